@@ -7,8 +7,8 @@ Targets
   fwloss_b200/libfwloss_b200.so   the C-ABI library (include/fwloss_b200.h):
                                   all CUDA kernels, compiled for sm_100a only.
   fw_radix_cuda<EXT_SUFFIX>       the drop-in Python module `fw_radix_cuda`
-                                  (csrc/fw_torch_binding.cpp), a host-only C++
-                                  torch extension linked against the library.
+                                  (csrc/fw_torch_*.cpp), a host-only C++ torch
+                                  extension linked against the library.
 """
 import os
 import subprocess
@@ -77,10 +77,12 @@ def build_lib(force=False, verbose=False):
 
 
 def build_ext(force=False):
-    src = os.path.join(CSRC, "fw_torch_binding.cpp")
-    deps = [src, os.path.join(INCLUDE, "fwloss_b200.h"), LIB]
+    srcs = [os.path.join(CSRC, f) for f in ("fw_torch_binding.cpp", "fw_torch_lm.cpp")]
+    deps = srcs + [os.path.join(INCLUDE, "fwloss_b200.h"), LIB]
     if not force and not _stale(EXT, deps):
         return EXT
+    from concurrent.futures import ThreadPoolExecutor
+
     import torch
     from torch.utils import cpp_extension as ce
 
@@ -88,10 +90,14 @@ def build_ext(force=False):
                                                    os.path.join(CUDA_HOME, "include")]
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", EXT + ".tmp",
-           "-DTORCH_EXTENSION_NAME=fw_radix_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-Wno-deprecated-declarations"]
-    cmd += [f"-I{p}" for p in incs]
+    os.makedirs(BUILD_DIR, exist_ok=True)
+    objs = [os.path.join(BUILD_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
+    todo = [(s, o) for s, o in zip(srcs, objs) if force or _stale(o, [s, os.path.join(INCLUDE, "fwloss_b200.h")])]
+    flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=fw_radix_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-Wno-deprecated-declarations"] + [f"-I{p}" for p in incs]
+    with ThreadPoolExecutor(max_workers=2) as ex:
+        list(ex.map(lambda so: subprocess.run(["g++", *flags, "-c", so[0], "-o", so[1]], check=True), todo))
+    cmd = ["g++", "-shared", "-o", EXT + ".tmp", *objs]
     cmd += [f"-L{p}" for p in libdirs] + [f"-Wl,-rpath,{p}" for p in libdirs]
     cmd += [f"-L{PKG}", "-lfwloss_b200", "-Wl,-rpath,$ORIGIN/fwloss_b200",
             "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]

@@ -1,0 +1,148 @@
+// Output layer in 8-bit integers:
+//   out[t, n] = (sum_k q[t, k] * wq[n, k]) * q_scale[t] * w_scale[n]
+// with an exact 32-bit integer sum on the tensor cores (tcgen05 kind::i8),
+// two fp32 multiplications and one rounding to the output's type.
+//
+// Two layouts of the same product:
+//   many tokens  tokens are the 128 rows of a tile, 256 weight rows its
+//                columns: bound by the tensor cores;
+//   few tokens   weight rows are the 128 rows of a tile and the tokens its
+//                16 .. 128 columns: every weight is read once, bound by HBM,
+//                so the small B tile leaves the shared memory to more stages.
+#include "fw_tc_gemm.cuh"
+
+namespace fwb200 {
+namespace {
+
+struct Int8Args {
+  const float* qs;
+  const float* ws;
+  void* out;
+  int64_t ldo;
+  int T, N, K;
+  int32_t* status;
+};
+
+template <class TO>
+struct Int8Many {
+  using Args = Int8Args;
+  static constexpr TcKind KIND = kTcS8;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int BN = 256, STAGES = 4;
+  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
+  __device__ static int tiles(const Args& a) { return ((a.T + 127) / 128) * ((a.N + 255) / 256); }
+  __device__ static TcTile tile(const Args& a, int w) {
+    const int mt = (a.T + 127) / 128, nt = (a.N + 255) / 256;
+    constexpr int kGroup = 16;  // token blocks that share the weight tiles in flight
+    const int g = w / (kGroup * nt), r = w - g * kGroup * nt;
+    const int gm = min(kGroup, mt - g * kGroup);
+    return {(g * kGroup + r % gm) * 128, (r / gm) * 256, 0, 0, (a.K + 127) / 128};
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
+                                  Done done) {
+    float* sm = reinterpret_cast<float*>(smem);
+    const int r0 = t.m0 + quad * 32;
+    const float qs = r0 + lane < a.T ? a.qs[r0 + lane] : 0.0f;
+    TO* out = static_cast<TO*>(a.out);
+    for (int c = 0; c < BN; c += 32) {
+      float v[32];
+      tmem_ld32(acc + c, v);
+      if (c + 32 == BN) done();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = (float)__float_as_int(v[i]) * qs;
+      __syncwarp();
+      const int n = t.n0 + c + lane;
+      if (n < a.N) {
+        const float ws = a.ws[n];
+        const int rows = min(32, a.T - r0);
+        for (int i = 0; i < rows; ++i) st_elem(out + (int64_t)(r0 + i) * a.ldo + n, sm[i * 33 + lane] * ws);
+      }
+      __syncwarp();
+    }
+  }
+};
+
+template <class TO, int NT>
+struct Int8Few {
+  using Args = Int8Args;
+  static constexpr TcKind KIND = kTcS8;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int BN = NT;
+  static constexpr int STAGES = NT <= 32 ? 10 : NT <= 64 ? 8 : 6;
+  static constexpr uint32_t EPI_BYTES = 0;
+  __device__ static int tiles(const Args& a) { return (a.N + 127) / 128; }
+  __device__ static TcTile tile(const Args& a, int w) { return {w * 128, 0, 0, 0, (a.K + 127) / 128}; }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
+                                  Done done) {
+    const int n = t.m0 + quad * 32 + lane;
+    const float ws = n < a.N ? a.ws[n] : 0.0f;
+    TO* out = static_cast<TO*>(a.out);
+    constexpr int STEP = NT < 32 ? 16 : 32;
+    for (int c = 0; c < NT; c += STEP) {
+      float v[STEP];
+      if constexpr (STEP == 32)
+        tmem_ld32(acc + c, v);
+      else
+        tmem_ld16(acc + c, v);
+      if (c + STEP == NT) done();
+      if (n >= a.N) continue;
+#pragma unroll
+      for (int i = 0; i < STEP; ++i) {
+        const int tok = c + i;
+        if (tok < a.T) st_elem(out + (int64_t)tok * a.ldo + n, (float)__float_as_int(v[i]) * a.qs[tok] * ws);
+      }
+    }
+  }
+};
+
+template <class P>
+cudaError_t run_int8(const void* a, int64_t rows_a, int64_t lda, const void* b, int64_t rows_b, int64_t ldb,
+                     const Int8Args& args, int64_t tiles, cudaStream_t st) {
+  CUtensorMap ma, mb;
+  if (!tc_map(&ma, kTcS8, a, rows_a, args.K, lda, kGemmBM) || !tc_map(&mb, kTcS8, b, rows_b, args.K, ldb, P::BN))
+    return cudaErrorInvalidValue;
+  return launch_gemm<P>(ma, mb, args, tiles, st);
+}
+
+template <class TO>
+cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Int8Args& a,
+                            cudaStream_t st) {
+  const int64_t nt = ((int64_t)a.N + 127) / 128;
+  if (a.T <= 16) return run_int8<Int8Few<TO, 16>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  if (a.T <= 128) return run_int8<Int8Few<TO, 128>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  const int64_t tiles = (((int64_t)a.T + 127) / 128) * (((int64_t)a.N + 255) / 256);
+  return run_int8<Int8Many<TO>>(q, a.T, ldq, w, a.N, ldw, a, tiles, st);
+}
+
+}  // namespace
+}  // namespace fwb200
+
+using namespace fwb200;
+
+extern "C" {
+
+int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const float* q_scale, const int8_t* wq, int64_t ldw,
+                   const float* w_scale, int64_t T, int64_t N, int64_t K, void* out, int64_t ldo, int32_t* status,
+                   void* stream) {
+  if (out_dtype != FWB_DTYPE_F32 && out_dtype != FWB_DTYPE_BF16 && out_dtype != FWB_DTYPE_F16) return FWB_E_DTYPE;
+  if (T < 0 || N < 1 || K < 1 || T > (1 << 30) || N > (1 << 30)) return FWB_E_SHAPE;
+  if (K > FWB_INT8_MAX_K || ((T + 127) / 128) * ((N + 255) / 256) > (1 << 30)) return FWB_E_CAPACITY;
+  if (ldq % 16 != 0 || ldw % 16 != 0 || ldq < K || ldw < K || ldo < N || ldq > ((int64_t)1 << 39) ||
+      ldw > ((int64_t)1 << 39) || ldo > ((int64_t)1 << 60) / (T > 0 ? T : 1))
+    return FWB_E_SHAPE;
+  if (T == 0) return FWB_OK;
+  if (!q || !q_scale || !wq || !w_scale || !out) return FWB_E_POINTER;
+  if (!aligned16(q) || !aligned16(wq)) return FWB_E_POINTER;
+  if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FWB_DTYPE_F32 ? 4 : 2)) return FWB_E_POINTER;
+  const Int8Args a = {q_scale, w_scale, out, ldo, (int)T, (int)N, (int)K, status};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (out_dtype == FWB_DTYPE_BF16) return launch_status(run_int8_linear<__nv_bfloat16>(q, ldq, wq, ldw, a, st));
+  if (out_dtype == FWB_DTYPE_F16) return launch_status(run_int8_linear<__half>(q, ldq, wq, ldw, a, st));
+  return launch_status(run_int8_linear<float>(q, ldq, wq, ldw, a, st));
+}
+
+}  // extern "C"

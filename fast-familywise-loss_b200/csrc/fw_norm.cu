@@ -1,0 +1,626 @@
+// Root-mean-square norm of a residual stream: the addition, the norm, its
+// gradient, and the form whose output is 8-bit integers with a scale per row
+// (the input of the 8-bit output layer).
+//
+//   s = x + residual, rounded to the stream's type      (s = x without one)
+//   y = s * rstd * w,   rstd = 1 / sqrt(mean(s^2) + eps)
+//   q = rint(y / scale), scale = max|y| / 127           (8-bit form)
+//
+// s is defined as the stored, rounded sum, so the gradient (which reads the
+// stored stream) is the gradient of exactly this function:
+//   a = dy * w,  c = sum(a * s) * rstd^2 / D
+//   ds = rstd * (a - s * c) + ds_out,  dx = dresidual = ds
+//   dw = sum over rows of dy * s * rstd
+// Sums, statistics and gains are fp32; each output is rounded once.
+//
+// Bound by HBM: forward reads x and residual and writes s and y, backward
+// reads dy, s and ds_out and writes ds, each once.  A row lives in the
+// registers of a group of G threads (a warp, or a CTA of up to 512) as CH
+// slots of 16 bytes per thread (fw_rowslots.cuh).  The grid is persistent
+// with a group count that is a multiple of 8, so that the rows one group
+// visits all start at the same distance from a 16-byte boundary: a thread
+// keeps the same columns from row to row, hence its gains and its part of dw
+// stay in registers for any D.  dw parts are written once per CTA and added
+// in a fixed order by a second kernel.
+#include <cuda_runtime.h>
+
+#include <climits>
+
+#include "fw_host.cuh"
+#include "fw_rowslots.cuh"
+
+namespace fwb200 {
+namespace {
+
+enum { kNormOut = 0, kNormInt8 = 1, kInt8Only = 2 };
+
+struct NormArgs {
+  const void* x;
+  const void* res;
+  const void* w;
+  void* s;
+  void* y;
+  float* rstd;
+  int8_t* q;
+  float* qscale;
+  int64_t ldx, ldr, lds, ldy, ldq;
+  int64_t rows, D;
+  float eps;
+  int w_f32;  // gains are fp32 whatever T is
+  int vec;    // x, residual, s and y rows share their distance from a 16-byte boundary
+};
+
+struct NormGradArgs {
+  const void* dy;
+  const void* s;
+  const void* dso;
+  const void* w;
+  const float* rstd;
+  void* dx;
+  float* part;  // [gridDim.x, D]
+  int64_t lddy, lds, ldo, lddx;
+  int64_t rows, D;
+  int w_f32;
+  int vec;
+};
+
+template <class T>
+__device__ __forceinline__ int row_off(const void* base, int64_t row, int64_t ld, int vec) {
+  if (!vec) return 0;
+  return (int)((reinterpret_cast<uintptr_t>(base) + (uintptr_t)(row * ld) * sizeof(T)) & 15u) / (int)sizeof(T);
+}
+
+// Gains of slot e0.., zero outside the row.
+template <class T>
+__device__ __forceinline__ void load_gain(const void* w, int w_f32, int64_t e0, int64_t D, float* out) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t e = e0 + j;
+    float g = 0.0f;
+    if (e >= 0 && e < D) g = w_f32 ? static_cast<const float*>(w)[e] : ld_elem(static_cast<const T*>(w) + e);
+    out[j] = g;
+  }
+}
+
+// Sum (or NaN-propagating maximum) over the G threads of a group; `buf` holds
+// one float per warp and alternates between two halves so that one barrier
+// per call is enough.
+template <int G, bool MAX>
+__device__ __forceinline__ float group_reduce(float v, float* buf, int& flip) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float u = __shfl_xor_sync(kFull, v, o);
+    v = MAX ? max_nan(v, u) : v + u;
+  }
+  if constexpr (G > 32) {
+    float* b = buf + flip * (G / 32);
+    flip ^= 1;
+    if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float t = b[0];
+#pragma unroll
+    for (int i = 1; i < G / 32; ++i) t = MAX ? max_nan(t, b[i]) : t + b[i];
+    v = t;
+  }
+  return v;
+}
+
+template <int G>
+__host__ __device__ constexpr int cta_threads() {
+  return G < 128 ? 128 : G;
+}
+
+template <class T, int G, int CH, int MODE>
+__global__ void __launch_bounds__(cta_threads<G>()) fw_norm_kernel(NormArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int R = cta_threads<G>() / G;
+  __shared__ float red[2 * (G / 32)];
+  extern __shared__ __align__(16) int8_t qrow_all[];
+  const int t = threadIdx.x % G;
+  const int grp = threadIdx.x / G;
+  const int64_t step = (int64_t)gridDim.x * R;
+  const int64_t first = (int64_t)blockIdx.x * R + grp;
+  if (first >= a.rows) return;  // a whole group; groups of one CTA share no barrier unless R == 1
+  int flip = 0;
+  const int off = row_off<T>(a.x, first, a.ldx, a.vec);
+  float gain[CH * V];
+  if constexpr (MODE != kInt8Only) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, (int64_t)(k * G + t) * V - off, a.D, gain + k * V);
+  }
+  const float inv_d = 1.0f / (float)a.D;
+  for (int64_t r = first; r < a.rows; r += step) {
+    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
+    uint4 xs[CH], rs[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) xs[k] = load_slot(xr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
+    if (a.res) {
+      const T* rr = static_cast<const T*>(a.res) + r * a.ldr;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) rs[k] = load_slot(rr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
+    }
+    float v[CH * V];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) unpack16<T>(xs[k], v + k * V);
+    if (a.res) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        float u[V];
+        unpack16<T>(rs[k], u);
+#pragma unroll
+        for (int j = 0; j < V; ++j) u[j] += v[k * V + j];
+        const uint4 p = pack16<T>(u);
+        unpack16<T>(p, v + k * V);
+        if (a.s) store_slot(static_cast<T*>(a.s) + r * a.lds, (int64_t)(k * G + t) * V - off, a.D, a.vec, p);
+      }
+    }
+    if constexpr (MODE != kInt8Only) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CH * V; ++i) ss = fmaf(v[i], v[i], ss);
+      ss = group_reduce<G, false>(ss, red, flip);
+      const float rstd = 1.0f / sqrtf(fmaf(ss, inv_d, a.eps));
+      if (a.rstd && t == 0) a.rstd[r] = rstd;
+#pragma unroll
+      for (int i = 0; i < CH * V; ++i) v[i] = v[i] * rstd * gain[i];
+    }
+    if constexpr (MODE == kNormOut) {
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        store_slot(static_cast<T*>(a.y) + r * a.ldy, (int64_t)(k * G + t) * V - off, a.D, a.vec, pack16<T>(v + k * V));
+    } else {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < CH * V; ++i) m = max_nan(m, fabsf(v[i]));  // slots past the row hold 0 * 0
+      m = group_reduce<G, true>(m, red, flip);
+      const float scale = m / 127.0f;
+      if (t == 0) a.qscale[r] = scale;
+      const bool live = scale > 0.0f && scale < CUDART_INF_F;  // otherwise the row is 0 (or NaN) through its scale
+      const int64_t w16 = (a.D + 15) / 16;
+      int8_t* qs = qrow_all + (int64_t)grp * w16 * 16;
+      if (t < 16 && a.D + t < w16 * 16) qs[a.D + t] = 0;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const int64_t e0 = (int64_t)(k * G + t) * V - off;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          const int64_t e = e0 + j;
+          if (e >= 0 && e < a.D) {
+            const float u = live ? rintf(__fdiv_rn(v[k * V + j], scale)) : 0.0f;
+            qs[e] = (int8_t)fminf(fmaxf(u, -127.0f), 127.0f);
+          }
+        }
+      }
+      if constexpr (G > 32)
+        __syncthreads();
+      else
+        __syncwarp();
+      for (int64_t i = t; i < w16; i += G)
+        reinterpret_cast<uint4*>(a.q + r * a.ldq)[i] = reinterpret_cast<const uint4*>(qs)[i];
+      if constexpr (G > 32)
+        __syncthreads();
+      else
+        __syncwarp();
+    }
+  }
+}
+
+// Rows too long for a CTA's registers: passes over the row in memory.
+template <class T, int MODE>
+__global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
+  __shared__ float red[2 * 32];
+  int flip = 0;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
+    const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
+    auto elem = [&](int64_t e) {
+      float v = ld_elem(xr + e);
+      return rr ? Elem<T>::to_f(Elem<T>::from_f(v + ld_elem(rr + e))) : v;
+    };
+    auto gain = [&](int64_t e) {
+      return a.w_f32 ? static_cast<const float*>(a.w)[e] : ld_elem(static_cast<const T*>(a.w) + e);
+    };
+    float rstd = 1.0f;
+    if constexpr (MODE != kInt8Only) {
+      float ss = 0.0f;
+      for (int64_t e = threadIdx.x; e < a.D; e += 1024) {
+        const float v = elem(e);
+        ss = fmaf(v, v, ss);
+      }
+      ss = group_reduce<1024, false>(ss, red, flip);
+      rstd = 1.0f / sqrtf(ss / (float)a.D + a.eps);
+      if (a.rstd && threadIdx.x == 0) a.rstd[r] = rstd;
+    }
+    float m = 0.0f;
+    for (int64_t e = threadIdx.x; e < a.D; e += 1024) {
+      float v = elem(e);
+      if (rr && a.s) st_elem(static_cast<T*>(a.s) + r * a.lds + e, v);
+      if constexpr (MODE != kInt8Only) v = v * rstd * gain(e);
+      if constexpr (MODE == kNormOut)
+        st_elem(static_cast<T*>(a.y) + r * a.ldy + e, v);
+      else
+        m = max_nan(m, fabsf(v));
+    }
+    if constexpr (MODE != kNormOut) {
+      m = group_reduce<1024, true>(m, red, flip);
+      const float scale = m / 127.0f;
+      if (threadIdx.x == 0) a.qscale[r] = scale;
+      const bool live = scale > 0.0f && scale < CUDART_INF_F;
+      for (int64_t e = threadIdx.x; e < (a.D + 15) / 16 * 16; e += 1024) {
+        float u = 0.0f;
+        if (e < a.D && live) {
+          float v = elem(e);
+          if constexpr (MODE != kInt8Only) v = v * rstd * gain(e);
+          u = rintf(__fdiv_rn(v, scale));
+        }
+        a.q[r * a.ldq + e] = (int8_t)fminf(fmaxf(u, -127.0f), 127.0f);
+      }
+    }
+  }
+}
+
+template <class T, int G, int CH>
+__global__ void __launch_bounds__(cta_threads<G>()) fw_norm_grad_kernel(NormGradArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  constexpr int R = cta_threads<G>() / G;
+  __shared__ float red[2 * (G / 32)];
+  extern __shared__ __align__(16) float dw_row[];  // [D], R > 1 only
+  const int t = threadIdx.x % G;
+  const int grp = threadIdx.x / G;
+  const int64_t step = (int64_t)gridDim.x * R;
+  const int64_t first = (int64_t)blockIdx.x * R + grp;
+  int flip = 0;
+  const int off = row_off<T>(a.s, first, a.lds, a.vec);
+  float gain[CH * V], dw[CH * V];
+#pragma unroll
+  for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, (int64_t)(k * G + t) * V - off, a.D, gain + k * V);
+#pragma unroll
+  for (int i = 0; i < CH * V; ++i) dw[i] = 0.0f;
+  const float inv_d = 1.0f / (float)a.D;
+  for (int64_t r = first; r < a.rows; r += step) {
+    const T* sr = static_cast<const T*>(a.s) + r * a.lds;
+    const T* gr = static_cast<const T*>(a.dy) + r * a.lddy;
+    uint4 ss[CH], gs[CH], os[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      ss[k] = load_slot(sr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
+      gs[k] = load_slot(gr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
+    }
+    if (a.dso) {
+      const T* orow = static_cast<const T*>(a.dso) + r * a.ldo;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) os[k] = load_slot(orow, (int64_t)(k * G + t) * V - off, a.D, a.vec);
+    } else {
+#pragma unroll
+      for (int k = 0; k < CH; ++k) os[k] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    const float rstd = a.rstd[r];
+    float c = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      float s[V], g[V];
+      unpack16<T>(ss[k], s);
+      unpack16<T>(gs[k], g);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float n = s[j] * rstd;
+        c = fmaf(g[j] * gain[k * V + j], n, c);
+        dw[k * V + j] = fmaf(g[j], n, dw[k * V + j]);
+      }
+    }
+    c = group_reduce<G, false>(c, red, flip) * inv_d;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      float s[V], g[V], o[V];
+      unpack16<T>(ss[k], s);
+      unpack16<T>(gs[k], g);
+      unpack16<T>(os[k], o);
+#pragma unroll
+      for (int j = 0; j < V; ++j) o[j] = fmaf(rstd, fmaf(g[j], gain[k * V + j], -(s[j] * rstd) * c), o[j]);
+      store_slot(static_cast<T*>(a.dx) + r * a.lddx, (int64_t)(k * G + t) * V - off, a.D, a.vec, pack16<T>(o));
+    }
+  }
+  if (!a.part) return;
+  float* part = a.part + (int64_t)blockIdx.x * a.D;
+  if constexpr (R == 1) {
+#pragma unroll
+    for (int i = 0; i < CH * V; ++i) {
+      const int64_t e = (int64_t)((i / V) * G + t) * V - off + i % V;
+      if (e >= 0 && e < a.D) part[e] = dw[i];
+    }
+  } else {
+    for (int64_t e = threadIdx.x; e < a.D; e += blockDim.x) dw_row[e] = 0.0f;
+    for (int g = 0; g < R; ++g) {  // the CTA's groups in order: their rows start at different distances
+      __syncthreads();
+      if (grp == g) {
+#pragma unroll
+        for (int i = 0; i < CH * V; ++i) {
+          const int64_t e = (int64_t)((i / V) * G + t) * V - off + i % V;
+          if (e >= 0 && e < a.D) dw_row[e] += dw[i];
+        }
+      }
+    }
+    __syncthreads();
+    for (int64_t e = threadIdx.x; e < a.D; e += blockDim.x) part[e] = dw_row[e];
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(1024) fw_norm_grad_long_kernel(NormGradArgs a) {
+  __shared__ float red[2 * 32];
+  int flip = 0;
+  float* part = a.part ? a.part + (int64_t)blockIdx.x * a.D : nullptr;
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const T* sr = static_cast<const T*>(a.s) + r * a.lds;
+    const T* gr = static_cast<const T*>(a.dy) + r * a.lddy;
+    const float rstd = a.rstd[r];
+    auto gain = [&](int64_t e) {
+      return a.w_f32 ? static_cast<const float*>(a.w)[e] : ld_elem(static_cast<const T*>(a.w) + e);
+    };
+    float c = 0.0f;
+    for (int64_t e = threadIdx.x; e < a.D; e += 1024) {
+      const float n = ld_elem(sr + e) * rstd, g = ld_elem(gr + e);
+      c = fmaf(g * gain(e), n, c);
+      if (part) part[e] = r == blockIdx.x ? g * n : fmaf(g, n, part[e]);  // this thread's own columns
+    }
+    c = group_reduce<1024, false>(c, red, flip) / (float)a.D;
+    for (int64_t e = threadIdx.x; e < a.D; e += 1024) {
+      const float o = a.dso ? ld_elem(static_cast<const T*>(a.dso) + r * a.ldo + e) : 0.0f;
+      const float v = fmaf(rstd, fmaf(ld_elem(gr + e), gain(e), -(ld_elem(sr + e) * rstd) * c), o);
+      st_elem(static_cast<T*>(a.dx) + r * a.lddx + e, v);
+    }
+  }
+}
+
+// dw[e] = sum over the parts in order; 32 columns and 8 interleaved runs of
+// parts per CTA.
+template <class T>
+__global__ void __launch_bounds__(256) fw_norm_dw_kernel(const float* __restrict__ part, int64_t n, int64_t D,
+                                                         T* __restrict__ dw) {
+  __shared__ float sm[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t e = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.0f;
+  if (e < D)
+    for (int64_t p = w; p < n; p += 8) s += part[p * D + e];
+  sm[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && e < D) {
+    float t = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t += sm[i][lane];
+    st_elem(dw + e, t);
+  }
+}
+
+// Threads per row and slots per thread by the row's slot count: a warp up to
+// 64 slots; CTAs of 128, 256 and 512 threads so that a thread holds at most
+// 2 slots (4 in the longest); the memory-pass kernels beyond 2048.
+struct NormShape {
+  int G, CH;
+};
+
+NormShape norm_shape(int64_t D, int64_t esize, bool vec) {
+  const int64_t V = 16 / esize;
+  const int64_t n = (D + V - 1) / V + (vec && (D * esize) % 16 != 0 ? 1 : 0);
+  if (n <= 32) return {32, 1};
+  if (n <= 64) return {32, 2};
+  if (n <= 128) return {128, 1};
+  if (n <= 256) return {128, 2};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {512, 2};
+  if (n <= 2048) return {512, 4};
+  return {0, 0};
+}
+
+// Persistent grid: enough CTAs for about 1024 resident threads per SM, a
+// multiple of 8 unless every group has at most one row.
+int64_t norm_grid(int64_t rows, int G) {
+  const int threads = G == 0 ? 1024 : (G < 128 ? 128 : G);
+  const int64_t R = G == 0 ? 1 : threads / G;
+  const int64_t need = (rows + R - 1) / R;
+  int64_t cap = (int64_t)sm_count() * (G == 0 ? 2 : 1024 / threads);
+  cap = (cap + 7) / 8 * 8;
+  return need < cap ? need : cap;
+}
+
+bool same_slots(const void* p, int64_t ld, const void* q, int64_t ldq, int64_t esize) {
+  return ((reinterpret_cast<uintptr_t>(p) ^ reinterpret_cast<uintptr_t>(q)) & 15u) == 0 &&
+         ((ld - ldq) * esize) % 16 == 0;
+}
+
+bool elem_aligned(const void* p, int64_t esize) { return reinterpret_cast<uintptr_t>(p) % esize == 0; }
+
+int esize_of(int dtype) { return dtype == FWB_DTYPE_F32 ? 4 : 2; }
+
+int norm_check(int dtype, int wdtype, int64_t rows, int64_t D) {
+  if (dtype != FWB_DTYPE_F32 && dtype != FWB_DTYPE_BF16 && dtype != FWB_DTYPE_F16) return FWB_E_DTYPE;
+  if (wdtype != dtype && wdtype != FWB_DTYPE_F32) return FWB_E_DTYPE;
+  if (rows < 0 || D < 1 || D > (int64_t)INT_MAX - 64) return FWB_E_SHAPE;
+  return FWB_OK;
+}
+
+bool ld_ok(int64_t ld, int64_t rows, int64_t D) {
+  return ld >= D && (rows <= 0 || ld <= ((int64_t)1 << 60) / rows);
+}
+
+template <class T, int MODE>
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
+  const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
+  const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
+  const int R = sh.G == 32 ? 4 : 1;
+  const size_t smem = MODE == kNormOut ? 0 : (size_t)R * (size_t)((a.D + 15) / 16 * 16);
+  if (sh.G == 32 && sh.CH == 1) fw_norm_kernel<T, 32, 1, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 32) fw_norm_kernel<T, 32, 2, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128 && sh.CH == 1) fw_norm_kernel<T, 128, 1, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128) fw_norm_kernel<T, 128, 2, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 256) fw_norm_kernel<T, 256, 2, MODE><<<grid, 256, smem, st>>>(a);
+  else if (sh.G == 512 && sh.CH == 2) fw_norm_kernel<T, 512, 2, MODE><<<grid, 512, smem, st>>>(a);
+  else if (sh.G == 512) fw_norm_kernel<T, 512, 4, MODE><<<grid, 512, smem, st>>>(a);
+  else fw_norm_long_kernel<T, MODE><<<grid, 1024, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
+  const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
+  const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
+  const size_t smem = sh.G == 32 ? (size_t)a.D * sizeof(float) : 0;
+  if (sh.G == 32 && sh.CH == 1) fw_norm_grad_kernel<T, 32, 1><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 32) fw_norm_grad_kernel<T, 32, 2><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128 && sh.CH == 1) fw_norm_grad_kernel<T, 128, 1><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128) fw_norm_grad_kernel<T, 128, 2><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 256) fw_norm_grad_kernel<T, 256, 2><<<grid, 256, smem, st>>>(a);
+  else if (sh.G == 512 && sh.CH == 2) fw_norm_grad_kernel<T, 512, 2><<<grid, 512, smem, st>>>(a);
+  else if (sh.G == 512) fw_norm_grad_kernel<T, 512, 4><<<grid, 512, smem, st>>>(a);
+  else fw_norm_grad_long_kernel<T><<<grid, 1024, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <int MODE>
+int run_norm(int dtype, const NormArgs& a, cudaStream_t st) {
+  if (dtype == FWB_DTYPE_BF16) return launch_status(launch_norm<__nv_bfloat16, MODE>(a, st));
+  if (dtype == FWB_DTYPE_F16) return launch_status(launch_norm<__half, MODE>(a, st));
+  return launch_status(launch_norm<float, MODE>(a, st));
+}
+
+// Shared by the entry points: argument checks and the slot test.
+int norm_args(int dtype, int wdtype, const void* x, int64_t ldx, const void* res, int64_t ldr, const void* w,
+              int64_t rows, int64_t D, float eps, void* s, int64_t lds, NormArgs* a) {
+  if (int rc = norm_check(dtype, wdtype, rows, D)) return rc;
+  if (!ld_ok(ldx, rows, D) || (res && !ld_ok(ldr, rows, D)) || (s && !ld_ok(lds, rows, D))) return FWB_E_SHAPE;
+  if (!(eps >= 0.0f)) return FWB_E_SHAPE;
+  const int es = esize_of(dtype);
+  if (!elem_aligned(x, es) || !elem_aligned(res, es) || !elem_aligned(s, es) || !elem_aligned(w, esize_of(wdtype)))
+    return FWB_E_POINTER;
+  a->x = x;
+  a->res = res;
+  a->w = w;
+  a->s = s;
+  a->ldx = ldx;
+  a->ldr = ldr;
+  a->lds = lds;
+  a->rows = rows;
+  a->D = D;
+  a->eps = eps;
+  a->w_f32 = wdtype == FWB_DTYPE_F32 && dtype != FWB_DTYPE_F32;
+  a->vec = (!res || same_slots(x, ldx, res, ldr, es)) && (!s || same_slots(x, ldx, s, lds, es));
+  return FWB_OK;
+}
+
+int int8_rows_check(const int8_t* q, int64_t ldq, int64_t rows, int64_t D) {
+  if (ldq % 16 != 0 || ldq < (D + 15) / 16 * 16 || (rows > 0 && ldq > ((int64_t)1 << 60) / rows)) return FWB_E_SHAPE;
+  return aligned16(q) ? FWB_OK : FWB_E_POINTER;
+}
+
+}  // namespace
+}  // namespace fwb200
+
+using namespace fwb200;
+
+extern "C" {
+
+int fw_rms_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                const void* weight, int64_t rows, int64_t D, float eps, void* sum, int64_t lds, void* y, int64_t ldy,
+                float* rstd, void* stream) {
+  NormArgs a = {};
+  if (int rc = norm_args(dtype, wdtype, x, ldx, residual, ldr, weight, rows, D, eps, sum, lds, &a)) return rc;
+  if (!ld_ok(ldy, rows, D)) return FWB_E_SHAPE;
+  if (rows == 0) return FWB_OK;
+  if (!x || !weight || !y || (residual && !sum)) return FWB_E_POINTER;
+  const int es = esize_of(dtype);
+  if (!elem_aligned(y, es)) return FWB_E_POINTER;
+  a.y = y;
+  a.ldy = ldy;
+  a.rstd = rstd;
+  a.vec = a.vec && same_slots(x, ldx, y, ldy, es);
+  return run_norm<kNormOut>(dtype, a, static_cast<cudaStream_t>(stream));
+}
+
+int fw_rms_norm_int8(int dtype, int wdtype, const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                     const void* weight, int64_t rows, int64_t D, float eps, void* sum, int64_t lds, int8_t* q,
+                     int64_t ldq, float* scale, void* stream) {
+  NormArgs a = {};
+  if (int rc = norm_args(dtype, wdtype, x, ldx, residual, ldr, weight, rows, D, eps, sum, lds, &a)) return rc;
+  if (rows == 0) return FWB_OK;
+  if (!x || !weight || !q || !scale || (residual && !sum)) return FWB_E_POINTER;
+  if (int rc = int8_rows_check(q, ldq, rows, D)) return rc;
+  a.q = q;
+  a.ldq = ldq;
+  a.qscale = scale;
+  return run_norm<kNormInt8>(dtype, a, static_cast<cudaStream_t>(stream));
+}
+
+int fw_quantize_rows_int8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t D, int8_t* q, int64_t ldq,
+                          float* scale, void* stream) {
+  NormArgs a = {};
+  if (int rc = norm_args(dtype, dtype, x, ldx, nullptr, 0, nullptr, rows, D, 0.0f, nullptr, 0, &a)) return rc;
+  if (rows == 0) return FWB_OK;
+  if (!x || !q || !scale) return FWB_E_POINTER;
+  if (int rc = int8_rows_check(q, ldq, rows, D)) return rc;
+  a.q = q;
+  a.ldq = ldq;
+  a.qscale = scale;
+  return run_norm<kInt8Only>(dtype, a, static_cast<cudaStream_t>(stream));
+}
+
+// An upper bound on the parts of dweight that fw_rms_norm_grad writes, by the
+// largest grid of any shape it may choose.
+int64_t fw_rms_norm_grad_parts(int64_t rows) {
+  if (rows < 0) return 0;
+  const int64_t cap = ((int64_t)sm_count() * 8 + 7) / 8 * 8;
+  return rows < cap ? rows : cap;
+}
+
+int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy, const void* sum, int64_t lds,
+                     const void* dsum, int64_t ldo, const void* weight, const float* rstd, int64_t rows, int64_t D,
+                     void* dx, int64_t lddx, float* parts, int64_t nparts, void* dweight, void* stream) {
+  if (int rc = norm_check(dtype, wdtype, rows, D)) return rc;
+  if (!ld_ok(lddy, rows, D) || !ld_ok(lds, rows, D) || !ld_ok(lddx, rows, D) || (dsum && !ld_ok(ldo, rows, D)))
+    return FWB_E_SHAPE;
+  const int es = esize_of(dtype);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dweight && !elem_aligned(dweight, esize_of(wdtype))) return FWB_E_POINTER;
+  if (rows == 0) {
+    if (dweight && cudaMemsetAsync(dweight, 0, (size_t)D * esize_of(wdtype), st) != cudaSuccess) return FWB_E_LAUNCH;
+    return FWB_OK;
+  }
+  if (!dy || !sum || !weight || !rstd || !dx || (dweight && !parts)) return FWB_E_POINTER;
+  if (!elem_aligned(dy, es) || !elem_aligned(sum, es) || !elem_aligned(dsum, es) || !elem_aligned(dx, es) ||
+      !elem_aligned(weight, esize_of(wdtype)))
+    return FWB_E_POINTER;
+  NormGradArgs a = {};
+  a.dy = dy;
+  a.s = sum;
+  a.dso = dsum;
+  a.w = weight;
+  a.rstd = rstd;
+  a.dx = dx;
+  a.part = dweight ? parts : nullptr;
+  a.lddy = lddy;
+  a.lds = lds;
+  a.ldo = ldo;
+  a.lddx = lddx;
+  a.rows = rows;
+  a.D = D;
+  a.w_f32 = wdtype == FWB_DTYPE_F32 && dtype != FWB_DTYPE_F32;
+  a.vec = same_slots(sum, lds, dy, lddy, es) && same_slots(sum, lds, dx, lddx, es) &&
+          (!dsum || same_slots(sum, lds, dsum, ldo, es));
+  const int64_t grid = norm_grid(rows, norm_shape(D, es, a.vec).G);
+  if (dweight && nparts < grid) return FWB_E_CAPACITY;
+  cudaError_t e = dtype == FWB_DTYPE_BF16  ? launch_norm_grad<__nv_bfloat16>(a, st)
+                  : dtype == FWB_DTYPE_F16 ? launch_norm_grad<__half>(a, st)
+                                           : launch_norm_grad<float>(a, st);
+  if (e != cudaSuccess || !dweight) return launch_status(e);
+  const dim3 g2((unsigned)((D + 31) / 32));
+  if (wdtype == FWB_DTYPE_BF16)
+    fw_norm_dw_kernel<__nv_bfloat16><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<__nv_bfloat16*>(dweight));
+  else if (wdtype == FWB_DTYPE_F16)
+    fw_norm_dw_kernel<__half><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<__half*>(dweight));
+  else
+    fw_norm_dw_kernel<float><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<float*>(dweight));
+  return launch_status(cudaGetLastError());
+}
+
+}  // extern "C"

@@ -1,0 +1,96 @@
+// Rows cut into 16-byte slots of memory, for kernels that keep a row in
+// registers whatever its length and start address.
+//
+// A row of D elements that starts `off` elements past a 16-byte boundary is
+// covered by slots k = 0, 1, ...; slot k holds elements k * V - off + j,
+// j < V = 16 / sizeof(T).  Slots inside the row are one 16-byte access; the
+// first and the last touch only the row's own elements, one by one.  Tensors
+// whose rows start at the same distance from a boundary share the slots; if
+// they do not (`vec` false), off is 0 and every slot is read element by
+// element.
+#pragma once
+
+#include "fw_device.cuh"
+
+namespace fwb200 {
+
+__device__ __forceinline__ uint4 ld_global16(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+template <class T>
+__device__ __forceinline__ uint4 load_slot(const T* row, int64_t e0, int64_t D, bool vec) {
+  constexpr int V = 16 / sizeof(T);
+  if (vec && e0 >= 0 && e0 + V <= D) return ld_stream16(row + e0);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t e = e0 + j;
+    if (e >= 0 && e < D) {
+      if constexpr (sizeof(T) == 4)
+        w[j] = __float_as_uint(row[e]);
+      else
+        w[j >> 1] |= (uint32_t)*reinterpret_cast<const unsigned short*>(row + e) << (16 * (j & 1));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <class T>
+__device__ __forceinline__ void store_slot(T* row, int64_t e0, int64_t D, bool vec, const uint4& u) {
+  constexpr int V = 16 / sizeof(T);
+  if (vec && e0 >= 0 && e0 + V <= D) {
+    *reinterpret_cast<uint4*>(row + e0) = u;
+    return;
+  }
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int64_t e = e0 + j;
+    if (e >= 0 && e < D) {
+      if constexpr (sizeof(T) == 4)
+        row[e] = __uint_as_float(w[j]);
+      else
+        *reinterpret_cast<unsigned short*>(row + e) = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
+    }
+  }
+}
+
+// The 16 bytes at `p`, which may start anywhere a T may; [begin, end) is the
+// row.  A full slot read through its two aligned neighbours and a funnel
+// shift, except where a neighbour would leave the row.
+template <class T>
+__device__ __forceinline__ uint4 load_shifted(const T* p, const T* begin, const T* end) {
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(p);
+  const uint32_t m = (uint32_t)(addr & 15u);
+  if (m == 0) return ld_stream16(p);
+  const uintptr_t lo = addr - m;
+  if (lo >= reinterpret_cast<uintptr_t>(begin) && lo + 32 <= reinterpret_cast<uintptr_t>(end)) {
+    const uint4 a = ld_global16(reinterpret_cast<const void*>(lo));
+    const uint4 b = ld_global16(reinterpret_cast<const void*>(lo + 16));
+    const uint32_t s = (m & 3u) * 8u;
+    uint32_t w[5];
+    switch (m >> 2) {  // the same for the whole row
+      case 0: w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x; break;
+      case 1: w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y; break;
+      case 2: w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z; break;
+      default: w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w; break;
+    }
+    return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s),
+                      __funnelshift_r(w[2], w[3], s), __funnelshift_r(w[3], w[4], s));
+  }
+  return load_slot(p, 0, 16 / (int)sizeof(T), false);
+}
+
+// Slot of a row whose own slots lie elsewhere: elements e0 .. e0 + V of the
+// row at `row`, zero outside [0, D).
+template <class T>
+__device__ __forceinline__ uint4 load_slot_shifted(const T* row, int64_t e0, int64_t D) {
+  constexpr int V = 16 / sizeof(T);
+  if (e0 >= 0 && e0 + V <= D) return load_shifted(row + e0, row, row + D);
+  return load_slot(row, e0, D, false);
+}
+
+}  // namespace fwb200

@@ -662,6 +662,8 @@ void segment_grad_weight(torch::Tensor hidden, torch::Tensor sorted_keys, torch:
            "fw_segment_grad_weight");
 }
 
+void register_lm_operators(pybind11::module_& m);  // fw_torch_lm.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 (sm_100a) Familywise loss: drop-in for the fw_radix_cuda module";
   m.def("fw_forward", &fw_forward, "FW forward (support as candidate lists)");
@@ -706,5 +708,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("shard_solve", &shard_solve, "class-sharded step 3: global solve from gathered summaries",
         py::arg("gathered"), py::arg("rank"), py::arg("col_start"), py::arg("z_local"), py::arg("targets"),
         py::arg("grad_scale"), py::arg("grad"), py::arg("local_idx"), py::arg("status") = py::none());
+  register_lm_operators(m);
   m.def("version", []() { return std::string(fw_version()); });
 }

@@ -1,0 +1,691 @@
+// Softmax cross entropy of an output layer, logits z = H W^T never stored:
+//   lse_r = log sum_j exp z_rj,  loss_r = lse_r - z_r,y(r)
+//   G_rj = g_r (exp(z_rj - lse_r) - 1[j = y(r)]),  dH = G W,  dW = G^T H
+// for H [B, D] and W [V, D] in bfloat16 or float16; logits, statistics and
+// sums in fp32.
+//
+// Forward: live rows are packed (rows whose label is ignore_index take no
+// part in anything, whatever they hold), one tensor-core product gives each
+// 128 x 256 logit tile, whose epilogue keeps only each row's maximum and sum
+// of exponentials; a second kernel joins the tiles' pairs, takes the losses
+// and reduces them in a fixed order.
+// Backward, in pieces of the vocabulary: the logits of a piece again, their
+// epilogue writing G (16-bit, the product's operand type: the rounding is
+// relative to each entry, so it weighs as the rounding of the result does);
+// then dH += G W and dW = G^T H of the piece, G read in both orientations
+// from the one buffer (MN-major operands), each row of dW written once.
+// Bound by the tensor cores: 2 B V D operations for each of the four products.
+//
+// float16 G: exp(z - lse) / B may be under float16's smallest value, so rows
+// are scaled to the range of the type (largest upstream gradient to 2^15) and
+// the factor is taken out in fp32 after the sums.
+#include "fw_reduce.cuh"
+#include "fw_rowslots.cuh"
+#include "fw_tc_gemm.cuh"
+
+namespace fwb200 {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kF16Unit = 32768.0f;
+constexpr int kPackThreads = 256;
+
+// Device words at the start of the state.
+struct XentHead {
+  int32_t rows;    // live rows
+  uint32_t done;   // blocks of the joining kernel that have finished
+  int32_t status;  // status bits raised inside
+  float back;      // factor taken out after the sums (float16)
+};
+
+struct PackArgs {
+  const void* hidden;
+  const int64_t* y;
+  int64_t B, Bp, D, Dp, ldh, V, ignore;
+  void* hp;
+  int32_t* row_of;   // [Bp] packed -> given row, -1 past the last live one
+  int32_t* label;    // [Bp] -1: outside [0, V)
+  float* loss_rows;  // zero for ignored rows, per given row; may be NULL
+  XentHead* head;
+  int32_t* status;
+  int per_cta;
+};
+
+// Every CTA counts the live rows before its own by reading all labels, so
+// packing is one launch.
+template <class T>
+__global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) {
+  __shared__ int red[2][kPackThreads / 32];
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * a.per_cta;
+  int before = 0, total = 0;
+  for (int64_t i = threadIdx.x; i < a.B; i += kPackThreads) {
+    const int live = a.y[i] != a.ignore;
+    total += live;
+    before += i < r0 ? live : 0;
+  }
+  before = __reduce_add_sync(kFull, before);
+  total = __reduce_add_sync(kFull, total);
+  if (lane == 0) {
+    red[0][w] = before;
+    red[1][w] = total;
+  }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int i = 0; i < kPackThreads / 32; ++i) {
+    before += red[0][i];
+    total += red[1][i];
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.head->rows = total;
+    a.head->done = 0u;
+    a.head->status = 0;
+  }
+  const int64_t rows_up = ((int64_t)total + 127) / 128 * 128;
+  for (int i0 = 0; i0 < a.per_cta; i0 += 32) {
+    const int64_t rl = r0 + i0 + lane;
+    const int64_t yl = rl < a.B ? a.y[rl] : a.ignore;
+    const uint32_t live = __ballot_sync(kFull, rl < a.B && yl != a.ignore);
+    for (int i = w; i < 32 && i0 + i < a.per_cta; i += kPackThreads / 32) {
+      const int64_t r = r0 + i0 + i;
+      if (r >= a.Bp) break;
+      const bool alive = (live >> i) & 1u;
+      const int64_t ahead = before + __popc(live & ((1u << i) - 1u));
+      const int64_t dst = alive ? ahead : total + (r - ahead);
+      const int64_t y = __shfl_sync(kFull, yl, i);
+      if (lane == 0) {
+        const bool ok = y >= 0 && y < a.V;
+        a.row_of[dst] = alive ? (int32_t)r : -1;
+        a.label[dst] = alive && ok ? (int32_t)y : -1;
+        if (alive && !ok) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
+        if (!alive && r < a.B && a.loss_rows) a.loss_rows[r] = 0.0f;
+      }
+      if (dst >= rows_up) continue;
+      T* out = static_cast<T*>(a.hp) + dst * a.Dp;
+      const T* in = static_cast<const T*>(a.hidden) + (alive ? r : 0) * a.ldh;
+      for (int64_t e = (int64_t)lane * V; e < a.Dp; e += 32 * V)
+        *reinterpret_cast<uint4*>(out + e) = alive ? load_slot_shifted(in, e, a.D) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    before += __popc(live);
+  }
+}
+
+// Rows of an unaligned matrix copied to 16-byte boundaries.
+template <class T>
+__global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_t ld, T* dst, int64_t ldd, int64_t rows,
+                                                            int64_t D) {
+  constexpr int V = 16 / sizeof(T);
+  const int lane = threadIdx.x & 31;
+  const int64_t slabs = (ldd + 32 * V * 4 - 1) / (32 * V * 4);
+  const int64_t nw = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows * slabs; i += nw) {
+    const int64_t r = i / slabs, e0 = ((i - r * slabs) * 128 + lane) * V;
+    uint4 u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t e = e0 + k * 32 * V;
+      if (e < ldd) u[k] = load_slot_shifted(src + r * ld, e, D);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t e = e0 + k * 32 * V;
+      if (e < ldd) *reinterpret_cast<uint4*>(dst + r * ldd + e) = u[k];
+    }
+  }
+}
+
+// Order of tiles: blocks of `group` m-blocks, m fastest inside one, so that
+// the tiles in flight share their operands in L2.
+__device__ __forceinline__ void tile_order(int w, int mt, int nt, int group, int* m, int* n) {
+  const int g = w / (group * nt), r = w - g * group * nt;
+  const int gm = min(group, mt - g * group);
+  *m = g * group + r % gm;
+  *n = r / gm;
+}
+
+// ------------------------------------------------------------ forward
+struct LseArgs {
+  const XentHead* head;
+  const int32_t* label;
+  float2* part;  // [tiles of V, Bp]: maximum, sum of exp(z - maximum)
+  float* zy;     // [Bp]
+  int64_t Bp;
+  int V, D;
+  int32_t* status;
+};
+
+template <TcKind K>
+struct LseTile {
+  using Args = LseArgs;
+  static constexpr TcKind KIND = K;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int BN = 256, STAGES = 4;
+  static constexpr uint32_t EPI_BYTES = 0;
+  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * ((a.V + 255) / 256); }
+  __device__ static TcTile tile(const Args& a, int w) {
+    int m, n;
+    tile_order(w, (a.head->rows + 127) / 128, (a.V + 255) / 256, 32, &m, &n);
+    return {m * 128, n * 256, 0, 0, (a.D + 63) / 64};
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
+                                  Done done) {
+    const int row = t.m0 + quad * 32 + lane;  // < Bp
+    const int y = a.label[row];
+    float m = -CUDART_INF_F, s = 0.0f;
+    for (int c = 0; c < BN; c += 32) {
+      const int valid = min(32, a.V - (t.n0 + c));
+      float v[32];
+      tmem_ld32(acc + c, v);
+      if (c + 32 == BN) done();
+      if (valid <= 0) continue;
+      float top = -CUDART_INF_F;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        if (i >= valid) v[i] = -CUDART_INF_F;
+        if (t.n0 + c + i == y) a.zy[row] = v[i];
+        top = max_nan(top, v[i]);
+      }
+      if (top > m || top != top) {  // the maximum moves, or is NaN
+        const float to = top;
+        s = m == -CUDART_INF_F ? s : s * exp2f((m - to) * kLog2e);
+        m = to;
+      }
+      if (m == -CUDART_INF_F) continue;  // nothing but -inf so far
+#pragma unroll
+      for (int i = 0; i < 32; ++i) s += exp2f((v[i] - m) * kLog2e);
+    }
+    a.part[(int64_t)(t.n0 / BN) * a.Bp + row] = make_float2(m, s);
+  }
+};
+
+struct JoinArgs {
+  XentHead* head;
+  const float2* part;
+  const float* zy;
+  const int32_t* label;
+  const int32_t* row_of;
+  float* lse;        // [Bp], packed
+  float* loss_pack;  // [Bp], packed
+  float* loss;       // [B] (reduction none) or one value
+  int64_t Bp;
+  int ntiles;
+  int reduction;
+  int32_t* status;
+};
+
+constexpr int kJoinWarps = 8;
+
+// 32 rows per CTA, the tiles' pairs split over its warps; the last CTA to
+// finish adds the losses in a fixed order.
+__global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_kernel(JoinArgs a) {
+  __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32];
+  __shared__ double sd[kJoinWarps];
+  __shared__ bool last;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rows = a.head->rows;
+  const int row = blockIdx.x * 32 + lane;
+  float m = -CUDART_INF_F, s = 0.0f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int t = w; t < a.ntiles; t += kJoinWarps) {
+      const float2 p = a.part[(int64_t)t * a.Bp + row];
+      const float to = max_nan(m, p.x);
+      if (to == -CUDART_INF_F) continue;
+      s = (m == -CUDART_INF_F ? 0.0f : s * exp2f((m - to) * kLog2e)) +
+          (p.x == -CUDART_INF_F ? 0.0f : p.y * exp2f((p.x - to) * kLog2e));
+      m = to;
+    }
+  }
+  sm[w][lane] = m;
+  ss[w][lane] = s;
+  __syncthreads();
+  if (w == 0 && row < rows) {
+    float M = sm[0][lane];
+#pragma unroll
+    for (int i = 1; i < kJoinWarps; ++i) M = max_nan(M, sm[i][lane]);
+    float S = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kJoinWarps; ++i)
+      if (sm[i][lane] != -CUDART_INF_F) S += ss[i][lane] * exp2f((sm[i][lane] - M) * kLog2e);
+    const bool ok = a.label[row] >= 0 && a.head->status == 0;
+    const float lse = ok ? M + logf(S) : CUDART_NAN_F;  // a NaN row stays NaN in the gradient too
+    const float loss = ok ? lse - a.zy[row] : CUDART_NAN_F;
+    a.lse[row] = lse;
+    a.loss_pack[row] = loss;
+    if (!(fabsf(lse) < CUDART_INF_F) && a.label[row] >= 0) raise_status(a.status, FWB_STATUS_NONFINITE);
+    if (a.reduction == FWB_REDUCE_NONE) a.loss[a.row_of[row]] = loss;
+  }
+  if (a.reduction == FWB_REDUCE_NONE) return;
+  __threadfence();
+  __syncthreads();
+  if (threadIdx.x == 0) last = atomicAdd(&a.head->done, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double d = 0.0;
+  for (int i = threadIdx.x; i < rows; i += kJoinWarps * 32) d += (double)__ldcg(a.loss_pack + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(kFull, d, o);
+  if (lane == 0) sd[w] = d;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kJoinWarps; ++i) d += sd[i];
+    a.loss[0] = (float)(a.reduction == FWB_REDUCE_MEAN ? d / (double)rows : d);
+  }
+}
+
+// ------------------------------------------------------------ backward
+struct CoefArgs {
+  XentHead* head;
+  const int32_t* row_of;
+  const float* go;
+  float* coef;  // [Bp], packed
+  int per_row, mean, f16;
+};
+
+// Factor of each packed row's G, and the factor taken out after the sums.
+__global__ void __launch_bounds__(1024) fw_xent_coef_kernel(CoefArgs a) {
+  __shared__ float red[32];
+  const int rows = a.head->rows;
+  const float over = a.mean ? 1.0f / (float)rows : 1.0f;
+  float unit = 1.0f;
+  if (a.f16) {
+    float top = a.per_row ? 0.0f : fabsf(a.go[0] * over);
+    if (a.per_row) {
+      for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, fabsf(a.go[a.row_of[i]] * over));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
+      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+      __syncthreads();
+      top = red[0];
+      for (int i = 1; i < 32; ++i) top = max_nan(top, red[i]);
+    }
+    unit = top == 0.0f ? 1.0f : top;
+    if (threadIdx.x == 0) a.head->back = unit / kF16Unit;
+  } else if (threadIdx.x == 0) {
+    a.head->back = 1.0f;
+  }
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float g = a.go[a.per_row ? a.row_of[i] : 0] * over;
+    a.coef[i] = a.f16 ? g / unit * kF16Unit : g;
+  }
+}
+
+struct GradArgs {
+  const XentHead* head;
+  const int32_t* label;
+  const float* lse;
+  const float* coef;
+  void* g;  // [Bp, ldg]
+  int64_t ldg;
+  int V, D;
+  int v0, vn;  // first column of the piece, its columns rounded up to 256
+  int32_t* status;
+};
+
+template <class T, TcKind K>
+struct GradTile {
+  using Args = GradArgs;
+  static constexpr TcKind KIND = K;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr int BN = 256, STAGES = 4;
+  static constexpr uint32_t EPI_BYTES = 0;
+  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * (a.vn / 256); }
+  __device__ static TcTile tile(const Args& a, int w) {
+    int m, n;
+    tile_order(w, (a.head->rows + 127) / 128, a.vn / 256, 32, &m, &n);
+    return {m * 128, a.v0 + n * 256, 0, 0, (a.D + 63) / 64};
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
+                                  Done done) {
+    const int row = t.m0 + quad * 32 + lane;
+    const bool live = row < a.head->rows;
+    const int y = live ? a.label[row] : -1;
+    const float lse = live ? a.lse[row] : 0.0f;
+    const float coef = live ? a.coef[row] : 0.0f;
+    T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
+    for (int c = 0; c < BN; c += 32) {
+      float v[32];
+      tmem_ld32(acc + c, v);
+      if (c + 32 == BN) done();
+      const int valid = live ? min(32, a.V - (t.n0 + c)) : 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        float p = exp2f((v[i] - lse) * kLog2e);
+        if (t.n0 + c + i == y) p -= 1.0f;
+        v[i] = i < valid ? p * coef : 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(g + c + 8 * i) = pack16<T>(v + 8 * i);
+    }
+  }
+};
+
+struct DHiddenArgs {
+  const XentHead* head;
+  const int32_t* row_of;
+  float* sum;  // [Bp, D] when the vocabulary has several pieces
+  void* out;   // [B, D]
+  int D;
+  int v0, vn;
+  int first, last;
+  int32_t* status;
+};
+
+// The warp's 32 x 32 block of values, one row per thread, handed to f(row,
+// column, value) with the lanes along the columns.
+template <class F>
+__device__ __forceinline__ void by_columns(float* sm, const float (&v)[32], int lane, int rows, int cols, F f) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
+  __syncwarp();
+  if (lane < cols)
+    for (int i = 0; i < rows; ++i) f(i, lane, sm[i * 33 + lane]);
+  __syncwarp();
+}
+
+template <class T, TcKind K>
+struct DHiddenTile {
+  using Args = DHiddenArgs;
+  static constexpr TcKind KIND = K;
+  static constexpr bool A_MN = false, B_MN = true;
+  static constexpr int BN = 256, STAGES = 4;
+  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
+  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * ((a.D + 255) / 256); }
+  __device__ static TcTile tile(const Args& a, int w) {
+    int m, n;
+    tile_order(w, (a.head->rows + 127) / 128, (a.D + 255) / 256, 12, &m, &n);
+    return {m * 128, n * 256, 0, a.v0, a.vn / 64};
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
+                                  Done done) {
+    float* sm = reinterpret_cast<float*>(smem);
+    const int r0 = t.m0 + quad * 32;
+    const int rows = min(32, a.head->rows - r0);
+    const float back = a.head->back;
+    const int mine = lane < rows ? a.row_of[r0 + lane] : 0;
+    for (int c = 0; c < BN; c += 32) {
+      float v[32];
+      tmem_ld32(acc + c, v);
+      if (c + 32 == BN) done();
+      const int c0 = t.n0 + c;
+      const int cols = min(32, a.D - c0);
+      if (cols <= 0 || rows <= 0) continue;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
+      __syncwarp();
+      for (int i = 0; i < rows; ++i) {
+        const int64_t to = __shfl_sync(kFull, mine, i);
+        if (lane < cols) {
+          float x = sm[i * 33 + lane];
+          const int64_t at = (int64_t)(r0 + i) * a.D + c0 + lane;
+          if (!a.first) x += a.sum[at];
+          if (a.last)
+            st_elem(static_cast<T*>(a.out) + to * a.D + c0 + lane, x * back);
+          else
+            a.sum[at] = x;
+        }
+      }
+      __syncwarp();
+    }
+  }
+};
+
+struct DWeightArgs {
+  const XentHead* head;
+  void* out;  // [V, D]
+  int V, D;
+  int v0, vn;
+  int32_t* status;
+};
+
+template <class T, TcKind K>
+struct DWeightTile {
+  using Args = DWeightArgs;
+  static constexpr TcKind KIND = K;
+  static constexpr bool A_MN = true, B_MN = true;
+  static constexpr int BN = 256, STAGES = 4;
+  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
+  __device__ static int mtiles(const Args& a) { return (min(a.vn, a.V - a.v0) + 127) / 128; }
+  __device__ static int tiles(const Args& a) { return mtiles(a) * ((a.D + 255) / 256); }
+  __device__ static TcTile tile(const Args& a, int w) {
+    int m, n;
+    tile_order(w, mtiles(a), (a.D + 255) / 256, 8, &m, &n);
+    return {m * 128, n * 256, 0, 0, (a.head->rows + 63) / 64};
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
+                                  Done done) {
+    float* sm = reinterpret_cast<float*>(smem);
+    const int r0 = a.v0 + t.m0 + quad * 32;
+    const int rows = min(32, a.V - r0);
+    const float back = a.head->back;
+    for (int c = 0; c < BN; c += 32) {
+      float v[32];
+      tmem_ld32(acc + c, v);
+      if (c + 32 == BN) done();
+      const int c0 = t.n0 + c;
+      const int cols = min(32, a.D - c0);
+      if (cols <= 0 || rows <= 0) continue;
+      if (t.nk == 0) {  // no live row: the accumulator was never written
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+      }
+      by_columns(sm, v, lane, rows, cols, [&](int i, int j, float x) {
+        st_elem(static_cast<T*>(a.out) + (int64_t)(r0 + i) * a.D + c0 + j, t.nk == 0 ? 0.0f : x * back);
+      });
+    }
+  }
+};
+
+// ------------------------------------------------------------ host
+// Bytes of G that one piece of the vocabulary may take.
+constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+
+struct XentPlan {
+  int64_t Bp, Dp;
+  bool copy_w;
+  // state: what backward needs
+  int64_t row_of, label, lse, hp, wp, state_bytes;
+  // forward workspace
+  int64_t part, zy, loss_pack, fwd_bytes;
+  // backward workspace
+  int64_t piece, pieces, coef, g, sum, bwd_bytes;
+};
+
+XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
+  XentPlan p = {};
+  p.Bp = up(B, 128);
+  p.Dp = up(D, 8);
+  p.copy_w = copy_w;
+  int64_t at = 256;
+  p.row_of = at, at += up(4 * p.Bp, 256);
+  p.label = at, at += up(4 * p.Bp, 256);
+  p.lse = at, at += up(4 * p.Bp, 256);
+  p.hp = at, at += up(2 * p.Bp * p.Dp, 256);
+  p.wp = at, at += copy_w ? up(2 * V * p.Dp, 256) : 0;
+  p.state_bytes = at;
+  at = 0;
+  p.part = at, at += up(8 * p.Bp * ((V + 255) / 256), 256);
+  p.zy = at, at += up(4 * p.Bp, 256);
+  p.loss_pack = at, at += up(4 * p.Bp, 256);
+  p.fwd_bytes = at;
+  const int64_t Vp = up(V, 256);
+  p.pieces = (2 * p.Bp * Vp + kPieceBytes - 1) / kPieceBytes;
+  if (p.pieces < 1) p.pieces = 1;
+  p.piece = up((Vp + p.pieces - 1) / p.pieces, 256);
+  p.pieces = (Vp + p.piece - 1) / p.piece;
+  at = 0;
+  p.coef = at, at += up(4 * p.Bp, 256);
+  p.g = at, at += up(2 * p.Bp * p.piece, 256);
+  p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * D, 256) : 0;
+  p.bwd_bytes = at;
+  return p;
+}
+
+int xent_check(int dtype, int64_t B, int64_t D, int64_t V) {
+  if (dtype != FWB_DTYPE_BF16 && dtype != FWB_DTYPE_F16) return FWB_E_DTYPE;
+  if (B < 0 || D < 1 || V < 1 || B > (1 << 26) || D > (1 << 20) || V > (1 << 28)) return FWB_E_SHAPE;
+  if ((up(B, 128) / 128) * (up(V, 256) / 256) > (1 << 30)) return FWB_E_SHAPE;
+  return FWB_OK;
+}
+
+// Rows that a TMA tile load can read in place.
+bool tma_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+template <class T, TcKind K>
+int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* y, int64_t B,
+                int64_t D, int64_t V, int64_t ignore, int reduction, float* loss, char* state, char* ws,
+                int32_t* status, cudaStream_t st) {
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+  XentHead* head = reinterpret_cast<XentHead*>(state);
+  int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
+  int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
+  PackArgs pk = {hidden, y, B, p.Bp, D, p.Dp, ldh, V, ignore, state + p.hp, row_of, label,
+                 reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, B <= 8192 ? 8 : 64};
+  fw_xent_pack_kernel<T><<<(unsigned)((p.Bp + pk.per_cta - 1) / pk.per_cta), kPackThreads, 0, st>>>(pk);
+  const void* w = weight;
+  if (p.copy_w) {
+    const int64_t need = (V * ((p.Dp + 1023) / 1024) + 7) / 8, cap = (int64_t)sm_count() * 16;
+    fw_xent_align_kernel<T><<<(unsigned)(need < cap ? need : cap), 256, 0, st>>>(
+        static_cast<const T*>(weight), ldw, reinterpret_cast<T*>(state + p.wp), p.Dp, V, D);
+    w = state + p.wp;
+    ldw = p.Dp;
+  }
+  if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+  CUtensorMap mh, mw;
+  if (!tc_map(&mh, K, state + p.hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 256)) return FWB_E_LAUNCH;
+  LseArgs la = {head, label, reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.zy), p.Bp, (int)V,
+                (int)D, &head->status};
+  const int64_t nt = (V + 255) / 256;
+  if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 128) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
+  JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
+                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)nt, reduction, status};
+  fw_xent_join_kernel<<<(unsigned)(p.Bp / 32), kJoinWarps * 32, 0, st>>>(ja);
+  return launch_status(cudaGetLastError());
+}
+
+template <class T, TcKind K>
+int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int mean, const float* go,
+                 int per_row, char* state, char* ws, void* dhidden, void* dweight, int32_t* status, cudaStream_t st) {
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+  XentHead* head = reinterpret_cast<XentHead*>(state);
+  int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
+  int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
+  float* coef = reinterpret_cast<float*>(ws + p.coef);
+  const void* w = p.copy_w ? state + p.wp : weight;
+  if (p.copy_w) ldw = p.Dp;
+  // ignored rows' gradient; the live rows' is written below
+  if (dhidden && cudaMemsetAsync(dhidden, 0, (size_t)(2 * B * D), st) != cudaSuccess) return FWB_E_LAUNCH;
+  const CoefArgs ca = {head, row_of, go, coef, per_row, mean, K == kTcF16};
+  fw_xent_coef_kernel<<<1, 1024, 0, st>>>(ca);
+  if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+  CUtensorMap mh, mw, mg, wmn, gmn, hmn;
+  char* hp = state + p.hp;
+  char* g = ws + p.g;
+  if (!tc_map(&mh, K, hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 256) ||
+      !tc_map(&mg, K, g, p.Bp, p.piece, p.piece, 128) || !tc_map(&wmn, K, w, V, D, ldw, 64) ||
+      !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hp, p.Bp, D, p.Dp, 64))
+    return FWB_E_LAUNCH;
+  const int64_t Vp = up(V, 256), mb = p.Bp / 128, nd = (D + 255) / 256;
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
+    const GradArgs ga = {head, label, reinterpret_cast<float*>(state + p.lse), coef, g, p.piece, (int)V, (int)D, v0,
+                         vn, status};
+    if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
+    if (dhidden) {
+      const DHiddenArgs da = {head, row_of, reinterpret_cast<float*>(ws + p.sum), dhidden, (int)D, v0, vn, i == 0,
+                              i == p.pieces - 1, status};
+      if (launch_gemm<DHiddenTile<T, K>>(mg, wmn, da, mb * nd, st) != cudaSuccess) return FWB_E_LAUNCH;
+    }
+    if (dweight) {
+      const DWeightArgs da = {head, dweight, (int)V, (int)D, v0, vn, status};
+      if (launch_gemm<DWeightTile<T, K>>(gmn, hmn, da, (int64_t)(vn / 128) * nd, st) != cudaSuccess)
+        return FWB_E_LAUNCH;
+    }
+  }
+  return FWB_OK;
+}
+
+}  // namespace
+}  // namespace fwb200
+
+using namespace fwb200;
+
+extern "C" {
+
+int64_t fw_xent_state_bytes(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw) {
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
+  return xent_plan(B, D, V, !tma_rows(weight, ldw)).state_bytes;
+}
+
+int64_t fw_xent_workspace(int64_t B, int64_t D, int64_t V, int backward) {
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
+  const XentPlan p = xent_plan(B, D, V, false);
+  return backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+int fw_xent_forward(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* y,
+                    int64_t B, int64_t D, int64_t V, int64_t ignore_index, int reduction, float* loss, void* state,
+                    int64_t state_bytes, void* workspace, int64_t workspace_bytes, int32_t* status, void* stream) {
+  if (int rc = xent_check(dtype, B, D, V)) return rc;
+  if (reduction < FWB_REDUCE_NONE || reduction > FWB_REDUCE_SUM || ldh < D || ldw < D || ldh > ((int64_t)1 << 38) ||
+      ldw > ((int64_t)1 << 38))
+    return FWB_E_SHAPE;
+  if (B > 0 && (!hidden || !y)) return FWB_E_POINTER;
+  if (!weight || !state || !workspace || (!loss && (B > 0 || reduction != FWB_REDUCE_NONE))) return FWB_E_POINTER;
+  if (reinterpret_cast<uintptr_t>(hidden) % 2 || reinterpret_cast<uintptr_t>(weight) % 2 || !aligned16(state) ||
+      !aligned16(workspace))
+    return FWB_E_POINTER;
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+  if (state_bytes < p.state_bytes || workspace_bytes < p.fwd_bytes) return FWB_E_CAPACITY;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (B == 0) {  // no rows: the mean is 0 / 0
+    if (cudaMemsetAsync(state, 0, sizeof(XentHead), st) != cudaSuccess) return FWB_E_LAUNCH;
+    if (reduction == FWB_REDUCE_NONE) return FWB_OK;
+    return cudaMemsetAsync(loss, reduction == FWB_REDUCE_MEAN ? 0xff : 0, 4, st) == cudaSuccess ? FWB_OK : FWB_E_LAUNCH;
+  }
+  char* s = static_cast<char*>(state);
+  char* w = static_cast<char*>(workspace);
+  return dtype == FWB_DTYPE_BF16 ? run_forward<__nv_bfloat16, kTcBf16>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index,
+                                                                       reduction, loss, s, w, status, st)
+                                 : run_forward<__half, kTcF16>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index,
+                                                               reduction, loss, s, w, status, st);
+}
+
+int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int reduction,
+                     const float* grad_output, void* state, int64_t state_bytes, void* workspace,
+                     int64_t workspace_bytes, void* dhidden, void* dweight, int32_t* status, void* stream) {
+  if (int rc = xent_check(dtype, B, D, V)) return rc;
+  if (reduction < FWB_REDUCE_NONE || reduction > FWB_REDUCE_SUM || ldw < D || ldw > ((int64_t)1 << 38))
+    return FWB_E_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (B == 0) {
+    if (dweight && cudaMemsetAsync(dweight, 0, (size_t)(2 * V * D), st) != cudaSuccess) return FWB_E_LAUNCH;
+    return FWB_OK;
+  }
+  if (!weight || !grad_output || !state || !workspace) return FWB_E_POINTER;
+  if (reinterpret_cast<uintptr_t>(weight) % 2 || reinterpret_cast<uintptr_t>(dhidden) % 2 ||
+      reinterpret_cast<uintptr_t>(dweight) % 2 || !aligned16(state) || !aligned16(workspace))
+    return FWB_E_POINTER;
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+  if (state_bytes < p.state_bytes || workspace_bytes < p.bwd_bytes) return FWB_E_CAPACITY;
+  if (!dhidden && !dweight) return FWB_OK;
+  char* s = static_cast<char*>(state);
+  char* w = static_cast<char*>(workspace);
+  const int per_row = reduction == FWB_REDUCE_NONE, mean = reduction == FWB_REDUCE_MEAN;
+  return dtype == FWB_DTYPE_BF16
+             ? run_backward<__nv_bfloat16, kTcBf16>(weight, ldw, B, D, V, mean, grad_output, per_row, s, w, dhidden,
+                                                    dweight, status, st)
+             : run_backward<__half, kTcF16>(weight, ldw, B, D, V, mean, grad_output, per_row, s, w, dhidden, dweight,
+                                            status, st);
+}
+
+}  // extern "C"

@@ -74,6 +74,24 @@ _SIGS["fw_loss_allreduce"] = ([_P, _I64, ctypes.c_double, _P, ctypes.c_int, ctyp
                                ctypes.c_double, _P], ctypes.c_int)
 _SIGS["fw_loss_allreduce_f64"] = ([_P, _I64, ctypes.c_double, _P, ctypes.c_int, ctypes.c_int, _P, _P,
                                    ctypes.c_double, _P], ctypes.c_int)
+_C_INT, _F32 = ctypes.c_int, ctypes.c_float
+_SIGS["fw_embed_rows"] = ([_C_INT, _P, _I64, _P, _I64, _I64, _I64, _F32, _P, _I64, _P, _P], _C_INT)
+_SIGS["fw_embed_grad_workspace"] = ([_I64, _I64, _I64], _I64)
+_SIGS["fw_embed_grad"] = ([_C_INT, _P, _I64, _P, _I64, _I64, _I64, _F32, _I64, _P, _P, _I64, _P, _P], _C_INT)
+_SIGS["fw_rms_norm"] = ([_C_INT, _C_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _P, _I64, _P, _I64, _P, _P], _C_INT)
+_SIGS["fw_rms_norm_int8"] = ([_C_INT, _C_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _F32, _P, _I64, _P, _I64, _P, _P],
+                             _C_INT)
+_SIGS["fw_quantize_rows_int8"] = ([_C_INT, _P, _I64, _I64, _I64, _P, _I64, _P, _P], _C_INT)
+_SIGS["fw_rms_norm_grad_parts"] = ([_I64], _I64)
+_SIGS["fw_rms_norm_grad"] = ([_C_INT, _C_INT, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I64, _P, _I64, _P, _I64, _P,
+                              _P], _C_INT)
+_SIGS["fw_int8_linear"] = ([_C_INT, _P, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P], _C_INT)
+_SIGS["fw_xent_state_bytes"] = ([_I64, _I64, _I64, _P, _I64], _I64)
+_SIGS["fw_xent_workspace"] = ([_I64, _I64, _I64, _C_INT], _I64)
+_SIGS["fw_xent_forward"] = ([_C_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _I64, _C_INT, _P, _P, _I64, _P, _I64,
+                             _P, _P], _C_INT)
+_SIGS["fw_xent_backward"] = ([_C_INT, _P, _I64, _I64, _I64, _I64, _C_INT, _P, _P, _I64, _P, _I64, _P, _P, _P, _P],
+                             _C_INT)
 DTYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ANY_FLOAT = (torch.float32, torch.bfloat16, torch.float16, torch.float64)
 

@@ -453,6 +453,114 @@ FWB_API int fw_lmhead_fused_loss_noalloc(int dtype, const void* hidden, int64_t 
                                          int32_t* fb_rows, int32_t* fb_count, int32_t* status,
                                          void* stream);
 
+/*
+ * Operators of a language model around the loss: the embedding table at its
+ * input, the norm of its residual stream, the softmax cross entropy and the
+ * 8-bit logits of its output layer.  No counterpart in the reference, which
+ * takes logits as input.  dtype: FWB_DTYPE_F32, _BF16 or _F16 unless said
+ * otherwise; arithmetic, sums and statistics are fp32; strides (ld*) are in
+ * elements; a row may start anywhere its element type may; outputs must not
+ * overlap inputs.
+ */
+
+/*
+ * out[t] = scale * weight[ids[t]] for ids[t] in [0, V); a row of NaN and
+ * FWB_STATUS_LABEL_RANGE for any other id.
+ */
+FWB_API int fw_embed_rows(int dtype, const int64_t* ids, int64_t T, const void* weight, int64_t ldw,
+                          int64_t V, int64_t D, float scale, void* out, int64_t ldo, int32_t* status,
+                          void* stream);
+
+/*
+ * dweight[v] = scale * sum of grad[t] over the t with ids[t] = v, added in
+ * position order (no atomics: the result does not vary), 0 for rows without a
+ * token; dweight is [V, D], contiguous, and every row is written.  Tokens
+ * equal to `padding` (-1: none) or outside [0, V) add nothing.  The workspace
+ * (16-byte aligned, fw_embed_grad_workspace bytes) holds the sorted tokens and
+ * partial rows.
+ */
+FWB_API int64_t fw_embed_grad_workspace(int64_t T, int64_t V, int64_t D);
+FWB_API int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, int64_t ldg,
+                          int64_t V, int64_t D, float scale, int64_t padding, void* dweight,
+                          void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+
+/*
+ * Root-mean-square norm: sum = x + residual, rounded to dtype (residual NULL:
+ * sum is x and is not written); y = sum * rstd * weight with
+ * rstd = 1 / sqrt(mean(sum^2) + eps), one per row, kept for the gradient
+ * (rstd may be NULL).  weight has dtype wdtype: dtype or FWB_DTYPE_F32.
+ */
+FWB_API int fw_rms_norm(int dtype, int wdtype, const void* x, int64_t ldx, const void* residual,
+                        int64_t ldr, const void* weight, int64_t rows, int64_t D, float eps, void* sum,
+                        int64_t lds, void* y, int64_t ldy, float* rstd, void* stream);
+
+/*
+ * The same norm with an 8-bit output: q = rint(y / scale[r]) with
+ * scale[r] = max|y| / 127.  Rows of q start on 16-byte boundaries: ldq is a
+ * multiple of 16 and at least D rounded up to 16; the columns from D up to
+ * that are set to 0.  A row whose largest value is 0 or not finite gives
+ * q = 0 and that scale.
+ */
+FWB_API int fw_rms_norm_int8(int dtype, int wdtype, const void* x, int64_t ldx, const void* residual,
+                             int64_t ldr, const void* weight, int64_t rows, int64_t D, float eps,
+                             void* sum, int64_t lds, int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/* The rows of x themselves in 8 bits (the layout of an 8-bit weight). */
+FWB_API int fw_quantize_rows_int8(int dtype, const void* x, int64_t ldx, int64_t rows, int64_t D,
+                                  int8_t* q, int64_t ldq, float* scale, void* stream);
+
+/*
+ * Gradient of fw_rms_norm from the stored sum (x without a residual) and rstd:
+ * dx (the gradient of x and of residual) with dsum, if given, added; dweight
+ * (dtype wdtype, may be NULL) through `parts`, fp32 [nparts, D] workspace with
+ * nparts = fw_rms_norm_grad_parts(rows), added in a fixed order.
+ */
+FWB_API int64_t fw_rms_norm_grad_parts(int64_t rows);
+FWB_API int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy, const void* sum,
+                             int64_t lds, const void* dsum, int64_t ldo, const void* weight,
+                             const float* rstd, int64_t rows, int64_t D, void* dx, int64_t lddx,
+                             float* parts, int64_t nparts, void* dweight, void* stream);
+
+/*
+ * out[t, n] = (sum_k q[t, k] * wq[n, k]) * q_scale[t] * w_scale[n]: the sum is
+ * an exact 32-bit integer (hence K <= FWB_INT8_MAX_K), the result is rounded
+ * once to out_dtype.  Rows of q and wq start on 16-byte boundaries (ldq and
+ * ldw multiples of 16); columns from K on are not read as values.
+ */
+#define FWB_INT8_MAX_K 131071
+FWB_API int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const float* q_scale,
+                           const int8_t* wq, int64_t ldw, const float* w_scale, int64_t T, int64_t N,
+                           int64_t K, void* out, int64_t ldo, int32_t* status, void* stream);
+
+/*
+ * Softmax cross entropy of logits = hidden [B, D] x weight [V, D]^T without
+ * storing the logits (FWB_DTYPE_BF16 or _F16; V <= 2^28).  Rows with
+ * y = ignore_index take no part, whatever hidden holds there (loss 0 under
+ * FWB_REDUCE_NONE; the mean is over the others); any other label outside
+ * [0, V) gives a NaN loss and FWB_STATUS_LABEL_RANGE.  loss: fp32, [B] for
+ * FWB_REDUCE_NONE, else one value.
+ * `state` (fw_xent_state_bytes, for the same weight pointer and stride) keeps
+ * what the gradient needs: packed live rows, their log-sum-exp, and a copy of
+ * the weight only if its rows do not start on 16-byte boundaries.
+ * fw_xent_backward writes dhidden [B, D] and dweight [V, D] (contiguous,
+ * either may be NULL) for grad_output ([B] for FWB_REDUCE_NONE, else one
+ * value), the logit gradient formed in pieces of the vocabulary.  Both
+ * buffers and the workspaces (fw_xent_workspace bytes) are 16-byte aligned.
+ */
+#define FWB_REDUCE_NONE 0
+#define FWB_REDUCE_MEAN 1
+#define FWB_REDUCE_SUM 2
+FWB_API int64_t fw_xent_state_bytes(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw);
+FWB_API int64_t fw_xent_workspace(int64_t B, int64_t D, int64_t V, int backward);
+FWB_API int fw_xent_forward(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                            const int64_t* y, int64_t B, int64_t D, int64_t V, int64_t ignore_index,
+                            int reduction, float* loss, void* state, int64_t state_bytes,
+                            void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
+FWB_API int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V,
+                             int reduction, const float* grad_output, void* state, int64_t state_bytes,
+                             void* workspace, int64_t workspace_bytes, void* dhidden, void* dweight,
+                             int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
