@@ -9,6 +9,11 @@
 // tokens are sorted by id (a stable radix sort), and a row's contributions
 // are added in position order, in fp32, so the result does not vary.
 //
+// The sort is one launch, a cluster of 8 CTAs that exchange digit counts and
+// entries through distributed shared memory, up to kClusterTokens tokens, and
+// two launches per digit beyond.  Up to kDirectTokens tokens nothing is
+// sorted: every warp finds its row's positions in the list itself.
+//
 // Skewed ids (the commonest token may take a tenth of the positions) are cut
 // at fixed chunks of kChunk sorted entries: a run of equal ids inside one
 // chunk is summed by the warp that owns the table row; a run that crosses a
@@ -18,6 +23,7 @@
 //
 // Rows are read and written in 16-byte slots of the destination row, whatever
 // the alignment of either (fw_rowslots.cuh).
+#include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -33,13 +39,21 @@ constexpr int kChunk = 32;       // sorted entries per partial sum
 constexpr int kSortThreads = 256;
 constexpr int kSortItems = 8;
 constexpr int kSortTile = kSortThreads * kSortItems;
-constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kClusterCtas = 8;
+constexpr int kClusterThreads = 512;
+constexpr int kClusterTile = kClusterThreads * kSortItems;
+constexpr int kClusterTokens = kClusterCtas * kClusterTile;
 constexpr int kMaxDigitBits = 9;
 constexpr int kMaxBins = 1 << kMaxDigitBits;
 
-__host__ __device__ constexpr int slots_of(int64_t D, int esize) {  // at any alignment
-  return (int)((D * esize + 15) / 16 + 1);
+constexpr int kDirectTokens = 256;
+
+// Slots of a row of a contiguous matrix (one more where rows start anywhere).
+__host__ __device__ constexpr int slots_of(int64_t D, int esize) {
+  return (int)((D * esize + 15) / 16 + (D * esize % 16 != 0 ? 1 : 0));
 }
+
+int slabs_of(int64_t D, int esize) { return (slots_of(D, esize) + 32 * kSlab - 1) / (32 * kSlab); }
 
 template <class T>
 __device__ __forceinline__ int dst_off(const T* row) {
@@ -118,10 +132,12 @@ __device__ __forceinline__ uint2 sort_entry(const SortArgs& a, int64_t i, bool r
 // thread goes to (place of its digit) + cnt[warp][digit] + rank[i], and
 // total[digit] is the tile's count.  Entry i of lane l of warp w is number
 // w * 32 * kSortItems + 32 * i + l of the tile.
+template <int THREADS>
 __device__ __forceinline__ void tile_rank(const uint32_t (&digit)[kSortItems], uint32_t (&rank)[kSortItems],
-                                          uint32_t (*cnt)[kMaxBins + 1], uint32_t* total, int bins) {
+                                          uint16_t (*cnt)[kMaxBins + 2], uint32_t* total, int bins) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  for (int i = threadIdx.x; i < kSortWarps * (kMaxBins + 1); i += kSortThreads) (&cnt[0][0])[i] = 0u;
+  uint32_t* words = reinterpret_cast<uint32_t*>(&cnt[0][0]);
+  for (int i = threadIdx.x; i < THREADS / 32 * (kMaxBins + 2) / 2; i += THREADS) words[i] = 0u;
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSortItems; ++i) {
@@ -129,17 +145,17 @@ __device__ __forceinline__ void tile_rank(const uint32_t (&digit)[kSortItems], u
     const uint32_t same = __match_any_sync(kFull, d);
     const uint32_t before = cnt[w][d];
     __syncwarp();
-    if (lane == __ffs(same) - 1) cnt[w][d] = before + __popc(same);
+    if (lane == __ffs(same) - 1) cnt[w][d] = (uint16_t)(before + __popc(same));
     __syncwarp();
     rank[i] = before + __popc(same & ((1u << lane) - 1u));
   }
   __syncthreads();
-  for (int d = threadIdx.x; d < bins; d += kSortThreads) {
+  for (int d = threadIdx.x; d < bins; d += THREADS) {
     uint32_t run = 0u;
 #pragma unroll
-    for (int q = 0; q < kSortWarps; ++q) {
+    for (int q = 0; q < THREADS / 32; ++q) {
       const uint32_t c = cnt[q][d];
-      cnt[q][d] = run;
+      cnt[q][d] = (uint16_t)run;
       run += c;
     }
     total[d] = run;
@@ -148,8 +164,10 @@ __device__ __forceinline__ void tile_rank(const uint32_t (&digit)[kSortItems], u
 }
 
 // Exclusive scan of total[0 .. bins) in place by the whole CTA.
+template <int THREADS>
 __device__ __forceinline__ void scan_bins(uint32_t* total, uint32_t* warp_sum, int bins) {
-  constexpr int kPer = kMaxBins / kSortThreads;
+  constexpr int kPer = kMaxBins / THREADS;
+  static_assert(kPer * THREADS == kMaxBins, "whole bins per thread");
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   uint32_t v[kPer], s = 0u;
 #pragma unroll
@@ -196,8 +214,8 @@ __global__ void __launch_bounds__(kSortThreads) fw_sort_hist_kernel(SortArgs a) 
 // its own digit counts in the tiles before it), so no scan kernel runs
 // between the histograms and the scatter.
 __global__ void __launch_bounds__(kSortThreads) fw_sort_scatter_kernel(SortArgs a) {
-  __shared__ uint32_t cnt[kSortWarps][kMaxBins + 1];
-  __shared__ uint32_t total[kMaxBins], place[kMaxBins], warp_sum[kSortWarps];
+  __shared__ __align__(4) uint16_t cnt[kSortThreads / 32][kMaxBins + 2];
+  __shared__ uint32_t total[kMaxBins], place[kMaxBins], warp_sum[kSortThreads / 32];
   const int bins = 1 << a.bits;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t t0 = (int64_t)blockIdx.x * kSortTile;
@@ -209,7 +227,7 @@ __global__ void __launch_bounds__(kSortThreads) fw_sort_scatter_kernel(SortArgs 
     ent[i] = e < a.T ? sort_entry(a, e, false) : make_uint2(0u, 0u);
     digit[i] = e < a.T ? (ent[i].x >> a.shift) & (bins - 1) : (uint32_t)bins;
   }
-  tile_rank(digit, rank, cnt, total, bins);
+  tile_rank<kSortThreads>(digit, rank, cnt, total, bins);
   for (int d = threadIdx.x; d < bins; d += kSortThreads) {
     uint32_t before = 0u, all = 0u;
 #pragma unroll 4
@@ -222,80 +240,116 @@ __global__ void __launch_bounds__(kSortThreads) fw_sort_scatter_kernel(SortArgs 
     total[d] = all;
   }
   __syncthreads();
-  scan_bins(total, warp_sum, bins);
+  scan_bins<kSortThreads>(total, warp_sum, bins);
 #pragma unroll
   for (int i = 0; i < kSortItems; ++i)
     if (digit[i] < (uint32_t)bins) a.dst[total[digit[i]] + place[digit[i]] + cnt[w][digit[i]] + rank[i]] = ent[i];
 }
 
-// Up to one tile of tokens: all passes in one CTA, entries in shared memory.
-__global__ void __launch_bounds__(kSortThreads) fw_sort_small_kernel(SortArgs a, int passes, int total_bits) {
-  __shared__ uint32_t cnt[kSortWarps][kMaxBins + 1];
-  __shared__ uint32_t total[kMaxBins], warp_sum[kSortWarps];
-  __shared__ uint2 buf[kSortTile];
+// All passes in one launch: a cluster holds the entries in shared memory, CTA
+// c the entries c * per .. of the current order.  Per pass the CTAs rank their
+// own entries, read each other's digit counts, and store every entry where it
+// belongs in the cluster.
+__global__ void __launch_bounds__(kClusterThreads) fw_sort_cluster_kernel(SortArgs a, int passes) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cl = cg::this_cluster();
+  extern __shared__ __align__(16) unsigned char sort_smem[];
+  uint2* buf = reinterpret_cast<uint2*>(sort_smem);  // two halves of kClusterTile entries
+  uint16_t(*cnt)[kMaxBins + 2] = reinterpret_cast<uint16_t(*)[kMaxBins + 2]>(sort_smem + 2 * kClusterTile * sizeof(uint2));
+  __shared__ uint32_t total[kMaxBins], base[kMaxBins], warp_sum[kClusterThreads / 32];
   const int bins = 1 << a.bits;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int nc = (int)cl.num_blocks(), me = (int)cl.block_rank();
+  const int T = (int)a.T;
+  const int per = (T + nc - 1) / nc;
+  const int first = me * per, mine = max(0, min(per, T - first));
   uint2 ent[kSortItems];
   uint32_t digit[kSortItems], rank[kSortItems];
 #pragma unroll
   for (int i = 0; i < kSortItems; ++i) {
     const int e = w * 32 * kSortItems + 32 * i + lane;
-    ent[i] = e < a.T ? sort_entry(a, e, true) : make_uint2(0u, 0u);
+    ent[i] = e < mine ? sort_entry(a, first + e, true) : make_uint2(0u, 0u);
   }
   for (int p = 0; p < passes; ++p) {
 #pragma unroll
     for (int i = 0; i < kSortItems; ++i) {
       const int e = w * 32 * kSortItems + 32 * i + lane;
-      if (p > 0 && e < a.T) ent[i] = buf[e];
-      digit[i] = e < a.T ? (ent[i].x >> (p * a.bits)) & (bins - 1) : (uint32_t)bins;
+      if (p > 0 && e < mine) ent[i] = buf[(p & 1) * kClusterTile + e];
+      digit[i] = e < mine ? (ent[i].x >> (p * a.bits)) & (bins - 1) : (uint32_t)bins;
     }
-    tile_rank(digit, rank, cnt, total, bins);  // its barriers also end the reads of buf
-    scan_bins(total, warp_sum, bins);
+    tile_rank<kClusterThreads>(digit, rank, cnt, total, bins);
+    cl.sync();  // the counts of every CTA are in place
+    uint32_t before[kMaxBins / kClusterThreads], all[kMaxBins / kClusterThreads];
 #pragma unroll
-    for (int i = 0; i < kSortItems; ++i)
-      if (digit[i] < (uint32_t)bins) buf[total[digit[i]] + cnt[w][digit[i]] + rank[i]] = ent[i];
+    for (int k = 0; k < kMaxBins / kClusterThreads; ++k) {
+      const int d = k * kClusterThreads + threadIdx.x;
+      before[k] = all[k] = 0u;
+      if (d < bins)
+        for (int q = 0; q < nc; ++q) {
+          const uint32_t c = cl.map_shared_rank(total, q)[d];
+          before[k] += q < me ? c : 0u;
+          all[k] += c;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kMaxBins / kClusterThreads; ++k) {
+      const int d = k * kClusterThreads + threadIdx.x;
+      if (d < bins) base[d] = all[k];
+    }
     __syncthreads();
+    scan_bins<kClusterThreads>(base, warp_sum, bins);
+#pragma unroll
+    for (int k = 0; k < kMaxBins / kClusterThreads; ++k) {
+      const int d = k * kClusterThreads + threadIdx.x;
+      if (d < bins) base[d] += before[k];
+    }
+    __syncthreads();
+    const bool end = p == passes - 1;
+    uint2* next = buf + ((p + 1) & 1) * kClusterTile;
+#pragma unroll
+    for (int i = 0; i < kSortItems; ++i) {
+      if (digit[i] >= (uint32_t)bins) continue;
+      const int to = (int)(base[digit[i]] + cnt[w][digit[i]] + rank[i]);
+      if (end)
+        a.dst[to] = ent[i];
+      else
+        cl.map_shared_rank(next, to / per)[to % per] = ent[i];
+    }
+    cl.sync();  // entries in place; nobody reads these counts any more
   }
-  for (int e = threadIdx.x; e < a.T; e += kSortThreads) a.dst[e] = buf[e];
 }
 
 // ------------------------------------------------------------ row sums
 struct EmbedGradArgs {
   const uint2* sorted;
+  const int32_t* start;  // [V + 1] first sorted entry of each row
+  const int64_t* ids;    // direct form
   const void* g;
   void* dw;
   float* part;  // [2 * chunks, pitch]
-  int64_t T, V, D, ldg, pitch;
+  int64_t T, V, D, ldg, pitch, padding;
   float scale;
   int nslabs;
+  int part_blocks;
+  int32_t* status;
 };
 
-// First sorted entry in [lo, hi) whose key is at least v; the whole warp.
-__device__ __forceinline__ int64_t lower_bound_warp(const uint2* s, int64_t lo, int64_t hi, uint32_t v, int lane) {
-  while (lo < hi) {
-    const int64_t step = (hi - lo + 31) / 32;
-    const int64_t at = lo + lane * step;
-    const bool less = at < hi && s[at].x < v;
-    const int c = __popc(__ballot_sync(kFull, less));
-    const int64_t nhi = lo + c * step;
-    if (c > 0) lo += (c - 1) * step + 1;
-    hi = nhi < hi ? nhi : hi;
-  }
-  return lo;
-}
-
-// Adds rows sorted[i0 .. i1) of g, in that order, to the slots of this lane.
-template <class T>
-__device__ __forceinline__ void add_rows(const EmbedGradArgs& a, int64_t i0, int64_t i1, int64_t e0, float* acc) {
+// Adds rows pos of the n <= 32 entries (lane i holds the i-th position) of g,
+// in that order, to the slots of this lane.  ALIGNED: every row of g and dw
+// starts on a 16-byte boundary.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void add_rows(const EmbedGradArgs& a, uint32_t pos, int n, int64_t e0, float* acc) {
   constexpr int V = 16 / sizeof(T);
 #pragma unroll 2
-  for (int64_t i = i0; i < i1; ++i) {
-    const T* row = static_cast<const T*>(a.g) + (int64_t)a.sorted[i].y * a.ldg;
+  for (int i = 0; i < n; ++i) {
+    const T* row = static_cast<const T*>(a.g) + (int64_t)__shfl_sync(kFull, pos, i) * a.ldg;
     uint4 u[kSlab];
 #pragma unroll
     for (int k = 0; k < kSlab; ++k) {
       const int64_t e = e0 + (int64_t)k * 32 * V;
-      u[k] = e < a.D ? load_slot_shifted(row, e, a.D) : make_uint4(0u, 0u, 0u, 0u);
+      u[k] = e >= a.D  ? make_uint4(0u, 0u, 0u, 0u)
+             : ALIGNED ? ld_stream16(row + e)
+                       : load_slot_shifted(row, e, a.D);
     }
 #pragma unroll
     for (int k = 0; k < kSlab; ++k) {
@@ -307,77 +361,113 @@ __device__ __forceinline__ void add_rows(const EmbedGradArgs& a, int64_t i0, int
   }
 }
 
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int64_t e0, const float* acc) {
+  constexpr int V = 16 / sizeof(T);
+#pragma unroll
+  for (int k = 0; k < kSlab; ++k) {
+    const int64_t e = e0 + (int64_t)k * 32 * V;
+    if (e >= a.D) continue;
+    float s[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] = acc[k * V + j] * a.scale;
+    if (ALIGNED)
+      *reinterpret_cast<uint4*>(dst + e) = pack16<T>(s);
+    else
+      store_slot(dst, e, a.D, true, pack16<T>(s));
+  }
+}
+
 // Partial rows of the runs that cross a chunk boundary: row 2c is the part in
 // chunk c of a run that began before it, row 2c + 1 the part of a run that
 // begins in it and goes on.
-template <class T>
-__global__ void __launch_bounds__(256) fw_embed_part_kernel(EmbedGradArgs a) {
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int slab, int lane) {
   constexpr int V = 16 / sizeof(T);
-  const int lane = threadIdx.x & 31;
-  const int64_t chunks = (a.T + kChunk - 1) / kChunk;
-  const int64_t work = chunks * a.nslabs;
-  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
-    const int64_t c = i / a.nslabs;
-    const int slab = (int)(i - c * a.nslabs);
-    const int64_t b = c * kChunk, n = min((int64_t)kChunk, a.T - b);
-    const uint32_t key = lane < n ? a.sorted[b + lane].x : 0xffffffffu;
-    const uint32_t first = __shfl_sync(kFull, key, 0), last = __shfl_sync(kFull, key, (int)n - 1);
-    const bool from = b > 0 && a.sorted[b - 1].x == first;
-    const bool on = b + n < a.T && a.sorted[b + n].x == last;
-    for (int half = 0; half < 2; ++half) {
-      int64_t i0 = b, i1 = b + n;
-      if (half == 0) {
-        if (!from || first >= (uint32_t)a.V) continue;
-        i1 = b + __popc(__ballot_sync(kFull, lane < n && key == first));
-      } else {
-        if (!on || last >= (uint32_t)a.V || (from && first == last)) continue;
-        i0 = b + n - __popc(__ballot_sync(kFull, lane < n && key == last));
-      }
-      float acc[kSlab * V];
+  const int64_t b = c * kChunk;
+  const int n = (int)min((int64_t)kChunk, a.T - b);
+  const uint2 ent = lane < n ? a.sorted[b + lane] : make_uint2(0xffffffffu, 0u);
+  const uint32_t first = __shfl_sync(kFull, ent.x, 0), last = __shfl_sync(kFull, ent.x, n - 1);
+  const bool from = b > 0 && a.sorted[b - 1].x == first;
+  const bool on = b + n < a.T && a.sorted[b + n].x == last;
+  for (int half = 0; half < 2; ++half) {
+    int i0 = 0, i1 = n;
+    if (half == 0) {
+      if (!from || first >= (uint32_t)a.V) continue;
+      i1 = __popc(__ballot_sync(kFull, lane < n && ent.x == first));
+    } else {
+      if (!on || last >= (uint32_t)a.V || (from && first == last)) continue;
+      i0 = n - __popc(__ballot_sync(kFull, lane < n && ent.x == last));
+    }
+    float acc[kSlab * V];
 #pragma unroll
-      for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
-      const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V;
-      add_rows<T>(a, i0, i1, e0, acc);
-      float* out = a.part + (2 * c + half) * a.pitch;
+    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
+    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V;
+    add_rows<T, ALIGNED>(a, __shfl_sync(kFull, ent.y, (i0 + lane) & 31), i1 - i0, e0, acc);
+    float* out = a.part + (2 * c + half) * a.pitch;
 #pragma unroll
-      for (int k = 0; k < kSlab; ++k) {
-        const int64_t e = e0 + (int64_t)k * 32 * V;
-        if (e < a.D) {
+    for (int k = 0; k < kSlab; ++k) {
+      const int64_t e = e0 + (int64_t)k * 32 * V;
+      if (e < a.D) {
 #pragma unroll
-          for (int j = 0; j < V; j += 4)  // pitch is a multiple of V
-            *reinterpret_cast<float4*>(out + e + j) =
-                make_float4(acc[k * V + j], acc[k * V + j + 1], acc[k * V + j + 2], acc[k * V + j + 3]);
-        }
+        for (int j = 0; j < V; j += 4)  // pitch is a multiple of V
+          *reinterpret_cast<float4*>(out + e + j) =
+              make_float4(acc[k * V + j], acc[k * V + j + 1], acc[k * V + j + 2], acc[k * V + j + 3]);
       }
     }
   }
 }
 
-// One warp per table row.
-template <class T>
+// What the row sums need of the sorted tokens: the partial rows (first
+// part_blocks CTAs) and where each row's entries start (the others).
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) fw_embed_part_kernel(EmbedGradArgs a, int32_t* start) {
+  const int lane = threadIdx.x & 31;
+  if ((int)blockIdx.x < a.part_blocks) {
+    const int64_t chunks = (a.T + kChunk - 1) / kChunk;
+    const int64_t work = chunks * a.nslabs;
+    const int64_t nw = (int64_t)a.part_blocks * (blockDim.x / 32);
+    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw)
+      sum_chunk<T, ALIGNED>(a, i / a.nslabs, (int)(i % a.nslabs), lane);
+    return;
+  }
+  const int64_t n = (int64_t)(gridDim.x - a.part_blocks) * blockDim.x;
+  for (int64_t v = (int64_t)(blockIdx.x - a.part_blocks) * blockDim.x + threadIdx.x; v <= a.V; v += n) {
+    int64_t lo = 0, hi = a.T;  // first entry whose key is at least v
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (a.sorted[mid].x < (uint32_t)v)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    start[v] = (int32_t)lo;
+  }
+}
+
+// One warp per table row and slab of it.
+template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) fw_embed_grad_kernel(EmbedGradArgs a) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
-  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
-  for (int64_t v = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); v < a.V; v += nw) {
-    const int64_t i0 = lower_bound_warp(a.sorted, 0, a.T, (uint32_t)v, lane);
-    const uint32_t hit = __ballot_sync(kFull, i0 + lane < a.T && a.sorted[i0 + lane].x == (uint32_t)v);
-    int64_t i1 = i0 + __popc(hit);
-    if (hit == kFull) i1 = lower_bound_warp(a.sorted, i1, a.T, (uint32_t)v + 1u, lane);
-    const int64_t c0 = i0 / kChunk, c1 = i1 > i0 ? (i1 - 1) / kChunk : c0;
+  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32), work = a.V * a.nslabs;
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
+    const int64_t v = i / a.nslabs;
+    const int slab = (int)(i - v * a.nslabs);
+    const int i0 = a.start[v], i1 = a.start[v + 1];
     T* dst = static_cast<T*>(a.dw) + v * a.D;
-    const int off = dst_off(dst);
-    for (int slab = 0; slab < a.nslabs; ++slab) {
-      float acc[kSlab * V];
+    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V - (ALIGNED ? 0 : dst_off(dst));
+    float acc[kSlab * V];
 #pragma unroll
-      for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
-      const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V - off;
+    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
+    if (i0 < i1) {
+      const int c0 = i0 / kChunk, c1 = (i1 - 1) / kChunk;
       if (c0 == c1) {
-        add_rows<T>(a, i0, i1, e0, acc);
+        const uint32_t pos = i0 + lane < i1 ? a.sorted[i0 + lane].y : 0u;
+        add_rows<T, ALIGNED>(a, pos, i1 - i0, e0, acc);
       } else {
-        for (int64_t c = c0; c <= c1; ++c) {
-          const float* p = a.part + (2 * c + (c == c0 ? 1 : 0)) * a.pitch;
+        for (int c = c0; c <= c1; ++c) {
+          const float* p = a.part + (2 * (int64_t)c + (c == c0 ? 1 : 0)) * a.pitch;
 #pragma unroll
           for (int j = 0; j < kSlab * V; ++j) {
             const int64_t e = e0 + (int64_t)(j / V) * 32 * V + j % V;
@@ -385,23 +475,51 @@ __global__ void __launch_bounds__(256) fw_embed_grad_kernel(EmbedGradArgs a) {
           }
         }
       }
-#pragma unroll
-      for (int k = 0; k < kSlab; ++k) {
-        const int64_t e = e0 + (int64_t)k * 32 * V;
-        if (e >= a.D) continue;
-        float s[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] = acc[k * V + j] * a.scale;
-        store_slot(dst, e, a.D, true, pack16<T>(s));
-      }
     }
+    store_sum<T, ALIGNED>(a, dst, e0, acc);
+  }
+}
+
+// Few tokens: every warp looks for its row in the list of ids.
+template <class T, bool ALIGNED>
+__global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ int32_t key[kDirectTokens];
+  const int n = (int)a.T;
+  for (int i = threadIdx.x; i < kDirectTokens; i += 256) {
+    const int64_t id = i < n ? a.ids[i] : -1;
+    const bool ok = id >= 0 && id < a.V;
+    if (i < n && !ok && blockIdx.x == 0) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
+    key[i] = ok && id != a.padding ? (int32_t)id : -1;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 31;
+  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32), work = a.V * a.nslabs;
+  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
+    const int64_t v = i / a.nslabs;
+    const int slab = (int)(i - v * a.nslabs);
+    T* dst = static_cast<T*>(a.dw) + v * a.D;
+    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V - (ALIGNED ? 0 : dst_off(dst));
+    float acc[kSlab * V];
+#pragma unroll
+    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
+    for (int t0 = 0; t0 < n; t0 += 32) {
+      const uint32_t hit = __ballot_sync(kFull, key[t0 + lane] == (int32_t)v);
+      if (hit == 0u) continue;
+      uint32_t pos = 0u;  // lane i: the i-th hit
+      int at = 0;
+      for (uint32_t h = hit; h != 0u; h &= h - 1u, ++at)
+        if (lane == at) pos = (uint32_t)(t0 + __ffs(h) - 1);
+      add_rows<T, ALIGNED>(a, pos, at, e0, acc);
+    }
+    store_sum<T, ALIGNED>(a, dst, e0, acc);
   }
 }
 
 struct EmbedPlan {
   int passes, bits;
   int64_t tiles, chunks, pitch;
-  int64_t hist_at, part_at, bytes;  // workspace: two entry arrays, histograms, partial rows
+  int64_t hist_at, start_at, part_at, bytes;  // workspace: entries (two arrays), histograms, row starts, partial rows
 };
 
 EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
@@ -413,9 +531,12 @@ EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
   p.tiles = (T + kSortTile - 1) / kSortTile;
   p.chunks = (T + kChunk - 1) / kChunk;
   p.pitch = (D + 7) / 8 * 8;
-  p.hist_at = (2 * T * (int64_t)sizeof(uint2) + 255) / 256 * 256;
-  p.part_at = (p.hist_at + p.tiles * ((int64_t)4 << p.bits) + 255) / 256 * 256;
-  p.bytes = p.part_at + (p.chunks > 1 ? 2 * p.chunks * p.pitch * 4 : 0);
+  if (T <= kDirectTokens) return p;
+  const bool one = T <= kClusterTokens;
+  p.hist_at = ((one ? 1 : 2) * T * (int64_t)sizeof(uint2) + 255) / 256 * 256;
+  p.start_at = (p.hist_at + (one ? 0 : p.tiles * ((int64_t)4 << p.bits)) + 255) / 256 * 256;
+  p.part_at = (p.start_at + 4 * (V + 1) + 255) / 256 * 256;
+  p.bytes = p.part_at + 2 * p.chunks * p.pitch * 4;
   return p;
 }
 
@@ -424,16 +545,58 @@ bool embed_sizes_ok(int64_t T, int64_t V, int64_t D) {
          D <= (int64_t)1 << 24;
 }
 
-template <class T>
-cudaError_t launch_embed_grad(const EmbedGradArgs& a, int64_t chunks, cudaStream_t st) {
-  if (chunks > 1) {
-    const int64_t warps = chunks * a.nslabs;
-    const int64_t g = (warps + 7) / 8, cap = (int64_t)sm_count() * 64;
-    fw_embed_part_kernel<T><<<(unsigned)(g < cap ? g : cap), 256, 0, st>>>(a);
+unsigned warps_grid(int64_t warps) {
+  const int64_t need = (warps + 7) / 8, cap = (int64_t)sm_count() * 64;
+  return (unsigned)(need < cap ? need : cap);
+}
+
+template <class T, bool ALIGNED>
+cudaError_t launch_embed_grad(EmbedGradArgs a, int64_t chunks, int32_t* start, cudaStream_t st) {
+  if (a.T <= kDirectTokens) {
+    fw_embed_direct_kernel<T, ALIGNED><<<warps_grid(a.V * a.nslabs), 256, 0, st>>>(a);
+    return cudaGetLastError();
   }
-  const int64_t g = (a.V + 7) / 8, cap = (int64_t)sm_count() * 64;
-  fw_embed_grad_kernel<T><<<(unsigned)(g < cap ? g : cap), 256, 0, st>>>(a);
+  a.part_blocks = (int)warps_grid(chunks * a.nslabs);
+  fw_embed_part_kernel<T, ALIGNED><<<a.part_blocks + warps_grid((a.V + 32) / 32), 256, 0, st>>>(a, start);
+  a.start = start;
+  fw_embed_grad_kernel<T, ALIGNED><<<warps_grid(a.V * a.nslabs), 256, 0, st>>>(a);
   return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_embed_grad(const EmbedGradArgs& a, int64_t chunks, int32_t* start, cudaStream_t st) {
+  const int64_t es = sizeof(T);
+  const bool aligned = aligned16(a.g) && aligned16(a.dw) && a.ldg * es % 16 == 0 && a.D * es % 16 == 0;
+  return aligned ? launch_embed_grad<T, true>(a, chunks, start, st) : launch_embed_grad<T, false>(a, chunks, start, st);
+}
+
+cudaError_t sort_cluster(const SortArgs& s, int passes, cudaStream_t st) {
+  constexpr int kSmem = 2 * kClusterTile * (int)sizeof(uint2) + kClusterThreads / 32 * (kMaxBins + 2) * 2;
+  static std::atomic<bool> attr_set[kMaxDevices] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= kMaxDevices || !attr_set[dev].load(std::memory_order_acquire)) {
+    e = cudaFuncSetAttribute(fw_sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return e;
+    if (dev < kMaxDevices) attr_set[dev].store(true, std::memory_order_release);
+  }
+  // as many CTAs as tiles ask for: a power of two, so that few tokens do not exchange with idle CTAs
+  int ctas = 1;
+  while (ctas < kClusterCtas && (int64_t)ctas * (kClusterTile / 4) < s.T) ctas *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kClusterThreads);
+  cfg.dynamicSmemBytes = kSmem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, fw_sort_cluster_kernel, s, passes);
 }
 
 }  // namespace
@@ -453,7 +616,7 @@ int fw_embed_rows(int dtype, const int64_t* ids, int64_t T, const void* weight, 
   const int es = dtype == FWB_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(weight) % es || reinterpret_cast<uintptr_t>(out) % es) return FWB_E_POINTER;
   EmbedArgs a = {ids, weight, out, T, V, D, ldw, ldo, scale, status, 0};
-  a.nslabs = (slots_of(D, es) + 32 * kSlab - 1) / (32 * kSlab);
+  a.nslabs = slabs_of(D, es);
   const int64_t need = (T * a.nslabs + 7) / 8, cap = (int64_t)sm_count() * 64;
   const unsigned grid = (unsigned)(need < cap ? need : cap);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -476,40 +639,41 @@ int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, in
   const int es = dtype == FWB_DTYPE_F32 ? 4 : 2;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (T == 0) return cudaMemsetAsync(dweight, 0, (size_t)(V * D * es), st) == cudaSuccess ? FWB_OK : FWB_E_LAUNCH;
-  if (!ids || !grad || !workspace) return FWB_E_POINTER;
+  const EmbedPlan p = embed_plan(T, V, D);
+  if (!ids || !grad || (p.bytes > 0 && !workspace)) return FWB_E_POINTER;
   if (reinterpret_cast<uintptr_t>(grad) % es || reinterpret_cast<uintptr_t>(dweight) % es || !aligned16(workspace))
     return FWB_E_POINTER;
-  const EmbedPlan p = embed_plan(T, V, D);
   if (workspace_bytes < p.bytes) return FWB_E_CAPACITY;
   char* ws = static_cast<char*>(workspace);
-  uint2* ent[2] = {reinterpret_cast<uint2*>(ws), reinterpret_cast<uint2*>(ws) + T};
-  SortArgs s = {};
-  s.ids = ids;
-  s.hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
-  s.T = T;
-  s.V = V;
-  s.padding = padding;
-  s.bits = p.bits;
-  s.tiles = (int)p.tiles;
-  s.status = status;
-  const uint2* sorted;
-  if (p.tiles == 1) {
-    s.dst = ent[0];
-    fw_sort_small_kernel<<<1, kSortThreads, 0, st>>>(s, p.passes, p.bits * p.passes);
-    sorted = ent[0];
-  } else {
-    for (int i = 0; i < p.passes; ++i) {
-      s.src = i == 0 ? nullptr : ent[(i - 1) & 1];
-      s.dst = ent[i & 1];
-      s.shift = i * p.bits;
-      fw_sort_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
-      fw_sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
-    }
-    sorted = ent[(p.passes - 1) & 1];
-  }
-  if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
   EmbedGradArgs a = {};
-  a.sorted = sorted;
+  if (T > kDirectTokens) {
+    uint2* ent[2] = {reinterpret_cast<uint2*>(ws), reinterpret_cast<uint2*>(ws) + T};
+    SortArgs s = {};
+    s.ids = ids;
+    s.hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
+    s.T = T;
+    s.V = V;
+    s.padding = padding;
+    s.bits = p.bits;
+    s.tiles = (int)p.tiles;
+    s.status = status;
+    a.sorted = ent[0];
+    if (T <= kClusterTokens) {
+      s.dst = ent[0];
+      if (sort_cluster(s, p.passes, st) != cudaSuccess) return FWB_E_LAUNCH;
+    } else {
+      for (int i = 0; i < p.passes; ++i) {
+        s.src = i == 0 ? nullptr : ent[(i - 1) & 1];
+        s.dst = ent[i & 1];
+        s.shift = i * p.bits;
+        fw_sort_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
+        fw_sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
+      }
+      a.sorted = ent[(p.passes - 1) & 1];
+      if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+    }
+  }
+  a.ids = ids;
   a.g = grad;
   a.dw = dweight;
   a.part = reinterpret_cast<float*>(ws + p.part_at);
@@ -518,11 +682,14 @@ int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, in
   a.D = D;
   a.ldg = ldg;
   a.pitch = p.pitch;
+  a.padding = padding;
   a.scale = scale;
-  a.nslabs = (slots_of(D, es) + 32 * kSlab - 1) / (32 * kSlab);
-  return launch_status(dtype == FWB_DTYPE_BF16  ? launch_embed_grad<__nv_bfloat16>(a, p.chunks, st)
-                       : dtype == FWB_DTYPE_F16 ? launch_embed_grad<__half>(a, p.chunks, st)
-                                                : launch_embed_grad<float>(a, p.chunks, st));
+  a.nslabs = slabs_of(D, es);
+  a.status = status;
+  int32_t* start = reinterpret_cast<int32_t*>(ws + p.start_at);
+  return launch_status(dtype == FWB_DTYPE_BF16  ? launch_embed_grad<__nv_bfloat16>(a, p.chunks, start, st)
+                       : dtype == FWB_DTYPE_F16 ? launch_embed_grad<__half>(a, p.chunks, start, st)
+                                                : launch_embed_grad<float>(a, p.chunks, start, st));
 }
 
 }  // extern "C"

@@ -15,7 +15,7 @@
 //
 // Bound by HBM: forward reads x and residual and writes s and y, backward
 // reads dy, s and ds_out and writes ds, each once.  A row lives in the
-// registers of a group of G threads (a warp, or a CTA of up to 512) as CH
+// registers of a group of G threads (a warp, or a CTA of up to 1024) as CH
 // slots of 16 bytes per thread (fw_rowslots.cuh).  The grid is persistent
 // with a group count that is a multiple of 8, so that the rows one group
 // visits all start at the same distance from a 16-byte boundary: a thread
@@ -106,15 +106,38 @@ __device__ __forceinline__ float group_reduce(float v, float* buf, int& flip) {
   return v;
 }
 
+// y in steps of the scale, to the nearest, as a byte; `steps` = 1 / scale, 0
+// for a row that has no such step (its y may be NaN).
+__device__ __forceinline__ uint32_t int8_step(float y, float steps) {
+  const float u = steps > 0.0f ? fminf(fmaxf(rintf(y * steps), -127.0f), 127.0f) : 0.0f;
+  return (uint32_t)(int)u & 0xffu;
+}
+
 template <int G>
 __host__ __device__ constexpr int cta_threads() {
   return G < 128 ? 128 : G;
 }
 
+// The slots of one row that a thread holds.
+template <class T, int CH>
+struct Slots {
+  uint4 u[CH];
+  __device__ __forceinline__ void load(const void* base, int64_t row, int64_t ld, int64_t e0, int64_t step, int64_t D,
+                                       int vec) {
+    const T* p = static_cast<const T*>(base) + row * ld;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) u[k] = load_slot(p, e0 + k * step, D, vec);
+  }
+};
+
+// The loads of a group's next row are issued before the current row is
+// reduced (CH = 1: the registers allow it), so that the memory pipe does not
+// drain at the reductions.
 template <class T, int G, int CH, int MODE>
-__global__ void __launch_bounds__(cta_threads<G>()) fw_norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_norm_kernel(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
+  constexpr bool AHEAD = CH == 1;
   __shared__ float red[2 * (G / 32)];
   extern __shared__ __align__(16) int8_t qrow_all[];
   const int t = threadIdx.x % G;
@@ -124,36 +147,35 @@ __global__ void __launch_bounds__(cta_threads<G>()) fw_norm_kernel(NormArgs a) {
   if (first >= a.rows) return;  // a whole group; groups of one CTA share no barrier unless R == 1
   int flip = 0;
   const int off = row_off<T>(a.x, first, a.ldx, a.vec);
+  const int64_t e0 = (int64_t)t * V - off;
+  Slots<T, CH> xs, rs;
+  xs.load(a.x, first, a.ldx, e0, G * V, a.D, a.vec);
+  if (a.res) rs.load(a.res, first, a.ldr, e0, G * V, a.D, a.vec);
   float gain[CH * V];
   if constexpr (MODE != kInt8Only) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, (int64_t)(k * G + t) * V - off, a.D, gain + k * V);
+    for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, e0 + k * (G * V), a.D, gain + k * V);
   }
   const float inv_d = 1.0f / (float)a.D;
   for (int64_t r = first; r < a.rows; r += step) {
-    const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
-    uint4 xs[CH], rs[CH];
-#pragma unroll
-    for (int k = 0; k < CH; ++k) xs[k] = load_slot(xr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
-    if (a.res) {
-      const T* rr = static_cast<const T*>(a.res) + r * a.ldr;
-#pragma unroll
-      for (int k = 0; k < CH; ++k) rs[k] = load_slot(rr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
-    }
     float v[CH * V];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) unpack16<T>(xs[k], v + k * V);
+    for (int k = 0; k < CH; ++k) unpack16<T>(xs.u[k], v + k * V);
     if (a.res) {
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         float u[V];
-        unpack16<T>(rs[k], u);
+        unpack16<T>(rs.u[k], u);
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] += v[k * V + j];
-        const uint4 p = pack16<T>(u);
-        unpack16<T>(p, v + k * V);
-        if (a.s) store_slot(static_cast<T*>(a.s) + r * a.lds, (int64_t)(k * G + t) * V - off, a.D, a.vec, p);
+        rs.u[k] = pack16<T>(u);
+        unpack16<T>(rs.u[k], v + k * V);
+        store_slot(static_cast<T*>(a.s) + r * a.lds, e0 + k * (G * V), a.D, a.vec, rs.u[k]);
       }
+    }
+    if (AHEAD && r + step < a.rows) {
+      xs.load(a.x, r + step, a.ldx, e0, G * V, a.D, a.vec);
+      if (a.res) rs.load(a.res, r + step, a.ldr, e0, G * V, a.D, a.vec);
     }
     if constexpr (MODE != kInt8Only) {
       float ss = 0.0f;
@@ -168,7 +190,7 @@ __global__ void __launch_bounds__(cta_threads<G>()) fw_norm_kernel(NormArgs a) {
     if constexpr (MODE == kNormOut) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
-        store_slot(static_cast<T*>(a.y) + r * a.ldy, (int64_t)(k * G + t) * V - off, a.D, a.vec, pack16<T>(v + k * V));
+        store_slot(static_cast<T*>(a.y) + r * a.ldy, e0 + k * (G * V), a.D, a.vec, pack16<T>(v + k * V));
     } else {
       float m = 0.0f;
 #pragma unroll
@@ -176,32 +198,51 @@ __global__ void __launch_bounds__(cta_threads<G>()) fw_norm_kernel(NormArgs a) {
       m = group_reduce<G, true>(m, red, flip);
       const float scale = m / 127.0f;
       if (t == 0) a.qscale[r] = scale;
-      const bool live = scale > 0.0f && scale < CUDART_INF_F;  // otherwise the row is 0 (or NaN) through its scale
-      const int64_t w16 = (a.D + 15) / 16;
-      int8_t* qs = qrow_all + (int64_t)grp * w16 * 16;
-      if (t < 16 && a.D + t < w16 * 16) qs[a.D + t] = 0;
+      // a row of zeros, or not finite, is 0 (or NaN) through its scale
+      const float steps = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / scale : 0.0f;
+      const int64_t w16 = (a.D + 15) / 16 * 16;
+      if (off == 0) {  // the slots' bytes lie together in q
 #pragma unroll
-      for (int k = 0; k < CH; ++k) {
-        const int64_t e0 = (int64_t)(k * G + t) * V - off;
+        for (int k = 0; k < CH; ++k) {
+          const int64_t e = e0 + k * (G * V);
+          if (e >= w16) continue;
+          uint32_t b[V / 4];
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          const int64_t e = e0 + j;
-          if (e >= 0 && e < a.D) {
-            const float u = live ? rintf(__fdiv_rn(v[k * V + j], scale)) : 0.0f;
-            qs[e] = (int8_t)fminf(fmaxf(u, -127.0f), 127.0f);
-          }
+          for (int j = 0; j < V; j += 4)
+            b[j / 4] = int8_step(v[k * V + j], steps) | (int8_step(v[k * V + j + 1], steps) << 8) |
+                       (int8_step(v[k * V + j + 2], steps) << 16) | (int8_step(v[k * V + j + 3], steps) << 24);
+          if constexpr (V == 8)
+            *reinterpret_cast<uint2*>(a.q + r * a.ldq + e) = make_uint2(b[0], b[1]);
+          else
+            *reinterpret_cast<uint32_t*>(a.q + r * a.ldq + e) = b[0];
         }
+        if constexpr (CH * G * V < 16 * 64) {  // short rows: the padding may lie past the last slot
+          for (int64_t e = (int64_t)(CH * G + t) * V; e < w16; e += G * V)
+            for (int j = 0; j < V; ++j) a.q[r * a.ldq + e + j] = 0;
+        }
+      } else {  // through shared memory
+        int8_t* qs = qrow_all + (int64_t)grp * w16;
+        if (t < 16 && a.D + t < w16) qs[a.D + t] = 0;
+#pragma unroll
+        for (int i = 0; i < CH * V; ++i) {
+          const int64_t e = e0 + (i / V) * (G * V) + i % V;
+          if (e >= 0 && e < a.D) qs[e] = (int8_t)int8_step(v[i], steps);
+        }
+        if constexpr (G > 32)
+          __syncthreads();
+        else
+          __syncwarp();
+        for (int64_t i = t; i < w16 / 16; i += G)
+          reinterpret_cast<uint4*>(a.q + r * a.ldq)[i] = reinterpret_cast<const uint4*>(qs)[i];
+        if constexpr (G > 32)
+          __syncthreads();
+        else
+          __syncwarp();
       }
-      if constexpr (G > 32)
-        __syncthreads();
-      else
-        __syncwarp();
-      for (int64_t i = t; i < w16; i += G)
-        reinterpret_cast<uint4*>(a.q + r * a.ldq)[i] = reinterpret_cast<const uint4*>(qs)[i];
-      if constexpr (G > 32)
-        __syncthreads();
-      else
-        __syncwarp();
+    }
+    if (!AHEAD && r + step < a.rows) {
+      xs.load(a.x, r + step, a.ldx, e0, G * V, a.D, a.vec);
+      if (a.res) rs.load(a.res, r + step, a.ldr, e0, G * V, a.D, a.vec);
     }
   }
 }
@@ -246,24 +287,24 @@ __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
       m = group_reduce<1024, true>(m, red, flip);
       const float scale = m / 127.0f;
       if (threadIdx.x == 0) a.qscale[r] = scale;
-      const bool live = scale > 0.0f && scale < CUDART_INF_F;
+      const float steps = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / scale : 0.0f;
       for (int64_t e = threadIdx.x; e < (a.D + 15) / 16 * 16; e += 1024) {
-        float u = 0.0f;
-        if (e < a.D && live) {
-          float v = elem(e);
+        float v = 0.0f;
+        if (e < a.D) {
+          v = elem(e);
           if constexpr (MODE != kInt8Only) v = v * rstd * gain(e);
-          u = rintf(__fdiv_rn(v, scale));
         }
-        a.q[r * a.ldq + e] = (int8_t)fminf(fmaxf(u, -127.0f), 127.0f);
+        a.q[r * a.ldq + e] = (int8_t)int8_step(v, steps);
       }
     }
   }
 }
 
 template <class T, int G, int CH>
-__global__ void __launch_bounds__(cta_threads<G>()) fw_norm_grad_kernel(NormGradArgs a) {
+__global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_norm_grad_kernel(NormGradArgs a) {
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
+  constexpr bool AHEAD = CH == 1;
   __shared__ float red[2 * (G / 32)];
   extern __shared__ __align__(16) float dw_row[];  // [D], R > 1 only
   const int t = threadIdx.x % G;
@@ -278,33 +319,31 @@ __global__ void __launch_bounds__(cta_threads<G>()) fw_norm_grad_kernel(NormGrad
 #pragma unroll
   for (int i = 0; i < CH * V; ++i) dw[i] = 0.0f;
   const float inv_d = 1.0f / (float)a.D;
+  const int64_t e0 = (int64_t)t * V - off;
+  Slots<T, CH> ss, gs, os;
+  float rstd = 0.0f;
+  auto fetch = [&](int64_t r) {
+    ss.load(a.s, r, a.lds, e0, G * V, a.D, a.vec);
+    gs.load(a.dy, r, a.lddy, e0, G * V, a.D, a.vec);
+    if (a.dso) os.load(a.dso, r, a.ldo, e0, G * V, a.D, a.vec);
+    rstd = a.rstd[r];
+  };
+  if (first < a.rows) fetch(first);
   for (int64_t r = first; r < a.rows; r += step) {
-    const T* sr = static_cast<const T*>(a.s) + r * a.lds;
-    const T* gr = static_cast<const T*>(a.dy) + r * a.lddy;
-    uint4 ss[CH], gs[CH], os[CH];
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      ss[k] = load_slot(sr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
-      gs[k] = load_slot(gr, (int64_t)(k * G + t) * V - off, a.D, a.vec);
-    }
-    if (a.dso) {
-      const T* orow = static_cast<const T*>(a.dso) + r * a.ldo;
-#pragma unroll
-      for (int k = 0; k < CH; ++k) os[k] = load_slot(orow, (int64_t)(k * G + t) * V - off, a.D, a.vec);
-    } else {
-#pragma unroll
-      for (int k = 0; k < CH; ++k) os[k] = make_uint4(0u, 0u, 0u, 0u);
-    }
-    const float rstd = a.rstd[r];
+    // the current row stays packed: unpacking twice costs fewer registers
+    const Slots<T, CH> cs = ss, cg = gs;
+    Slots<T, CH> co = os;
+    const float rs = rstd;
+    if (AHEAD && r + step < a.rows) fetch(r + step);
     float c = 0.0f;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float s[V], g[V];
-      unpack16<T>(ss[k], s);
-      unpack16<T>(gs[k], g);
+      unpack16<T>(cs.u[k], s);
+      unpack16<T>(cg.u[k], g);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const float n = s[j] * rstd;
+        const float n = s[j] * rs;
         c = fmaf(g[j] * gain[k * V + j], n, c);
         dw[k * V + j] = fmaf(g[j], n, dw[k * V + j]);
       }
@@ -313,13 +352,15 @@ __global__ void __launch_bounds__(cta_threads<G>()) fw_norm_grad_kernel(NormGrad
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float s[V], g[V], o[V];
-      unpack16<T>(ss[k], s);
-      unpack16<T>(gs[k], g);
-      unpack16<T>(os[k], o);
+      unpack16<T>(cs.u[k], s);
+      unpack16<T>(cg.u[k], g);
+      if (!a.dso) co.u[k] = make_uint4(0u, 0u, 0u, 0u);
+      unpack16<T>(co.u[k], o);
 #pragma unroll
-      for (int j = 0; j < V; ++j) o[j] = fmaf(rstd, fmaf(g[j], gain[k * V + j], -(s[j] * rstd) * c), o[j]);
-      store_slot(static_cast<T*>(a.dx) + r * a.lddx, (int64_t)(k * G + t) * V - off, a.D, a.vec, pack16<T>(o));
+      for (int j = 0; j < V; ++j) o[j] = fmaf(rs, fmaf(-(s[j] * rs), c, g[j] * gain[k * V + j]), o[j]);
+      store_slot(static_cast<T*>(a.dx) + r * a.lddx, e0 + k * (G * V), a.D, a.vec, pack16<T>(o));
     }
+    if (!AHEAD && r + step < a.rows) fetch(r + step);
   }
   if (!a.part) return;
   float* part = a.part + (int64_t)blockIdx.x * a.D;
@@ -373,30 +414,32 @@ __global__ void __launch_bounds__(1024) fw_norm_grad_long_kernel(NormGradArgs a)
   }
 }
 
-// dw[e] = sum over the parts in order; 32 columns and 8 interleaved runs of
-// parts per CTA.
+// dw[e] = sum over the parts, in a fixed order: 32 columns per CTA, each of
+// its 32 warps adds every 32nd part.
 template <class T>
-__global__ void __launch_bounds__(256) fw_norm_dw_kernel(const float* __restrict__ part, int64_t n, int64_t D,
-                                                         T* __restrict__ dw) {
-  __shared__ float sm[8][33];
+__global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restrict__ part, int64_t n, int64_t D,
+                                                          T* __restrict__ dw) {
+  __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + lane;
   float s = 0.0f;
-  if (e < D)
-    for (int64_t p = w; p < n; p += 8) s += part[p * D + e];
+  if (e < D) {
+#pragma unroll 8
+    for (int64_t p = w; p < n; p += 32) s += part[p * D + e];
+  }
   sm[w][lane] = s;
   __syncthreads();
-  if (w == 0 && e < D) {
-    float t = 0.0f;
+  // warp w takes column w of the block
+  s = sm[lane][w];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) t += sm[i][lane];
-    st_elem(dw + e, t);
-  }
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFull, s, o);
+  const int64_t c = (int64_t)blockIdx.x * 32 + w;
+  if (lane == 0 && c < D) st_elem(dw + c, s);
 }
 
-// Threads per row and slots per thread by the row's slot count: a warp up to
-// 64 slots; CTAs of 128, 256 and 512 threads so that a thread holds at most
-// 2 slots (4 in the longest); the memory-pass kernels beyond 2048.
+// Threads per row by the row's slot count: a warp, or a CTA with one slot per
+// thread (two in the longest), so that a thread's 64 registers hold the row
+// and the next one; the memory-pass kernels beyond 2048 slots.
 struct NormShape {
   int G, CH;
 };
@@ -405,12 +448,11 @@ NormShape norm_shape(int64_t D, int64_t esize, bool vec) {
   const int64_t V = 16 / esize;
   const int64_t n = (D + V - 1) / V + (vec && (D * esize) % 16 != 0 ? 1 : 0);
   if (n <= 32) return {32, 1};
-  if (n <= 64) return {32, 2};
   if (n <= 128) return {128, 1};
-  if (n <= 256) return {128, 2};
-  if (n <= 512) return {256, 2};
-  if (n <= 1024) return {512, 2};
-  if (n <= 2048) return {512, 4};
+  if (n <= 256) return {256, 1};
+  if (n <= 512) return {512, 1};
+  if (n <= 1024) return {1024, 1};
+  if (n <= 2048) return {1024, 2};
   return {0, 0};
 }
 
@@ -451,13 +493,12 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
   const int R = sh.G == 32 ? 4 : 1;
   const size_t smem = MODE == kNormOut ? 0 : (size_t)R * (size_t)((a.D + 15) / 16 * 16);
-  if (sh.G == 32 && sh.CH == 1) fw_norm_kernel<T, 32, 1, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 32) fw_norm_kernel<T, 32, 2, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128 && sh.CH == 1) fw_norm_kernel<T, 128, 1, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128) fw_norm_kernel<T, 128, 2, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 256) fw_norm_kernel<T, 256, 2, MODE><<<grid, 256, smem, st>>>(a);
-  else if (sh.G == 512 && sh.CH == 2) fw_norm_kernel<T, 512, 2, MODE><<<grid, 512, smem, st>>>(a);
-  else if (sh.G == 512) fw_norm_kernel<T, 512, 4, MODE><<<grid, 512, smem, st>>>(a);
+  if (sh.G == 32) fw_norm_kernel<T, 32, 1, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128) fw_norm_kernel<T, 128, 1, MODE><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 256) fw_norm_kernel<T, 256, 1, MODE><<<grid, 256, smem, st>>>(a);
+  else if (sh.G == 512) fw_norm_kernel<T, 512, 1, MODE><<<grid, 512, smem, st>>>(a);
+  else if (sh.G == 1024 && sh.CH == 1) fw_norm_kernel<T, 1024, 1, MODE><<<grid, 1024, smem, st>>>(a);
+  else if (sh.G == 1024) fw_norm_kernel<T, 1024, 2, MODE><<<grid, 1024, smem, st>>>(a);
   else fw_norm_long_kernel<T, MODE><<<grid, 1024, 0, st>>>(a);
   return cudaGetLastError();
 }
@@ -467,13 +508,12 @@ cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
   const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
   const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
   const size_t smem = sh.G == 32 ? (size_t)a.D * sizeof(float) : 0;
-  if (sh.G == 32 && sh.CH == 1) fw_norm_grad_kernel<T, 32, 1><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 32) fw_norm_grad_kernel<T, 32, 2><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128 && sh.CH == 1) fw_norm_grad_kernel<T, 128, 1><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128) fw_norm_grad_kernel<T, 128, 2><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 256) fw_norm_grad_kernel<T, 256, 2><<<grid, 256, smem, st>>>(a);
-  else if (sh.G == 512 && sh.CH == 2) fw_norm_grad_kernel<T, 512, 2><<<grid, 512, smem, st>>>(a);
-  else if (sh.G == 512) fw_norm_grad_kernel<T, 512, 4><<<grid, 512, smem, st>>>(a);
+  if (sh.G == 32) fw_norm_grad_kernel<T, 32, 1><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 128) fw_norm_grad_kernel<T, 128, 1><<<grid, 128, smem, st>>>(a);
+  else if (sh.G == 256) fw_norm_grad_kernel<T, 256, 1><<<grid, 256, smem, st>>>(a);
+  else if (sh.G == 512) fw_norm_grad_kernel<T, 512, 1><<<grid, 512, smem, st>>>(a);
+  else if (sh.G == 1024 && sh.CH == 1) fw_norm_grad_kernel<T, 1024, 1><<<grid, 1024, smem, st>>>(a);
+  else if (sh.G == 1024) fw_norm_grad_kernel<T, 1024, 2><<<grid, 1024, smem, st>>>(a);
   else fw_norm_grad_long_kernel<T><<<grid, 1024, 0, st>>>(a);
   return cudaGetLastError();
 }
@@ -615,11 +655,11 @@ int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy, const 
   if (e != cudaSuccess || !dweight) return launch_status(e);
   const dim3 g2((unsigned)((D + 31) / 32));
   if (wdtype == FWB_DTYPE_BF16)
-    fw_norm_dw_kernel<__nv_bfloat16><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<__nv_bfloat16*>(dweight));
+    fw_norm_dw_kernel<__nv_bfloat16><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<__nv_bfloat16*>(dweight));
   else if (wdtype == FWB_DTYPE_F16)
-    fw_norm_dw_kernel<__half><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<__half*>(dweight));
+    fw_norm_dw_kernel<__half><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<__half*>(dweight));
   else
-    fw_norm_dw_kernel<float><<<g2, 256, 0, st>>>(parts, grid, D, static_cast<float*>(dweight));
+    fw_norm_dw_kernel<float><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<float*>(dweight));
   return launch_status(cudaGetLastError());
 }
 
