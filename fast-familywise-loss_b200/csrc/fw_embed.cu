@@ -14,12 +14,17 @@
 // two launches per digit beyond.  Up to kDirectTokens tokens nothing is
 // sorted: every warp finds its row's positions in the list itself.
 //
-// Skewed ids (the commonest token may take a tenth of the positions) are cut
-// at fixed chunks of kChunk sorted entries: a run of equal ids inside one
-// chunk is summed by the warp that owns the table row; a run that crosses a
-// chunk boundary is first summed chunk by chunk into fp32 partial rows by
-// other warps.  The longest serial sum is then kChunk rows plus one partial
-// per chunk.
+// Skewed ids (the commonest token may take a tenth of the positions) do not
+// unbalance the sums: a warp takes kChunk sorted entries and 512 bytes of
+// their rows, whoever they belong to, with kAhead rows in flight.  A run of
+// equal ids that ends inside its chunk is finished there and its table row
+// written; the parts of a run that crosses chunks go to fp32 partial rows,
+// which a last small launch adds up in order.
+//
+// The rows of dW without a token, most of the bytes for a large vocabulary,
+// are zeroed by CTAs that run beside the sort (each marks its rows' tokens in
+// a bitmap, from the unsorted list), or beside the sums for more tokens than
+// one cluster sorts.
 //
 // Rows are read and written in 16-byte slots of the destination row, whatever
 // the alignment of either (fw_rowslots.cuh).
@@ -35,7 +40,8 @@ namespace fwb200 {
 namespace {
 
 constexpr int kSlab = 4;         // slots per lane and step: 2 KB of a row per warp
-constexpr int kChunk = 32;       // sorted entries per partial sum
+constexpr int kChunk = 32;       // sorted entries per warp
+constexpr int kAhead = 8;        // rows of g in flight per warp
 constexpr int kSortThreads = 256;
 constexpr int kSortItems = 8;
 constexpr int kSortTile = kSortThreads * kSortItems;
@@ -246,11 +252,55 @@ __global__ void __launch_bounds__(kSortThreads) fw_sort_scatter_kernel(SortArgs 
     if (digit[i] < (uint32_t)bins) a.dst[total[digit[i]] + place[digit[i]] + cnt[w][digit[i]] + rank[i]] = ent[i];
 }
 
+// Zeroes row v of dw: the lanes of a warp over its slots.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void zero_row(T* dst, int64_t D, int nslots, int lane) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t off = ALIGNED ? 0 : dst_off(dst);
+#pragma unroll 4
+  for (int64_t slot = lane; slot < nslots; slot += 32) {
+    const int64_t e0 = slot * V - off;
+    if (e0 >= D) continue;
+    if (ALIGNED)
+      *reinterpret_cast<uint4*>(dst + e0) = make_uint4(0u, 0u, 0u, 0u);
+    else
+      store_slot(dst, e0, D, true, make_uint4(0u, 0u, 0u, 0u));
+  }
+}
+
+struct ZeroArgs {
+  void* dw;
+  int64_t D;
+  int nslots;
+  int rows;  // rows per CTA, at most kZeroRows
+};
+
+constexpr int kZeroRows = 1024;
+
+// Rows first .. first + a.rows of dw that no entry names, by a whole CTA.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void zero_unnamed(const SortArgs& s, const ZeroArgs& z, int64_t first, uint32_t* named) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  for (int i = threadIdx.x; i < kZeroRows / 32; i += kClusterThreads) named[i] = 0u;
+  __syncthreads();
+#pragma unroll 4
+  for (int64_t t = threadIdx.x; t < s.T; t += kClusterThreads) {
+    const int64_t r = s.ids[t] - first;
+    if (r >= 0 && r < z.rows && r + first != s.padding) atomicOr(&named[r >> 5], 1u << (r & 31));
+  }
+  __syncthreads();
+  const int n = (int)min((int64_t)z.rows, s.V - first);
+  for (int r = w; r < n; r += kClusterThreads / 32)
+    if (!(named[r >> 5] >> (r & 31) & 1u))
+      zero_row<T, ALIGNED>(static_cast<T*>(z.dw) + (first + r) * z.D, z.D, z.nslots, lane);
+}
+
 // All passes in one launch: a cluster holds the entries in shared memory, CTA
 // c the entries c * per .. of the current order.  Per pass the CTAs rank their
 // own entries, read each other's digit counts, and store every entry where it
-// belongs in the cluster.
-__global__ void __launch_bounds__(kClusterThreads) fw_sort_cluster_kernel(SortArgs a, int passes) {
+// belongs in the cluster.  The grid's other clusters zero.
+template <class TW, bool ALIGNED>
+__global__ void __launch_bounds__(kClusterThreads, 2) fw_sort_cluster_kernel(SortArgs a, int passes, ZeroArgs z) {
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char sort_smem[];
@@ -260,6 +310,13 @@ __global__ void __launch_bounds__(kClusterThreads) fw_sort_cluster_kernel(SortAr
   const int bins = 1 << a.bits;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int nc = (int)cl.num_blocks(), me = (int)cl.block_rank();
+  if ((int)blockIdx.x >= nc) {
+    for (int64_t v = (int64_t)(blockIdx.x - nc) * z.rows; v < a.V; v += (int64_t)(gridDim.x - nc) * z.rows) {
+      zero_unnamed<TW, ALIGNED>(a, z, v, total);
+      __syncthreads();
+    }
+    return;
+  }
   const int T = (int)a.T;
   const int per = (T + nc - 1) / nc;
   const int first = me * per, mine = max(0, min(per, T - first));
@@ -322,117 +379,110 @@ __global__ void __launch_bounds__(kClusterThreads) fw_sort_cluster_kernel(SortAr
 // ------------------------------------------------------------ row sums
 struct EmbedGradArgs {
   const uint2* sorted;
-  const int32_t* start;  // [V + 1] first sorted entry of each row
-  const int64_t* ids;    // direct form
+  const int64_t* ids;  // direct form
   const void* g;
   void* dw;
   float* part;  // [2 * chunks, pitch]
   int64_t T, V, D, ldg, pitch, padding;
   float scale;
-  int nslabs;
-  int part_blocks;
+  int nslots;       // slots of a row, at any alignment
+  int sum_blocks;   // CTAs that add rows; the others zero
   int32_t* status;
 };
-
-// Adds rows pos of the n <= 32 entries (lane i holds the i-th position) of g,
-// in that order, to the slots of this lane.  ALIGNED: every row of g and dw
-// starts on a 16-byte boundary.
-template <class T, bool ALIGNED>
-__device__ __forceinline__ void add_rows(const EmbedGradArgs& a, uint32_t pos, int n, int64_t e0, float* acc) {
-  constexpr int V = 16 / sizeof(T);
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const T* row = static_cast<const T*>(a.g) + (int64_t)__shfl_sync(kFull, pos, i) * a.ldg;
-    uint4 u[kSlab];
-#pragma unroll
-    for (int k = 0; k < kSlab; ++k) {
-      const int64_t e = e0 + (int64_t)k * 32 * V;
-      u[k] = e >= a.D  ? make_uint4(0u, 0u, 0u, 0u)
-             : ALIGNED ? ld_stream16(row + e)
-                       : load_slot_shifted(row, e, a.D);
-    }
-#pragma unroll
-    for (int k = 0; k < kSlab; ++k) {
-      float v[V];
-      unpack16<T>(u[k], v);
-#pragma unroll
-      for (int j = 0; j < V; ++j) acc[k * V + j] += v[j];
-    }
-  }
-}
 
 template <class T, bool ALIGNED>
 __device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int64_t e0, const float* acc) {
   constexpr int V = 16 / sizeof(T);
+  if (e0 >= a.D) return;
+  float s[V];
 #pragma unroll
-  for (int k = 0; k < kSlab; ++k) {
-    const int64_t e = e0 + (int64_t)k * 32 * V;
-    if (e >= a.D) continue;
-    float s[V];
-#pragma unroll
-    for (int j = 0; j < V; ++j) s[j] = acc[k * V + j] * a.scale;
-    if (ALIGNED)
-      *reinterpret_cast<uint4*>(dst + e) = pack16<T>(s);
-    else
-      store_slot(dst, e, a.D, true, pack16<T>(s));
-  }
+  for (int j = 0; j < V; ++j) s[j] = acc[j] * a.scale;
+  if (ALIGNED)
+    *reinterpret_cast<uint4*>(dst + e0) = pack16<T>(s);
+  else
+    store_slot(dst, e0, a.D, true, pack16<T>(s));
 }
 
-// Partial rows of the runs that cross a chunk boundary: row 2c is the part in
-// chunk c of a run that began before it, row 2c + 1 the part of a run that
-// begins in it and goes on.
+// Start of slot `slot` in the row at dst: every row's own slots, so that a
+// run's partial rows (kept by slot) and its table row agree.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int slab, int lane) {
+__device__ __forceinline__ int64_t slot_elem(const T* dst, int64_t slot) {
+  constexpr int V = 16 / sizeof(T);
+  return slot * V - (ALIGNED ? 0 : dst_off(dst));
+}
+
+// Adds the rows of chunk c, slots slot .. of which this lane has one, in
+// order.  Partial row 2c is the part of a run that began in an earlier chunk,
+// 2c + 1 the part of a run that begins here and goes on.
+template <class T, bool ALIGNED>
+__device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int64_t slot, int lane) {
   constexpr int V = 16 / sizeof(T);
   const int64_t b = c * kChunk;
   const int n = (int)min((int64_t)kChunk, a.T - b);
-  const uint2 ent = lane < n ? a.sorted[b + lane] : make_uint2(0xffffffffu, 0u);
+  const uint2 ent = lane < n ? a.sorted[b + lane] : make_uint2((uint32_t)a.V, 0u);
   const uint32_t first = __shfl_sync(kFull, ent.x, 0), last = __shfl_sync(kFull, ent.x, n - 1);
   const bool from = b > 0 && a.sorted[b - 1].x == first;
   const bool on = b + n < a.T && a.sorted[b + n].x == last;
-  for (int half = 0; half < 2; ++half) {
-    int i0 = 0, i1 = n;
-    if (half == 0) {
-      if (!from || first >= (uint32_t)a.V) continue;
-      i1 = __popc(__ballot_sync(kFull, lane < n && ent.x == first));
-    } else {
-      if (!on || last >= (uint32_t)a.V || (from && first == last)) continue;
-      i0 = n - __popc(__ballot_sync(kFull, lane < n && ent.x == last));
+  // per entry, as bits: its run begins here / ends here, and where the sum goes
+  const uint32_t up = __shfl_up_sync(kFull, ent.x, 1), down = __shfl_down_sync(kFull, ent.x, 1);
+  const uint32_t begins = __ballot_sync(kFull, lane == 0 || up != ent.x);
+  const uint32_t ends = __ballot_sync(kFull, lane == n - 1 || down != ent.x);
+  const uint32_t to0 = __ballot_sync(kFull, from && ent.x == first);
+  const uint32_t to1 = __ballot_sync(kFull, on && ent.x == last) & ~to0;
+  const int live = __popc(__ballot_sync(kFull, ent.x < (uint32_t)a.V));  // the others sort behind
+  float acc[V];
+  for (int i0 = 0; i0 < live; i0 += kAhead) {
+    uint4 u[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const T* row = static_cast<const T*>(a.g) + (int64_t)__shfl_sync(kFull, ent.y, (i0 + i) & 31) * a.ldg;
+      int64_t e0 = slot * V;
+      if (!ALIGNED)
+        e0 -= dst_off(static_cast<const T*>(a.dw) + (int64_t)__shfl_sync(kFull, ent.x, (i0 + i) & 31) * a.D);
+      u[i] = i0 + i >= live || e0 >= a.D ? make_uint4(0u, 0u, 0u, 0u)
+             : ALIGNED                   ? ld_stream16(row + e0)
+                                         : load_slot_shifted(row, e0, a.D);
     }
-    float acc[kSlab * V];
 #pragma unroll
-    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
-    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V;
-    add_rows<T, ALIGNED>(a, __shfl_sync(kFull, ent.y, (i0 + lane) & 31), i1 - i0, e0, acc);
-    float* out = a.part + (2 * c + half) * a.pitch;
+    for (int i = 0; i < kAhead; ++i) {
+      const int at = i0 + i;
+      if (at >= live) break;
+      float v[V];
+      unpack16<T>(u[i], v);
+      const bool begin = begins >> at & 1u;
 #pragma unroll
-    for (int k = 0; k < kSlab; ++k) {
-      const int64_t e = e0 + (int64_t)k * 32 * V;
-      if (e < a.D) {
+      for (int j = 0; j < V; ++j) acc[j] = begin ? v[j] : acc[j] + v[j];
+      if (!(ends >> at & 1u)) continue;
+      if (!((to0 | to1) >> at & 1u)) {
+        T* dst = static_cast<T*>(a.dw) + (int64_t)__shfl_sync(kFull, ent.x, at) * a.D;
+        store_sum<T, ALIGNED>(a, dst, slot_elem<T, ALIGNED>(dst, slot), acc);
+      } else if (slot < a.nslots) {
+        float* out = a.part + (2 * c + (to1 >> at & 1u)) * a.pitch + slot * V;
 #pragma unroll
-        for (int j = 0; j < V; j += 4)  // pitch is a multiple of V
-          *reinterpret_cast<float4*>(out + e + j) =
-              make_float4(acc[k * V + j], acc[k * V + j + 1], acc[k * V + j + 2], acc[k * V + j + 3]);
+        for (int j = 0; j < V; j += 4)
+          *reinterpret_cast<float4*>(out + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
       }
     }
   }
 }
 
-// What the row sums need of the sorted tokens: the partial rows (first
-// part_blocks CTAs) and where each row's entries start (the others).
+// sum_blocks of the CTAs add; the others, spread among them (more tokens than
+// one cluster sorts), look for the rows without a token and zero them: 8 rows
+// per warp, one binary search per lane.
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) fw_embed_part_kernel(EmbedGradArgs a, int32_t* start) {
-  const int lane = threadIdx.x & 31;
-  if ((int)blockIdx.x < a.part_blocks) {
-    const int64_t chunks = (a.T + kChunk - 1) / kChunk;
-    const int64_t work = chunks * a.nslabs;
-    const int64_t nw = (int64_t)a.part_blocks * (blockDim.x / 32);
-    for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw)
-      sum_chunk<T, ALIGNED>(a, i / a.nslabs, (int)(i % a.nslabs), lane);
+__global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) fw_embed_sum_kernel(EmbedGradArgs a) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t total = gridDim.x, adding = a.sum_blocks;
+  const int64_t before = blockIdx.x * adding / total;  // adding CTAs ahead of this one
+  if ((blockIdx.x + 1) * adding / total != before) {
+    const int64_t slabs = (a.nslots + 31) / 32;
+    const int64_t work = (a.T + kChunk - 1) / kChunk * slabs;
+    for (int64_t i = before * 8 + w; i < work; i += adding * 8)
+      sum_chunk<T, ALIGNED>(a, i / slabs, i % slabs * 32 + lane, lane);
     return;
   }
-  const int64_t n = (int64_t)(gridDim.x - a.part_blocks) * blockDim.x;
-  for (int64_t v = (int64_t)(blockIdx.x - a.part_blocks) * blockDim.x + threadIdx.x; v <= a.V; v += n) {
+  for (int64_t v0 = ((blockIdx.x - before) * 8 + w) * 8; v0 < a.V; v0 += (total - adding) * 64) {
+    const int64_t v = v0 + (lane & 7);
     int64_t lo = 0, hi = a.T;  // first entry whose key is at least v
     while (lo < hi) {
       const int64_t mid = (lo + hi) / 2;
@@ -441,42 +491,49 @@ __global__ void __launch_bounds__(256) fw_embed_part_kernel(EmbedGradArgs a, int
       else
         hi = mid;
     }
-    start[v] = (int32_t)lo;
+    const bool none = v < a.V && !(lo < a.T && a.sorted[lo].x == (uint32_t)v);
+    for (uint32_t empty = __ballot_sync(kFull, none) & 0xffu; empty != 0u; empty &= empty - 1u)
+      zero_row<T, ALIGNED>(static_cast<T*>(a.dw) + (v0 + __ffs(empty) - 1) * a.D, a.D, a.nslots, lane);
   }
 }
 
-// One warp per table row and slab of it.
+// Runs that cross chunks: one warp per chunk that such a run begins in and
+// slab of its row.
 template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) fw_embed_grad_kernel(EmbedGradArgs a) {
+__global__ void __launch_bounds__(256) fw_embed_join_kernel(EmbedGradArgs a) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
-  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32), work = a.V * a.nslabs;
+  const int64_t slabs = (a.nslots + 31) / 32, chunks = (a.T + kChunk - 1) / kChunk, work = chunks * slabs;
+  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
-    const int64_t v = i / a.nslabs;
-    const int slab = (int)(i - v * a.nslabs);
-    const int i0 = a.start[v], i1 = a.start[v + 1];
-    T* dst = static_cast<T*>(a.dw) + v * a.D;
-    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V - (ALIGNED ? 0 : dst_off(dst));
-    float acc[kSlab * V];
+    const int64_t c = i / slabs, slot = i % slabs * 32 + lane, b = c * kChunk;
+    if (b + kChunk >= a.T) continue;
+    const uint32_t key = a.sorted[b + kChunk - 1].x;
+    if (key >= (uint32_t)a.V || a.sorted[b + kChunk].x != key) continue;          // nothing goes on
+    if (a.sorted[b].x == key && b > 0 && a.sorted[b - 1].x == key) continue;  // it began earlier
+    int64_t end = c + 1;  // the last chunk of the run, found 32 chunks at a time
+    for (;;) {
+      const int64_t next = end + 1 + lane;  // does chunk `next` begin with the key?
+      const uint32_t more = __ballot_sync(kFull, next < chunks && a.sorted[next * kChunk].x == key);
+      end += more == kFull ? 32 : __ffs(~more) - 1;
+      if (more != kFull) break;
+    }
+    float acc[V];
 #pragma unroll
-    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
-    if (i0 < i1) {
-      const int c0 = i0 / kChunk, c1 = (i1 - 1) / kChunk;
-      if (c0 == c1) {
-        const uint32_t pos = i0 + lane < i1 ? a.sorted[i0 + lane].y : 0u;
-        add_rows<T, ALIGNED>(a, pos, i1 - i0, e0, acc);
-      } else {
-        for (int c = c0; c <= c1; ++c) {
-          const float* p = a.part + (2 * (int64_t)c + (c == c0 ? 1 : 0)) * a.pitch;
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+    if (slot < a.nslots) {
+#pragma unroll 8
+      for (int64_t q = c; q <= end; ++q) {
+        const float4* p = reinterpret_cast<const float4*>(a.part + (2 * q + (q == c ? 1 : 0)) * a.pitch + slot * V);
 #pragma unroll
-          for (int j = 0; j < kSlab * V; ++j) {
-            const int64_t e = e0 + (int64_t)(j / V) * 32 * V + j % V;
-            if (e >= 0 && e < a.D) acc[j] += p[e];
-          }
+        for (int j = 0; j < V / 4; ++j) {
+          const float4 x = p[j];
+          acc[4 * j] += x.x, acc[4 * j + 1] += x.y, acc[4 * j + 2] += x.z, acc[4 * j + 3] += x.w;
         }
       }
+      T* dst = static_cast<T*>(a.dw) + (int64_t)key * a.D;
+      store_sum<T, ALIGNED>(a, dst, slot_elem<T, ALIGNED>(dst, slot), acc);
     }
-    store_sum<T, ALIGNED>(a, dst, e0, acc);
   }
 }
 
@@ -494,23 +551,26 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
   }
   __syncthreads();
   const int lane = threadIdx.x & 31;
-  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32), work = a.V * a.nslabs;
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
-    const int64_t v = i / a.nslabs;
-    const int slab = (int)(i - v * a.nslabs);
+  const int64_t slabs = (a.nslots + 31) / 32;
+  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32), work = a.V * slabs;
+  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); w < work; w += nw) {
+    const int64_t v = w / slabs;
     T* dst = static_cast<T*>(a.dw) + v * a.D;
-    const int64_t e0 = (int64_t)(slab * kSlab * 32 + lane) * V - (ALIGNED ? 0 : dst_off(dst));
-    float acc[kSlab * V];
+    const int64_t e0 = slot_elem<T, ALIGNED>(dst, w % slabs * 32 + lane);
+    float acc[V];
 #pragma unroll
-    for (int j = 0; j < kSlab * V; ++j) acc[j] = 0.0f;
+    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
     for (int t0 = 0; t0 < n; t0 += 32) {
-      const uint32_t hit = __ballot_sync(kFull, key[t0 + lane] == (int32_t)v);
-      if (hit == 0u) continue;
-      uint32_t pos = 0u;  // lane i: the i-th hit
-      int at = 0;
-      for (uint32_t h = hit; h != 0u; h &= h - 1u, ++at)
-        if (lane == at) pos = (uint32_t)(t0 + __ffs(h) - 1);
-      add_rows<T, ALIGNED>(a, pos, at, e0, acc);
+      uint32_t hit = __ballot_sync(kFull, key[t0 + lane] == (int32_t)v);
+      if (e0 >= a.D) continue;
+#pragma unroll 4
+      for (; hit != 0u; hit &= hit - 1u) {
+        const T* row = static_cast<const T*>(a.g) + (int64_t)(t0 + __ffs(hit) - 1) * a.ldg;
+        float x[V];
+        unpack16<T>(ALIGNED ? ld_stream16(row + e0) : load_slot_shifted(row, e0, a.D), x);
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[j] += x[j];
+      }
     }
     store_sum<T, ALIGNED>(a, dst, e0, acc);
   }
@@ -519,7 +579,7 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
 struct EmbedPlan {
   int passes, bits;
   int64_t tiles, chunks, pitch;
-  int64_t hist_at, start_at, part_at, bytes;  // workspace: entries (two arrays), histograms, row starts, partial rows
+  int64_t hist_at, part_at, bytes;  // workspace: entries, histograms, partial rows
 };
 
 EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
@@ -530,12 +590,11 @@ EmbedPlan embed_plan(int64_t T, int64_t V, int64_t D) {
   p.bits = (total + p.passes - 1) / p.passes;
   p.tiles = (T + kSortTile - 1) / kSortTile;
   p.chunks = (T + kChunk - 1) / kChunk;
-  p.pitch = (D + 7) / 8 * 8;
+  p.pitch = (D + 7) / 8 * 8 + 8;  // whole slots at any alignment
   if (T <= kDirectTokens) return p;
   const bool one = T <= kClusterTokens;
   p.hist_at = ((one ? 1 : 2) * T * (int64_t)sizeof(uint2) + 255) / 256 * 256;
-  p.start_at = (p.hist_at + (one ? 0 : p.tiles * ((int64_t)4 << p.bits)) + 255) / 256 * 256;
-  p.part_at = (p.start_at + 4 * (V + 1) + 255) / 256 * 256;
+  p.part_at = (p.hist_at + (one ? 0 : p.tiles * ((int64_t)4 << p.bits)) + 255) / 256 * 256;
   p.bytes = p.part_at + 2 * p.chunks * p.pitch * 4;
   return p;
 }
@@ -551,41 +610,31 @@ unsigned warps_grid(int64_t warps) {
 }
 
 template <class T, bool ALIGNED>
-cudaError_t launch_embed_grad(EmbedGradArgs a, int64_t chunks, int32_t* start, cudaStream_t st) {
-  if (a.T <= kDirectTokens) {
-    fw_embed_direct_kernel<T, ALIGNED><<<warps_grid(a.V * a.nslabs), 256, 0, st>>>(a);
-    return cudaGetLastError();
-  }
-  a.part_blocks = (int)warps_grid(chunks * a.nslabs);
-  fw_embed_part_kernel<T, ALIGNED><<<a.part_blocks + warps_grid((a.V + 32) / 32), 256, 0, st>>>(a, start);
-  a.start = start;
-  fw_embed_grad_kernel<T, ALIGNED><<<warps_grid(a.V * a.nslabs), 256, 0, st>>>(a);
-  return cudaGetLastError();
-}
-
-template <class T>
-cudaError_t launch_embed_grad(const EmbedGradArgs& a, int64_t chunks, int32_t* start, cudaStream_t st) {
-  const int64_t es = sizeof(T);
-  const bool aligned = aligned16(a.g) && aligned16(a.dw) && a.ldg * es % 16 == 0 && a.D * es % 16 == 0;
-  return aligned ? launch_embed_grad<T, true>(a, chunks, start, st) : launch_embed_grad<T, false>(a, chunks, start, st);
-}
-
-cudaError_t sort_cluster(const SortArgs& s, int passes, cudaStream_t st) {
+cudaError_t sort_cluster(const SortArgs& s, int passes, const EmbedGradArgs& g, cudaStream_t st) {
   constexpr int kSmem = 2 * kClusterTile * (int)sizeof(uint2) + kClusterThreads / 32 * (kMaxBins + 2) * 2;
+  auto kernel = fw_sort_cluster_kernel<T, ALIGNED>;
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev >= kMaxDevices || !attr_set[dev].load(std::memory_order_acquire)) {
-    e = cudaFuncSetAttribute(fw_sort_cluster_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) attr_set[dev].store(true, std::memory_order_release);
   }
-  // as many CTAs as tiles ask for: a power of two, so that few tokens do not exchange with idle CTAs
+  // as many sorting CTAs as the tokens ask for, so that few do not exchange with idle ones
   int ctas = 1;
   while (ctas < kClusterCtas && (int64_t)ctas * (kClusterTile / 4) < s.T) ctas *= 2;
+  // zeroing: about 1 MB of rows per CTA, fewer where that leaves SMs without any
+  const int64_t row = g.D * (int64_t)sizeof(T), two = 2 * (int64_t)sm_count() - ctas;
+  int64_t rows = ((int64_t)1 << 20) / row;
+  if (rows > (s.V + two - 1) / two) rows = (s.V + two - 1) / two;
+  rows = rows < 1 ? 1 : rows > kZeroRows ? kZeroRows : rows;
+  int64_t zero = (s.V + rows - 1) / rows;
+  if (zero > 65536) zero = 65536;
+  const ZeroArgs z = {g.dw, g.D, g.nslots, (int)rows};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
+  cfg.gridDim = dim3((unsigned)(ctas + (zero + ctas - 1) / ctas * ctas));
   cfg.blockDim = dim3(kClusterThreads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
@@ -596,7 +645,45 @@ cudaError_t sort_cluster(const SortArgs& s, int passes, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, fw_sort_cluster_kernel, s, passes);
+  return cudaLaunchKernelEx(&cfg, kernel, s, passes, z);
+}
+
+template <class T, bool ALIGNED>
+cudaError_t launch_embed_grad(EmbedGradArgs a, SortArgs s, const EmbedPlan& p, uint2* other, cudaStream_t st) {
+  const int64_t slabs = (a.nslots + 31) / 32;
+  if (a.T <= kDirectTokens) {
+    fw_embed_direct_kernel<T, ALIGNED><<<warps_grid(a.V * slabs), 256, 0, st>>>(a);
+    return cudaGetLastError();
+  }
+  a.sorted = s.dst;
+  unsigned zero = 0;
+  if (a.T <= kClusterTokens) {
+    const cudaError_t e = sort_cluster<T, ALIGNED>(s, p.passes, a, st);
+    if (e != cudaSuccess) return e;
+  } else {
+    uint2* ent[2] = {s.dst, other};
+    for (int i = 0; i < p.passes; ++i) {
+      s.src = i == 0 ? nullptr : ent[(i - 1) & 1];
+      s.dst = ent[i & 1];
+      s.shift = i * p.bits;
+      fw_sort_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
+      fw_sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
+    }
+    a.sorted = ent[(p.passes - 1) & 1];
+    zero = warps_grid((a.V + 7) / 8);
+  }
+  a.sum_blocks = (int)warps_grid(p.chunks * slabs);
+  fw_embed_sum_kernel<T, ALIGNED><<<a.sum_blocks + zero, 256, 0, st>>>(a);
+  fw_embed_join_kernel<T, ALIGNED><<<warps_grid(p.chunks * slabs), 256, 0, st>>>(a);
+  return cudaGetLastError();
+}
+
+template <class T>
+cudaError_t launch_embed_grad(const EmbedGradArgs& a, const SortArgs& s, const EmbedPlan& p, uint2* other,
+                              cudaStream_t st) {
+  const int64_t es = sizeof(T);
+  const bool aligned = aligned16(a.g) && aligned16(a.dw) && a.ldg * es % 16 == 0 && a.D * es % 16 == 0;
+  return aligned ? launch_embed_grad<T, true>(a, s, p, other, st) : launch_embed_grad<T, false>(a, s, p, other, st);
 }
 
 }  // namespace
@@ -645,34 +732,17 @@ int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, in
     return FWB_E_POINTER;
   if (workspace_bytes < p.bytes) return FWB_E_CAPACITY;
   char* ws = static_cast<char*>(workspace);
+  SortArgs s = {};
+  s.ids = ids;
+  s.dst = reinterpret_cast<uint2*>(ws);
+  s.hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
+  s.T = T;
+  s.V = V;
+  s.padding = padding;
+  s.bits = p.bits;
+  s.tiles = (int)p.tiles;
+  s.status = status;
   EmbedGradArgs a = {};
-  if (T > kDirectTokens) {
-    uint2* ent[2] = {reinterpret_cast<uint2*>(ws), reinterpret_cast<uint2*>(ws) + T};
-    SortArgs s = {};
-    s.ids = ids;
-    s.hist = reinterpret_cast<uint32_t*>(ws + p.hist_at);
-    s.T = T;
-    s.V = V;
-    s.padding = padding;
-    s.bits = p.bits;
-    s.tiles = (int)p.tiles;
-    s.status = status;
-    a.sorted = ent[0];
-    if (T <= kClusterTokens) {
-      s.dst = ent[0];
-      if (sort_cluster(s, p.passes, st) != cudaSuccess) return FWB_E_LAUNCH;
-    } else {
-      for (int i = 0; i < p.passes; ++i) {
-        s.src = i == 0 ? nullptr : ent[(i - 1) & 1];
-        s.dst = ent[i & 1];
-        s.shift = i * p.bits;
-        fw_sort_hist_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
-        fw_sort_scatter_kernel<<<(unsigned)p.tiles, kSortThreads, 0, st>>>(s);
-      }
-      a.sorted = ent[(p.passes - 1) & 1];
-      if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
-    }
-  }
   a.ids = ids;
   a.g = grad;
   a.dw = dweight;
@@ -684,12 +754,12 @@ int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, in
   a.pitch = p.pitch;
   a.padding = padding;
   a.scale = scale;
-  a.nslabs = slabs_of(D, es);
+  a.nslots = slots_of(D, es);
   a.status = status;
-  int32_t* start = reinterpret_cast<int32_t*>(ws + p.start_at);
-  return launch_status(dtype == FWB_DTYPE_BF16  ? launch_embed_grad<__nv_bfloat16>(a, p.chunks, start, st)
-                       : dtype == FWB_DTYPE_F16 ? launch_embed_grad<__half>(a, p.chunks, start, st)
-                                                : launch_embed_grad<float>(a, p.chunks, start, st));
+  uint2* other = reinterpret_cast<uint2*>(ws) + T;  // second array of entries, more than kClusterTokens only
+  return launch_status(dtype == FWB_DTYPE_BF16  ? launch_embed_grad<__nv_bfloat16>(a, s, p, other, st)
+                       : dtype == FWB_DTYPE_F16 ? launch_embed_grad<__half>(a, s, p, other, st)
+                                                : launch_embed_grad<float>(a, s, p, other, st));
 }
 
 }  // extern "C"

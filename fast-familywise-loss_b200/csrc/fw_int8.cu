@@ -4,8 +4,8 @@
 // two fp32 multiplications and one rounding to the output's type.
 //
 // Two layouts of the same product:
-//   many tokens  tokens are the 128 rows of a tile, 256 weight rows its
-//                columns: bound by the tensor cores;
+//   many tokens  tokens are the 256 rows of a tile (two CTAs), 256 weight
+//                rows its columns: bound by the tensor cores;
 //   few tokens   weight rows are the 128 rows of a tile and the tokens its
 //                16 .. 128 columns: every weight is read once, bound by HBM,
 //                so the small B tile leaves the shared memory to more stages.
@@ -20,45 +20,46 @@ struct Int8Args {
   void* out;
   int64_t ldo;
   int T, N, K;
+  int vec;  // rows of out start on 16-byte boundaries
   int32_t* status;
 };
+
+struct NoState {};
 
 template <class TO>
 struct Int8Many {
   using Args = Int8Args;
+  using State = NoState;
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int BN = 256, STAGES = 4;
-  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
-  __device__ static int tiles(const Args& a) { return ((a.T + 127) / 128) * ((a.N + 255) / 256); }
+  static constexpr int CG = 2, BN = 256, STAGES = 6, KC = 0, EW = 8;
+  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
+  __device__ static int tiles(const Args& a) { return ((a.T + 255) / 256) * ((a.N + 255) / 256); }
   __device__ static TcTile tile(const Args& a, int w) {
-    const int mt = (a.T + 127) / 128, nt = (a.N + 255) / 256;
+    const int mt = (a.T + 255) / 256, nt = (a.N + 255) / 256;
     constexpr int kGroup = 16;  // token blocks that share the weight tiles in flight
     const int g = w / (kGroup * nt), r = w - g * kGroup * nt;
     const int gm = min(kGroup, mt - g * kGroup);
-    return {(g * kGroup + r % gm) * 128, (r / gm) * 256, 0, 0, (a.K + 127) / 128};
+    return {(g * kGroup + r % gm) * 256, (r / gm) * 256, 0, 0, (a.K + 127) / 128};
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
-                                  Done done) {
-    float* sm = reinterpret_cast<float*>(smem);
-    const int r0 = t.m0 + quad * 32;
-    const float qs = r0 + lane < a.T ? a.qs[r0 + lane] : 0.0f;
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+    float* sm = reinterpret_cast<float*>(p.smem);
+    const int r0 = t.m0 + p.row;
+    const float qs = r0 + p.lane < a.T ? a.qs[r0 + p.lane] : 0.0f;
     TO* out = static_cast<TO*>(a.out);
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
+      const int n0 = t.n0 + c;
+      const float ws = n0 + p.lane < a.N ? a.ws[n0 + p.lane] : 0.0f;
       float v[32];
-      tmem_ld32(acc + c, v);
-      if (c + 32 == BN) done();
+      tmem_ld32(p.taddr + c, v);
+      if (c + 32 == (p.share + 1) * (BN / 2)) done();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = (float)__float_as_int(v[i]) * qs;
-      __syncwarp();
-      const int n = t.n0 + c + lane;
-      if (n < a.N) {
-        const float ws = a.ws[n];
-        const int rows = min(32, a.T - r0);
-        for (int i = 0; i < rows; ++i) st_elem(out + (int64_t)(r0 + i) * a.ldo + n, sm[i * 33 + lane] * ws);
-      }
-      __syncwarp();
+      for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * qs * __shfl_sync(kFull, ws, i);
+      const int rows = a.T - r0;
+      store_block<TO>(sm, v, p.lane, a.N - n0, a.vec, [&](int i) -> TO* {
+        return i < rows ? out + (int64_t)(r0 + i) * a.ldo + n0 : nullptr;
+      });
     }
   }
 };
@@ -66,26 +67,26 @@ struct Int8Many {
 template <class TO, int NT>
 struct Int8Few {
   using Args = Int8Args;
+  using State = NoState;
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int BN = NT;
+  static constexpr int CG = 1, BN = NT, KC = 0, EW = 4;
   static constexpr int STAGES = NT <= 32 ? 10 : NT <= 64 ? 8 : 6;
   static constexpr uint32_t EPI_BYTES = 0;
   __device__ static int tiles(const Args& a) { return (a.N + 127) / 128; }
   __device__ static TcTile tile(const Args& a, int w) { return {w * 128, 0, 0, 0, (a.K + 127) / 128}; }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
-                                  Done done) {
-    const int n = t.m0 + quad * 32 + lane;
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+    const int n = t.m0 + p.row + p.lane;
     const float ws = n < a.N ? a.ws[n] : 0.0f;
     TO* out = static_cast<TO*>(a.out);
     constexpr int STEP = NT < 32 ? 16 : 32;
     for (int c = 0; c < NT; c += STEP) {
       float v[STEP];
       if constexpr (STEP == 32)
-        tmem_ld32(acc + c, v);
+        tmem_ld32(p.taddr + c, v);
       else
-        tmem_ld16(acc + c, v);
+        tmem_ld16(p.taddr + c, v);
       if (c + STEP == NT) done();
       if (n >= a.N) continue;
 #pragma unroll
@@ -101,7 +102,7 @@ template <class P>
 cudaError_t run_int8(const void* a, int64_t rows_a, int64_t lda, const void* b, int64_t rows_b, int64_t ldb,
                      const Int8Args& args, int64_t tiles, cudaStream_t st) {
   CUtensorMap ma, mb;
-  if (!tc_map(&ma, kTcS8, a, rows_a, args.K, lda, kGemmBM) || !tc_map(&mb, kTcS8, b, rows_b, args.K, ldb, P::BN))
+  if (!tc_map(&ma, kTcS8, a, rows_a, args.K, lda, kGemmBM) || !tc_map(&mb, kTcS8, b, rows_b, args.K, ldb, P::BN / P::CG))
     return cudaErrorInvalidValue;
   return launch_gemm<P>(ma, mb, args, tiles, st);
 }
@@ -114,7 +115,7 @@ cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64
   if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 128) return run_int8<Int8Few<TO, 128>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  const int64_t tiles = (((int64_t)a.T + 127) / 128) * (((int64_t)a.N + 255) / 256);
+  const int64_t tiles = (((int64_t)a.T + 255) / 256) * (((int64_t)a.N + 255) / 256);
   return run_int8<Int8Many<TO>>(q, a.T, ldq, w, a.N, ldw, a, tiles, st);
 }
 
@@ -138,7 +139,9 @@ int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const float* q_s
   if (!q || !q_scale || !wq || !w_scale || !out) return FWB_E_POINTER;
   if (!aligned16(q) || !aligned16(wq)) return FWB_E_POINTER;
   if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FWB_DTYPE_F32 ? 4 : 2)) return FWB_E_POINTER;
-  const Int8Args a = {q_scale, w_scale, out, ldo, (int)T, (int)N, (int)K, status};
+  const int64_t es = out_dtype == FWB_DTYPE_F32 ? 4 : 2;
+  const int vec = aligned16(out) && ldo * es % 16 == 0 && N * es % 16 == 0;
+  const Int8Args a = {q_scale, w_scale, out, ldo, (int)T, (int)N, (int)K, vec, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (out_dtype == FWB_DTYPE_BF16) return launch_status(run_int8_linear<__nv_bfloat16>(q, ldq, wq, ldw, a, st));
   if (out_dtype == FWB_DTYPE_F16) return launch_status(run_int8_linear<__half>(q, ldq, wq, ldw, a, st));

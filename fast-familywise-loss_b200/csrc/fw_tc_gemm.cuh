@@ -2,20 +2,32 @@
 // uses it: the loop shared by the cross-entropy kernels and the 8-bit output
 // layer.
 //
-// One CTA per SM (persistent), 6 warps, as in the fused LM-head kernel:
-//   warp 0       TMA producer, kGemmStages stages of a 128 x 128-byte A tile
-//                and a BN x 128-byte B tile (128-byte swizzle);
-//   warp 1       TMEM allocation, MMA issuer: four tcgen05.mma (32 bytes of
-//                K each) per stage into one of two BN-column accumulators;
-//   warps 2..5   epilogue, one accumulator row per thread.
+// A tile is 128 * CG rows by BN columns, made by CG = 1 or 2 CTAs.  With 2 (a
+// cluster, one CTA per SM of a pair) each CTA loads its 128 rows of A and half
+// of the rows of B, one tcgen05.mma.cta_group::2 reads both halves, and each
+// CTA keeps its own 128 rows of the accumulator: per product step an SM reads
+// 32 KB of shared memory instead of 48 KB, which is what bounds a 128 x 256
+// tile of 8-bit operands (188 of the 128 bytes per clock it could read) and
+// costs power with 16-bit ones.
+//
+// Persistent CTAs of 2 + EW warps:
+//   warp 0       TMA producer, STAGES stages of 128 bytes of K (128-byte
+//                swizzle);
+//   warp 1       TMEM allocation; in the first CTA of a pair the MMA issuer:
+//                four tcgen05.mma (32 bytes of K each) per stage into one of
+//                two BN-column accumulators;
+//   the others   epilogue, one accumulator row per thread, the columns split
+//                over EW / 4 warps.
 // The two accumulators let the epilogue of a tile run under the next tile's
-// products.  An operand is either K-major (its rows run along K, 128 bytes of
-// K per stage) or MN-major (its rows run along M or N; the stage then holds
-// 64 rows of K of as many 64-element column groups as the tile needs).
+// products.  An operator may take the accumulator over every KC stages of K
+// (a tile's parts, added by its epilogue in fp32 registers).  An operand is
+// either K-major (its rows run along K) or MN-major (its rows run along M or
+// N; a stage then holds 64 rows of K of as many 64-element column groups as
+// the tile needs).
 //
 // Every wait is bounded; on a timeout all roles leave their loops, the copies
 // and products in flight are waited for (bounded) and TMEM is released, as in
-// the fused LM-head kernel.
+// the fused LM-head kernel; the CTAs of a pair leave together.
 #pragma once
 
 #include "fw_host.cuh"
@@ -24,19 +36,18 @@
 namespace fwb200 {
 namespace {
 
-constexpr int kGemmBM = 128;
+constexpr int kGemmBM = 128;        // accumulator rows per CTA
 constexpr int kGemmRowBytes = 128;  // bytes of K per stage (K-major) = one swizzle row
-constexpr int kGemmThreads = 192;
 constexpr uint32_t kGemmABytes = kGemmBM * kGemmRowBytes;
 
 enum TcKind { kTcBf16, kTcF16, kTcS8 };
 
-__host__ __device__ constexpr uint32_t gemm_idesc(TcKind kind, bool a_mn, bool b_mn, int bn) {
+__host__ __device__ constexpr uint32_t gemm_idesc(TcKind kind, bool a_mn, bool b_mn, int m, int n) {
   // accumulator: fp32 (1) or s32 (2); operands: f16 0, bf16 1 / u8 0, s8 1
   const uint32_t d = kind == kTcS8 ? 2u : 1u;
   const uint32_t ab = kind == kTcF16 ? 0u : 1u;
   return (d << 4) | (ab << 7) | (ab << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) |
-         ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kGemmBM >> 4) << 24);
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // MN-major operand in the 128-byte swizzle: 64 elements of M or N by 8 of K
@@ -47,17 +58,78 @@ __device__ __forceinline__ uint64_t umma_desc_mn(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-template <bool I8>
+template <int CG, bool I8>
 __device__ __forceinline__ void umma_issue(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                            uint32_t accumulate) {
-  if constexpr (I8)
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+#define FWB_MMA(group, kind)                                                       \
+  asm volatile(                                                                    \
+      "{\n\t.reg .pred p;\n\t"                                                     \
+      "setp.ne.b32 p, %4, 0;\n\t"                                                  \
+      "tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d), \
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate))
+  if constexpr (CG == 2 && I8)
+    FWB_MMA("2", "i8");
+  else if constexpr (CG == 2)
+    FWB_MMA("2", "f16");
+  else if constexpr (I8)
+    FWB_MMA("1", "i8");
   else
-    umma_bf16(tmem_d, adesc, bdesc, idesc, accumulate);
+    FWB_MMA("1", "f16");
+#undef FWB_MMA
+}
+
+// Arrives, once the products issued so far are complete, on the barrier at
+// this offset in every CTA of the group.
+template <int CG>
+__device__ __forceinline__ void umma_commit_group(uint64_t* bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+  else
+    umma_commit(bar);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Address, in the cluster's window, of `p`'s place in CTA `rank`.
+__device__ __forceinline__ uint32_t in_cta(const void* p, uint32_t rank) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  return a;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+// Tile load into this CTA that counts on a barrier given by its address in
+// the cluster's window (the pair's first CTA holds it).
+template <int CG>
+__device__ __forceinline__ void tma_load_group(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_arrive_at(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
 
 // Where a tile is and how many stages of K it has.
@@ -67,45 +139,62 @@ struct TcTile {
   int nk;      // stages of K (0: the accumulator is not written)
 };
 
-// P is the operator: static members KIND, A_MN, B_MN, BN, STAGES, smem for its epilogue
-// (EPI_BYTES), and
-//   tiles(args)              number of tiles (read from device memory where
-//                            it depends on data)
-//   tile(args, w)            tile w
-//   epilogue(args, tile, acc_addr, quad, lane, has, smem, done)
-// `done()` hands the accumulator back once its last column has been read.
+// What an epilogue warp works on: 32 rows of the accumulator from row r0 of
+// the tile, and a share of its columns.
+struct TcPart {
+  uint32_t taddr;  // TMEM address of the warp's rows, column 0
+  int row;         // first row of the warp in the tile
+  int lane;
+  int share;       // which share of the columns
+  uint8_t* smem;   // EPI_BYTES / EW of scratch
+};
+
+// P is the operator: static members CG, KIND, A_MN, B_MN, BN, STAGES, KC (0:
+// all of K at once), EW, EPI_BYTES, and
+//   tiles(args)      number of tiles (read from device memory where it
+//                    depends on data)
+//   tile(args, w)    tile w
+//   struct State     what an epilogue thread keeps over a tile's parts
+//   epilogue(args, tile, part, state, k, parts, done): part k of the
+//                    tile's `parts`; done() hands the accumulator back once
+//                    its last column has been read.
 template <class P>
 struct GemmSmem {
-  static constexpr uint32_t kBBytes = P::BN * kGemmRowBytes;
+  static constexpr uint32_t kBRows = P::BN / P::CG;
+  static constexpr uint32_t kBBytes = kBRows * kGemmRowBytes;
   static constexpr uint32_t kStage = kGemmABytes + kBBytes;
   static constexpr uint32_t kBytes = 1024 + P::STAGES * kStage + P::EPI_BYTES + 256;
+  static constexpr int kThreads = 64 + 32 * P::EW;
+  static_assert(kBytes <= 232448, "shared memory of one CTA");
 };
 
 template <class P>
-__global__ void __launch_bounds__(kGemmThreads, 1)
+__global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     fw_tc_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                       const __grid_constant__ typename P::Args a) {
-  constexpr int S = P::STAGES;
+  constexpr int S = P::STAGES, CG = P::CG;
   constexpr uint32_t kBBytes = GemmSmem<P>::kBBytes;
   constexpr bool kI8 = P::KIND == kTcS8;
   constexpr uint32_t kTmemCols = 2 * P::BN < 32 ? 32 : 2 * P::BN;
-  constexpr uint32_t kIdesc = gemm_idesc(P::KIND, P::A_MN, P::B_MN, P::BN);
+  constexpr uint32_t kIdesc = gemm_idesc(P::KIND, P::A_MN, P::B_MN, kGemmBM * CG, P::BN);
+  constexpr int kStep = kI8 ? 128 : 64;  // elements of K per stage
   extern __shared__ uint8_t gemm_smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* smA = base;
   uint8_t* smB = base + S * kGemmABytes;
   uint8_t* smE = smB + S * kBBytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smE + P::EPI_BYTES);
-  uint64_t* full = bars;           // [S] TMA -> MMA
-  uint64_t* empty = bars + S;      // [S] MMA -> TMA
-  uint64_t* tfull = bars + 2 * S;  // [2] MMA -> epilogue
-  uint64_t* tempty = tfull + 2;    // [2] epilogue -> MMA
+  uint64_t* full = bars;           // [S] TMA -> MMA, in the first CTA, for both
+  uint64_t* empty = bars + S;      // [S] MMA -> TMA, in each CTA
+  uint64_t* tfull = bars + 2 * S;  // [2] MMA -> epilogue, in each CTA
+  uint64_t* tempty = tfull + 2;    // [2] epilogue -> MMA, in the first CTA, from both
   uint64_t* drain = tempty + 2;    // abort path
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int rank = CG == 2 ? (int)cluster_rank() : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -113,7 +202,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&tfull[i], 1);
-      mbar_init(&tempty[i], 4 * 32);
+      mbar_init(&tempty[i], P::EW * CG);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -121,42 +210,51 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(kTmemCols));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (CG == 2) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(kTmemCols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                   "r"(kTmemCols));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
   }
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // the pair's barriers exist
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
   const int ntiles = P::tiles(a);
+  const int w0 = (int)blockIdx.x / CG, wstep = (int)gridDim.x / CG;
   uint32_t issued = 0u, issued_par = 0u;  // stages with a copy issued, and its parity
   bool mma_any = false;
 
   if (warp == 0) {
     uint32_t s = 0, ph = 0;
-    for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
+    for (int w = w0; w < ntiles; w += wstep) {
       const TcTile t = P::tile(a, w);
+      const int m = t.m0 + rank * kGemmBM, n = t.n0 + rank * (P::BN / CG);
       for (int kb = 0; kb < t.nk; ++kb) {
         if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status)) goto done;
         if (lane == 0) {
-          mbar_expect_tx(&full[s], kGemmABytes + kBBytes);
-          constexpr int kStep = kI8 ? 128 : 64;  // elements of K per stage
+          if (rank == 0) mbar_expect_tx(&full[s], CG * (kGemmABytes + kBBytes));
+          const uint32_t bar = CG == 2 ? in_cta(&full[s], 0) : smem_u32(&full[s]);
           const int ka = t.ak + kb * kStep, kbb = t.bk + kb * kStep;
           if constexpr (P::A_MN) {
 #pragma unroll
             for (int i = 0; i < kGemmBM / 64; ++i)
-              tma_load_2d(smA + s * kGemmABytes + i * 8192, &tm_a, t.m0 + 64 * i, ka, &full[s]);
+              tma_load_group<CG>(smA + s * kGemmABytes + i * 8192, &tm_a, m + 64 * i, ka, bar);
           } else {
-            tma_load_2d(smA + s * kGemmABytes, &tm_a, ka, t.m0, &full[s]);
+            tma_load_group<CG>(smA + s * kGemmABytes, &tm_a, ka, m, bar);
           }
           if constexpr (P::B_MN) {
 #pragma unroll
-            for (int i = 0; i < P::BN / 64; ++i)
-              tma_load_2d(smB + s * kBBytes + i * 8192, &tm_b, t.n0 + 64 * i, kbb, &full[s]);
+            for (int i = 0; i < P::BN / CG / 64; ++i)
+              tma_load_group<CG>(smB + s * kBBytes + i * 8192, &tm_b, n + 64 * i, kbb, bar);
           } else {
-            tma_load_2d(smB + s * kBBytes, &tm_b, kbb, t.n0, &full[s]);
+            tma_load_group<CG>(smB + s * kBBytes, &tm_b, kbb, n, bar);
           }
         }
         issued |= 1u << s;
@@ -170,57 +268,72 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     }
   } else if (warp == 1) {
     uint32_t s = 0, ph = 0, acc = 0, aph = 0;
-    for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
-      const TcTile t = P::tile(a, w);
-      if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status)) goto done;
-      tc_fence_after();
-      const uint32_t d = tmem + acc * P::BN;
-      for (int kb = 0; kb < t.nk; ++kb) {
-        if (!mbar_wait(&full[s], ph, abort_flag, a.status)) goto done;
-        tc_fence_after();
-        if (lane == 0) {
-          const uint32_t sa = smem_u32(smA + s * kGemmABytes);
-          const uint32_t sb = smem_u32(smB + s * kBBytes);
+    if (rank == 0) {
+      for (int w = w0; w < ntiles; w += wstep) {
+        const TcTile t = P::tile(a, w);
+        const int kc = P::KC == 0 ? max(t.nk, 1) : P::KC;
+        for (int k0 = 0; k0 < max(t.nk, 1); k0 += kc) {
+          if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status)) goto done;
+          tc_fence_after();
+          const uint32_t d = tmem + acc * P::BN;
+          for (int kb = k0; kb < min(k0 + kc, t.nk); ++kb) {
+            if (!mbar_wait(&full[s], ph, abort_flag, a.status)) goto done;
+            tc_fence_after();
+            if (lane == 0) {
+              const uint32_t sa = smem_u32(smA + s * kGemmABytes);
+              const uint32_t sb = smem_u32(smB + s * kBBytes);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            // 16 rows of K (MN-major) or 32 bytes of K (K-major) further on
-            const uint64_t da = P::A_MN ? umma_desc_mn(sa + 2048 * k) : umma_desc_sw128(sa + 32 * k);
-            const uint64_t db = P::B_MN ? umma_desc_mn(sb + 2048 * k) : umma_desc_sw128(sb + 32 * k);
-            umma_issue<kI8>(d, da, db, kIdesc, (kb | k) != 0 ? 1u : 0u);
+              for (int k = 0; k < 4; ++k) {
+                // 16 rows of K (MN-major) or 32 bytes of K (K-major) further on
+                const uint64_t da = P::A_MN ? umma_desc_mn(sa + 2048 * k) : umma_desc_sw128(sa + 32 * k);
+                const uint64_t db = P::B_MN ? umma_desc_mn(sb + 2048 * k) : umma_desc_sw128(sb + 32 * k);
+                umma_issue<CG, kI8>(d, da, db, kIdesc, (kb != k0 || k != 0) ? 1u : 0u);
+              }
+              umma_commit_group<CG>(&empty[s]);
+            }
+            mma_any = true;
+            __syncwarp();
+            if (++s == S) {
+              s = 0;
+              ph ^= 1u;
+            }
           }
-          umma_commit(&empty[s]);
+          if (lane == 0) umma_commit_group<CG>(&tfull[acc]);
+          mma_any = true;
+          __syncwarp();
+          if (++acc == 2) {
+            acc = 0;
+            aph ^= 1u;
+          }
         }
-        mma_any = true;
-        __syncwarp();
-        if (++s == S) {
-          s = 0;
-          ph ^= 1u;
-        }
-      }
-      if (lane == 0) umma_commit(&tfull[acc]);
-      mma_any = true;
-      __syncwarp();
-      if (++acc == 2) {
-        acc = 0;
-        aph ^= 1u;
       }
     }
   } else {
     const int quad = warp & 3;  // TMEM lanes this warp may read
     uint32_t acc = 0, aph = 0;
-    for (int w = blockIdx.x; w < ntiles; w += gridDim.x) {
+    TcPart part;
+    part.row = rank * kGemmBM + quad * 32;
+    part.lane = lane;
+    part.share = (warp - 2) >> 2;
+    part.smem = smE + (warp - 2) * (P::EPI_BYTES / P::EW);
+    for (int w = w0; w < ntiles; w += wstep) {
       const TcTile t = P::tile(a, w);
-      if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
-      tc_fence_after();
-      const uint32_t addr = tmem + (uint32_t)((quad * 32) << 16) + acc * P::BN;
-      uint64_t* te = &tempty[acc];
-      P::epilogue(a, t, addr, quad, lane, smE + (warp - 2) * (P::EPI_BYTES / 4), [te] {
-        tc_fence_before();
-        mbar_arrive(te);
-      });
-      if (++acc == 2) {
-        acc = 0;
-        aph ^= 1u;
+      const int parts = P::KC == 0 ? 1 : max((t.nk + P::KC - 1) / (P::KC == 0 ? 1 : P::KC), 1);
+      typename P::State state;
+      for (int k = 0; k < parts; ++k) {
+        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
+        tc_fence_after();
+        part.taddr = tmem + (uint32_t)((quad * 32) << 16) + acc * P::BN;
+        const uint32_t te = CG == 2 ? in_cta(&tempty[acc], 0) : smem_u32(&tempty[acc]);
+        P::epilogue(a, t, part, state, k, parts, [te, lane] {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_at(te);
+        });
+        if (++acc == 2) {
+          acc = 0;
+          aph ^= 1u;
+        }
       }
     }
   }
@@ -228,20 +341,61 @@ done:
   __syncwarp();
   if (*abort_flag && lane == 0) {
     if (warp == 0) {
-      for (int st = 0; st < S; ++st)
-        if (issued & (1u << st)) mbar_drain(&full[st], (issued_par >> st) & 1u);
+      if (rank == 0)
+        for (int st = 0; st < S; ++st)
+          if (issued & (1u << st)) mbar_drain(&full[st], (issued_par >> st) & 1u);
+      // the pair's other copies count on the first CTA's barriers: time for them to land
+      const uint64_t t0 = global_ns();
+      for (int i = 0; i < (1 << 20) && global_ns() - t0 < 1000000ull; ++i) {
+      }
     } else if (warp == 1 && mma_any) {
-      umma_commit(drain);
+      umma_commit_group<CG>(drain);
       mbar_drain(drain, 0u);
     }
   }
   __syncwarp();
   tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) cluster_sync();  // nobody reads or signals the other's shared memory any more
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    if constexpr (CG == 2)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }
+}
+
+// The warp's 32 x 32 block of values, one row per thread, turned through
+// shared memory and stored as rows of T: 16 bytes per lane where the rows are
+// aligned (`vec`), else one element per lane.  row_ptr(i) is where column 0 of
+// the block's row i goes, or NULL.
+template <class T, class RowPtr>
+__device__ __forceinline__ void store_block(float* sm, const float (&v)[32], int lane, int cols, bool vec,
+                                            RowPtr row_ptr) {
+  constexpr int V = 16 / sizeof(T), LANES = 32 / V, ROWS = 32 / LANES;  // lanes per row, rows per step
+#pragma unroll
+  for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
+  __syncwarp();
+  if (vec) {
+    const int c = (lane % LANES) * V;
+#pragma unroll
+    for (int i0 = 0; i0 < 32; i0 += ROWS) {
+      const int i = i0 + lane / LANES;
+      T* p = row_ptr(i);
+      float x[V];
+#pragma unroll
+      for (int j = 0; j < V; ++j) x[j] = sm[i * 33 + c + j];
+      if (p && c < cols) *reinterpret_cast<uint4*>(p + c) = pack16<T>(x);  // cols is a multiple of V
+    }
+  } else {
+#pragma unroll 4
+    for (int i = 0; i < 32; ++i) {
+      T* p = row_ptr(i);
+      if (p && lane < cols) st_elem(p + lane, sm[i * 33 + lane]);
+    }
+  }
+  __syncwarp();
 }
 
 // ------------------------------------------------------------------- host
@@ -298,12 +452,21 @@ cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const type
     if (e != cudaSuccess) return e;
     if (dev < kMaxDevices) attr_set[dev].store(true, std::memory_order_release);
   }
-  const int64_t sms = sm_count();
+  int64_t grid = max_tiles * P::CG;
+  const int64_t sms = sm_count() / P::CG * P::CG;
+  if (grid > sms) grid = sms;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(max_tiles < sms ? max_tiles : sms));
-  cfg.blockDim = dim3(kGemmThreads);
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(GemmSmem<P>::kThreads);
   cfg.dynamicSmemBytes = GemmSmem<P>::kBytes;
   cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = P::CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = P::CG > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, fw_tc_gemm_kernel<P>, ma, mb, a);
 }
 

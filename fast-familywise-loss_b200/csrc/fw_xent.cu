@@ -6,7 +6,7 @@
 //
 // Forward: live rows are packed (rows whose label is ignore_index take no
 // part in anything, whatever they hold), one tensor-core product gives each
-// 128 x 256 logit tile, whose epilogue keeps only each row's maximum and sum
+// 256 x 256 logit tile, whose epilogue keeps only each row's maximum and sum
 // of exponentials; a second kernel joins the tiles' pairs, takes the losses
 // and reduces them in a fixed order.
 // Backward, in pieces of the vocabulary: the logits of a piece again, their
@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
     a.head->done = 0u;
     a.head->status = 0;
   }
-  const int64_t rows_up = ((int64_t)total + 127) / 128 * 128;
+  const int64_t rows_up = ((int64_t)total + 255) / 256 * 256;
   for (int i0 = 0; i0 < a.per_cta; i0 += 32) {
     const int64_t rl = r0 + i0 + lane;
     const int64_t yl = rl < a.B ? a.y[rl] : a.ignore;
@@ -136,6 +136,12 @@ __global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_
   }
 }
 
+struct NoState {};
+
+constexpr int kTileM = 256, kTileN = 256;  // of a pair of CTAs
+
+__device__ __forceinline__ int row_tiles(const XentHead* h) { return (h->rows + kTileM - 1) / kTileM; }
+
 // Order of tiles: blocks of `group` m-blocks, m fastest inside one, so that
 // the tiles in flight share their operands in L2.
 __device__ __forceinline__ void tile_order(int w, int mt, int nt, int group, int* m, int* n) {
@@ -149,55 +155,64 @@ __device__ __forceinline__ void tile_order(int w, int mt, int nt, int group, int
 struct LseArgs {
   const XentHead* head;
   const int32_t* label;
-  float2* part;  // [tiles of V, Bp]: maximum, sum of exp(z - maximum)
+  float2* part;  // [half tiles of V, Bp]: maximum, sum of exp(z - maximum)
   float* zy;     // [Bp]
   int64_t Bp;
   int V, D;
   int32_t* status;
 };
 
+// The accumulator is taken over every kLseStages stages of K and added up in
+// registers: the tensor cores' fp32 additions round towards zero, so a logit
+// shrinks by a part that grows with the length of the sum.
+constexpr int kLseStages = 8;
+
 template <TcKind K>
 struct LseTile {
   using Args = LseArgs;
+  struct State {
+    float z[kTileN / 2];
+  };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int BN = 256, STAGES = 4;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = kLseStages, EW = 8;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * ((a.V + 255) / 256); }
+  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * ((a.V + BN - 1) / BN); }
   __device__ static TcTile tile(const Args& a, int w) {
     int m, n;
-    tile_order(w, (a.head->rows + 127) / 128, (a.V + 255) / 256, 32, &m, &n);
-    return {m * 128, n * 256, 0, 0, (a.D + 63) / 64};
+    tile_order(w, row_tiles(a.head), (a.V + BN - 1) / BN, 16, &m, &n);
+    return {m * kTileM, n * BN, 0, 0, (a.D + 63) / 64};
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State& st, int k, int parts,
                                   Done done) {
-    const int row = t.m0 + quad * 32 + lane;  // < Bp
-    const int y = a.label[row];
-    float m = -CUDART_INF_F, s = 0.0f;
-    for (int c = 0; c < BN; c += 32) {
-      const int valid = min(32, a.V - (t.n0 + c));
-      float v[32];
-      tmem_ld32(acc + c, v);
-      if (c + 32 == BN) done();
-      if (valid <= 0) continue;
-      float top = -CUDART_INF_F;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        if (i >= valid) v[i] = -CUDART_INF_F;
-        if (t.n0 + c + i == y) a.zy[row] = v[i];
-        top = max_nan(top, v[i]);
-      }
-      if (top > m || top != top) {  // the maximum moves, or is NaN
-        const float to = top;
-        s = m == -CUDART_INF_F ? s : s * exp2f((m - to) * kLog2e);
-        m = to;
-      }
-      if (m == -CUDART_INF_F) continue;  // nothing but -inf so far
+    for (int c = 0; c < BN / 2; c += 16) {
+      float v[16];
+      tmem_ld16(p.taddr + p.share * (BN / 2) + c, v);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) s += exp2f((v[i] - m) * kLog2e);
+      for (int i = 0; i < 16; ++i) st.z[c + i] = k == 0 ? v[i] : st.z[c + i] + v[i];
     }
-    a.part[(int64_t)(t.n0 / BN) * a.Bp + row] = make_float2(m, s);
+    done();
+    if (k < parts - 1) return;
+    const int row = t.m0 + p.row + p.lane;  // < Bp
+    const int n0 = t.n0 + p.share * (BN / 2);
+    const int y = a.label[row] - n0;
+    const int valid = a.V - n0;
+    float m = -CUDART_INF_F, s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < BN / 2; ++i) {
+      if (i >= valid) st.z[i] = -CUDART_INF_F;
+      if (i == y) a.zy[row] = st.z[i];
+      m = max_nan(m, st.z[i]);
+    }
+    if (m != -CUDART_INF_F) {  // a NaN maximum, or +inf, makes the sum NaN
+      float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int i = 0; i < BN / 2; ++i) s4[i & 3] += exp2f((st.z[i] - m) * kLog2e);
+      s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+    }
+    a.part[(int64_t)(n0 / (BN / 2)) * a.Bp + row] = make_float2(m, s);
   }
 };
 
@@ -329,35 +344,35 @@ struct GradArgs {
 template <class T, TcKind K>
 struct GradTile {
   using Args = GradArgs;
+  using State = NoState;
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int BN = 256, STAGES = 4;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = 0, EW = 8;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * (a.vn / 256); }
+  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * (a.vn / BN); }
   __device__ static TcTile tile(const Args& a, int w) {
     int m, n;
-    tile_order(w, (a.head->rows + 127) / 128, a.vn / 256, 32, &m, &n);
-    return {m * 128, a.v0 + n * 256, 0, 0, (a.D + 63) / 64};
+    tile_order(w, row_tiles(a.head), a.vn / BN, 16, &m, &n);
+    return {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64};
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t*,
-                                  Done done) {
-    const int row = t.m0 + quad * 32 + lane;
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+    const int row = t.m0 + p.row + p.lane;
     const bool live = row < a.head->rows;
     const int y = live ? a.label[row] : -1;
     const float lse = live ? a.lse[row] : 0.0f;
     const float coef = live ? a.coef[row] : 0.0f;
     T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
-      tmem_ld32(acc + c, v);
-      if (c + 32 == BN) done();
+      tmem_ld32(p.taddr + c, v);
+      if (c + 32 == (p.share + 1) * (BN / 2)) done();
       const int valid = live ? min(32, a.V - (t.n0 + c)) : 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float p = exp2f((v[i] - lse) * kLog2e);
-        if (t.n0 + c + i == y) p -= 1.0f;
-        v[i] = i < valid ? p * coef : 0.0f;
+        float q = exp2f((v[i] - lse) * kLog2e);
+        if (t.n0 + c + i == y) q -= 1.0f;
+        v[i] = i < valid ? q * coef : 0.0f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(g + c + 8 * i) = pack16<T>(v + 8 * i);
@@ -368,70 +383,66 @@ struct GradTile {
 struct DHiddenArgs {
   const XentHead* head;
   const int32_t* row_of;
-  float* sum;  // [Bp, D] when the vocabulary has several pieces
+  float* sum;  // [Bp, lds] where the vocabulary has several pieces, else NULL
   void* out;   // [B, D]
-  int D;
+  int D, lds;
+  int vec;  // rows of out start on 16-byte boundaries
   int v0, vn;
   int first, last;
   int32_t* status;
 };
 
-// The warp's 32 x 32 block of values, one row per thread, handed to f(row,
-// column, value) with the lanes along the columns.
-template <class F>
-__device__ __forceinline__ void by_columns(float* sm, const float (&v)[32], int lane, int rows, int cols, F f) {
-#pragma unroll
-  for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
-  __syncwarp();
-  if (lane < cols)
-    for (int i = 0; i < rows; ++i) f(i, lane, sm[i * 33 + lane]);
-  __syncwarp();
-}
-
 template <class T, TcKind K>
 struct DHiddenTile {
   using Args = DHiddenArgs;
+  using State = NoState;
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = true;
-  static constexpr int BN = 256, STAGES = 4;
-  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
-  __device__ static int tiles(const Args& a) { return ((a.head->rows + 127) / 128) * ((a.D + 255) / 256); }
+  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8;
+  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
+  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * ((a.D + BN - 1) / BN); }
   __device__ static TcTile tile(const Args& a, int w) {
     int m, n;
-    tile_order(w, (a.head->rows + 127) / 128, (a.D + 255) / 256, 12, &m, &n);
-    return {m * 128, n * 256, 0, a.v0, a.vn / 64};
+    tile_order(w, row_tiles(a.head), (a.D + BN - 1) / BN, 8, &m, &n);
+    return {m * kTileM, n * BN, 0, a.v0, a.vn / 64};
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
-                                  Done done) {
-    float* sm = reinterpret_cast<float*>(smem);
-    const int r0 = t.m0 + quad * 32;
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+    float* sm = reinterpret_cast<float*>(p.smem);
+    const int r0 = t.m0 + p.row;
     const int rows = min(32, a.head->rows - r0);
     const float back = a.head->back;
-    const int mine = lane < rows ? a.row_of[r0 + lane] : 0;
-    for (int c = 0; c < BN; c += 32) {
+    const int mine = p.lane < rows ? a.row_of[r0 + p.lane] : -1;
+    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
-      tmem_ld32(acc + c, v);
-      if (c + 32 == BN) done();
+      tmem_ld32(p.taddr + c, v);
+      if (c + 32 == (p.share + 1) * (BN / 2)) done();
       const int c0 = t.n0 + c;
       const int cols = min(32, a.D - c0);
       if (cols <= 0 || rows <= 0) continue;
+      if (a.sum) {  // several pieces: the rows of the sum so far are this thread's own
+        float* s = a.sum + (int64_t)(r0 + p.lane) * a.lds + c0;  // lds: D rounded up to 32
+        if (!a.first) {
 #pragma unroll
-      for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
-      __syncwarp();
-      for (int i = 0; i < rows; ++i) {
-        const int64_t to = __shfl_sync(kFull, mine, i);
-        if (lane < cols) {
-          float x = sm[i * 33 + lane];
-          const int64_t at = (int64_t)(r0 + i) * a.D + c0 + lane;
-          if (!a.first) x += a.sum[at];
-          if (a.last)
-            st_elem(static_cast<T*>(a.out) + to * a.D + c0 + lane, x * back);
-          else
-            a.sum[at] = x;
+          for (int i = 0; i < 32; i += 4) {
+            const float4 x = *reinterpret_cast<const float4*>(s + i);
+            v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
+          }
+        }
+        if (!a.last) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(s + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          continue;
         }
       }
-      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] *= back;
+      T* out = static_cast<T*>(a.out);
+      store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
+        const int r = __shfl_sync(kFull, mine, i);
+        return r >= 0 ? out + (int64_t)r * a.D + c0 : nullptr;
+      });
     }
   }
 };
@@ -441,43 +452,43 @@ struct DWeightArgs {
   void* out;  // [V, D]
   int V, D;
   int v0, vn;
+  int vec;  // rows of out start on 16-byte boundaries
   int32_t* status;
 };
 
 template <class T, TcKind K>
 struct DWeightTile {
   using Args = DWeightArgs;
+  using State = NoState;
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = true, B_MN = true;
-  static constexpr int BN = 256, STAGES = 4;
-  static constexpr uint32_t EPI_BYTES = 4 * 32 * 33 * 4;
-  __device__ static int mtiles(const Args& a) { return (min(a.vn, a.V - a.v0) + 127) / 128; }
-  __device__ static int tiles(const Args& a) { return mtiles(a) * ((a.D + 255) / 256); }
+  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8;
+  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
+  __device__ static int mtiles(const Args& a) { return (min(a.vn, a.V - a.v0) + kTileM - 1) / kTileM; }
+  __device__ static int tiles(const Args& a) { return mtiles(a) * ((a.D + BN - 1) / BN); }
   __device__ static TcTile tile(const Args& a, int w) {
     int m, n;
-    tile_order(w, mtiles(a), (a.D + 255) / 256, 8, &m, &n);
-    return {m * 128, n * 256, 0, 0, (a.head->rows + 63) / 64};
+    tile_order(w, mtiles(a), (a.D + BN - 1) / BN, 5, &m, &n);
+    return {m * kTileM, n * BN, 0, 0, (a.head->rows + 63) / 64};
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, uint32_t acc, int quad, int lane, uint8_t* smem,
-                                  Done done) {
-    float* sm = reinterpret_cast<float*>(smem);
-    const int r0 = a.v0 + t.m0 + quad * 32;
-    const int rows = min(32, a.V - r0);
+  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+    float* sm = reinterpret_cast<float*>(p.smem);
+    const int r0 = a.v0 + t.m0 + p.row;
+    const int rows = a.V - r0;
     const float back = a.head->back;
-    for (int c = 0; c < BN; c += 32) {
+    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
-      tmem_ld32(acc + c, v);
-      if (c + 32 == BN) done();
+      tmem_ld32(p.taddr + c, v);
+      if (c + 32 == (p.share + 1) * (BN / 2)) done();
       const int c0 = t.n0 + c;
       const int cols = min(32, a.D - c0);
       if (cols <= 0 || rows <= 0) continue;
-      if (t.nk == 0) {  // no live row: the accumulator was never written
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-      }
-      by_columns(sm, v, lane, rows, cols, [&](int i, int j, float x) {
-        st_elem(static_cast<T*>(a.out) + (int64_t)(r0 + i) * a.D + c0 + j, t.nk == 0 ? 0.0f : x * back);
+      for (int i = 0; i < 32; ++i) v[i] = t.nk == 0 ? 0.0f : v[i] * back;  // no live row: nothing was accumulated
+      T* out = static_cast<T*>(a.out);
+      store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
+        return i < rows ? out + (int64_t)(r0 + i) * a.D + c0 : nullptr;
       });
     }
   }
@@ -502,7 +513,7 @@ struct XentPlan {
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   XentPlan p = {};
-  p.Bp = up(B, 128);
+  p.Bp = up(B, 256);
   p.Dp = up(D, 8);
   p.copy_w = copy_w;
   int64_t at = 256;
@@ -513,7 +524,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.wp = at, at += copy_w ? up(2 * V * p.Dp, 256) : 0;
   p.state_bytes = at;
   at = 0;
-  p.part = at, at += up(8 * p.Bp * ((V + 255) / 256), 256);
+  p.part = at, at += up(8 * p.Bp * ((V + 127) / 128 + 1), 256);
   p.zy = at, at += up(4 * p.Bp, 256);
   p.loss_pack = at, at += up(4 * p.Bp, 256);
   p.fwd_bytes = at;
@@ -525,7 +536,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   at = 0;
   p.coef = at, at += up(4 * p.Bp, 256);
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
-  p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * D, 256) : 0;
+  p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * up(D, 32), 256) : 0;
   p.bwd_bytes = at;
   return p;
 }
@@ -533,7 +544,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
 int xent_check(int dtype, int64_t B, int64_t D, int64_t V) {
   if (dtype != FWB_DTYPE_BF16 && dtype != FWB_DTYPE_F16) return FWB_E_DTYPE;
   if (B < 0 || D < 1 || V < 1 || B > (1 << 26) || D > (1 << 20) || V > (1 << 28)) return FWB_E_SHAPE;
-  if ((up(B, 128) / 128) * (up(V, 256) / 256) > (1 << 30)) return FWB_E_SHAPE;
+  if ((up(B, 256) / 256) * (up(V, 256) / 256) > (1 << 30)) return FWB_E_SHAPE;
   return FWB_OK;
 }
 
@@ -561,13 +572,13 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   }
   if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
   CUtensorMap mh, mw;
-  if (!tc_map(&mh, K, state + p.hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 256)) return FWB_E_LAUNCH;
+  if (!tc_map(&mh, K, state + p.hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 128)) return FWB_E_LAUNCH;
   LseArgs la = {head, label, reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.zy), p.Bp, (int)V,
                 (int)D, &head->status};
   const int64_t nt = (V + 255) / 256;
-  if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 128) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
+  if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
   JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
-                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)nt, reduction, status};
+                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + 127) / 128), reduction, status};
   fw_xent_join_kernel<<<(unsigned)(p.Bp / 32), kJoinWarps * 32, 0, st>>>(ja);
   return launch_status(cudaGetLastError());
 }
@@ -590,24 +601,25 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   CUtensorMap mh, mw, mg, wmn, gmn, hmn;
   char* hp = state + p.hp;
   char* g = ws + p.g;
-  if (!tc_map(&mh, K, hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 256) ||
+  if (!tc_map(&mh, K, hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 128) ||
       !tc_map(&mg, K, g, p.Bp, p.piece, p.piece, 128) || !tc_map(&wmn, K, w, V, D, ldw, 64) ||
       !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hp, p.Bp, D, p.Dp, 64))
     return FWB_E_LAUNCH;
-  const int64_t Vp = up(V, 256), mb = p.Bp / 128, nd = (D + 255) / 256;
+  const int64_t Vp = up(V, 256), mb = p.Bp / 256, nd = (D + 255) / 256;
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
     const GradArgs ga = {head, label, reinterpret_cast<float*>(state + p.lse), coef, g, p.piece, (int)V, (int)D, v0,
                          vn, status};
     if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
     if (dhidden) {
-      const DHiddenArgs da = {head, row_of, reinterpret_cast<float*>(ws + p.sum), dhidden, (int)D, v0, vn, i == 0,
+      const DHiddenArgs da = {head, row_of, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr, dhidden,
+                              (int)D, (int)up(D, 32), aligned16(dhidden) && D % 8 == 0, v0, vn, i == 0,
                               i == p.pieces - 1, status};
       if (launch_gemm<DHiddenTile<T, K>>(mg, wmn, da, mb * nd, st) != cudaSuccess) return FWB_E_LAUNCH;
     }
     if (dweight) {
-      const DWeightArgs da = {head, dweight, (int)V, (int)D, v0, vn, status};
-      if (launch_gemm<DWeightTile<T, K>>(gmn, hmn, da, (int64_t)(vn / 128) * nd, st) != cudaSuccess)
+      const DWeightArgs da = {head, dweight, (int)V, (int)D, v0, vn, aligned16(dweight) && D % 8 == 0, status};
+      if (launch_gemm<DWeightTile<T, K>>(gmn, hmn, da, (int64_t)(vn / 256) * nd, st) != cudaSuccess)
         return FWB_E_LAUNCH;
     }
   }
