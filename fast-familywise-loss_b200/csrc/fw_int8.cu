@@ -7,8 +7,13 @@
 //   many tokens  tokens are the 256 rows of a tile (two CTAs), 256 weight
 //                rows its columns: bound by the tensor cores;
 //   few tokens   weight rows are the 128 rows of a tile and the tokens its
-//                16 .. 128 columns: every weight is read once, bound by HBM,
-//                so the small B tile leaves the shared memory to more stages.
+//                16 .. 128 columns: every weight is read once, bound by HBM.
+//                The weight rows are dealt out evenly over the SMs in steps of
+//                8 (whole tiles would leave up to half of them idle in the
+//                last round), tiles of fewer than 128 rows loading only the
+//                32-row boxes they need, and the first weights are brought
+//                into L2 while the kernel before (the norm that makes q) still
+//                runs.
 #include "fw_tc_gemm.cuh"
 
 namespace fwb200 {
@@ -21,6 +26,7 @@ struct Int8Args {
   int64_t ldo;
   int T, N, K;
   int vec;  // rows of out start on 16-byte boundaries
+  int per;  // few tokens: weight rows per CTA
   int32_t* status;
 };
 
@@ -32,15 +38,18 @@ struct Int8Many {
   using State = NoState;
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int CG = 2, BN = 256, STAGES = 6, KC = 0, EW = 8;
+  static constexpr bool TWO = false, A_MN2 = false;
+  static constexpr int CG = 2, BN = 256, STAGES = 6, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
-  __device__ static int tiles(const Args& a) { return ((a.T + 255) / 256) * ((a.N + 255) / 256); }
-  __device__ static TcTile tile(const Args& a, int w) {
+  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
     const int mt = (a.T + 255) / 256, nt = (a.N + 255) / 256;
+    const int w = tile_in_turn(group, groups, i, mt * nt);
+    if (w < 0) return false;
     constexpr int kGroup = 16;  // token blocks that share the weight tiles in flight
     const int g = w / (kGroup * nt), r = w - g * kGroup * nt;
     const int gm = min(kGroup, mt - g * kGroup);
-    return {(g * kGroup + r % gm) * 256, (r / gm) * 256, 0, 0, (a.K + 127) / 128};
+    *t = {(g * kGroup + r % gm) * 256, (r / gm) * 256, 0, 0, (a.K + 127) / 128, 128, 0};
+    return true;
   }
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
@@ -70,15 +79,21 @@ struct Int8Few {
   using State = NoState;
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int CG = 1, BN = NT, KC = 0, EW = 4;
+  static constexpr bool TWO = false, A_MN2 = false;
+  static constexpr int CG = 1, BN = NT, KC = 0, EW = 4, A_BOX = 32, AHEAD = 16;
   static constexpr int STAGES = NT <= 32 ? 10 : NT <= 64 ? 8 : 6;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static int tiles(const Args& a) { return (a.N + 127) / 128; }
-  __device__ static TcTile tile(const Args& a, int w) { return {w * 128, 0, 0, 0, (a.K + 127) / 128}; }
+  __device__ static bool get(const Args& a, int group, int, int i, TcTile* t) {
+    const int end = min(a.N, (group + 1) * a.per), m0 = group * a.per + i * 128;
+    if (m0 >= end) return false;
+    *t = {m0, 0, 0, 0, (a.K + 127) / 128, min(128, end - m0), 0};
+    return true;
+  }
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
     const int n = t.m0 + p.row + p.lane;
-    const float ws = n < a.N ? a.ws[n] : 0.0f;
+    const bool mine = p.row + p.lane < t.rows;
+    const float ws = mine ? a.ws[n] : 0.0f;
     TO* out = static_cast<TO*>(a.out);
     constexpr int STEP = NT < 32 ? 16 : 32;
     for (int c = 0; c < NT; c += STEP) {
@@ -88,7 +103,7 @@ struct Int8Few {
       else
         tmem_ld16(p.taddr + c, v);
       if (c + STEP == NT) done();
-      if (n >= a.N) continue;
+      if (!mine) continue;
 #pragma unroll
       for (int i = 0; i < STEP; ++i) {
         const int tok = c + i;
@@ -101,16 +116,18 @@ struct Int8Few {
 template <class P>
 cudaError_t run_int8(const void* a, int64_t rows_a, int64_t lda, const void* b, int64_t rows_b, int64_t ldb,
                      const Int8Args& args, int64_t tiles, cudaStream_t st) {
-  CUtensorMap ma, mb;
-  if (!tc_map(&ma, kTcS8, a, rows_a, args.K, lda, kGemmBM) || !tc_map(&mb, kTcS8, b, rows_b, args.K, ldb, P::BN / P::CG))
+  CUtensorMap ma, ma2, mb;
+  if (!tc_map(&ma, kTcS8, a, rows_a, args.K, lda, kGemmBM) || !tc_map(&ma2, kTcS8, a, rows_a, args.K, lda, P::A_BOX) ||
+      !tc_map(&mb, kTcS8, b, rows_b, args.K, ldb, P::BN / P::CG))
     return cudaErrorInvalidValue;
-  return launch_gemm<P>(ma, mb, args, tiles, st);
+  return launch_gemm<P>(ma, mb, args, tiles, st, &ma2);
 }
 
 template <class TO>
-cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, const Int8Args& a,
+cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, Int8Args a,
                             cudaStream_t st) {
-  const int64_t nt = ((int64_t)a.N + 127) / 128;
+  a.per = (int)(((int64_t)a.N + sm_count() - 1) / sm_count() + 7) / 8 * 8;
+  const int64_t nt = ((int64_t)a.N + a.per - 1) / a.per;
   if (a.T <= 16) return run_int8<Int8Few<TO, 16>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
@@ -141,7 +158,7 @@ int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const float* q_s
   if (reinterpret_cast<uintptr_t>(out) % (out_dtype == FWB_DTYPE_F32 ? 4 : 2)) return FWB_E_POINTER;
   const int64_t es = out_dtype == FWB_DTYPE_F32 ? 4 : 2;
   const int vec = aligned16(out) && ldo * es % 16 == 0 && N * es % 16 == 0;
-  const Int8Args a = {q_scale, w_scale, out, ldo, (int)T, (int)N, (int)K, vec, status};
+  const Int8Args a = {q_scale, w_scale, out, ldo, (int)T, (int)N, (int)K, vec, 0, status};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (out_dtype == FWB_DTYPE_BF16) return launch_status(run_int8_linear<__nv_bfloat16>(q, ldq, wq, ldw, a, st));
   if (out_dtype == FWB_DTYPE_F16) return launch_status(run_int8_linear<__half>(q, ldq, wq, ldw, a, st));

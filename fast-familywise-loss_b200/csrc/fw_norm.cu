@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   const int grp = threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * R;
   const int64_t first = (int64_t)blockIdx.x * R + grp;
+  // the 8-bit product that follows may start its weights (it waits for this grid before it reads q)
+  if constexpr (MODE == kNormInt8) allow_dependent_launch();
   if (first >= a.rows) return;  // a whole group; groups of one CTA share no barrier unless R == 1
   int flip = 0;
   const int off = row_off<T>(a.x, first, a.ldx, a.vec);

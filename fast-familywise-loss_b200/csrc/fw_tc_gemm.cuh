@@ -137,7 +137,24 @@ struct TcTile {
   int m0, n0;  // first row of M, first row of N
   int ak, bk;  // start along K, in elements, of A and of B
   int nk;      // stages of K (0: the accumulator is not written)
+  int rows;    // rows of A that matter, at most 128 (operators with A_BOX < 128)
+  int kind;    // which of two products (operators with TWO)
 };
+
+// The i-th of `n` tiles for CTA group `g` of `groups` when they are dealt out
+// in turn; -1 past the end.
+__device__ __forceinline__ int tile_in_turn(int g, int groups, int i, int n) {
+  const int64_t w = (int64_t)i * groups + g;
+  return w < n ? (int)w : -1;
+}
+
+// Lets a kernel launched as a programmatic dependent of the one before it
+// read that one's results from here on (no effect otherwise).
+__device__ __forceinline__ void wait_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 
 // What an epilogue warp works on: 32 rows of the accumulator from row r0 of
 // the tile, and a share of its columns.
@@ -150,10 +167,14 @@ struct TcPart {
 };
 
 // P is the operator: static members CG, KIND, A_MN, B_MN, BN, STAGES, KC (0:
-// all of K at once), EW, EPI_BYTES, and
-//   tiles(args)      number of tiles (read from device memory where it
-//                    depends on data)
-//   tile(args, w)    tile w
+// all of K at once), EW, EPI_BYTES and
+//   TWO              tiles of kind 1 are another product, of A2 (A_MN2) and B2
+//   A_BOX            rows per load of A: 128; fewer where tiles need not be
+//                    whole, and A2 then is A in boxes of that many rows
+//   AHEAD            loads of A brought into L2 before the previous kernel's
+//                    results are waited for (0: none; A is not written by it,
+//                    or the copy in L2 is brought up to date by the write)
+//   get(args, group, groups, i, &tile)  i-th tile of a CTA group; false: done
 //   struct State     what an epilogue thread keeps over a tile's parts
 //   epilogue(args, tile, part, state, k, parts, done): part k of the
 //                    tile's `parts`; done() hands the accumulator back once
@@ -171,12 +192,12 @@ struct GemmSmem {
 template <class P>
 __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     fw_tc_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+                      const __grid_constant__ CUtensorMap tm_a2, const __grid_constant__ CUtensorMap tm_b2,
                       const __grid_constant__ typename P::Args a) {
   constexpr int S = P::STAGES, CG = P::CG;
   constexpr uint32_t kBBytes = GemmSmem<P>::kBBytes;
   constexpr bool kI8 = P::KIND == kTcS8;
   constexpr uint32_t kTmemCols = 2 * P::BN < 32 ? 32 : 2 * P::BN;
-  constexpr uint32_t kIdesc = gemm_idesc(P::KIND, P::A_MN, P::B_MN, kGemmBM * CG, P::BN);
   constexpr int kStep = kI8 ? 128 : 64;  // elements of K per stage
   extern __shared__ uint8_t gemm_smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -195,6 +216,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)cluster_rank() : 0;
+  const int group = (int)blockIdx.x / CG, groups = (int)gridDim.x / CG;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -208,6 +230,14 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if constexpr (P::AHEAD > 0) {
+    if (threadIdx.x == 32 * 2) {
+      TcTile t;
+      if (P::get(a, group, groups, 0, &t))
+        for (int kb = 0; kb < min(t.nk, P::AHEAD); ++kb)
+          for (int i = 0; i < t.rows; i += P::A_BOX) tma_prefetch_2d(&tm_a2, t.ak + kb * kStep, t.m0 + i);
+    }
   }
   if (warp == 1) {
     if constexpr (CG == 2) {
@@ -225,36 +255,44 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   if constexpr (CG == 2) cluster_sync();  // the pair's barriers exist
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  wait_prior_kernel();  // every thread: what follows reads its results
+  allow_dependent_launch();
 
-  const int ntiles = P::tiles(a);
-  const int w0 = (int)blockIdx.x / CG, wstep = (int)gridDim.x / CG;
   uint32_t issued = 0u, issued_par = 0u;  // stages with a copy issued, and its parity
   bool mma_any = false;
+  TcTile t;
 
   if (warp == 0) {
     uint32_t s = 0, ph = 0;
-    for (int w = w0; w < ntiles; w += wstep) {
-      const TcTile t = P::tile(a, w);
+    for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
       const int m = t.m0 + rank * kGemmBM, n = t.n0 + rank * (P::BN / CG);
+      const CUtensorMap* ma = P::TWO && t.kind ? &tm_a2 : &tm_a;
+      const CUtensorMap* mb = P::TWO && t.kind ? &tm_b2 : &tm_b;
+      const bool a_mn = P::TWO && t.kind ? P::A_MN2 : P::A_MN;
+      const uint32_t bytes =
+          P::A_BOX == 128 ? kGemmABytes : (uint32_t)((t.rows + P::A_BOX - 1) / P::A_BOX * P::A_BOX * kGemmRowBytes);
       for (int kb = 0; kb < t.nk; ++kb) {
         if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status)) goto done;
         if (lane == 0) {
-          if (rank == 0) mbar_expect_tx(&full[s], CG * (kGemmABytes + kBBytes));
+          if (rank == 0) mbar_expect_tx(&full[s], CG * (bytes + kBBytes));
           const uint32_t bar = CG == 2 ? in_cta(&full[s], 0) : smem_u32(&full[s]);
           const int ka = t.ak + kb * kStep, kbb = t.bk + kb * kStep;
-          if constexpr (P::A_MN) {
+          if (a_mn) {
 #pragma unroll
             for (int i = 0; i < kGemmBM / 64; ++i)
-              tma_load_group<CG>(smA + s * kGemmABytes + i * 8192, &tm_a, m + 64 * i, ka, bar);
+              tma_load_group<CG>(smA + s * kGemmABytes + i * 8192, ma, m + 64 * i, ka, bar);
+          } else if (P::A_BOX == 128 || t.rows == 128) {
+            tma_load_group<CG>(smA + s * kGemmABytes, ma, ka, m, bar);
           } else {
-            tma_load_group<CG>(smA + s * kGemmABytes, &tm_a, ka, m, bar);
+            for (int i = 0; i < t.rows; i += P::A_BOX)
+              tma_load_group<CG>(smA + s * kGemmABytes + i * kGemmRowBytes, &tm_a2, ka, m + i, bar);
           }
           if constexpr (P::B_MN) {
 #pragma unroll
             for (int i = 0; i < P::BN / CG / 64; ++i)
-              tma_load_group<CG>(smB + s * kBBytes + i * 8192, &tm_b, n + 64 * i, kbb, bar);
+              tma_load_group<CG>(smB + s * kBBytes + i * 8192, mb, n + 64 * i, kbb, bar);
           } else {
-            tma_load_group<CG>(smB + s * kBBytes, &tm_b, kbb, n, bar);
+            tma_load_group<CG>(smB + s * kBBytes, mb, kbb, n, bar);
           }
         }
         issued |= 1u << s;
@@ -269,8 +307,9 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   } else if (warp == 1) {
     uint32_t s = 0, ph = 0, acc = 0, aph = 0;
     if (rank == 0) {
-      for (int w = w0; w < ntiles; w += wstep) {
-        const TcTile t = P::tile(a, w);
+      for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
+        const bool a_mn = P::TWO && t.kind ? P::A_MN2 : P::A_MN;
+        const uint32_t idesc = gemm_idesc(P::KIND, a_mn, P::B_MN, kGemmBM * CG, P::BN);
         const int kc = P::KC == 0 ? max(t.nk, 1) : P::KC;
         for (int k0 = 0; k0 < max(t.nk, 1); k0 += kc) {
           if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status)) goto done;
@@ -285,9 +324,9 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
 #pragma unroll
               for (int k = 0; k < 4; ++k) {
                 // 16 rows of K (MN-major) or 32 bytes of K (K-major) further on
-                const uint64_t da = P::A_MN ? umma_desc_mn(sa + 2048 * k) : umma_desc_sw128(sa + 32 * k);
+                const uint64_t da = a_mn ? umma_desc_mn(sa + 2048 * k) : umma_desc_sw128(sa + 32 * k);
                 const uint64_t db = P::B_MN ? umma_desc_mn(sb + 2048 * k) : umma_desc_sw128(sb + 32 * k);
-                umma_issue<CG, kI8>(d, da, db, kIdesc, (kb != k0 || k != 0) ? 1u : 0u);
+                umma_issue<CG, kI8>(d, da, db, idesc, (kb != k0 || k != 0) ? 1u : 0u);
               }
               umma_commit_group<CG>(&empty[s]);
             }
@@ -316,10 +355,9 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     part.lane = lane;
     part.share = (warp - 2) >> 2;
     part.smem = smE + (warp - 2) * (P::EPI_BYTES / P::EW);
-    for (int w = w0; w < ntiles; w += wstep) {
-      const TcTile t = P::tile(a, w);
+    for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
       const int parts = P::KC == 0 ? 1 : max((t.nk + P::KC - 1) / (P::KC == 0 ? 1 : P::KC), 1);
-      typename P::State state;
+      typename P::State state{};
       for (int k = 0; k < parts; ++k) {
         if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
         tc_fence_after();
@@ -432,16 +470,22 @@ inline bool tc_map(CUtensorMap* m, TcKind kind, const void* ptr, int64_t rows, i
   const CUtensorMapDataType dt = kind == kTcS8   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                                  : kind == kTcF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  auto encode = [&] {
+    return fn(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  };
+  if (encode()) return true;
+  // a host thread that has not used the device yet has no context current
+  int dev = 0;
+  return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode();
 }
 
 // At most one CTA per SM; `max_tiles` bounds the grid where the tile count is
-// known on the device only.
+// known on the device only.  A programmatic dependent of the kernel before it.
 template <class P>
 cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const typename P::Args& a, int64_t max_tiles,
-                        cudaStream_t st) {
+                        cudaStream_t st, const CUtensorMap* ma2 = nullptr, const CUtensorMap* mb2 = nullptr) {
   static std::atomic<bool> attr_set[kMaxDevices] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -460,14 +504,31 @@ cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const type
   cfg.blockDim = dim3(GemmSmem<P>::kThreads);
   cfg.dynamicSmemBytes = GemmSmem<P>::kBytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = P::CG;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = P::CG;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = P::CG > 1 ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, fw_tc_gemm_kernel<P>, ma, mb, a);
+  cfg.numAttrs = P::CG > 1 ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, fw_tc_gemm_kernel<P>, ma, mb, ma2 ? *ma2 : ma, mb2 ? *mb2 : mb, a);
+}
+
+// The same for another kernel of the chain.
+template <class... KArgs, class... Args>
+cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
 }
 
 }  // namespace

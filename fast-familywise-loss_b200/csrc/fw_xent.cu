@@ -12,8 +12,9 @@
 // Backward, in pieces of the vocabulary: the logits of a piece again, their
 // epilogue writing G (16-bit, the product's operand type: the rounding is
 // relative to each entry, so it weighs as the rounding of the result does);
-// then dH += G W and dW = G^T H of the piece, G read in both orientations
-// from the one buffer (MN-major operands), each row of dW written once.
+// then dH += G W and dW = G^T H of the piece in one launch, G read in both
+// orientations from the one buffer (MN-major operands), each row of dW written
+// once.
 // Bound by the tensor cores: 2 B V D operations for each of the four products.
 //
 // float16 G: exp(z - lse) / B may be under float16's smallest value, so rows
@@ -35,7 +36,7 @@ struct XentHead {
   int32_t rows;    // live rows
   uint32_t done;   // blocks of the joining kernel that have finished
   int32_t status;  // status bits raised inside
-  float back;      // factor taken out after the sums (float16)
+  float top;       // largest upstream gradient of a live row (float16, one per row)
 };
 
 struct PackArgs {
@@ -43,7 +44,7 @@ struct PackArgs {
   const int64_t* y;
   int64_t B, Bp, D, Dp, ldh, V, ignore;
   void* hp;
-  int32_t* row_of;   // [Bp] packed -> given row, -1 past the last live one
+  int32_t* row_of;   // [Bp] packed -> given row (behind the live ones the ignored ones, then -1)
   int32_t* label;    // [Bp] -1: outside [0, V)
   float* loss_rows;  // zero for ignored rows, per given row; may be NULL
   XentHead* head;
@@ -57,6 +58,7 @@ template <class T>
 __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) {
   __shared__ int red[2][kPackThreads / 32];
   constexpr int V = 16 / sizeof(T);
+  allow_dependent_launch();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * a.per_cta;
   int before = 0, total = 0;
@@ -97,7 +99,7 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
       const int64_t y = __shfl_sync(kFull, yl, i);
       if (lane == 0) {
         const bool ok = y >= 0 && y < a.V;
-        a.row_of[dst] = alive ? (int32_t)r : -1;
+        a.row_of[dst] = r < a.B ? (int32_t)r : -1;
         a.label[dst] = alive && ok ? (int32_t)y : -1;
         if (alive && !ok) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
         if (!alive && r < a.B && a.loss_rows) a.loss_rows[r] = 0.0f;
@@ -138,6 +140,15 @@ __global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_
 
 struct NoState {};
 
+// 2^x by the hardware's instruction (relative error 2^-22, results under
+// 2^-126 flushed to 0); volatile, so that the compiler does not hold many
+// arguments in registers to interleave them.
+__device__ __forceinline__ float exp2_hw(float x) {
+  float y;
+  asm volatile("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 constexpr int kTileM = 256, kTileN = 256;  // of a pair of CTAs
 
 __device__ __forceinline__ int row_tiles(const XentHead* h) { return (h->rows + kTileM - 1) / kTileM; }
@@ -155,7 +166,7 @@ __device__ __forceinline__ void tile_order(int w, int mt, int nt, int group, int
 struct LseArgs {
   const XentHead* head;
   const int32_t* label;
-  float2* part;  // [half tiles of V, Bp]: maximum, sum of exp(z - maximum)
+  float2* part;  // [kLseCols columns of V, Bp]: maximum, sum of exp(z - maximum)
   float* zy;     // [Bp]
   int64_t Bp;
   int V, D;
@@ -166,42 +177,46 @@ struct LseArgs {
 // registers: the tensor cores' fp32 additions round towards zero, so a logit
 // shrinks by a part that grows with the length of the sum.
 constexpr int kLseStages = 8;
+constexpr int kLseCols = 128;  // columns of a tile per epilogue thread: they stay in its registers
 
 template <TcKind K>
 struct LseTile {
   using Args = LseArgs;
   struct State {
-    float z[kTileN / 2];
+    float z[kLseCols] = {};
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = kLseStages, EW = 8;
+  static constexpr bool TWO = false, A_MN2 = false;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = kLseStages, EW = 4 * BN / kLseCols, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * ((a.V + BN - 1) / BN); }
-  __device__ static TcTile tile(const Args& a, int w) {
+  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
+    const int mt = row_tiles(a.head), nt = (a.V + BN - 1) / BN, w = tile_in_turn(group, groups, i, mt * nt);
+    if (w < 0) return false;
     int m, n;
-    tile_order(w, row_tiles(a.head), (a.V + BN - 1) / BN, 16, &m, &n);
-    return {m * kTileM, n * BN, 0, 0, (a.D + 63) / 64};
+    tile_order(w, mt, nt, 16, &m, &n);
+    *t = {m * kTileM, n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
+    return true;
   }
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State& st, int k, int parts,
                                   Done done) {
 #pragma unroll
-    for (int c = 0; c < BN / 2; c += 16) {
+    for (int c = 0; c < kLseCols; c += 16) {
       float v[16];
-      tmem_ld16(p.taddr + p.share * (BN / 2) + c, v);
+      tmem_ld16(p.taddr + p.share * kLseCols + c, v);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) st.z[c + i] = k == 0 ? v[i] : st.z[c + i] + v[i];
+      for (int i = 0; i < 16; ++i) st.z[c + i] += v[i];
     }
     done();
     if (k < parts - 1) return;
     const int row = t.m0 + p.row + p.lane;  // < Bp
-    const int n0 = t.n0 + p.share * (BN / 2);
+    const int n0 = t.n0 + p.share * kLseCols;
     const int y = a.label[row] - n0;
     const int valid = a.V - n0;
     float m = -CUDART_INF_F, s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < BN / 2; ++i) {
+    for (int i = 0; i < kLseCols; ++i) {
       if (i >= valid) st.z[i] = -CUDART_INF_F;
       if (i == y) a.zy[row] = st.z[i];
       m = max_nan(m, st.z[i]);
@@ -209,10 +224,10 @@ struct LseTile {
     if (m != -CUDART_INF_F) {  // a NaN maximum, or +inf, makes the sum NaN
       float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < BN / 2; ++i) s4[i & 3] += exp2f((st.z[i] - m) * kLog2e);
+      for (int i = 0; i < kLseCols; ++i) s4[i & 3] += exp2_hw((st.z[i] - m) * kLog2e);
       s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
     }
-    a.part[(int64_t)(n0 / (BN / 2)) * a.Bp + row] = make_float2(m, s);
+    a.part[(int64_t)(n0 / kLseCols) * a.Bp + row] = make_float2(m, s);
   }
 };
 
@@ -231,7 +246,7 @@ struct JoinArgs {
   int32_t* status;
 };
 
-constexpr int kJoinWarps = 8;
+constexpr int kJoinWarps = 32;
 
 // 32 rows per CTA, the tiles' pairs split over its warps; the last CTA to
 // finish adds the losses in a fixed order.
@@ -240,6 +255,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_kernel(JoinArgs 
   __shared__ double sd[kJoinWarps];
   __shared__ bool last;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  wait_prior_kernel();
   const int rows = a.head->rows;
   const int row = blockIdx.x * 32 + lane;
   float m = -CUDART_INF_F, s = 0.0f;
@@ -266,6 +282,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_kernel(JoinArgs 
     for (int i = 0; i < kJoinWarps; ++i)
       if (sm[i][lane] != -CUDART_INF_F) S += ss[i][lane] * exp2f((sm[i][lane] - M) * kLog2e);
     const bool ok = a.label[row] >= 0 && a.head->status == 0;
+    if (lane == 0 && a.head->status != 0) raise_status(a.status, a.head->status);
     const float lse = ok ? M + logf(S) : CUDART_NAN_F;  // a NaN row stays NaN in the gradient too
     const float loss = ok ? lse - a.zy[row] : CUDART_NAN_F;
     a.lse[row] = lse;
@@ -293,47 +310,48 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_kernel(JoinArgs 
 }
 
 // ------------------------------------------------------------ backward
-struct CoefArgs {
-  XentHead* head;
-  const int32_t* row_of;
-  const float* go;
-  float* coef;  // [Bp], packed
+// The upstream gradient and the scale of G.
+struct Upstream {
+  const float* go;  // one per given row, or one
   int per_row, mean, f16;
+
+  __device__ float over(const XentHead* h) const { return mean ? 1.0f / (float)h->rows : 1.0f; }
+  // float16: what G's rows are scaled by, largest upstream factor to kF16Unit
+  __device__ float unit(const XentHead* h) const {
+    if (!f16) return 1.0f;
+    const float top = per_row ? h->top : fabsf(go[0] * over(h));
+    return top == 0.0f ? 1.0f : top;
+  }
+  // factor of the row of G, given row r
+  __device__ float coef(const XentHead* h, int r) const {
+    const float g = go[per_row ? r : 0] * over(h);
+    return f16 ? g / unit(h) * kF16Unit : g;
+  }
+  // factor taken out after the sums
+  __device__ float back(const XentHead* h) const { return f16 ? unit(h) / kF16Unit : 1.0f; }
 };
 
-// Factor of each packed row's G, and the factor taken out after the sums.
-__global__ void __launch_bounds__(1024) fw_xent_coef_kernel(CoefArgs a) {
+__global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const int32_t* row_of, const float* go) {
   __shared__ float red[32];
-  const int rows = a.head->rows;
-  const float over = a.mean ? 1.0f / (float)rows : 1.0f;
-  float unit = 1.0f;
-  if (a.f16) {
-    float top = a.per_row ? 0.0f : fabsf(a.go[0] * over);
-    if (a.per_row) {
-      for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, fabsf(a.go[a.row_of[i]] * over));
+  const int rows = head->rows;
+  float top = 0.0f;
+  for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, fabsf(go[row_of[i]]));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
-      if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
-      __syncthreads();
-      top = red[0];
-      for (int i = 1; i < 32; ++i) top = max_nan(top, red[i]);
-    }
-    unit = top == 0.0f ? 1.0f : top;
-    if (threadIdx.x == 0) a.head->back = unit / kF16Unit;
-  } else if (threadIdx.x == 0) {
-    a.head->back = 1.0f;
-  }
-  for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float g = a.go[a.per_row ? a.row_of[i] : 0] * over;
-    a.coef[i] = a.f16 ? g / unit * kF16Unit : g;
+  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < 32; ++i) top = max_nan(top, red[i]);
+    head->top = top;
   }
 }
 
 struct GradArgs {
   const XentHead* head;
   const int32_t* label;
+  const int32_t* row_of;
   const float* lse;
-  const float* coef;
+  Upstream up;
   void* g;  // [Bp, ldg]
   int64_t ldg;
   int V, D;
@@ -347,13 +365,16 @@ struct GradTile {
   using State = NoState;
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
-  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = 0, EW = 8;
+  static constexpr bool TWO = false, A_MN2 = false;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * (a.vn / BN); }
-  __device__ static TcTile tile(const Args& a, int w) {
+  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
+    const int mt = row_tiles(a.head), nt = a.vn / BN, w = tile_in_turn(group, groups, i, mt * nt);
+    if (w < 0) return false;
     int m, n;
-    tile_order(w, row_tiles(a.head), a.vn / BN, 16, &m, &n);
-    return {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64};
+    tile_order(w, mt, nt, 16, &m, &n);
+    *t = {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
+    return true;
   }
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
@@ -361,7 +382,7 @@ struct GradTile {
     const bool live = row < a.head->rows;
     const int y = live ? a.label[row] : -1;
     const float lse = live ? a.lse[row] : 0.0f;
-    const float coef = live ? a.coef[row] : 0.0f;
+    const float coef = live ? a.up.coef(a.head, a.row_of[row]) : 0.0f;
     T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
@@ -370,7 +391,7 @@ struct GradTile {
       const int valid = live ? min(32, a.V - (t.n0 + c)) : 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float q = exp2f((v[i] - lse) * kLog2e);
+        float q = exp2_hw((v[i] - lse) * kLog2e);
         if (t.n0 + c + i == y) q -= 1.0f;
         v[i] = i < valid ? q * coef : 0.0f;
       }
@@ -380,47 +401,100 @@ struct GradTile {
   }
 };
 
-struct DHiddenArgs {
+// dH += G W and dW = G^T H of a piece, in one launch: the few long tiles of dH
+// (all of the piece's columns are their K) would leave most of the last round
+// of SMs idle, so the tiles of dW fill it up.
+struct ProductArgs {
   const XentHead* head;
   const int32_t* row_of;
-  float* sum;  // [Bp, lds] where the vocabulary has several pieces, else NULL
-  void* out;   // [B, D]
-  int D, lds;
-  int vec;  // rows of out start on 16-byte boundaries
-  int v0, vn;
+  Upstream up;
+  float* sum;     // dH so far, [Bp, lds], where the vocabulary has several pieces, else NULL
+  void* dhidden;  // [B, D] or NULL
+  void* dweight;  // [V, D] or NULL
+  int Bp, V, D, lds;
+  int v0, vn;  // first column of the piece, its columns rounded up to 256
   int first, last;
+  int vec;  // rows of dhidden and dweight start on 16-byte boundaries
   int32_t* status;
 };
 
 template <class T, TcKind K>
-struct DHiddenTile {
-  using Args = DHiddenArgs;
+struct ProductTile {
+  using Args = ProductArgs;
   using State = NoState;
   static constexpr TcKind KIND = K;
-  static constexpr bool A_MN = false, B_MN = true;
-  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8;
+  static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
-  __device__ static int tiles(const Args& a) { return row_tiles(a.head) * ((a.D + BN - 1) / BN); }
-  __device__ static TcTile tile(const Args& a, int w) {
+
+  // Tiles: `long_` of dH with vn / 64 stages each, then `shorts` of dW with
+  // rows / 64, then (last piece) those of dH that hold only ignored rows.  A
+  // CTA group takes its long tiles in turn; with `more` groups having one more
+  // than the others, the short ones go to the others first, until all are
+  // level, then to all in turn.
+  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
+    const int nt = (a.D + BN - 1) / BN, mt = a.dhidden ? row_tiles(a.head) : 0;
+    const int k_long = a.vn / 64, k_short = (a.head->rows + 63) / 64;
+    const int vt = a.dweight ? (min(a.vn, a.V - a.v0) + kTileM - 1) / kTileM : 0;
+    const int dead = a.dhidden && a.last ? a.Bp / kTileM - mt : 0;
+    const int n_long = mt * nt, n_short = vt * nt, n_rest = n_short + dead * nt;
+    const int q = n_long / groups, more = n_long % groups;
+    const int mine = q + (group < more ? 1 : 0);
     int m, n;
-    tile_order(w, row_tiles(a.head), (a.D + BN - 1) / BN, 8, &m, &n);
-    return {m * kTileM, n * BN, 0, a.v0, a.vn / 64};
+    if (i < mine) {
+      tile_order(i * groups + group, mt, nt, 8, &m, &n);
+      *t = {m * kTileM, n * BN, 0, a.v0, k_long, 128, 0};
+      return true;
+    }
+    i -= mine;
+    int lead = 0;  // rounds of short tiles that only the groups with fewer long ones take
+    if (more > 0) {
+      lead = k_short > 0 ? (k_long + k_short / 2) / k_short : 0;
+      lead = min(lead, (n_rest + groups - more - 1) / (groups - more));
+    }
+    int64_t w;
+    if (group >= more && i < lead) {
+      w = (int64_t)i * (groups - more) + (group - more);
+    } else {
+      if (group >= more) i -= lead;
+      w = (int64_t)lead * (groups - more) + (int64_t)i * groups + group;
+    }
+    if (w >= n_rest) return false;
+    if (w < n_short) {
+      tile_order((int)w, vt, nt, 5, &m, &n);
+      *t = {m * kTileM, n * BN, 0, 0, k_short, 128, 1};
+    } else {
+      const int d = (int)w - n_short;
+      *t = {(mt + d / nt) * kTileM, d % nt * BN, 0, 0, 0, 128, 0};
+    }
+    return true;
   }
+
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
     float* sm = reinterpret_cast<float*>(p.smem);
+    const float back = a.up.back(a.head);
     const int r0 = t.m0 + p.row;
-    const int rows = min(32, a.head->rows - r0);
-    const float back = a.head->back;
-    const int mine = p.lane < rows ? a.row_of[r0 + p.lane] : -1;
+    const int live = a.head->rows - r0;  // dH: the warp's rows behind these are ignored ones
+    const int mine = t.kind == 0 ? a.row_of[r0 + p.lane] : -1;
+    const int rows = a.V - (a.v0 + r0);  // dW
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
       tmem_ld32(p.taddr + c, v);
       if (c + 32 == (p.share + 1) * (BN / 2)) done();
       const int c0 = t.n0 + c;
       const int cols = min(32, a.D - c0);
-      if (cols <= 0 || rows <= 0) continue;
-      if (a.sum) {  // several pieces: the rows of the sum so far are this thread's own
+      if (cols <= 0) continue;
+      if (t.kind == 1) {
+        if (rows <= 0) continue;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = t.nk == 0 ? 0.0f : v[i] * back;  // no live row: nothing was accumulated
+        T* out = static_cast<T*>(a.dweight) + (int64_t)(a.v0 + r0) * a.D + c0;
+        store_block<T>(sm, v, p.lane, cols, a.vec,
+                       [&](int i) -> T* { return i < rows ? out + (int64_t)i * a.D : nullptr; });
+        continue;
+      }
+      if (a.sum && t.nk > 0) {  // several pieces: this thread's own row of the sum so far
         float* s = a.sum + (int64_t)(r0 + p.lane) * a.lds + c0;  // lds: D rounded up to 32
         if (!a.first) {
 #pragma unroll
@@ -437,58 +511,11 @@ struct DHiddenTile {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= back;
-      T* out = static_cast<T*>(a.out);
+      for (int i = 0; i < 32; ++i) v[i] = p.lane < live && t.nk > 0 ? v[i] * back : 0.0f;
+      T* out = static_cast<T*>(a.dhidden) + c0;
       store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
         const int r = __shfl_sync(kFull, mine, i);
-        return r >= 0 ? out + (int64_t)r * a.D + c0 : nullptr;
-      });
-    }
-  }
-};
-
-struct DWeightArgs {
-  const XentHead* head;
-  void* out;  // [V, D]
-  int V, D;
-  int v0, vn;
-  int vec;  // rows of out start on 16-byte boundaries
-  int32_t* status;
-};
-
-template <class T, TcKind K>
-struct DWeightTile {
-  using Args = DWeightArgs;
-  using State = NoState;
-  static constexpr TcKind KIND = K;
-  static constexpr bool A_MN = true, B_MN = true;
-  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8;
-  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
-  __device__ static int mtiles(const Args& a) { return (min(a.vn, a.V - a.v0) + kTileM - 1) / kTileM; }
-  __device__ static int tiles(const Args& a) { return mtiles(a) * ((a.D + BN - 1) / BN); }
-  __device__ static TcTile tile(const Args& a, int w) {
-    int m, n;
-    tile_order(w, mtiles(a), (a.D + BN - 1) / BN, 5, &m, &n);
-    return {m * kTileM, n * BN, 0, 0, (a.head->rows + 63) / 64};
-  }
-  template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
-    float* sm = reinterpret_cast<float*>(p.smem);
-    const int r0 = a.v0 + t.m0 + p.row;
-    const int rows = a.V - r0;
-    const float back = a.head->back;
-    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
-      float v[32];
-      tmem_ld32(p.taddr + c, v);
-      if (c + 32 == (p.share + 1) * (BN / 2)) done();
-      const int c0 = t.n0 + c;
-      const int cols = min(32, a.D - c0);
-      if (cols <= 0 || rows <= 0) continue;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = t.nk == 0 ? 0.0f : v[i] * back;  // no live row: nothing was accumulated
-      T* out = static_cast<T*>(a.out);
-      store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
-        return i < rows ? out + (int64_t)(r0 + i) * a.D + c0 : nullptr;
+        return r >= 0 ? out + (int64_t)r * a.D : nullptr;
       });
     }
   }
@@ -496,7 +523,7 @@ struct DWeightTile {
 
 // ------------------------------------------------------------ host
 // Bytes of G that one piece of the vocabulary may take.
-constexpr int64_t kPieceBytes = (int64_t)512 << 20;
+constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
@@ -508,7 +535,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, zy, loss_pack, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, coef, g, sum, bwd_bytes;
+  int64_t piece, pieces, g, sum, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
@@ -524,7 +551,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.wp = at, at += copy_w ? up(2 * V * p.Dp, 256) : 0;
   p.state_bytes = at;
   at = 0;
-  p.part = at, at += up(8 * p.Bp * ((V + 127) / 128 + 1), 256);
+  p.part = at, at += up(8 * p.Bp * up(V, kTileN) / kLseCols, 256);
   p.zy = at, at += up(4 * p.Bp, 256);
   p.loss_pack = at, at += up(4 * p.Bp, 256);
   p.fwd_bytes = at;
@@ -534,7 +561,6 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.piece = up((Vp + p.pieces - 1) / p.pieces, 256);
   p.pieces = (Vp + p.piece - 1) / p.piece;
   at = 0;
-  p.coef = at, at += up(4 * p.Bp, 256);
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
   p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * up(D, 32), 256) : 0;
   p.bwd_bytes = at;
@@ -578,9 +604,8 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   const int64_t nt = (V + 255) / 256;
   if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
   JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
-                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + 127) / 128), reduction, status};
-  fw_xent_join_kernel<<<(unsigned)(p.Bp / 32), kJoinWarps * 32, 0, st>>>(ja);
-  return launch_status(cudaGetLastError());
+                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + kLseCols - 1) / kLseCols), reduction, status};
+  return launch_status(launch_after(fw_xent_join_kernel, dim3((unsigned)(p.Bp / 32)), dim3(kJoinWarps * 32), st, ja));
 }
 
 template <class T, TcKind K>
@@ -590,13 +615,10 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   XentHead* head = reinterpret_cast<XentHead*>(state);
   int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
   int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
-  float* coef = reinterpret_cast<float*>(ws + p.coef);
   const void* w = p.copy_w ? state + p.wp : weight;
   if (p.copy_w) ldw = p.Dp;
-  // ignored rows' gradient; the live rows' is written below
-  if (dhidden && cudaMemsetAsync(dhidden, 0, (size_t)(2 * B * D), st) != cudaSuccess) return FWB_E_LAUNCH;
-  const CoefArgs ca = {head, row_of, go, coef, per_row, mean, K == kTcF16};
-  fw_xent_coef_kernel<<<1, 1024, 0, st>>>(ca);
+  const Upstream u = {go, per_row, mean, K == kTcF16};
+  if (u.f16 && per_row) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go);
   if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
   CUtensorMap mh, mw, mg, wmn, gmn, hmn;
   char* hp = state + p.hp;
@@ -606,22 +628,17 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
       !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hp, p.Bp, D, p.Dp, 64))
     return FWB_E_LAUNCH;
   const int64_t Vp = up(V, 256), mb = p.Bp / 256, nd = (D + 255) / 256;
+  const int vec = aligned16(dhidden) && aligned16(dweight) && D % 8 == 0;
+  float* sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
-    const GradArgs ga = {head, label, reinterpret_cast<float*>(state + p.lse), coef, g, p.piece, (int)V, (int)D, v0,
-                         vn, status};
+    const GradArgs ga = {head, label, row_of, reinterpret_cast<float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
+                         v0, vn, status};
     if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
-    if (dhidden) {
-      const DHiddenArgs da = {head, row_of, p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr, dhidden,
-                              (int)D, (int)up(D, 32), aligned16(dhidden) && D % 8 == 0, v0, vn, i == 0,
-                              i == p.pieces - 1, status};
-      if (launch_gemm<DHiddenTile<T, K>>(mg, wmn, da, mb * nd, st) != cudaSuccess) return FWB_E_LAUNCH;
-    }
-    if (dweight) {
-      const DWeightArgs da = {head, dweight, (int)V, (int)D, v0, vn, aligned16(dweight) && D % 8 == 0, status};
-      if (launch_gemm<DWeightTile<T, K>>(gmn, hmn, da, (int64_t)(vn / 256) * nd, st) != cudaSuccess)
-        return FWB_E_LAUNCH;
-    }
+    const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
+                            i == 0, i == p.pieces - 1, vec, status};
+    const int64_t tiles = (dhidden ? mb * nd : 0) + (dweight ? vn / 256 * nd : 0);
+    if (launch_gemm<ProductTile<T, K>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
   }
   return FWB_OK;
 }
