@@ -408,6 +408,11 @@ __device__ __forceinline__ void allow_dependent_launch() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// In a kernel launched as a programmatic dependent: waits for the grids before
+// it to complete and their writes to be visible (no effect in others).  Every
+// thread of such a kernel calls it before it touches memory.
+__device__ __forceinline__ void wait_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void raise_status(int32_t* status, int bits) {
   if (status) atomicOr(reinterpret_cast<int*>(status), bits);
 }

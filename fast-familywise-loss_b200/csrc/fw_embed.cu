@@ -79,6 +79,8 @@ struct EmbedArgs {
 template <class T>
 __global__ void __launch_bounds__(256) fw_embed_rows_kernel(EmbedArgs a) {
   constexpr int V = 16 / sizeof(T);
+  wait_prior_kernel();
+  allow_dependent_launch();
   const int lane = threadIdx.x & 31;
   const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
   const int64_t work = a.T * a.nslabs;
@@ -301,6 +303,8 @@ __device__ __forceinline__ void zero_unnamed(const SortArgs& s, const ZeroArgs& 
 // belongs in the cluster.  The grid's other clusters zero.
 template <class TW, bool ALIGNED>
 __global__ void __launch_bounds__(kClusterThreads, 2) fw_sort_cluster_kernel(SortArgs a, int passes, ZeroArgs z) {
+  wait_prior_kernel();
+  allow_dependent_launch();
   namespace cg = cooperative_groups;
   cg::cluster_group cl = cg::this_cluster();
   extern __shared__ __align__(16) unsigned char sort_smem[];
@@ -471,6 +475,8 @@ __device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int
 // per warp, one binary search per lane.
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) fw_embed_sum_kernel(EmbedGradArgs a) {
+  wait_prior_kernel();
+  allow_dependent_launch();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t total = gridDim.x, adding = a.sum_blocks;
   const int64_t before = blockIdx.x * adding / total;  // adding CTAs ahead of this one
@@ -502,6 +508,8 @@ __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) fw_embed_sum_kernel(Embe
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) fw_embed_join_kernel(EmbedGradArgs a) {
   constexpr int V = 16 / sizeof(T);
+  wait_prior_kernel();
+  allow_dependent_launch();
   const int lane = threadIdx.x & 31;
   const int64_t slabs = (a.nslots + 31) / 32, chunks = (a.T + kChunk - 1) / kChunk, work = chunks * slabs;
   const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
@@ -541,6 +549,8 @@ __global__ void __launch_bounds__(256) fw_embed_join_kernel(EmbedGradArgs a) {
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
   constexpr int V = 16 / sizeof(T);
+  wait_prior_kernel();
+  allow_dependent_launch();
   __shared__ int32_t key[kDirectTokens];
   const int n = (int)a.T;
   for (int i = threadIdx.x; i < kDirectTokens; i += 256) {
@@ -633,33 +643,20 @@ cudaError_t sort_cluster(const SortArgs& s, int passes, const EmbedGradArgs& g, 
   int64_t zero = (s.V + rows - 1) / rows;
   if (zero > 65536) zero = 65536;
   const ZeroArgs z = {g.dw, g.D, g.nslots, (int)rows};
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(ctas + (zero + ctas - 1) / ctas * ctas));
-  cfg.blockDim = dim3(kClusterThreads);
-  cfg.dynamicSmemBytes = kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, s, passes, z);
+  return launch_dependent(kernel, ctas + (zero + ctas - 1) / ctas * ctas, kClusterThreads, kSmem, ctas, st, s, passes, z);
 }
 
 template <class T, bool ALIGNED>
 cudaError_t launch_embed_grad(EmbedGradArgs a, SortArgs s, const EmbedPlan& p, uint2* other, cudaStream_t st) {
   const int64_t slabs = (a.nslots + 31) / 32;
   if (a.T <= kDirectTokens) {
-    fw_embed_direct_kernel<T, ALIGNED><<<warps_grid(a.V * slabs), 256, 0, st>>>(a);
-    return cudaGetLastError();
+    return launch_dependent(fw_embed_direct_kernel<T, ALIGNED>, warps_grid(a.V * slabs), 256, 0, 1, st, a);
   }
   a.sorted = s.dst;
   unsigned zero = 0;
+  cudaError_t e = cudaSuccess;
   if (a.T <= kClusterTokens) {
-    const cudaError_t e = sort_cluster<T, ALIGNED>(s, p.passes, a, st);
-    if (e != cudaSuccess) return e;
+    e = sort_cluster<T, ALIGNED>(s, p.passes, a, st);
   } else {
     uint2* ent[2] = {s.dst, other};
     for (int i = 0; i < p.passes; ++i) {
@@ -671,11 +668,13 @@ cudaError_t launch_embed_grad(EmbedGradArgs a, SortArgs s, const EmbedPlan& p, u
     }
     a.sorted = ent[(p.passes - 1) & 1];
     zero = warps_grid((a.V + 7) / 8);
+    e = cudaGetLastError();
   }
+  if (e != cudaSuccess) return e;
   a.sum_blocks = (int)warps_grid(p.chunks * slabs);
-  fw_embed_sum_kernel<T, ALIGNED><<<a.sum_blocks + zero, 256, 0, st>>>(a);
-  fw_embed_join_kernel<T, ALIGNED><<<warps_grid(p.chunks * slabs), 256, 0, st>>>(a);
-  return cudaGetLastError();
+  e = launch_dependent(fw_embed_sum_kernel<T, ALIGNED>, a.sum_blocks + zero, 256, 0, 1, st, a);
+  if (e != cudaSuccess) return e;
+  return launch_dependent(fw_embed_join_kernel<T, ALIGNED>, warps_grid(p.chunks * slabs), 256, 0, 1, st, a);
 }
 
 template <class T>
@@ -705,12 +704,12 @@ int fw_embed_rows(int dtype, const int64_t* ids, int64_t T, const void* weight, 
   EmbedArgs a = {ids, weight, out, T, V, D, ldw, ldo, scale, status, 0};
   a.nslabs = slabs_of(D, es);
   const int64_t need = (T * a.nslabs + 7) / 8, cap = (int64_t)sm_count() * 64;
-  const unsigned grid = (unsigned)(need < cap ? need : cap);
+  const int64_t grid = need < cap ? need : cap;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == FWB_DTYPE_BF16) fw_embed_rows_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a);
-  else if (dtype == FWB_DTYPE_F16) fw_embed_rows_kernel<__half><<<grid, 256, 0, st>>>(a);
-  else fw_embed_rows_kernel<float><<<grid, 256, 0, st>>>(a);
-  return launch_status(cudaGetLastError());
+  return launch_status(
+      dtype == FWB_DTYPE_BF16  ? launch_dependent(fw_embed_rows_kernel<__nv_bfloat16>, grid, 256, 0, 1, st, a)
+      : dtype == FWB_DTYPE_F16 ? launch_dependent(fw_embed_rows_kernel<__half>, grid, 256, 0, 1, st, a)
+                               : launch_dependent(fw_embed_rows_kernel<float>, grid, 256, 0, 1, st, a));
 }
 
 int64_t fw_embed_grad_workspace(int64_t T, int64_t V, int64_t D) {

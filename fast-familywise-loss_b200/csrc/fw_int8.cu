@@ -8,10 +8,10 @@
 //                rows its columns: bound by the tensor cores;
 //   few tokens   weight rows are the 128 rows of a tile and the tokens its
 //                16 .. 128 columns: every weight is read once, bound by HBM.
-//                The weight rows are dealt out evenly over the SMs in steps of
-//                8 (whole tiles would leave up to half of them idle in the
-//                last round), tiles of fewer than 128 rows loading only the
-//                32-row boxes they need, and the first weights are brought
+//                The rows that do not make a whole round of tiles are dealt
+//                out evenly over the SMs in steps of 8 (a last round of whole
+//                tiles would leave up to all but one of them idle), loading
+//                only the 32-row boxes they need, and the first weights are brought
 //                into L2 while the kernel before (the norm that makes q) still
 //                runs.
 #include "fw_tc_gemm.cuh"
@@ -26,7 +26,7 @@ struct Int8Args {
   int64_t ldo;
   int T, N, K;
   int vec;  // rows of out start on 16-byte boundaries
-  int per;  // few tokens: weight rows per CTA
+  int per;  // few tokens: weight rows per CTA behind the whole tiles
   int32_t* status;
 };
 
@@ -83,10 +83,17 @@ struct Int8Few {
   static constexpr int CG = 1, BN = NT, KC = 0, EW = 4, A_BOX = 32, AHEAD = 16;
   static constexpr int STAGES = NT <= 32 ? 10 : NT <= 64 ? 8 : 6;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static bool get(const Args& a, int group, int, int i, TcTile* t) {
-    const int end = min(a.N, (group + 1) * a.per), m0 = group * a.per + i * 128;
-    if (m0 >= end) return false;
-    *t = {m0, 0, 0, 0, (a.K + 127) / 128, min(128, end - m0), 0};
+  // whole tiles in turn, then what is left in equal parts
+  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
+    const int rounds = a.N / 128 / groups;
+    int m0 = (i * groups + group) * 128, rows = 128;
+    if (i >= rounds) {
+      if (i > rounds) return false;
+      m0 = rounds * groups * 128 + group * a.per;
+      rows = min(a.per, a.N - m0);
+      if (rows <= 0) return false;
+    }
+    *t = {m0, 0, 0, 0, (a.K + 127) / 128, rows, 0};
     return true;
   }
   template <class Done>
@@ -126,8 +133,9 @@ cudaError_t run_int8(const void* a, int64_t rows_a, int64_t lda, const void* b, 
 template <class TO>
 cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64_t ldw, Int8Args a,
                             cudaStream_t st) {
-  a.per = (int)(((int64_t)a.N + sm_count() - 1) / sm_count() + 7) / 8 * 8;
-  const int64_t nt = ((int64_t)a.N + a.per - 1) / a.per;
+  const int sms = sm_count(), left = a.N % (128 * sms);
+  a.per = ((left + sms - 1) / sms + 7) / 8 * 8;
+  const int64_t nt = a.N / 128 >= sms ? sms : (left + a.per - 1) / a.per;  // CTAs
   if (a.T <= 16) return run_int8<Int8Few<TO, 16>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);

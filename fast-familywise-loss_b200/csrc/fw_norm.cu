@@ -144,8 +144,8 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   const int grp = threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * R;
   const int64_t first = (int64_t)blockIdx.x * R + grp;
-  // the 8-bit product that follows may start its weights (it waits for this grid before it reads q)
-  if constexpr (MODE == kNormInt8) allow_dependent_launch();
+  wait_prior_kernel();
+  allow_dependent_launch();
   if (first >= a.rows) return;  // a whole group; groups of one CTA share no barrier unless R == 1
   int flip = 0;
   const int off = row_off<T>(a.x, first, a.ldx, a.vec);
@@ -254,6 +254,8 @@ template <class T, int MODE>
 __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
   __shared__ float red[2 * 32];
   int flip = 0;
+  wait_prior_kernel();
+  allow_dependent_launch();
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* xr = static_cast<const T*>(a.x) + r * a.ldx;
     const T* rr = a.res ? static_cast<const T*>(a.res) + r * a.ldr : nullptr;
@@ -309,6 +311,8 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   constexpr bool AHEAD = CH == 1;
   __shared__ float red[2 * (G / 32)];
   extern __shared__ __align__(16) float dw_row[];  // [D], R > 1 only
+  wait_prior_kernel();
+  allow_dependent_launch();
   const int t = threadIdx.x % G;
   const int grp = threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * R;
@@ -393,6 +397,8 @@ template <class T>
 __global__ void __launch_bounds__(1024) fw_norm_grad_long_kernel(NormGradArgs a) {
   __shared__ float red[2 * 32];
   int flip = 0;
+  wait_prior_kernel();
+  allow_dependent_launch();
   float* part = a.part ? a.part + (int64_t)blockIdx.x * a.D : nullptr;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T* sr = static_cast<const T*>(a.s) + r * a.lds;
@@ -424,6 +430,8 @@ __global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restric
   __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + lane;
+  wait_prior_kernel();
+  allow_dependent_launch();
   float s = 0.0f;
   if (e < D) {
 #pragma unroll 8
@@ -492,32 +500,34 @@ bool ld_ok(int64_t ld, int64_t rows, int64_t D) {
 template <class T, int MODE>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
-  const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
+  const int64_t grid = norm_grid(a.rows, sh.G);
+  cudaError_t e;
   const int R = sh.G == 32 ? 4 : 1;
   const size_t smem = MODE == kNormOut ? 0 : (size_t)R * (size_t)((a.D + 15) / 16 * 16);
-  if (sh.G == 32) fw_norm_kernel<T, 32, 1, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128) fw_norm_kernel<T, 128, 1, MODE><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 256) fw_norm_kernel<T, 256, 1, MODE><<<grid, 256, smem, st>>>(a);
-  else if (sh.G == 512) fw_norm_kernel<T, 512, 1, MODE><<<grid, 512, smem, st>>>(a);
-  else if (sh.G == 1024 && sh.CH == 1) fw_norm_kernel<T, 1024, 1, MODE><<<grid, 1024, smem, st>>>(a);
-  else if (sh.G == 1024) fw_norm_kernel<T, 1024, 2, MODE><<<grid, 1024, smem, st>>>(a);
-  else fw_norm_long_kernel<T, MODE><<<grid, 1024, 0, st>>>(a);
-  return cudaGetLastError();
+  if (sh.G == 32) e = launch_dependent(fw_norm_kernel<T, 32, 1, MODE>, grid, 128, smem, 1, st, a);
+  else if (sh.G == 128) e = launch_dependent(fw_norm_kernel<T, 128, 1, MODE>, grid, 128, smem, 1, st, a);
+  else if (sh.G == 256) e = launch_dependent(fw_norm_kernel<T, 256, 1, MODE>, grid, 256, smem, 1, st, a);
+  else if (sh.G == 512) e = launch_dependent(fw_norm_kernel<T, 512, 1, MODE>, grid, 512, smem, 1, st, a);
+  else if (sh.G == 1024 && sh.CH == 1) e = launch_dependent(fw_norm_kernel<T, 1024, 1, MODE>, grid, 1024, smem, 1, st, a);
+  else if (sh.G == 1024) e = launch_dependent(fw_norm_kernel<T, 1024, 2, MODE>, grid, 1024, smem, 1, st, a);
+  else e = launch_dependent(fw_norm_long_kernel<T, MODE>, grid, 1024, 0, 1, st, a);
+  return e;
 }
 
 template <class T>
 cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
   const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
-  const dim3 grid((unsigned)norm_grid(a.rows, sh.G));
+  const int64_t grid = norm_grid(a.rows, sh.G);
+  cudaError_t e;
   const size_t smem = sh.G == 32 ? (size_t)a.D * sizeof(float) : 0;
-  if (sh.G == 32) fw_norm_grad_kernel<T, 32, 1><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 128) fw_norm_grad_kernel<T, 128, 1><<<grid, 128, smem, st>>>(a);
-  else if (sh.G == 256) fw_norm_grad_kernel<T, 256, 1><<<grid, 256, smem, st>>>(a);
-  else if (sh.G == 512) fw_norm_grad_kernel<T, 512, 1><<<grid, 512, smem, st>>>(a);
-  else if (sh.G == 1024 && sh.CH == 1) fw_norm_grad_kernel<T, 1024, 1><<<grid, 1024, smem, st>>>(a);
-  else if (sh.G == 1024) fw_norm_grad_kernel<T, 1024, 2><<<grid, 1024, smem, st>>>(a);
-  else fw_norm_grad_long_kernel<T><<<grid, 1024, 0, st>>>(a);
-  return cudaGetLastError();
+  if (sh.G == 32) e = launch_dependent(fw_norm_grad_kernel<T, 32, 1>, grid, 128, smem, 1, st, a);
+  else if (sh.G == 128) e = launch_dependent(fw_norm_grad_kernel<T, 128, 1>, grid, 128, smem, 1, st, a);
+  else if (sh.G == 256) e = launch_dependent(fw_norm_grad_kernel<T, 256, 1>, grid, 256, smem, 1, st, a);
+  else if (sh.G == 512) e = launch_dependent(fw_norm_grad_kernel<T, 512, 1>, grid, 512, smem, 1, st, a);
+  else if (sh.G == 1024 && sh.CH == 1) e = launch_dependent(fw_norm_grad_kernel<T, 1024, 1>, grid, 1024, smem, 1, st, a);
+  else if (sh.G == 1024) e = launch_dependent(fw_norm_grad_kernel<T, 1024, 2>, grid, 1024, smem, 1, st, a);
+  else e = launch_dependent(fw_norm_grad_long_kernel<T>, grid, 1024, 0, 1, st, a);
+  return e;
 }
 
 template <int MODE>
@@ -655,14 +665,15 @@ int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy, const 
                   : dtype == FWB_DTYPE_F16 ? launch_norm_grad<__half>(a, st)
                                            : launch_norm_grad<float>(a, st);
   if (e != cudaSuccess || !dweight) return launch_status(e);
-  const dim3 g2((unsigned)((D + 31) / 32));
+  const int64_t g2 = (D + 31) / 32;
   if (wdtype == FWB_DTYPE_BF16)
-    fw_norm_dw_kernel<__nv_bfloat16><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<__nv_bfloat16*>(dweight));
+    e = launch_dependent(fw_norm_dw_kernel<__nv_bfloat16>, g2, 1024, 0, 1, st, parts, grid, D,
+                         static_cast<__nv_bfloat16*>(dweight));
   else if (wdtype == FWB_DTYPE_F16)
-    fw_norm_dw_kernel<__half><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<__half*>(dweight));
+    e = launch_dependent(fw_norm_dw_kernel<__half>, g2, 1024, 0, 1, st, parts, grid, D, static_cast<__half*>(dweight));
   else
-    fw_norm_dw_kernel<float><<<g2, 1024, 0, st>>>(parts, grid, D, static_cast<float*>(dweight));
-  return launch_status(cudaGetLastError());
+    e = launch_dependent(fw_norm_dw_kernel<float>, g2, 1024, 0, 1, st, parts, grid, D, static_cast<float*>(dweight));
+  return launch_status(e);
 }
 
 }  // extern "C"

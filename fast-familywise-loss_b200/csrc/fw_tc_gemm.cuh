@@ -148,10 +148,6 @@ __device__ __forceinline__ int tile_in_turn(int g, int groups, int i, int n) {
   return w < n ? (int)w : -1;
 }
 
-// Lets a kernel launched as a programmatic dependent of the one before it
-// read that one's results from here on (no effect otherwise).
-__device__ __forceinline__ void wait_prior_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
 }
@@ -499,36 +495,8 @@ cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const type
   int64_t grid = max_tiles * P::CG;
   const int64_t sms = sm_count() / P::CG * P::CG;
   if (grid > sms) grid = sms;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(GemmSmem<P>::kThreads);
-  cfg.dynamicSmemBytes = GemmSmem<P>::kBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = P::CG;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = P::CG > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, fw_tc_gemm_kernel<P>, ma, mb, ma2 ? *ma2 : ma, mb2 ? *mb2 : mb, a);
-}
-
-// The same for another kernel of the chain.
-template <class... KArgs, class... Args>
-cudaError_t launch_after(void (*kernel)(KArgs...), dim3 grid, dim3 block, cudaStream_t st, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+  return launch_dependent(fw_tc_gemm_kernel<P>, grid, GemmSmem<P>::kThreads, GemmSmem<P>::kBytes, P::CG, st, ma, mb,
+                          ma2 ? *ma2 : ma, mb2 ? *mb2 : mb, a);
 }
 
 }  // namespace

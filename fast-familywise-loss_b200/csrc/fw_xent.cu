@@ -58,6 +58,7 @@ template <class T>
 __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) {
   __shared__ int red[2][kPackThreads / 32];
   constexpr int V = 16 / sizeof(T);
+  wait_prior_kernel();
   allow_dependent_launch();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * a.per_cta;
@@ -587,7 +588,9 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
   PackArgs pk = {hidden, y, B, p.Bp, D, p.Dp, ldh, V, ignore, state + p.hp, row_of, label,
                  reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, B <= 8192 ? 8 : 64};
-  fw_xent_pack_kernel<T><<<(unsigned)((p.Bp + pk.per_cta - 1) / pk.per_cta), kPackThreads, 0, st>>>(pk);
+  if (launch_dependent(fw_xent_pack_kernel<T>, (p.Bp + pk.per_cta - 1) / pk.per_cta, kPackThreads, 0, 1, st, pk) !=
+      cudaSuccess)
+    return FWB_E_LAUNCH;
   const void* w = weight;
   if (p.copy_w) {
     const int64_t need = (V * ((p.Dp + 1023) / 1024) + 7) / 8, cap = (int64_t)sm_count() * 16;
@@ -605,7 +608,7 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
   JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
                  reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + kLseCols - 1) / kLseCols), reduction, status};
-  return launch_status(launch_after(fw_xent_join_kernel, dim3((unsigned)(p.Bp / 32)), dim3(kJoinWarps * 32), st, ja));
+  return launch_status(launch_dependent(fw_xent_join_kernel, p.Bp / 32, kJoinWarps * 32, 0, 1, st, ja));
 }
 
 template <class T, TcKind K>
