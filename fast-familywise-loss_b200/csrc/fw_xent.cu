@@ -10,16 +10,22 @@
 // of exponentials; a second kernel joins the tiles' pairs, takes the losses
 // and reduces them in a fixed order.
 // Backward, in pieces of the vocabulary: the logits of a piece again, their
-// epilogue writing G (16-bit, the product's operand type: the rounding is
+// epilogue writing G (16-bit, the products' operand type: the rounding is
 // relative to each entry, so it weighs as the rounding of the result does);
 // then dH += G W and dW = G^T H of the piece in one launch, G read in both
 // orientations from the one buffer (MN-major operands), each row of dW written
 // once.
 // Bound by the tensor cores: 2 B V D operations for each of the four products.
 //
-// float16 G: exp(z - lse) / B may be under float16's smallest value, so rows
-// are scaled to the range of the type (largest upstream gradient to 2^15) and
-// the factor is taken out in fp32 after the sums.
+// The upstream factors g_r stay out of the rounding of G, whose label entry
+// -g_r would carry the rounding of g_r into a whole row (and, if all g_r are
+// 1 / B, into everything).  One factor for all rows is applied in fp32 after
+// the sums.  Factors per row are split, g_r = s_r f_r with s_r a power of two:
+// s_r goes into G, f_r in [0.5, 1) multiplies the rows of dH in fp32 and the
+// rows of H that dW is made of.
+//
+// float16 G: exp(z - lse) may be under float16's smallest value, so G is
+// scaled by 2^15 (over the largest s_r), taken out after the sums.
 #include "fw_reduce.cuh"
 #include "fw_rowslots.cuh"
 #include "fw_tc_gemm.cuh"
@@ -36,7 +42,7 @@ struct XentHead {
   int32_t rows;    // live rows
   uint32_t done;   // blocks of the joining kernel that have finished
   int32_t status;  // status bits raised inside
-  float top;       // largest upstream gradient of a live row (float16, one per row)
+  float top;       // largest s_r of a live row (float16, factors per row)
 };
 
 struct PackArgs {
@@ -311,32 +317,46 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_kernel(JoinArgs 
 }
 
 // ------------------------------------------------------------ backward
-// The upstream gradient and the scale of G.
+// The power of two above |g| (|g| itself where there is none: 0, not finite).
+__device__ __forceinline__ float pow2_above(float g) {
+  const float m = fabsf(g);
+  if (!(m > 0.0f && m < CUDART_INF_F)) return m;
+  int e;
+  frexpf(m, &e);  // m = f 2^e, f in [0.5, 1)
+  return ldexpf(1.0f, min(e, 127));
+}
+
+// The upstream gradient: the factors of G's rows (powers of two) and what is
+// left of it.
 struct Upstream {
   const float* go;  // one per given row, or one
   int per_row, mean, f16;
 
-  __device__ float over(const XentHead* h) const { return mean ? 1.0f / (float)h->rows : 1.0f; }
-  // float16: what G's rows are scaled by, largest upstream factor to kF16Unit
-  __device__ float unit(const XentHead* h) const {
-    if (!f16) return 1.0f;
-    const float top = per_row ? h->top : fabsf(go[0] * over(h));
-    return top == 0.0f ? 1.0f : top;
+  // s_r, scaled to the range of the type
+  __device__ float in_g(const XentHead* h, int r) const {
+    if (!per_row) return f16 ? kF16Unit : 1.0f;
+    const float s = pow2_above(go[r]);
+    return f16 && h->top > 0.0f ? s / h->top * kF16Unit : s;
   }
-  // factor of the row of G, given row r
-  __device__ float coef(const XentHead* h, int r) const {
-    const float g = go[per_row ? r : 0] * over(h);
-    return f16 ? g / unit(h) * kF16Unit : g;
+  // f_r; 1 where the factor is in G (0, not finite) or common
+  __device__ float rest(int r) const {
+    if (!per_row) return 1.0f;
+    const float g = go[r], s = pow2_above(g);
+    return s > 0.0f && s < CUDART_INF_F ? g / s : 1.0f;
   }
-  // factor taken out after the sums
-  __device__ float back(const XentHead* h) const { return f16 ? unit(h) / kF16Unit : 1.0f; }
+  // common factor taken out after the sums
+  __device__ float back(const XentHead* h) const {
+    if (per_row) return f16 && h->top > 0.0f ? h->top / kF16Unit : 1.0f;
+    const float g = mean ? go[0] / (float)h->rows : go[0];
+    return f16 ? g / kF16Unit : g;
+  }
 };
 
 __global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const int32_t* row_of, const float* go) {
   __shared__ float red[32];
   const int rows = head->rows;
   float top = 0.0f;
-  for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, fabsf(go[row_of[i]]));
+  for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, pow2_above(go[row_of[i]]));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
@@ -344,6 +364,25 @@ __global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const
   if (threadIdx.x == 0) {
     for (int i = 1; i < 32; ++i) top = max_nan(top, red[i]);
     head->top = top;
+  }
+}
+
+// The packed rows of H times f_r: dW's operand where the factors differ.
+template <class T>
+__global__ void __launch_bounds__(256) fw_xent_scale_kernel(const XentHead* head, const int32_t* row_of, Upstream up,
+                                                            const T* hp, T* out, int64_t Dp) {
+  constexpr int V = 16 / sizeof(T);
+  const int rows = head->rows, rows_up = (rows + kTileM - 1) / kTileM * kTileM;
+  const int64_t slots = Dp / V;
+  for (int r = blockIdx.x; r < rows_up; r += gridDim.x) {
+    const float f = r < rows ? up.rest(row_of[r]) : 0.0f;
+    for (int64_t i = threadIdx.x; i < slots; i += 256) {
+      float v[V];
+      unpack16<T>(*reinterpret_cast<const uint4*>(hp + r * Dp + i * V), v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = r < rows ? v[j] * f : 0.0f;
+      *reinterpret_cast<uint4*>(out + r * Dp + i * V) = pack16<T>(v);
+    }
   }
 }
 
@@ -383,7 +422,7 @@ struct GradTile {
     const bool live = row < a.head->rows;
     const int y = live ? a.label[row] : -1;
     const float lse = live ? a.lse[row] : 0.0f;
-    const float coef = live ? a.up.coef(a.head, a.row_of[row]) : 0.0f;
+    const float coef = live ? a.up.in_g(a.head, a.row_of[row]) : 0.0f;
     T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
@@ -478,6 +517,7 @@ struct ProductTile {
     const int r0 = t.m0 + p.row;
     const int live = a.head->rows - r0;  // dH: the warp's rows behind these are ignored ones
     const int mine = t.kind == 0 ? a.row_of[r0 + p.lane] : -1;
+    const float row_back = t.kind == 0 && p.lane < live ? back * a.up.rest(mine) : 0.0f;
     const int rows = a.V - (a.v0 + r0);  // dW
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
@@ -512,7 +552,7 @@ struct ProductTile {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = p.lane < live && t.nk > 0 ? v[i] * back : 0.0f;
+      for (int i = 0; i < 32; ++i) v[i] = p.lane < live && t.nk > 0 ? v[i] * row_back : 0.0f;
       T* out = static_cast<T*>(a.dhidden) + c0;
       store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
         const int r = __shfl_sync(kFull, mine, i);
@@ -536,7 +576,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, zy, loss_pack, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, g, sum, bwd_bytes;
+  int64_t piece, pieces, g, sum, hs, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
@@ -564,6 +604,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   at = 0;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
   p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * up(D, 32), 256) : 0;
+  p.hs = at, at += up(2 * p.Bp * p.Dp, 256);  // factors per row
   p.bwd_bytes = at;
   return p;
 }
@@ -621,14 +662,23 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   const void* w = p.copy_w ? state + p.wp : weight;
   if (p.copy_w) ldw = p.Dp;
   const Upstream u = {go, per_row, mean, K == kTcF16};
-  if (u.f16 && per_row) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go);
-  if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+  char* hw = state + p.hp;  // dW's operand
+  if (per_row) {
+    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go);
+    if (dweight) {
+      hw = ws + p.hs;
+      const int64_t cap = (int64_t)sm_count() * 8;
+      fw_xent_scale_kernel<T><<<(unsigned)(p.Bp < cap ? p.Bp : cap), 256, 0, st>>>(
+          head, row_of, u, reinterpret_cast<const T*>(state + p.hp), reinterpret_cast<T*>(hw), p.Dp);
+    }
+    if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+  }
   CUtensorMap mh, mw, mg, wmn, gmn, hmn;
   char* hp = state + p.hp;
   char* g = ws + p.g;
   if (!tc_map(&mh, K, hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 128) ||
       !tc_map(&mg, K, g, p.Bp, p.piece, p.piece, 128) || !tc_map(&wmn, K, w, V, D, ldw, 64) ||
-      !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hp, p.Bp, D, p.Dp, 64))
+      !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hw, p.Bp, D, p.Dp, 64))
     return FWB_E_LAUNCH;
   const int64_t Vp = up(V, 256), mb = p.Bp / 256, nd = (D + 255) / 256;
   const int vec = aligned16(dhidden) && aligned16(dweight) && D % 8 == 0;
