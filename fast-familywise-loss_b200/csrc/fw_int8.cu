@@ -25,7 +25,7 @@ struct Int8Args {
   void* out;
   int64_t ldo;
   int T, N, K;
-  int vec;  // rows of out start on 16-byte boundaries
+  int vec;  // fp32 rows of out start on 16-byte boundaries
   int per;  // few tokens: weight rows per CTA behind the whole tiles
   int32_t* status;
 };
@@ -39,8 +39,8 @@ struct Int8Many {
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr bool TWO = false, A_MN2 = false;
-  static constexpr int CG = 2, BN = 256, STAGES = 6, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
-  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
+  static constexpr int CG = 2, BN = 256, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
+  static constexpr uint32_t EPI_BYTES = EW * (sizeof(TO) == 2 ? kStageBytes : 32 * 33 * 4);
   __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
     const int mt = (a.T + 255) / 256, nt = (a.N + 255) / 256;
     const int w = tile_in_turn(group, groups, i, mt * nt);
@@ -53,23 +53,26 @@ struct Int8Many {
   }
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
-    float* sm = reinterpret_cast<float*>(p.smem);
-    const int r0 = t.m0 + p.row;
-    const float qs = r0 + p.lane < a.T ? a.qs[r0 + p.lane] : 0.0f;
-    TO* out = static_cast<TO*>(a.out);
-    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
-      const int n0 = t.n0 + c;
-      const float ws = n0 + p.lane < a.N ? a.ws[n0 + p.lane] : 0.0f;
+    const int r0 = t.m0 + p.row, rows = a.T - r0, s0 = p.share * (BN / 2);
+    const float qs = p.lane < rows ? a.qs[r0 + p.lane] : 0.0f;
+    TO* out = static_cast<TO*>(a.out) + t.n0 + s0;
+    for (int c = 0; c < BN / 2; c += 32) {
+      const int n = t.n0 + s0 + c + p.lane;
+      const float ws = n < a.N ? a.ws[n] : 0.0f;
       float v[32];
-      tmem_ld32(p.taddr + c, v);
-      if (c + 32 == (p.share + 1) * (BN / 2)) done();
+      tmem_ld32(p.taddr + s0 + c, v);
+      if (c + 32 == BN / 2) done();
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * qs * __shfl_sync(kFull, ws, i);
-      const int rows = a.T - r0;
-      store_block<TO>(sm, v, p.lane, a.N - n0, a.vec, [&](int i) -> TO* {
-        return i < rows ? out + (int64_t)(r0 + i) * a.ldo + n0 : nullptr;
-      });
+      if constexpr (sizeof(TO) == 2)
+        stage_block<TO>(reinterpret_cast<uint32_t*>(p.smem), v, p.lane, c);
+      else
+        store_block(reinterpret_cast<float*>(p.smem), v, p.lane, a.N - (t.n0 + s0 + c), a.vec,
+                    [&](int i) -> float* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo + c : nullptr; });
     }
+    if constexpr (sizeof(TO) == 2)
+      store_staged<TO>(reinterpret_cast<uint32_t*>(p.smem), p.lane, min(BN / 2, a.N - (t.n0 + s0)),
+                       [&](int i) -> TO* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo : nullptr; });
   }
 };
 

@@ -400,14 +400,14 @@ done:
   }
 }
 
-// The warp's 32 x 32 block of values, one row per thread, turned through
-// shared memory and stored as rows of T: 16 bytes per lane where the rows are
+// The warp's 32 x 32 block of fp32 values, one row per thread, turned through
+// shared memory and stored as rows: 16 bytes per lane where the rows are
 // aligned (`vec`), else one element per lane.  row_ptr(i) is where column 0 of
 // the block's row i goes, or NULL.
-template <class T, class RowPtr>
+template <class RowPtr>
 __device__ __forceinline__ void store_block(float* sm, const float (&v)[32], int lane, int cols, bool vec,
                                             RowPtr row_ptr) {
-  constexpr int V = 16 / sizeof(T), LANES = 32 / V, ROWS = 32 / LANES;  // lanes per row, rows per step
+  constexpr int V = 4, LANES = 32 / V, ROWS = 32 / LANES;  // lanes per row, rows per step
 #pragma unroll
   for (int i = 0; i < 32; ++i) sm[lane * 33 + i] = v[i];
   __syncwarp();
@@ -416,18 +416,62 @@ __device__ __forceinline__ void store_block(float* sm, const float (&v)[32], int
 #pragma unroll
     for (int i0 = 0; i0 < 32; i0 += ROWS) {
       const int i = i0 + lane / LANES;
-      T* p = row_ptr(i);
-      float x[V];
-#pragma unroll
-      for (int j = 0; j < V; ++j) x[j] = sm[i * 33 + c + j];
-      if (p && c < cols) *reinterpret_cast<uint4*>(p + c) = pack16<T>(x);  // cols is a multiple of V
+      float* p = row_ptr(i);
+      const float* x = sm + i * 33 + c;
+      if (p && c < cols) *reinterpret_cast<float4*>(p + c) = make_float4(x[0], x[1], x[2], x[3]);  // cols: a multiple of V
     }
   } else {
 #pragma unroll 4
     for (int i = 0; i < 32; ++i) {
-      T* p = row_ptr(i);
-      if (p && lane < cols) st_elem(p + lane, sm[i * 33 + lane]);
+      float* p = row_ptr(i);
+      if (p && lane < cols) p[lane] = sm[i * 33 + lane];
     }
+  }
+  __syncwarp();
+}
+
+// A warp's 32 x 128 block of 16-bit values: staged one row per thread, then
+// stored row by row.  Rows may start anywhere: the stores are the 16-byte
+// slots of the destination, single elements only at a segment's two ends (32
+// lanes of 2 bytes each would write parts of sectors, at a fifth of the rate).
+constexpr int kStageWords = 65;  // 32-bit words of a row: 64, and one against bank conflicts
+constexpr uint32_t kStageBytes = 32 * kStageWords * 4;
+
+template <class T>
+__device__ __forceinline__ void stage_block(uint32_t* sm, const float (&v)[32], int lane, int c) {
+  static_assert(sizeof(T) == 2, "16-bit types");
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    sm[lane * kStageWords + c / 2 + i] = Elem<T>::f_to_bits(v[2 * i]) | (Elem<T>::f_to_bits(v[2 * i + 1]) << 16);
+}
+
+// `cols` columns of every row, 16 lanes per row; row_ptr(i) is where column 0
+// of row i goes, or NULL.
+template <class T, class RowPtr>
+__device__ __forceinline__ void store_staged(const uint32_t* sm, int lane, int cols, RowPtr row_ptr) {
+  __syncwarp();
+  const int k = lane & 15;
+#pragma unroll 4
+  for (int i0 = 0; i0 < 32; i0 += 2) {
+    const int i = i0 + (lane >> 4);
+    unsigned short* p = reinterpret_cast<unsigned short*>(row_ptr(i));
+    const uint32_t* row = sm + i * kStageWords;
+    // elements before the first slot, slots, elements behind the last
+    const int head = min((int)(-(reinterpret_cast<uintptr_t>(p) >> 1) & 7u), cols);
+    const int whole = (cols - head) >> 3, tail = head + whole * 8;
+    if (p && k < whole) {
+      const int e0 = head + k * 8;
+      const uint32_t* w = row + (e0 >> 1);
+      uint4 u = make_uint4(w[0], w[1], w[2], w[3]);
+      if (head & 1) {
+        const uint32_t last = w[4];
+        u = make_uint4(__funnelshift_r(u.x, u.y, 16), __funnelshift_r(u.y, u.z, 16), __funnelshift_r(u.z, u.w, 16),
+                       __funnelshift_r(u.w, last, 16));
+      }
+      *reinterpret_cast<uint4*>(p + e0) = u;
+    }
+    const int e = k < 8 ? k : tail + k - 8;  // lanes 0..7: head, 8..15: tail
+    if (p && e < (k < 8 ? head : cols)) p[e] = (unsigned short)(row[e >> 1] >> (16 * (e & 1)));
   }
   __syncwarp();
 }

@@ -443,18 +443,20 @@ struct GradTile {
 
 // dH += G W and dW = G^T H of a piece, in one launch: the few long tiles of dH
 // (all of the piece's columns are their K) would leave most of the last round
-// of SMs idle, so the tiles of dW fill it up.
+// of SMs idle, so the tiles of dW fill it up.  With fewer tiles of dH than CTA
+// pairs, K is cut into `splits` parts with an fp32 sum each, which a last
+// small kernel adds in order.
 struct ProductArgs {
   const XentHead* head;
   const int32_t* row_of;
   Upstream up;
-  float* sum;     // dH so far, [Bp, lds], where the vocabulary has several pieces, else NULL
+  float* sum;     // dH so far, [splits, Bp, lds]; NULL for one piece and one split
   void* dhidden;  // [B, D] or NULL
   void* dweight;  // [V, D] or NULL
   int Bp, V, D, lds;
   int v0, vn;  // first column of the piece, its columns rounded up to 256
   int first, last;
-  int vec;  // rows of dhidden and dweight start on 16-byte boundaries
+  int splits;
   int32_t* status;
 };
 
@@ -464,26 +466,27 @@ struct ProductTile {
   using State = NoState;
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
-  static constexpr int CG = 2, BN = kTileN, STAGES = 6, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
-  static constexpr uint32_t EPI_BYTES = EW * 32 * 33 * 4;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
+  static constexpr uint32_t EPI_BYTES = EW * kStageBytes;
 
-  // Tiles: `long_` of dH with vn / 64 stages each, then `shorts` of dW with
-  // rows / 64, then (last piece) those of dH that hold only ignored rows.  A
-  // CTA group takes its long tiles in turn; with `more` groups having one more
+  // Tiles: the long ones of dH with vn / 64 / splits stages each, then the
+  // short ones of dW with rows / 64, then (last piece, one split) those of dH
+  // that hold only ignored rows.  A CTA group takes its long tiles in turn; with `more` groups having one more
   // than the others, the short ones go to the others first, until all are
   // level, then to all in turn.
   __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
     const int nt = (a.D + BN - 1) / BN, mt = a.dhidden ? row_tiles(a.head) : 0;
-    const int k_long = a.vn / 64, k_short = (a.head->rows + 63) / 64;
+    const int k_all = a.vn / 64, k_long = (k_all + a.splits - 1) / a.splits, k_short = (a.head->rows + 63) / 64;
     const int vt = a.dweight ? (min(a.vn, a.V - a.v0) + kTileM - 1) / kTileM : 0;
-    const int dead = a.dhidden && a.last ? a.Bp / kTileM - mt : 0;
-    const int n_long = mt * nt, n_short = vt * nt, n_rest = n_short + dead * nt;
+    const int dead = a.dhidden && a.last && a.splits == 1 ? a.Bp / kTileM - mt : 0;
+    const int n_one = mt * nt, n_long = n_one * a.splits, n_short = vt * nt, n_rest = n_short + dead * nt;
     const int q = n_long / groups, more = n_long % groups;
     const int mine = q + (group < more ? 1 : 0);
     int m, n;
     if (i < mine) {
-      tile_order(i * groups + group, mt, nt, 8, &m, &n);
-      *t = {m * kTileM, n * BN, 0, a.v0, k_long, 128, 0};
+      const int w = i * groups + group, part = w / n_one, k0 = (int)((int64_t)k_all * part / a.splits);
+      tile_order(w - part * n_one, mt, nt, 8, &m, &n);
+      *t = {m * kTileM, n * BN, k0 * 64, a.v0 + k0 * 64, (int)((int64_t)k_all * (part + 1) / a.splits) - k0, part, 0};
       return true;
     }
     i -= mine;
@@ -502,65 +505,93 @@ struct ProductTile {
     if (w >= n_rest) return false;
     if (w < n_short) {
       tile_order((int)w, vt, nt, 5, &m, &n);
-      *t = {m * kTileM, n * BN, 0, 0, k_short, 128, 1};
+      *t = {m * kTileM, n * BN, 0, 0, k_short, 0, 1};
     } else {
       const int d = (int)w - n_short;
-      *t = {(mt + d / nt) * kTileM, d % nt * BN, 0, 0, 0, 128, 0};
+      *t = {(mt + d / nt) * kTileM, d % nt * BN, 0, 0, 0, 0, 0};
     }
     return true;
   }
 
   template <class Done>
   __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
-    float* sm = reinterpret_cast<float*>(p.smem);
+    uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
     const float back = a.up.back(a.head);
-    const int r0 = t.m0 + p.row;
-    const int live = a.head->rows - r0;  // dH: the warp's rows behind these are ignored ones
-    const int mine = t.kind == 0 ? a.row_of[r0 + p.lane] : -1;
-    const float row_back = t.kind == 0 && p.lane < live ? back * a.up.rest(mine) : 0.0f;
-    const int rows = a.V - (a.v0 + r0);  // dW
-    for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
+    const int r0 = t.m0 + p.row, s0 = p.share * (BN / 2);
+    const int cols = a.D - (t.n0 + s0);
+    const bool dh = t.kind == 0, any = t.nk > 0;  // without stages of K the accumulator was never written
+    const int live = a.head->rows - r0;           // dH: the warp's rows behind these are ignored ones
+    const int mine = dh ? a.row_of[r0 + p.lane] : -1;
+    const bool zero = !any || (dh && p.lane >= live);
+    const float f = zero ? 0.0f : dh ? back * a.up.rest(mine) : back;
+    const bool summed = dh && a.sum && any;  // t.rows: the split
+    const bool store = dh ? a.splits == 1 && a.last : true;
+    float* sum = summed ? a.sum + ((int64_t)t.rows * a.Bp + r0 + p.lane) * a.lds + t.n0 + s0 : nullptr;
+    for (int c = 0; c < BN / 2; c += 32) {
       float v[32];
-      tmem_ld32(p.taddr + c, v);
-      if (c + 32 == (p.share + 1) * (BN / 2)) done();
-      const int c0 = t.n0 + c;
-      const int cols = min(32, a.D - c0);
-      if (cols <= 0) continue;
-      if (t.kind == 1) {
-        if (rows <= 0) continue;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = t.nk == 0 ? 0.0f : v[i] * back;  // no live row: nothing was accumulated
-        T* out = static_cast<T*>(a.dweight) + (int64_t)(a.v0 + r0) * a.D + c0;
-        store_block<T>(sm, v, p.lane, cols, a.vec,
-                       [&](int i) -> T* { return i < rows ? out + (int64_t)i * a.D : nullptr; });
-        continue;
-      }
-      if (a.sum && t.nk > 0) {  // several pieces: this thread's own row of the sum so far
-        float* s = a.sum + (int64_t)(r0 + p.lane) * a.lds + c0;  // lds: D rounded up to 32
+      tmem_ld32(p.taddr + s0 + c, v);
+      if (c + 32 == BN / 2) done();
+      if (c >= cols) continue;
+      if (summed) {  // this thread's own row of the sum so far; lds is D rounded up to 32
         if (!a.first) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const float4 x = *reinterpret_cast<const float4*>(s + i);
+            const float4 x = *reinterpret_cast<const float4*>(sum + c + i);
             v[i] += x.x, v[i + 1] += x.y, v[i + 2] += x.z, v[i + 3] += x.w;
           }
         }
-        if (!a.last) {
+        if (!store) {
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<float4*>(s + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          continue;
+            *reinterpret_cast<float4*>(sum + c + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
         }
       }
+      if (!store) continue;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = p.lane < live && t.nk > 0 ? v[i] * row_back : 0.0f;
-      T* out = static_cast<T*>(a.dhidden) + c0;
-      store_block<T>(sm, v, p.lane, cols, a.vec, [&](int i) -> T* {
-        const int r = __shfl_sync(kFull, mine, i);
-        return r >= 0 ? out + (int64_t)r * a.D : nullptr;
-      });
+      for (int i = 0; i < 32; ++i) v[i] = zero ? 0.0f : v[i] * f;
+      stage_block<T>(sm, v, p.lane, c);
     }
+    if (!store || cols <= 0) return;
+    const int rows = a.V - (a.v0 + r0);  // dW
+    T* out = (dh ? static_cast<T*>(a.dhidden) : static_cast<T*>(a.dweight) + (int64_t)(a.v0 + r0) * a.D) + t.n0 + s0;
+    store_staged<T>(sm, p.lane, min(cols, BN / 2), [&](int i) -> T* {
+      const int r = dh ? __shfl_sync(kFull, mine, i) : i < rows ? i : -1;
+      return r >= 0 ? out + (int64_t)r * a.D : nullptr;
+    });
   }
 };
+
+// dH from the sums of its splits; one warp per row and 128 columns.
+template <class T>
+__global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
+  wait_prior_kernel();
+  allow_dependent_launch();
+  const int lane = threadIdx.x & 31;
+  const int slabs = (a.D + 127) / 128;
+  const int64_t work = (int64_t)a.Bp * slabs, nw = (int64_t)gridDim.x * 8;
+  const int rows = a.head->rows;
+  const float back = a.up.back(a.head);
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < work; i += nw) {
+    const int r = (int)(i / slabs), c = (int)(i % slabs) * 128 + lane * 4;
+    const int to = a.row_of[r];
+    if (to < 0 || c >= a.D) continue;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (r < rows) {
+#pragma unroll 4
+      for (int q = 0; q < a.splits; ++q) {
+        const float4 x = *reinterpret_cast<const float4*>(a.sum + ((int64_t)q * a.Bp + r) * a.lds + c);
+        v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      const float f = back * a.up.rest(to);
+      v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+    }
+    T* out = static_cast<T*>(a.dhidden) + (int64_t)to * a.D + c;
+    const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < a.D) st_elem(out + j, x[j]);
+  }
+}
 
 // ------------------------------------------------------------ host
 // Bytes of G that one piece of the vocabulary may take.
@@ -576,7 +607,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, zy, loss_pack, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, g, sum, hs, bwd_bytes;
+  int64_t piece, pieces, splits, g, sum, hs, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
@@ -603,7 +634,11 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.pieces = (Vp + p.piece - 1) / p.piece;
   at = 0;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
-  p.sum = at, at += p.pieces > 1 ? up(4 * p.Bp * up(D, 32), 256) : 0;
+  // dH's tiles for every CTA pair, at least 16 stages of K each
+  p.splits = B > 0 ? sm_count() / 2 / ((p.Bp / kTileM) * ((D + kTileN - 1) / kTileN)) : 1;
+  if (p.splits > p.piece / 64 / 16) p.splits = p.piece / 64 / 16;
+  if (p.splits < 1) p.splits = 1;
+  p.sum = at, at += p.pieces > 1 || p.splits > 1 ? up(4 * p.splits * p.Bp * up(D, 32), 256) : 0;
   p.hs = at, at += up(2 * p.Bp * p.Dp, 256);  // factors per row
   p.bwd_bytes = at;
   return p;
@@ -681,17 +716,21 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
       !tc_map(&gmn, K, g, p.Bp, p.piece, p.piece, 64) || !tc_map(&hmn, K, hw, p.Bp, D, p.Dp, 64))
     return FWB_E_LAUNCH;
   const int64_t Vp = up(V, 256), mb = p.Bp / 256, nd = (D + 255) / 256;
-  const int vec = aligned16(dhidden) && aligned16(dweight) && D % 8 == 0;
-  float* sum = p.pieces > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
+  float* sum = p.pieces > 1 || p.splits > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
     const GradArgs ga = {head, label, row_of, reinterpret_cast<float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
                          v0, vn, status};
     if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
     const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
-                            i == 0, i == p.pieces - 1, vec, status};
-    const int64_t tiles = (dhidden ? mb * nd : 0) + (dweight ? vn / 256 * nd : 0);
+                            i == 0, i == p.pieces - 1, (int)p.splits, status};
+    const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
     if (launch_gemm<ProductTile<T, K>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
+    if (dhidden && pa.last && p.splits > 1) {
+      const int64_t need = (p.Bp * ((D + 127) / 128) + 7) / 8, cap = (int64_t)sm_count() * 16;
+      if (launch_dependent(fw_xent_dhidden_kernel<T>, need < cap ? need : cap, 256, 0, 1, st, pa) != cudaSuccess)
+        return FWB_E_LAUNCH;
+    }
   }
   return FWB_OK;
 }
