@@ -41,18 +41,26 @@ struct Int8Many {
   static constexpr bool TWO = false, A_MN2 = false;
   static constexpr int CG = 2, BN = 256, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = EW * (sizeof(TO) == 2 ? kStageBytes : 32 * 33 * 4);
-  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
-    const int mt = (a.T + 255) / 256, nt = (a.N + 255) / 256;
-    const int w = tile_in_turn(group, groups, i, mt * nt);
-    if (w < 0) return false;
-    constexpr int kGroup = 16;  // token blocks that share the weight tiles in flight
-    const int g = w / (kGroup * nt), r = w - g * kGroup * nt;
-    const int gm = min(kGroup, mt - g * kGroup);
-    *t = {(g * kGroup + r % gm) * 256, (r / gm) * 256, 0, 0, (a.K + 127) / 128, 128, 0};
+  struct Plan {
+    TileOrder order;
+    int first, step;
+  };
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
+    p->order.set((a.T + 255) / 256, (a.N + 255) / 256, 16);  // token blocks that share the weight tiles in flight
+    p->first = group;
+    p->step = groups;
+  }
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
+    const int w = p.first + i * p.step;
+    if (w >= p.order.count()) return false;
+    int m, n;
+    p.order.get(w, &m, &n);
+    *t = {m * 256, n * 256, 0, 0, (a.K + 127) / 128, 128, 0};
     return true;
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State&, int, int,
+                                  Done done) {
     const int r0 = t.m0 + p.row, rows = a.T - r0, s0 = p.share * (BN / 2);
     const float qs = p.lane < rows ? a.qs[r0 + p.lane] : 0.0f;
     TO* out = static_cast<TO*>(a.out) + t.n0 + s0;
@@ -86,13 +94,20 @@ struct Int8Few {
   static constexpr int CG = 1, BN = NT, KC = 0, EW = 4, A_BOX = 32, AHEAD = 16;
   static constexpr int STAGES = NT <= 32 ? 10 : NT <= 64 ? 8 : 6;
   static constexpr uint32_t EPI_BYTES = 0;
+  struct Plan {
+    int group, groups, rounds;
+  };
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
+    p->group = group;
+    p->groups = groups;
+    p->rounds = a.N / 128 / groups;
+  }
   // whole tiles in turn, then what is left in equal parts
-  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
-    const int rounds = a.N / 128 / groups;
-    int m0 = (i * groups + group) * 128, rows = 128;
-    if (i >= rounds) {
-      if (i > rounds) return false;
-      m0 = rounds * groups * 128 + group * a.per;
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
+    int m0 = (i * p.groups + p.group) * 128, rows = 128;
+    if (i >= p.rounds) {
+      if (i > p.rounds) return false;
+      m0 = p.rounds * p.groups * 128 + p.group * a.per;
       rows = min(a.per, a.N - m0);
       if (rows <= 0) return false;
     }
@@ -100,7 +115,8 @@ struct Int8Few {
     return true;
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State&, int, int,
+                                  Done done) {
     const int n = t.m0 + p.row + p.lane;
     const bool mine = p.row + p.lane < t.rows;
     const float ws = mine ? a.ws[n] : 0.0f;

@@ -141,12 +141,39 @@ struct TcTile {
   int kind;    // which of two products (operators with TWO)
 };
 
-// The i-th of `n` tiles for CTA group `g` of `groups` when they are dealt out
-// in turn; -1 past the end.
-__device__ __forceinline__ int tile_in_turn(int g, int groups, int i, int n) {
-  const int64_t w = (int64_t)i * groups + g;
-  return w < n ? (int)w : -1;
-}
+// Division of n < 2^31 by a divisor met again and again: a multiplication and
+// a shift (the multiplier is 2^32 (2^s - d) / d + 1 for 2^s >= d).
+struct FastDiv {
+  uint32_t d, mul, shift;
+  __device__ __forceinline__ void set(int divisor) {
+    d = (uint32_t)max(divisor, 1);
+    shift = d > 1 ? 32 - __clz((int)d - 1) : 0;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d) + 1u;
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+  }
+};
+
+// Order of mt x nt tiles: blocks of `group` rows of tiles, the row fastest
+// inside one, so that the tiles in flight share their operands in L2.
+struct TileOrder {
+  int mt, nt, group;
+  FastDiv by_block, by_group, by_tail;
+  __device__ __forceinline__ void set(int m_tiles, int n_tiles, int group_) {
+    mt = m_tiles, nt = n_tiles, group = group_;
+    by_block.set(group * nt);
+    by_group.set(group);
+    by_tail.set(mt % group);
+  }
+  __device__ __forceinline__ int count() const { return mt * nt; }
+  __device__ __forceinline__ void get(int w, int* m, int* n) const {
+    const int g = by_block.div(w), r = w - g * group * nt;
+    const bool tail = (g + 1) * group > mt;
+    *n = tail ? by_tail.div(r) : by_group.div(r);
+    *m = g * group + r - *n * (tail ? (int)by_tail.d : group);
+  }
+};
 
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
@@ -170,9 +197,11 @@ struct TcPart {
 //   AHEAD            loads of A brought into L2 before the previous kernel's
 //                    results are waited for (0: none; A is not written by it,
 //                    or the copy in L2 is brought up to date by the write)
-//   get(args, group, groups, i, &tile)  i-th tile of a CTA group; false: done
+//   struct Plan, plan(args, group, groups, &plan)  what the tiles of a CTA
+//                    group follow from, worked out once per CTA
+//   get(args, plan, i, &tile)  i-th tile of the CTA group; false: done
 //   struct State     what an epilogue thread keeps over a tile's parts
-//   epilogue(args, tile, part, state, k, parts, done): part k of the
+//   epilogue(args, plan, tile, part, state, k, parts, done): part k of the
 //                    tile's `parts`; done() hands the accumulator back once
 //                    its last column has been read.
 template <class P>
@@ -213,6 +242,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   const int lane = threadIdx.x & 31;
   const int rank = CG == 2 ? (int)cluster_rank() : 0;
   const int group = (int)blockIdx.x / CG, groups = (int)gridDim.x / CG;
+  __shared__ typename P::Plan plan;
   if (threadIdx.x == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(&full[s], 1);
@@ -229,8 +259,10 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   }
   if constexpr (P::AHEAD > 0) {
     if (threadIdx.x == 32 * 2) {
+      typename P::Plan early;
+      P::plan(a, group, groups, &early);
       TcTile t;
-      if (P::get(a, group, groups, 0, &t))
+      if (P::get(a, early, 0, &t))
         for (int kb = 0; kb < min(t.nk, P::AHEAD); ++kb)
           for (int i = 0; i < t.rows; i += P::A_BOX) tma_prefetch_2d(&tm_a2, t.ak + kb * kStep, t.m0 + i);
     }
@@ -253,6 +285,8 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   wait_prior_kernel();  // every thread: what follows reads its results
   allow_dependent_launch();
+  if (threadIdx.x == 0) P::plan(a, group, groups, &plan);
+  __syncthreads();
 
   uint32_t issued = 0u, issued_par = 0u;  // stages with a copy issued, and its parity
   bool mma_any = false;
@@ -260,7 +294,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
 
   if (warp == 0) {
     uint32_t s = 0, ph = 0;
-    for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
+    for (int it = 0; P::get(a, plan, it, &t); ++it) {
       const int m = t.m0 + rank * kGemmBM, n = t.n0 + rank * (P::BN / CG);
       const CUtensorMap* ma = P::TWO && t.kind ? &tm_a2 : &tm_a;
       const CUtensorMap* mb = P::TWO && t.kind ? &tm_b2 : &tm_b;
@@ -303,7 +337,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
   } else if (warp == 1) {
     uint32_t s = 0, ph = 0, acc = 0, aph = 0;
     if (rank == 0) {
-      for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
+      for (int it = 0; P::get(a, plan, it, &t); ++it) {
         const bool a_mn = P::TWO && t.kind ? P::A_MN2 : P::A_MN;
         const uint32_t idesc = gemm_idesc(P::KIND, a_mn, P::B_MN, kGemmBM * CG, P::BN);
         const int kc = P::KC == 0 ? max(t.nk, 1) : P::KC;
@@ -351,7 +385,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     part.lane = lane;
     part.share = (warp - 2) >> 2;
     part.smem = smE + (warp - 2) * (P::EPI_BYTES / P::EW);
-    for (int it = 0; P::get(a, group, groups, it, &t); ++it) {
+    for (int it = 0; P::get(a, plan, it, &t); ++it) {
       const int parts = P::KC == 0 ? 1 : max((t.nk + P::KC - 1) / (P::KC == 0 ? 1 : P::KC), 1);
       typename P::State state{};
       for (int k = 0; k < parts; ++k) {
@@ -359,7 +393,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
         tc_fence_after();
         part.taddr = tmem + (uint32_t)((quad * 32) << 16) + acc * P::BN;
         const uint32_t te = CG == 2 ? in_cta(&tempty[acc], 0) : smem_u32(&tempty[acc]);
-        P::epilogue(a, t, part, state, k, parts, [te, lane] {
+        P::epilogue(a, plan, t, part, state, k, parts, [te, lane] {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_at(te);

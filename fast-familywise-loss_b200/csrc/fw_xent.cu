@@ -160,14 +160,22 @@ constexpr int kTileM = 256, kTileN = 256;  // of a pair of CTAs
 
 __device__ __forceinline__ int row_tiles(const XentHead* h) { return (h->rows + kTileM - 1) / kTileM; }
 
-// Order of tiles: blocks of `group` m-blocks, m fastest inside one, so that
-// the tiles in flight share their operands in L2.
-__device__ __forceinline__ void tile_order(int w, int mt, int nt, int group, int* m, int* n) {
-  const int g = w / (group * nt), r = w - g * group * nt;
-  const int gm = min(group, mt - g * group);
-  *m = g * group + r % gm;
-  *n = r / gm;
-}
+// Tiles dealt out in turn.
+struct TurnPlan {
+  TileOrder order;
+  int first, step;
+  __device__ __forceinline__ void set(int mt, int nt, int group, int groups) {
+    order.set(mt, nt, 16);
+    first = group;
+    step = groups;
+  }
+  __device__ __forceinline__ bool get(int i, int* m, int* n) const {
+    const int w = first + i * step;
+    if (w >= order.count()) return false;
+    order.get(w, m, n);
+    return true;
+  }
+};
 
 // ------------------------------------------------------------ forward
 struct LseArgs {
@@ -197,17 +205,19 @@ struct LseTile {
   static constexpr bool TWO = false, A_MN2 = false;
   static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = kLseStages, EW = 4 * BN / kLseCols, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
-    const int mt = row_tiles(a.head), nt = (a.V + BN - 1) / BN, w = tile_in_turn(group, groups, i, mt * nt);
-    if (w < 0) return false;
+  using Plan = TurnPlan;
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
+    p->set(row_tiles(a.head), (a.V + BN - 1) / BN, group, groups);
+  }
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
     int m, n;
-    tile_order(w, mt, nt, 16, &m, &n);
+    if (!p.get(i, &m, &n)) return false;
     *t = {m * kTileM, n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
     return true;
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State& st, int k, int parts,
-                                  Done done) {
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int k,
+                                  int parts, Done done) {
 #pragma unroll
     for (int c = 0; c < kLseCols; c += 16) {
       float v[16];
@@ -408,16 +418,19 @@ struct GradTile {
   static constexpr bool TWO = false, A_MN2 = false;
   static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
   static constexpr uint32_t EPI_BYTES = 0;
-  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
-    const int mt = row_tiles(a.head), nt = a.vn / BN, w = tile_in_turn(group, groups, i, mt * nt);
-    if (w < 0) return false;
+  using Plan = TurnPlan;
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
+    p->set(row_tiles(a.head), a.vn / BN, group, groups);
+  }
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
     int m, n;
-    tile_order(w, mt, nt, 16, &m, &n);
+    if (!p.get(i, &m, &n)) return false;
     *t = {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
     return true;
   }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State&, int, int,
+                                  Done done) {
     const int row = t.m0 + p.row + p.lane;
     const bool live = row < a.head->rows;
     const int y = live ? a.label[row] : -1;
@@ -443,21 +456,37 @@ struct GradTile {
 
 // dH += G W and dW = G^T H of a piece, in one launch: the few long tiles of dH
 // (all of the piece's columns are their K) would leave most of the last round
-// of SMs idle, so the tiles of dW fill it up.  With fewer tiles of dH than CTA
-// pairs, K is cut into `splits` parts with an fp32 sum each, which a last
-// small kernel adds in order.
+// of SMs idle, so the tiles of dW fill it up.  Where one of them is longer than
+// a CTA pair's share of all stages, K is cut into splits with an fp32 sum
+// each, which a last small kernel adds in order.
+
+// A short tile in stages of K: its stages, or its epilogue where that takes longer.
+__device__ __forceinline__ int short_cost(int stages) { return max(stages, 16); }
+
 struct ProductArgs {
   const XentHead* head;
   const int32_t* row_of;
   Upstream up;
-  float* sum;     // dH so far, [splits, Bp, lds]; NULL for one piece and one split
+  float* sum;     // dH so far, [max_splits, Bp, lds]; not there for one piece and one split
   void* dhidden;  // [B, D] or NULL
   void* dweight;  // [V, D] or NULL
   int Bp, V, D, lds;
   int v0, vn;  // first column of the piece, its columns rounded up to 256
   int first, last;
-  int splits;
+  int piece;       // columns of a whole piece, a multiple of 256
+  int max_splits;  // sums there is room for
+  int pairs;       // CTA pairs of the launch
   int32_t* status;
+
+  __device__ int v_tiles() const { return dweight ? (min(vn, V - v0) + kTileM - 1) / kTileM : 0; }
+  // The same for every piece (whole ones are taken to reckon with).
+  __device__ int splits() const {
+    if (max_splits == 1 || !dhidden) return 1;
+    const int64_t nt = (D + kTileN - 1) / kTileN, k = piece / 64, mt = row_tiles(head);
+    const int64_t all = nt * (mt * k + (dweight ? (int64_t)(piece / kTileM) * short_cost((head->rows + 63) / 64) : 0));
+    const int64_t share = max((all + pairs - 1) / pairs, (int64_t)16);
+    return (int)min((int64_t)max_splits, (k + share - 1) / share);
+  }
 };
 
 template <class T, TcKind K>
@@ -471,52 +500,74 @@ struct ProductTile {
 
   // Tiles: the long ones of dH with vn / 64 / splits stages each, then the
   // short ones of dW with rows / 64, then (last piece, one split) those of dH
-  // that hold only ignored rows.  A CTA group takes its long tiles in turn; with `more` groups having one more
-  // than the others, the short ones go to the others first, until all are
-  // level, then to all in turn.
-  __device__ static bool get(const Args& a, int group, int groups, int i, TcTile* t) {
+  // that hold only ignored rows.  A CTA group takes its long tiles in turn;
+  // with `more` groups having one more than the others, the short ones go to
+  // the others first, for `lead` rounds, until all are level, then to all in
+  // turn.
+  struct Plan {
+    TileOrder longs, shorts;
+    FastDiv by_tile, by_nt, by_split;
+    int group, groups, splits, k_all, k_short, n_one, n_rest, mine, more, lead;
+    float back;
+  };
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
     const int nt = (a.D + BN - 1) / BN, mt = a.dhidden ? row_tiles(a.head) : 0;
-    const int k_all = a.vn / 64, k_long = (k_all + a.splits - 1) / a.splits, k_short = (a.head->rows + 63) / 64;
-    const int vt = a.dweight ? (min(a.vn, a.V - a.v0) + kTileM - 1) / kTileM : 0;
-    const int dead = a.dhidden && a.last && a.splits == 1 ? a.Bp / kTileM - mt : 0;
-    const int n_one = mt * nt, n_long = n_one * a.splits, n_short = vt * nt, n_rest = n_short + dead * nt;
-    const int q = n_long / groups, more = n_long % groups;
-    const int mine = q + (group < more ? 1 : 0);
+    p->splits = a.splits();
+    p->k_all = a.vn / 64;
+    p->k_short = (a.head->rows + 63) / 64;
+    p->longs.set(mt, nt, 8);
+    p->shorts.set(a.v_tiles(), nt, 5);
+    p->n_one = mt * nt;
+    p->by_tile.set(p->n_one);
+    p->by_nt.set(nt);
+    p->by_split.set(p->splits);
+    p->n_rest = p->shorts.count() + (a.dhidden && a.last && p->splits == 1 ? (a.Bp / kTileM - mt) * nt : 0);
+    p->group = group;
+    p->groups = groups;
+    const int n_long = p->n_one * p->splits;
+    p->more = n_long % groups;
+    p->mine = n_long / groups + (group < p->more ? 1 : 0);
+    p->lead = 0;
+    if (p->more > 0) {
+      const int k_long = (p->k_all + p->splits - 1) / p->splits, cost = short_cost(p->k_short);
+      p->lead = min((k_long + cost / 2) / cost, (p->n_rest + groups - p->more - 1) / (groups - p->more));
+    }
+    p->back = a.up.back(a.head);
+  }
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
     int m, n;
-    if (i < mine) {
-      const int w = i * groups + group, part = w / n_one, k0 = (int)((int64_t)k_all * part / a.splits);
-      tile_order(w - part * n_one, mt, nt, 8, &m, &n);
-      *t = {m * kTileM, n * BN, k0 * 64, a.v0 + k0 * 64, (int)((int64_t)k_all * (part + 1) / a.splits) - k0, part, 0};
+    if (i < p.mine) {
+      const int w = i * p.groups + p.group, part = p.by_tile.div(w);
+      const int k0 = p.by_split.div(p.k_all * part), k1 = p.by_split.div(p.k_all * (part + 1));
+      p.longs.get(w - part * p.n_one, &m, &n);
+      *t = {m * kTileM, n * BN, k0 * 64, a.v0 + k0 * 64, k1 - k0, part, 0};
       return true;
     }
-    i -= mine;
-    int lead = 0;  // rounds of short tiles that only the groups with fewer long ones take
-    if (more > 0) {
-      lead = k_short > 0 ? (k_long + k_short / 2) / k_short : 0;
-      lead = min(lead, (n_rest + groups - more - 1) / (groups - more));
-    }
-    int64_t w;
-    if (group >= more && i < lead) {
-      w = (int64_t)i * (groups - more) + (group - more);
+    i -= p.mine;
+    const int others = p.groups - p.more;
+    int w;
+    if (p.group >= p.more && i < p.lead) {
+      w = i * others + (p.group - p.more);
     } else {
-      if (group >= more) i -= lead;
-      w = (int64_t)lead * (groups - more) + (int64_t)i * groups + group;
+      if (p.group >= p.more) i -= p.lead;
+      w = p.lead * others + i * p.groups + p.group;
     }
-    if (w >= n_rest) return false;
-    if (w < n_short) {
-      tile_order((int)w, vt, nt, 5, &m, &n);
-      *t = {m * kTileM, n * BN, 0, 0, k_short, 0, 1};
+    if (w >= p.n_rest) return false;
+    if (w < p.shorts.count()) {
+      p.shorts.get(w, &m, &n);
+      *t = {m * kTileM, n * BN, 0, 0, p.k_short, 0, 1};
     } else {
-      const int d = (int)w - n_short;
-      *t = {(mt + d / nt) * kTileM, d % nt * BN, 0, 0, 0, 0, 0};
+      const int d = w - p.shorts.count(), q = p.by_nt.div(d);
+      *t = {(p.longs.mt + q) * kTileM, (d - q * p.longs.nt) * BN, 0, 0, 0, 0, 0};
     }
     return true;
   }
 
   template <class Done>
-  __device__ static void epilogue(const Args& a, const TcTile& t, const TcPart& p, State&, int, int, Done done) {
+  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State&, int, int,
+                                  Done done) {
     uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
-    const float back = a.up.back(a.head);
+    const float back = plan.back;
     const int r0 = t.m0 + p.row, s0 = p.share * (BN / 2);
     const int cols = a.D - (t.n0 + s0);
     const bool dh = t.kind == 0, any = t.nk > 0;  // without stages of K the accumulator was never written
@@ -524,8 +575,9 @@ struct ProductTile {
     const int mine = dh ? a.row_of[r0 + p.lane] : -1;
     const bool zero = !any || (dh && p.lane >= live);
     const float f = zero ? 0.0f : dh ? back * a.up.rest(mine) : back;
-    const bool summed = dh && a.sum && any;  // t.rows: the split
-    const bool store = dh ? a.splits == 1 && a.last : true;
+    const bool one = plan.splits == 1;
+    const bool summed = dh && any && !(one && a.first && a.last);  // t.rows: the split
+    const bool store = dh ? one && a.last : true;
     float* sum = summed ? a.sum + ((int64_t)t.rows * a.Bp + r0 + p.lane) * a.lds + t.n0 + s0 : nullptr;
     for (int c = 0; c < BN / 2; c += 32) {
       float v[32];
@@ -569,7 +621,8 @@ __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
   const int lane = threadIdx.x & 31;
   const int slabs = (a.D + 127) / 128;
   const int64_t work = (int64_t)a.Bp * slabs, nw = (int64_t)gridDim.x * 8;
-  const int rows = a.head->rows;
+  const int rows = a.head->rows, splits = a.splits();
+  if (splits == 1) return;  // written by the product itself
   const float back = a.up.back(a.head);
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < work; i += nw) {
     const int r = (int)(i / slabs), c = (int)(i % slabs) * 128 + lane * 4;
@@ -578,7 +631,7 @@ __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
     float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (r < rows) {
 #pragma unroll 4
-      for (int q = 0; q < a.splits; ++q) {
+      for (int q = 0; q < splits; ++q) {
         const float4 x = *reinterpret_cast<const float4*>(a.sum + ((int64_t)q * a.Bp + r) * a.lds + c);
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
       }
@@ -596,6 +649,8 @@ __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
 // ------------------------------------------------------------ host
 // Bytes of G that one piece of the vocabulary may take.
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;
+// Bytes of dH's sums where they are split.
+constexpr int64_t kSumBytes = (int64_t)128 << 20;
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 
@@ -634,8 +689,10 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.pieces = (Vp + p.piece - 1) / p.piece;
   at = 0;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
-  // dH's tiles for every CTA pair, at least 16 stages of K each
-  p.splits = B > 0 ? sm_count() / 2 / ((p.Bp / kTileM) * ((D + kTileN - 1) / kTileN)) : 1;
+  // as many as one row tile could use, 16 stages of K each, within kSumBytes
+  p.splits = sm_count() / 2 / ((D + kTileN - 1) / kTileN);
+  const int64_t room = B > 0 ? kSumBytes / (4 * p.Bp * up(D, 32)) : 1;
+  if (p.splits > room) p.splits = room;
   if (p.splits > p.piece / 64 / 16) p.splits = p.piece / 64 / 16;
   if (p.splits < 1) p.splits = 1;
   p.sum = at, at += p.pieces > 1 || p.splits > 1 ? up(4 * p.splits * p.Bp * up(D, 32), 256) : 0;
@@ -722,9 +779,11 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
     const GradArgs ga = {head, label, row_of, reinterpret_cast<float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
                          v0, vn, status};
     if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
-    const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
-                            i == 0, i == p.pieces - 1, (int)p.splits, status};
     const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
+    const int64_t pairs = sm_count() / 2;
+    const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
+                            i == 0, i == p.pieces - 1, (int)p.piece, (int)p.splits,
+                            (int)(tiles < pairs ? tiles : pairs), status};
     if (launch_gemm<ProductTile<T, K>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
     if (dhidden && pa.last && p.splits > 1) {
       const int64_t need = (p.Bp * ((D + 127) / 128) + 7) / 8, cap = (int64_t)sm_count() * 16;
