@@ -4,8 +4,9 @@
 // two fp32 multiplications and one rounding to the output's type.
 //
 // Two layouts of the same product:
-//   many tokens  tokens are the 256 rows of a tile (two CTAs), 256 weight
-//                rows its columns: bound by the tensor cores;
+//   many tokens  tokens are the rows of a tile, weight rows its columns: 256 x
+//                256 tiles by two CTAs, bound by the tensor cores, or, where
+//                those are too few for the SMs, 128 x 128 tiles by one;
 //   few tokens   weight rows are the 128 rows of a tile and the tokens its
 //                16 .. 128 columns: every weight is read once, bound by HBM.
 //                The rows that do not make a whole round of tiles are dealt
@@ -30,23 +31,24 @@ struct Int8Args {
   int32_t* status;
 };
 
-struct NoState {};
-
-template <class TO>
+template <class TO, int SIDE>
 struct Int8Many {
   using Args = Int8Args;
-  using State = NoState;
+  struct State {
+    float qs, ws[4];
+  };
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr bool TWO = false, A_MN2 = false;
-  static constexpr int CG = 2, BN = 256, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
+  static constexpr int CG = SIDE / 128, BN = SIDE, STAGES = 5, KC = 0, EW = SIDE / 32, A_BOX = 128, AHEAD = 0;
+  static constexpr int COLS = 128;  // per epilogue warp
   static constexpr uint32_t EPI_BYTES = EW * (sizeof(TO) == 2 ? kStageBytes : 32 * 33 * 4);
   struct Plan {
     TileOrder order;
     int first, step;
   };
   __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
-    p->order.set((a.T + 255) / 256, (a.N + 255) / 256, 16);  // token blocks that share the weight tiles in flight
+    p->order.set((a.T + SIDE - 1) / SIDE, (a.N + SIDE - 1) / SIDE, 16);  // token blocks that share the weight tiles in flight
     p->first = group;
     p->step = groups;
   }
@@ -55,23 +57,27 @@ struct Int8Many {
     if (w >= p.order.count()) return false;
     int m, n;
     p.order.get(w, &m, &n);
-    *t = {m * 256, n * 256, 0, 0, (a.K + 127) / 128, 128, 0};
+    *t = {m * SIDE, n * SIDE, 0, 0, (a.K + 127) / 128, 128, 0};
     return true;
   }
+  __device__ static void begin(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st) {
+    const int row = t.m0 + p.row + p.lane, col = t.n0 + p.share * COLS + p.lane;
+    st.qs = row < a.T ? a.qs[row] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < COLS / 32; ++k) st.ws[k] = col + 32 * k < a.N ? a.ws[col + 32 * k] : 0.0f;
+  }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State&, int, int,
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
                                   Done done) {
-    const int r0 = t.m0 + p.row, rows = a.T - r0, s0 = p.share * (BN / 2);
-    const float qs = p.lane < rows ? a.qs[r0 + p.lane] : 0.0f;
+    const int r0 = t.m0 + p.row, rows = a.T - r0, s0 = p.share * COLS;
     TO* out = static_cast<TO*>(a.out) + t.n0 + s0;
-    for (int c = 0; c < BN / 2; c += 32) {
-      const int n = t.n0 + s0 + c + p.lane;
-      const float ws = n < a.N ? a.ws[n] : 0.0f;
+#pragma unroll
+    for (int c = 0; c < COLS; c += 32) {
       float v[32];
       tmem_ld32(p.taddr + s0 + c, v);
-      if (c + 32 == BN / 2) done();
+      if (c + 32 == COLS) done();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * qs * __shfl_sync(kFull, ws, i);
+      for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * st.qs * __shfl_sync(kFull, st.ws[c / 32], i);
       if constexpr (sizeof(TO) == 2)
         stage_block<TO>(reinterpret_cast<uint32_t*>(p.smem), v, p.lane, c);
       else
@@ -79,7 +85,7 @@ struct Int8Many {
                     [&](int i) -> float* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo + c : nullptr; });
     }
     if constexpr (sizeof(TO) == 2)
-      store_staged<TO>(reinterpret_cast<uint32_t*>(p.smem), p.lane, min(BN / 2, a.N - (t.n0 + s0)),
+      store_staged<TO>(reinterpret_cast<uint32_t*>(p.smem), p.lane, min(COLS, a.N - (t.n0 + s0)),
                        [&](int i) -> TO* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo : nullptr; });
   }
 };
@@ -87,7 +93,9 @@ struct Int8Many {
 template <class TO, int NT>
 struct Int8Few {
   using Args = Int8Args;
-  using State = NoState;
+  struct State {
+    float ws, qs[(NT + 31) / 32];  // lane i: tokens i, i + 32, ...
+  };
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr bool TWO = false, A_MN2 = false;
@@ -114,14 +122,20 @@ struct Int8Few {
     *t = {m0, 0, 0, 0, (a.K + 127) / 128, rows, 0};
     return true;
   }
+  __device__ static void begin(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st) {
+    const int row = p.row + p.lane;
+    st.ws = row < t.rows ? a.ws[t.m0 + row] : 0.0f;
+#pragma unroll
+    for (int k = 0; k < (NT + 31) / 32; ++k) st.qs[k] = k * 32 + p.lane < a.T ? a.qs[k * 32 + p.lane] : 0.0f;
+  }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State&, int, int,
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
                                   Done done) {
     const int n = t.m0 + p.row + p.lane;
     const bool mine = p.row + p.lane < t.rows;
-    const float ws = mine ? a.ws[n] : 0.0f;
-    TO* out = static_cast<TO*>(a.out);
+    TO* out = static_cast<TO*>(a.out) + n;
     constexpr int STEP = NT < 32 ? 16 : 32;
+#pragma unroll
     for (int c = 0; c < NT; c += STEP) {
       float v[STEP];
       if constexpr (STEP == 32)
@@ -129,11 +143,11 @@ struct Int8Few {
       else
         tmem_ld16(p.taddr + c, v);
       if (c + STEP == NT) done();
-      if (!mine) continue;
 #pragma unroll
       for (int i = 0; i < STEP; ++i) {
         const int tok = c + i;
-        if (tok < a.T) st_elem(out + (int64_t)tok * a.ldo + n, (float)__float_as_int(v[i]) * a.qs[tok] * ws);
+        const float x = (float)__float_as_int(v[i]) * __shfl_sync(kFull, st.qs[tok / 32], tok % 32) * st.ws;
+        if (mine && tok < a.T) st_elem(out + (int64_t)tok * a.ldo, x);
       }
     }
   }
@@ -159,8 +173,10 @@ cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64
   if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   if (a.T <= 128) return run_int8<Int8Few<TO, 128>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  const int64_t tiles = (((int64_t)a.T + 255) / 256) * (((int64_t)a.N + 255) / 256);
-  return run_int8<Int8Many<TO>>(q, a.T, ldq, w, a.N, ldw, a, tiles, st);
+  const int64_t big = (((int64_t)a.T + 255) / 256) * (((int64_t)a.N + 255) / 256);
+  if (big >= sms / 2) return run_int8<Int8Many<TO, 256>>(q, a.T, ldq, w, a.N, ldw, a, big, st);
+  const int64_t small = (((int64_t)a.T + 127) / 128) * (((int64_t)a.N + 127) / 128);
+  return run_int8<Int8Many<TO, 128>>(q, a.T, ldq, w, a.N, ldw, a, small, st);
 }
 
 }  // namespace

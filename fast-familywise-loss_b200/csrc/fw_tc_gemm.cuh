@@ -142,13 +142,15 @@ struct TcTile {
 };
 
 // Division of n < 2^31 by a divisor met again and again: a multiplication and
-// a shift (the multiplier is 2^32 (2^s - d) / d + 1 for 2^s >= d).
+// a shift.  The multiplier is floor(2^32 (2^s - d) / d) + 1 for the first
+// 2^s >= d; n < 2^31 leaves room for one more, so the quotient may be a rounded
+// one (a 64-bit integer division here costs a short kernel half a microsecond).
 struct FastDiv {
   uint32_t d, mul, shift;
   __device__ __forceinline__ void set(int divisor) {
     d = (uint32_t)max(divisor, 1);
     shift = d > 1 ? 32 - __clz((int)d - 1) : 0;
-    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d) + 1u;
+    mul = (uint32_t)(4294967296.0 * (double)((1u << shift) - d) / (double)d) + 1u;
   }
   __device__ __forceinline__ int div(int n) const {
     return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
@@ -174,6 +176,10 @@ struct TileOrder {
     *m = g * group + r - *n * (tail ? (int)by_tail.d : group);
   }
 };
+
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+}
 
 __device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap* map, int x, int y) {
   asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(map), "r"(x), "r"(y) : "memory");
@@ -201,6 +207,8 @@ struct TcPart {
 //                    group follow from, worked out once per CTA
 //   get(args, plan, i, &tile)  i-th tile of the CTA group; false: done
 //   struct State     what an epilogue thread keeps over a tile's parts
+//   begin(args, plan, tile, part, state)  before the tile's products are done:
+//                    loads that the epilogue would wait for
 //   epilogue(args, plan, tile, part, state, k, parts, done): part k of the
 //                    tile's `parts`; done() hands the accumulator back once
 //                    its last column has been read.
@@ -256,6 +264,12 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (threadIdx.x == 32 * 3) {
+    tma_prefetch_map(&tm_a);
+    tma_prefetch_map(&tm_b);
+    if constexpr (P::TWO || P::A_BOX < 128) tma_prefetch_map(&tm_a2);
+    if constexpr (P::TWO) tma_prefetch_map(&tm_b2);
   }
   if constexpr (P::AHEAD > 0) {
     if (threadIdx.x == 32 * 2) {
@@ -388,6 +402,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     for (int it = 0; P::get(a, plan, it, &t); ++it) {
       const int parts = P::KC == 0 ? 1 : max((t.nk + P::KC - 1) / (P::KC == 0 ? 1 : P::KC), 1);
       typename P::State state{};
+      P::begin(a, plan, t, part, state);
       for (int k = 0; k < parts; ++k) {
         if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
         tc_fence_after();
@@ -455,7 +470,7 @@ __device__ __forceinline__ void store_block(float* sm, const float (&v)[32], int
       if (p && c < cols) *reinterpret_cast<float4*>(p + c) = make_float4(x[0], x[1], x[2], x[3]);  // cols: a multiple of V
     }
   } else {
-#pragma unroll 4
+#pragma unroll 8
     for (int i = 0; i < 32; ++i) {
       float* p = row_ptr(i);
       if (p && lane < cols) p[lane] = sm[i * 33 + lane];

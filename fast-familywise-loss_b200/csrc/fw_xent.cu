@@ -145,8 +145,6 @@ __global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_
   }
 }
 
-struct NoState {};
-
 // 2^x by the hardware's instruction (relative error 2^-22, results under
 // 2^-126 flushed to 0); volatile, so that the compiler does not hold many
 // arguments in registers to interleave them.
@@ -199,6 +197,7 @@ struct LseTile {
   using Args = LseArgs;
   struct State {
     float z[kLseCols] = {};
+    int y;
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
@@ -215,6 +214,9 @@ struct LseTile {
     *t = {m * kTileM, n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
     return true;
   }
+  __device__ static void begin(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st) {
+    st.y = a.label[t.m0 + p.row + p.lane];
+  }
   template <class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int k,
                                   int parts, Done done) {
@@ -229,7 +231,7 @@ struct LseTile {
     if (k < parts - 1) return;
     const int row = t.m0 + p.row + p.lane;  // < Bp
     const int n0 = t.n0 + p.share * kLseCols;
-    const int y = a.label[row] - n0;
+    const int y = st.y - n0;
     const int valid = a.V - n0;
     float m = -CUDART_INF_F, s = 0.0f;
 #pragma unroll
@@ -412,7 +414,10 @@ struct GradArgs {
 template <class T, TcKind K>
 struct GradTile {
   using Args = GradArgs;
-  using State = NoState;
+  struct State {
+    float lse, coef;
+    int y;
+  };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr bool TWO = false, A_MN2 = false;
@@ -428,14 +433,19 @@ struct GradTile {
     *t = {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
     return true;
   }
-  template <class Done>
-  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State&, int, int,
-                                  Done done) {
+  __device__ static void begin(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st) {
     const int row = t.m0 + p.row + p.lane;
     const bool live = row < a.head->rows;
-    const int y = live ? a.label[row] : -1;
-    const float lse = live ? a.lse[row] : 0.0f;
-    const float coef = live ? a.up.in_g(a.head, a.row_of[row]) : 0.0f;
+    st.y = live ? a.label[row] : -2;  // -2: not a live row
+    st.lse = live ? a.lse[row] : 0.0f;
+    st.coef = live ? a.up.in_g(a.head, a.row_of[row]) : 0.0f;
+  }
+  template <class Done>
+  __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
+                                  Done done) {
+    const int row = t.m0 + p.row + p.lane, y = st.y;
+    const bool live = y != -2;
+    const float lse = st.lse, coef = st.coef;
     T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
@@ -482,17 +492,22 @@ struct ProductArgs {
   // The same for every piece (whole ones are taken to reckon with).
   __device__ int splits() const {
     if (max_splits == 1 || !dhidden) return 1;
-    const int64_t nt = (D + kTileN - 1) / kTileN, k = piece / 64, mt = row_tiles(head);
-    const int64_t all = nt * (mt * k + (dweight ? (int64_t)(piece / kTileM) * short_cost((head->rows + 63) / 64) : 0));
-    const int64_t share = max((all + pairs - 1) / pairs, (int64_t)16);
-    return (int)min((int64_t)max_splits, (k + share - 1) / share);
+    // in fp32: the share of a pair need not be exact, only the same everywhere
+    const float nt = (float)((D + kTileN - 1) / kTileN), k = (float)(piece / 64), mt = (float)row_tiles(head);
+    const float rest = dweight ? (float)(piece / kTileM) * (float)short_cost((head->rows + 63) / 64) : 0.0f;
+    const float share = fmaxf(nt * (mt * k + rest) / (float)pairs, 16.0f);
+    return min(max_splits, (int)ceilf(k / share));
   }
 };
 
 template <class T, TcKind K>
 struct ProductTile {
   using Args = ProductArgs;
-  using State = NoState;
+  struct State {
+    int mine;  // dH: the given row of this lane's row
+    float f;   // its factor
+    bool zero;
+  };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
   static constexpr int CG = 2, BN = kTileN, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
@@ -563,18 +578,21 @@ struct ProductTile {
     return true;
   }
 
+  __device__ static void begin(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st) {
+    // without stages of K the accumulator is never written; dH's rows behind the live ones are ignored ones
+    const int row = t.m0 + p.row + p.lane;
+    const bool dh = t.kind == 0;
+    st.mine = dh ? a.row_of[row] : -1;
+    st.zero = t.nk == 0 || (dh && row >= a.head->rows);
+    st.f = st.zero ? 0.0f : dh ? plan.back * a.up.rest(st.mine) : plan.back;
+  }
   template <class Done>
-  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State&, int, int,
-                                  Done done) {
+  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st, int,
+                                  int, Done done) {
     uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
-    const float back = plan.back;
     const int r0 = t.m0 + p.row, s0 = p.share * (BN / 2);
     const int cols = a.D - (t.n0 + s0);
-    const bool dh = t.kind == 0, any = t.nk > 0;  // without stages of K the accumulator was never written
-    const int live = a.head->rows - r0;           // dH: the warp's rows behind these are ignored ones
-    const int mine = dh ? a.row_of[r0 + p.lane] : -1;
-    const bool zero = !any || (dh && p.lane >= live);
-    const float f = zero ? 0.0f : dh ? back * a.up.rest(mine) : back;
+    const bool dh = t.kind == 0, any = t.nk > 0;
     const bool one = plan.splits == 1;
     const bool summed = dh && any && !(one && a.first && a.last);  // t.rows: the split
     const bool store = dh ? one && a.last : true;
@@ -600,14 +618,14 @@ struct ProductTile {
       }
       if (!store) continue;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = zero ? 0.0f : v[i] * f;
+      for (int i = 0; i < 32; ++i) v[i] = st.zero ? 0.0f : v[i] * st.f;
       stage_block<T>(sm, v, p.lane, c);
     }
     if (!store || cols <= 0) return;
     const int rows = a.V - (a.v0 + r0);  // dW
     T* out = (dh ? static_cast<T*>(a.dhidden) : static_cast<T*>(a.dweight) + (int64_t)(a.v0 + r0) * a.D) + t.n0 + s0;
     store_staged<T>(sm, p.lane, min(cols, BN / 2), [&](int i) -> T* {
-      const int r = dh ? __shfl_sync(kFull, mine, i) : i < rows ? i : -1;
+      const int r = dh ? __shfl_sync(kFull, st.mine, i) : i < rows ? i : -1;
       return r >= 0 ? out + (int64_t)r * a.D : nullptr;
     });
   }
