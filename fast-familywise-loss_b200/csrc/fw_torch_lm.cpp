@@ -60,6 +60,17 @@ int32_t* status_of(const OptTensor& s, const Tensor& like) {
   return s->data_ptr<int32_t>();
 }
 
+// The status word of a later backward.  Not a saved variable: clearing it in
+// between is its normal use.
+void keep_status(AutogradContext* ctx, const OptTensor& s) {
+  if (s.has_value()) ctx->saved_data["status"] = c10::IValue(*s);
+}
+
+OptTensor kept_status(AutogradContext* ctx) {
+  const auto it = ctx->saved_data.find("status");
+  return it == ctx->saved_data.end() ? OptTensor() : OptTensor(it->second.toTensor());
+}
+
 Tensor bytes(int64_t n, const Tensor& like) {
   return at::empty({n > 0 ? n : 1}, like.options().dtype(torch::kUInt8));
 }
@@ -122,15 +133,15 @@ Tensor embed_grad(const Tensor& ids, const Tensor& grad, int64_t V, double scale
 struct EmbedTokens : torch::autograd::Function<EmbedTokens> {
   static Tensor forward(AutogradContext* ctx, const Tensor& ids, const Tensor& weight, double scale, int64_t padding,
                         const OptTensor& status) {
-    ctx->save_for_backward({ids, status.value_or(Tensor())});
+    ctx->save_for_backward({ids});
+    keep_status(ctx, status);
     ctx->saved_data["a"] = c10::IValue(std::vector<double>{(double)weight.size(0), scale, (double)padding});
     return embed_rows(ids, weight, scale, status);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();
     const auto a = ctx->saved_data["a"].toDoubleVector();
-    const OptTensor status = saved[1].defined() ? OptTensor(saved[1]) : c10::nullopt;
-    auto dw = embed_grad(saved[0], g[0].detach(), (int64_t)a[0], a[1], (int64_t)a[2], status);
+    auto dw = embed_grad(saved[0], g[0].detach(), (int64_t)a[0], a[1], (int64_t)a[2], kept_status(ctx));
     return once({Tensor(), dw, Tensor(), Tensor(), Tensor()});
   }
 };
@@ -358,7 +369,8 @@ struct LmHeadCrossEntropy : torch::autograd::Function<LmHeadCrossEntropy> {
   static Tensor forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& target,
                         int64_t ignore_index, int64_t reduction, const OptTensor& status) {
     auto x = xent_forward(hidden, weight, target, ignore_index, reduction, status);
-    ctx->save_for_backward({weight, x.state, status.value_or(Tensor())});
+    ctx->save_for_backward({weight, x.state});
+    keep_status(ctx, status);
     ctx->saved_data["a"] = c10::IValue(std::vector<int64_t>{hidden.size(0), reduction});
     return x.loss;
   }
@@ -376,7 +388,7 @@ struct LmHeadCrossEntropy : torch::autograd::Function<LmHeadCrossEntropy> {
     if (want_w) dw = at::empty({V, D}, w.options());
     const int64_t nw = fw_xent_workspace(B, D, V, 1);
     auto ws = bytes(nw, w);
-    const OptTensor status = saved[2].defined() ? OptTensor(saved[2]) : c10::nullopt;
+    const OptTensor status = kept_status(ctx);
     ok(fw_xent_backward(code(w), w.data_ptr(), ld_of(w), B, D, V, (int)a[1], go.data_ptr<float>(), state.data_ptr(),
                         state.numel(), ws.data_ptr(), nw, want_h ? dh.data_ptr() : nullptr,
                         want_w ? dw.data_ptr() : nullptr, status_of(status, w), stream()),
