@@ -59,8 +59,6 @@ __host__ __device__ constexpr int slots_of(int64_t D, int esize) {
   return (int)((D * esize + 15) / 16 + (D * esize % 16 != 0 ? 1 : 0));
 }
 
-int slabs_of(int64_t D, int esize) { return (slots_of(D, esize) + 32 * kSlab - 1) / (32 * kSlab); }
-
 template <class T>
 __device__ __forceinline__ int dst_off(const T* row) {
   return (int)(reinterpret_cast<uintptr_t>(row) & 15u) / (int)sizeof(T);
@@ -73,7 +71,7 @@ struct EmbedArgs {
   int64_t T, V, D, ldw, ldo;
   float scale;
   int32_t* status;
-  int nslabs;
+  int nsteps, nslabs;  // 32 slots each; parts of at most kSlab of them
 };
 
 template <class T>
@@ -84,6 +82,8 @@ __global__ void __launch_bounds__(256) fw_embed_rows_kernel(EmbedArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
   const int64_t work = a.T * a.nslabs;
+  const int D = (int)a.D, steps = (a.nsteps + a.nslabs - 1) / a.nslabs;  // of 32 slots, per slab
+  const Span<T> table(a.w, a.V, a.ldw, a.D);
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
     const int64_t t = i / a.nslabs;
     const int slab = (int)(i - t * a.nslabs);
@@ -92,16 +92,16 @@ __global__ void __launch_bounds__(256) fw_embed_rows_kernel(EmbedArgs a) {
     if (!ok && lane == 0) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
     const T* src = static_cast<const T*>(a.w) + (ok ? id : 0) * a.ldw;
     T* dst = static_cast<T*>(a.out) + t * a.ldo;
-    const int off = dst_off(dst);
+    const int off = dst_off(dst), first = slab * steps;
     uint4 u[kSlab];
 #pragma unroll
     for (int k = 0; k < kSlab; ++k) {
-      const int64_t e0 = (int64_t)((slab * kSlab + k) * 32 + lane) * V - off;
-      u[k] = e0 < a.D ? load_slot_shifted(src, e0, a.D) : make_uint4(0u, 0u, 0u, 0u);
+      const int e0 = ((first + k) * 32 + lane) * V - off;
+      u[k] = k < steps && e0 < D ? load_slot_shifted(src, e0, table) : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
     for (int k = 0; k < kSlab; ++k) {
-      const int64_t e0 = (int64_t)((slab * kSlab + k) * 32 + lane) * V - off;
+      const int e0 = ((first + k) * 32 + lane) * V - off;
       if (a.scale != 1.0f || !ok) {
         float v[V];
         unpack16<T>(u[k], v);
@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256) fw_embed_rows_kernel(EmbedArgs a) {
         for (int j = 0; j < V; ++j) v[j] = ok ? v[j] * a.scale : CUDART_NAN_F;
         u[k] = pack16<T>(v);
       }
-      if (e0 < a.D) store_slot(dst, e0, a.D, true, u[k]);
+      if (k < steps && e0 < D) store_slot(dst, e0, D, true, u[k]);
     }
   }
 }
@@ -395,7 +395,7 @@ struct EmbedGradArgs {
 };
 
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int64_t e0, const float* acc) {
+__device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int e0, const float* acc) {
   constexpr int V = 16 / sizeof(T);
   if (e0 >= a.D) return;
   float s[V];
@@ -410,7 +410,7 @@ __device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int64_
 // Start of slot `slot` in the row at dst: every row's own slots, so that a
 // run's partial rows (kept by slot) and its table row agree.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ int64_t slot_elem(const T* dst, int64_t slot) {
+__device__ __forceinline__ int slot_elem(const T* dst, int slot) {
   constexpr int V = 16 / sizeof(T);
   return slot * V - (ALIGNED ? 0 : dst_off(dst));
 }
@@ -419,7 +419,7 @@ __device__ __forceinline__ int64_t slot_elem(const T* dst, int64_t slot) {
 // order.  Partial row 2c is the part of a run that began in an earlier chunk,
 // 2c + 1 the part of a run that begins here and goes on.
 template <class T, bool ALIGNED>
-__device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int64_t slot, int lane) {
+__device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, const Span<T>& span, int64_t c, int slot, int lane) {
   constexpr int V = 16 / sizeof(T);
   const int64_t b = c * kChunk;
   const int n = (int)min((int64_t)kChunk, a.T - b);
@@ -440,12 +440,12 @@ __device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, int64_t c, int
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       const T* row = static_cast<const T*>(a.g) + (int64_t)__shfl_sync(kFull, ent.y, (i0 + i) & 31) * a.ldg;
-      int64_t e0 = slot * V;
+      int e0 = slot * V;
       if (!ALIGNED)
         e0 -= dst_off(static_cast<const T*>(a.dw) + (int64_t)__shfl_sync(kFull, ent.x, (i0 + i) & 31) * a.D);
       u[i] = i0 + i >= live || e0 >= a.D ? make_uint4(0u, 0u, 0u, 0u)
              : ALIGNED                   ? ld_stream16(row + e0)
-                                         : load_slot_shifted(row, e0, a.D);
+                                         : load_slot_shifted(row, e0, span);
     }
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -478,13 +478,14 @@ __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) fw_embed_sum_kernel(Embe
   wait_prior_kernel();
   allow_dependent_launch();
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const Span<T> span(a.g, a.T, a.ldg, a.D);
   const int64_t total = gridDim.x, adding = a.sum_blocks;
   const int64_t before = blockIdx.x * adding / total;  // adding CTAs ahead of this one
   if ((blockIdx.x + 1) * adding / total != before) {
     const int64_t slabs = (a.nslots + 31) / 32;
     const int64_t work = (a.T + kChunk - 1) / kChunk * slabs;
     for (int64_t i = before * 8 + w; i < work; i += adding * 8)
-      sum_chunk<T, ALIGNED>(a, i / slabs, i % slabs * 32 + lane, lane);
+      sum_chunk<T, ALIGNED>(a, span, i / slabs, (int)(i % slabs) * 32 + lane, lane);
     return;
   }
   for (int64_t v0 = ((blockIdx.x - before) * 8 + w) * 8; v0 < a.V; v0 += (total - adding) * 64) {
@@ -514,7 +515,8 @@ __global__ void __launch_bounds__(256) fw_embed_join_kernel(EmbedGradArgs a) {
   const int64_t slabs = (a.nslots + 31) / 32, chunks = (a.T + kChunk - 1) / kChunk, work = chunks * slabs;
   const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
   for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
-    const int64_t c = i / slabs, slot = i % slabs * 32 + lane, b = c * kChunk;
+    const int64_t c = i / slabs, b = c * kChunk;
+    const int slot = (int)(i % slabs) * 32 + lane;
     if (b + kChunk >= a.T) continue;
     const uint32_t key = a.sorted[b + kChunk - 1].x;
     if (key >= (uint32_t)a.V || a.sorted[b + kChunk].x != key) continue;          // nothing goes on
@@ -553,6 +555,7 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
   allow_dependent_launch();
   __shared__ int32_t key[kDirectTokens];
   const int n = (int)a.T;
+  const Span<T> span(a.g, a.T, a.ldg, a.D);
   for (int i = threadIdx.x; i < kDirectTokens; i += 256) {
     const int64_t id = i < n ? a.ids[i] : -1;
     const bool ok = id >= 0 && id < a.V;
@@ -566,7 +569,7 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
   for (int64_t w = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); w < work; w += nw) {
     const int64_t v = w / slabs;
     T* dst = static_cast<T*>(a.dw) + v * a.D;
-    const int64_t e0 = slot_elem<T, ALIGNED>(dst, w % slabs * 32 + lane);
+    const int e0 = slot_elem<T, ALIGNED>(dst, (int)(w % slabs) * 32 + lane);
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) acc[j] = 0.0f;
@@ -577,7 +580,7 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
       for (; hit != 0u; hit &= hit - 1u) {
         const T* row = static_cast<const T*>(a.g) + (int64_t)(t0 + __ffs(hit) - 1) * a.ldg;
         float x[V];
-        unpack16<T>(ALIGNED ? ld_stream16(row + e0) : load_slot_shifted(row, e0, a.D), x);
+        unpack16<T>(ALIGNED ? ld_stream16(row + e0) : load_slot_shifted(row, e0, span), x);
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] += x[j];
       }
@@ -701,8 +704,9 @@ int fw_embed_rows(int dtype, const int64_t* ids, int64_t T, const void* weight, 
   if (!ids || !weight || !out) return FWB_E_POINTER;
   const int es = dtype == FWB_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(weight) % es || reinterpret_cast<uintptr_t>(out) % es) return FWB_E_POINTER;
-  EmbedArgs a = {ids, weight, out, T, V, D, ldw, ldo, scale, status, 0};
-  a.nslabs = slabs_of(D, es);
+  EmbedArgs a = {ids, weight, out, T, V, D, ldw, ldo, scale, status, 0, 0};
+  a.nsteps = (slots_of(D, es) + 31) / 32;
+  a.nslabs = (a.nsteps + kSlab - 1) / kSlab;
   const int64_t need = (T * a.nslabs + 7) / 8, cap = (int64_t)sm_count() * 64;
   const int64_t grid = need < cap ? need : cap;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

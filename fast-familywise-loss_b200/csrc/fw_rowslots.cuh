@@ -58,39 +58,56 @@ __device__ __forceinline__ void store_slot(T* row, int64_t e0, int64_t D, bool v
   }
 }
 
-// The 16 bytes at `p`, which may start anywhere a T may; [begin, end) is the
-// row.  A full slot read through its two aligned neighbours and a funnel
-// shift, except where a neighbour would leave the row.
+// First element of a matrix and the one behind its last.
 template <class T>
-__device__ __forceinline__ uint4 load_shifted(const T* p, const T* begin, const T* end) {
-  const uintptr_t addr = reinterpret_cast<uintptr_t>(p);
-  const uint32_t m = (uint32_t)(addr & 15u);
-  if (m == 0) return ld_stream16(p);
-  const uintptr_t lo = addr - m;
-  if (lo >= reinterpret_cast<uintptr_t>(begin) && lo + 32 <= reinterpret_cast<uintptr_t>(end)) {
-    const uint4 a = ld_global16(reinterpret_cast<const void*>(lo));
-    const uint4 b = ld_global16(reinterpret_cast<const void*>(lo + 16));
-    const uint32_t s = (m & 3u) * 8u;
-    uint32_t w[5];
-    switch (m >> 2) {  // the same for the whole row
-      case 0: w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x; break;
-      case 1: w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y; break;
-      case 2: w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z; break;
-      default: w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w; break;
+struct Span {
+  const T* lo;
+  const T* hi;
+  __device__ __forceinline__ Span(const void* base, int64_t rows, int64_t ld, int64_t D)
+      : lo(static_cast<const T*>(base)), hi(lo + (rows - 1) * ld + D) {}
+};
+
+// Elements p .. p + V one by one, those outside [lo, hi) as zero.
+template <class T>
+__device__ __forceinline__ uint4 load_elems(const T* p, const T* lo, const T* hi) {
+  constexpr int V = 16 / sizeof(T);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    if (p + j >= lo && p + j < hi) {
+      if constexpr (sizeof(T) == 4)
+        w[j] = __float_as_uint(p[j]);
+      else
+        w[j >> 1] |= (uint32_t)*reinterpret_cast<const unsigned short*>(p + j) << (16 * (j & 1));
     }
-    return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s),
-                      __funnelshift_r(w[2], w[3], s), __funnelshift_r(w[3], w[4], s));
   }
-  return load_slot(p, 0, 16 / (int)sizeof(T), false);
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Slot of a row whose own slots lie elsewhere: elements e0 .. e0 + V of the
-// row at `row`, zero outside [0, D).
+// The slot at row + e0 of a row that may start anywhere: its 16 bytes through
+// the two aligned neighbours they lie in and a funnel shift.  Elements outside
+// the row are whatever lies there (zero outside the span).
 template <class T>
-__device__ __forceinline__ uint4 load_slot_shifted(const T* row, int64_t e0, int64_t D) {
-  constexpr int V = 16 / sizeof(T);
-  if (e0 >= 0 && e0 + V <= D) return load_shifted(row + e0, row, row + D);
-  return load_slot(row, e0, D, false);
+__device__ __forceinline__ uint4 load_slot_shifted(const T* row, int e0, const Span<T>& span) {
+  const T* p = row + e0;
+  const uintptr_t addr = reinterpret_cast<uintptr_t>(p);
+  const uint32_t m = (uint32_t)(addr & 15u);
+  const uintptr_t lo = addr - m;
+  if (lo < reinterpret_cast<uintptr_t>(span.lo) || lo + (m ? 32 : 16) > reinterpret_cast<uintptr_t>(span.hi))
+    return load_elems(p, span.lo, span.hi);
+  const uint4 a = ld_global16(reinterpret_cast<const void*>(lo));
+  if (m == 0) return a;
+  const uint4 b = ld_global16(reinterpret_cast<const void*>(lo + 16));
+  const uint32_t s = (m & 3u) * 8u;
+  uint32_t w[5];
+  switch (m >> 2) {  // the same for the whole row
+    case 0: w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x; break;
+    case 1: w[0] = a.y, w[1] = a.z, w[2] = a.w, w[3] = b.x, w[4] = b.y; break;
+    case 2: w[0] = a.z, w[1] = a.w, w[2] = b.x, w[3] = b.y, w[4] = b.z; break;
+    default: w[0] = a.w, w[1] = b.x, w[2] = b.y, w[3] = b.z, w[4] = b.w; break;
+  }
+  return make_uint4(__funnelshift_r(w[0], w[1], s), __funnelshift_r(w[1], w[2], s), __funnelshift_r(w[2], w[3], s),
+                    __funnelshift_r(w[3], w[4], s));
 }
 
 }  // namespace fwb200

@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
     a.head->status = 0;
   }
   const int64_t rows_up = ((int64_t)total + 255) / 256 * 256;
+  const Span<T> span(a.hidden, a.B, a.ldh, a.D);
   for (int i0 = 0; i0 < a.per_cta; i0 += 32) {
     const int64_t rl = r0 + i0 + lane;
     const int64_t yl = rl < a.B ? a.y[rl] : a.ignore;
@@ -115,19 +116,21 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
       T* out = static_cast<T*>(a.hp) + dst * a.Dp;
       const T* in = static_cast<const T*>(a.hidden) + (alive ? r : 0) * a.ldh;
       for (int64_t e = (int64_t)lane * V; e < a.Dp; e += 32 * V)
-        *reinterpret_cast<uint4*>(out + e) = alive ? load_slot_shifted(in, e, a.D) : make_uint4(0u, 0u, 0u, 0u);
+        *reinterpret_cast<uint4*>(out + e) = alive ? load_slot_shifted(in, (int)e, span) : make_uint4(0u, 0u, 0u, 0u);
     }
     before += __popc(live);
   }
 }
 
-// Rows of an unaligned matrix copied to 16-byte boundaries.
+// Rows of an unaligned matrix copied to 16-byte boundaries.  (What lands in
+// the columns from D on is never read: the tensor maps end at D.)
 template <class T>
 __global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_t ld, T* dst, int64_t ldd, int64_t rows,
                                                             int64_t D) {
   constexpr int V = 16 / sizeof(T);
   const int lane = threadIdx.x & 31;
   const int64_t slabs = (ldd + 32 * V * 4 - 1) / (32 * V * 4);
+  const Span<T> span(src, rows, ld, D);
   const int64_t nw = (int64_t)gridDim.x * 8;
   for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < rows * slabs; i += nw) {
     const int64_t r = i / slabs, e0 = ((i - r * slabs) * 128 + lane) * V;
@@ -135,7 +138,7 @@ __global__ void __launch_bounds__(256) fw_xent_align_kernel(const T* src, int64_
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int64_t e = e0 + k * 32 * V;
-      if (e < ldd) u[k] = load_slot_shifted(src + r * ld, e, D);
+      if (e < ldd) u[k] = load_slot_shifted(src + r * ld, (int)e, span);
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
