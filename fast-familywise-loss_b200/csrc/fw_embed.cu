@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(256) fw_embed_rows_kernel(EmbedArgs a) {
         unpack16<T>(u[k], v);
 #pragma unroll
         for (int j = 0; j < V; ++j) v[j] = ok ? v[j] * a.scale : CUDART_NAN_F;
-        u[k] = pack16<T>(v);
+        u[k] = pack_slot<T>(v);
       }
       if (k < steps && e0 < D) store_slot(dst, e0, D, true, u[k]);
     }
@@ -402,9 +402,9 @@ __device__ __forceinline__ void store_sum(const EmbedGradArgs& a, T* dst, int e0
 #pragma unroll
   for (int j = 0; j < V; ++j) s[j] = acc[j] * a.scale;
   if (ALIGNED)
-    *reinterpret_cast<uint4*>(dst + e0) = pack16<T>(s);
+    *reinterpret_cast<uint4*>(dst + e0) = pack_slot<T>(s);
   else
-    store_slot(dst, e0, a.D, true, pack16<T>(s));
+    store_slot(dst, e0, a.D, true, pack_slot<T>(s));
 }
 
 // Start of slot `slot` in the row at dst: every row's own slots, so that a

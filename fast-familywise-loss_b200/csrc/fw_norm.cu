@@ -98,10 +98,17 @@ __device__ __forceinline__ float group_reduce(float v, float* buf, int& flip) {
     flip ^= 1;
     if ((threadIdx.x & 31) == 0) b[threadIdx.x >> 5] = v;
     __syncthreads();
-    float t = b[0];
+    // four partial results side by side, then their join: 16-byte loads, short chains
+    float t[4];
 #pragma unroll
-    for (int i = 1; i < G / 32; ++i) t = MAX ? max_nan(t, b[i]) : t + b[i];
-    v = t;
+    for (int i = 0; i < G / 128; ++i) {
+      const float4 x = reinterpret_cast<const float4*>(b)[i];
+      t[0] = i == 0 ? x.x : MAX ? max_nan(t[0], x.x) : t[0] + x.x;
+      t[1] = i == 0 ? x.y : MAX ? max_nan(t[1], x.y) : t[1] + x.y;
+      t[2] = i == 0 ? x.z : MAX ? max_nan(t[2], x.z) : t[2] + x.z;
+      t[3] = i == 0 ? x.w : MAX ? max_nan(t[3], x.w) : t[3] + x.w;
+    }
+    v = MAX ? max_nan(max_nan(t[0], t[1]), max_nan(t[2], t[3])) : (t[0] + t[1]) + (t[2] + t[3]);
   }
   return v;
 }
@@ -138,7 +145,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
   constexpr bool AHEAD = CH == 1;
-  __shared__ float red[2 * (G / 32)];
+  __shared__ __align__(16) float red[2 * (G / 32)];
   extern __shared__ __align__(16) int8_t qrow_all[];
   const int t = threadIdx.x % G;
   const int grp = threadIdx.x / G;
@@ -170,7 +177,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
         unpack16<T>(rs.u[k], u);
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] += v[k * V + j];
-        rs.u[k] = pack16<T>(u);
+        rs.u[k] = pack_slot<T>(u);
         unpack16<T>(rs.u[k], v + k * V);
         store_slot(static_cast<T*>(a.s) + r * a.lds, e0 + k * (G * V), a.D, a.vec, rs.u[k]);
       }
@@ -192,7 +199,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
     if constexpr (MODE == kNormOut) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
-        store_slot(static_cast<T*>(a.y) + r * a.ldy, e0 + k * (G * V), a.D, a.vec, pack16<T>(v + k * V));
+        store_slot(static_cast<T*>(a.y) + r * a.ldy, e0 + k * (G * V), a.D, a.vec, pack_slot<T>(v + k * V));
     } else {
       float m = 0.0f;
 #pragma unroll
@@ -252,7 +259,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
 // Rows too long for a CTA's registers: passes over the row in memory.
 template <class T, int MODE>
 __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
-  __shared__ float red[2 * 32];
+  __shared__ __align__(16) float red[2 * 32];
   int flip = 0;
   wait_prior_kernel();
   allow_dependent_launch();
@@ -309,7 +316,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
   constexpr bool AHEAD = CH == 1;
-  __shared__ float red[2 * (G / 32)];
+  __shared__ __align__(16) float red[2 * (G / 32)];
   extern __shared__ __align__(16) float dw_row[];  // [D], R > 1 only
   wait_prior_kernel();
   allow_dependent_launch();
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       unpack16<T>(co.u[k], o);
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = fmaf(rs, fmaf(-(s[j] * rs), c, g[j] * gain[k * V + j]), o[j]);
-      store_slot(static_cast<T*>(a.dx) + r * a.lddx, e0 + k * (G * V), a.D, a.vec, pack16<T>(o));
+      store_slot(static_cast<T*>(a.dx) + r * a.lddx, e0 + k * (G * V), a.D, a.vec, pack_slot<T>(o));
     }
     if (!AHEAD && r + step < a.rows) fetch(r + step);
   }
@@ -395,7 +402,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
 
 template <class T>
 __global__ void __launch_bounds__(1024) fw_norm_grad_long_kernel(NormGradArgs a) {
-  __shared__ float red[2 * 32];
+  __shared__ __align__(16) float red[2 * 32];
   int flip = 0;
   wait_prior_kernel();
   allow_dependent_launch();

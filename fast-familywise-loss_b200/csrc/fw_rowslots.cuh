@@ -58,6 +58,27 @@ __device__ __forceinline__ void store_slot(T* row, int64_t e0, int64_t D, bool v
   }
 }
 
+// Two values in one word, rounded to nearest by one instruction.
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  static_assert(sizeof(T) == 2, "16-bit types");
+  if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  } else {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+}
+
+template <class T>
+__device__ __forceinline__ uint4 pack_slot(const float* v) {
+  if constexpr (sizeof(T) == 4)
+    return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+  else
+    return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+}
+
 // First element of a matrix and the one behind its last.
 template <class T>
 struct Span {

@@ -31,6 +31,7 @@
 #pragma once
 
 #include "fw_host.cuh"
+#include "fw_rowslots.cuh"
 #include "fw_tc_ptx.cuh"
 
 namespace fwb200 {
@@ -491,7 +492,7 @@ __device__ __forceinline__ void stage_block(uint32_t* sm, const float (&v)[32], 
   static_assert(sizeof(T) == 2, "16-bit types");
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    sm[lane * kStageWords + c / 2 + i] = Elem<T>::f_to_bits(v[2 * i]) | (Elem<T>::f_to_bits(v[2 * i + 1]) << 16);
+    sm[lane * kStageWords + c / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
 }
 
 // `cols` columns of every row, 16 lanes per row; row_ptr(i) is where column 0

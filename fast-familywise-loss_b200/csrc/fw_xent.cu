@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(256) fw_xent_scale_kernel(const XentHead* head
       unpack16<T>(*reinterpret_cast<const uint4*>(hp + r * Dp + i * V), v);
 #pragma unroll
       for (int j = 0; j < V; ++j) v[j] = r < rows ? v[j] * f : 0.0f;
-      *reinterpret_cast<uint4*>(out + r * Dp + i * V) = pack16<T>(v);
+      *reinterpret_cast<uint4*>(out + r * Dp + i * V) = pack_slot<T>(v);
     }
   }
 }
@@ -462,7 +462,7 @@ struct GradTile {
         v[i] = i < valid ? q * coef : 0.0f;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(g + c + 8 * i) = pack16<T>(v + 8 * i);
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(g + c + 8 * i) = pack_slot<T>(v + 8 * i);
     }
   }
 };
