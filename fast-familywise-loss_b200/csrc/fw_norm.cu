@@ -14,14 +14,17 @@
 // Sums, statistics and gains are fp32; each output is rounded once.
 //
 // Bound by HBM: forward reads x and residual and writes s and y, backward
-// reads dy, s and ds_out and writes ds, each once.  A row lives in the
-// registers of a group of G threads (a warp, or a CTA of up to 1024) as CH
-// slots of 16 bytes per thread (fw_rowslots.cuh).  The grid is persistent
-// with a group count that is a multiple of 8, so that the rows one group
-// visits all start at the same distance from a 16-byte boundary: a thread
-// keeps the same columns from row to row, hence its gains and its part of dw
-// stay in registers for any D.  dw parts are written once per CTA and added
-// in a fixed order by a second kernel.
+// reads dy, s and ds_out and writes ds, each once.  A row belongs to a group
+// of G threads (a warp, or a CTA of up to 1024), CH slots of 16 bytes per
+// thread (fw_rowslots.cuh).  The next kAhead rows of a group are on their way
+// into shared memory (cp.async; each thread copies the slots it will read, so
+// no barrier is needed) while a row is reduced: a CTA-wide reduction would
+// otherwise drain the memory pipe at every row.  The grid is persistent with
+// a group count that is a multiple of 8, so that the rows one group visits
+// all start at the same distance from a 16-byte boundary: a thread keeps the
+// same columns from row to row, hence its gains and its part of dw stay in
+// registers for any D.  dw parts are written once per CTA and added in a
+// fixed order by a second kernel.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -125,28 +128,66 @@ __host__ __device__ constexpr int cta_threads() {
   return G < 128 ? 128 : G;
 }
 
-// The slots of one row that a thread holds.
-template <class T, int CH>
-struct Slots {
-  uint4 u[CH];
-  __device__ __forceinline__ void load(const void* base, int64_t row, int64_t ld, int64_t e0, int64_t step, int64_t D,
-                                       int vec) {
-    const T* p = static_cast<const T*>(base) + row * ld;
+constexpr int kAhead = 2;  // rows of a group in flight
+
+// A thread's slots of the rows in flight, of NT matrices, in shared memory
+// (slot k of stage d of matrix m at [(d * NT + m) * CH + k][t]).
+template <class T, int G, int CH, int NT>
+struct RowRing {
+  static constexpr int V = 16 / sizeof(T);
+  uint4* mine;
+  int e0, D;   // first element of slot 0 (negative where the row starts inside it), elements of a row
+  int vec;
+
+  __device__ __forceinline__ void init(uint4* smem, int grp, int t, int off, int D_, int vec_) {
+    mine = smem + (size_t)grp * kAhead * NT * CH * G + t;
+    e0 = t * V - off;
+    D = D_;
+    vec = vec_;
 #pragma unroll
-    for (int k = 0; k < CH; ++k) u[k] = load_slot(p, e0 + k * step, D, vec);
+    for (int i = 0; i < kAhead * NT * CH; ++i) mine[i * G] = make_uint4(0u, 0u, 0u, 0u);  // slots past the row stay 0
+  }
+  // Starts matrix m's row (number r of its matrix) on its way into stage d.
+  __device__ __forceinline__ void fetch(int d, int m, const T* row, int64_t r) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int e = e0 + k * (G * V);
+      if (e >= D) continue;
+      uint4* to = mine + ((d * NT + m) * CH + k) * G;
+      if (vec && (e >= 0 || r > 0)) {
+        // whole slots of memory: what lies before the row is masked when read, behind it is not read
+        const uint32_t bytes = min(16, (D - e) * (int)sizeof(T));
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(to)), "l"(row + e), "r"(bytes)
+                     : "memory");
+      } else {
+        *to = load_elems(row + e, row, row + D);
+      }
+    }
+  }
+  __device__ __forceinline__ static void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  // The oldest row in flight has landed.
+  __device__ __forceinline__ static void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory"); }
+  __device__ __forceinline__ void get(int d, int m, int k, float* v) const {
+    unpack16<T>(mine[((d * NT + m) * CH + k) * G], v);
+    if (k == 0 && e0 < 0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < -e0) v[j] = 0.0f;
+    }
   }
 };
 
-// The loads of a group's next row are issued before the current row is
-// reduced (CH = 1: the registers allow it), so that the memory pipe does not
-// drain at the reductions.
+template <class T, int G, int CH>
+__host__ __device__ constexpr size_t ring_bytes(int nt) {
+  return (size_t)(G < 128 ? 128 / G : 1) * kAhead * nt * CH * G * 16;
+}
+
 template <class T, int G, int CH, int MODE>
 __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_norm_kernel(NormArgs a) {
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
-  constexpr bool AHEAD = CH == 1;
   __shared__ __align__(16) float red[2 * (G / 32)];
-  extern __shared__ __align__(16) int8_t qrow_all[];
+  extern __shared__ __align__(16) uint4 norm_smem[];
   const int t = threadIdx.x % G;
   const int grp = threadIdx.x / G;
   const int64_t step = (int64_t)gridDim.x * R;
@@ -156,36 +197,45 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   if (first >= a.rows) return;  // a whole group; groups of one CTA share no barrier unless R == 1
   int flip = 0;
   const int off = row_off<T>(a.x, first, a.ldx, a.vec);
-  const int64_t e0 = (int64_t)t * V - off;
-  Slots<T, CH> xs, rs;
-  xs.load(a.x, first, a.ldx, e0, G * V, a.D, a.vec);
-  if (a.res) rs.load(a.res, first, a.ldr, e0, G * V, a.D, a.vec);
+  const int D = (int)a.D;  // fits: longer rows take the other kernel
+  RowRing<T, G, CH, 2> ring;
+  ring.init(norm_smem, grp, t, off, D, a.vec);
+  const int e0 = ring.e0;
+  auto fetch = [&](int d, int64_t r) {
+    if (r < a.rows) {
+      ring.fetch(d, 0, static_cast<const T*>(a.x) + r * a.ldx, r);
+      if (a.res) ring.fetch(d, 1, static_cast<const T*>(a.res) + r * a.ldr, r);
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) fetch(d, first + d * step);
   float gain[CH * V];
   if constexpr (MODE != kInt8Only) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, e0 + k * (G * V), a.D, gain + k * V);
+    for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, e0 + k * (G * V), D, gain + k * V);
   }
   const float inv_d = 1.0f / (float)a.D;
+  int d = 0;
   for (int64_t r = first; r < a.rows; r += step) {
+    ring.wait();
     float v[CH * V];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) unpack16<T>(xs.u[k], v + k * V);
+    for (int k = 0; k < CH; ++k) ring.get(d, 0, k, v + k * V);
     if (a.res) {
 #pragma unroll
       for (int k = 0; k < CH; ++k) {
         float u[V];
-        unpack16<T>(rs.u[k], u);
+        ring.get(d, 1, k, u);
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] += v[k * V + j];
-        rs.u[k] = pack_slot<T>(u);
-        unpack16<T>(rs.u[k], v + k * V);
-        store_slot(static_cast<T*>(a.s) + r * a.lds, e0 + k * (G * V), a.D, a.vec, rs.u[k]);
+        const uint4 p = pack_slot<T>(u);
+        unpack16<T>(p, v + k * V);
+        store_slot(static_cast<T*>(a.s) + r * a.lds, e0 + k * (G * V), D, a.vec, p);
       }
     }
-    if (AHEAD && r + step < a.rows) {
-      xs.load(a.x, r + step, a.ldx, e0, G * V, a.D, a.vec);
-      if (a.res) rs.load(a.res, r + step, a.ldr, e0, G * V, a.D, a.vec);
-    }
+    fetch(d, r + kAhead * step);
+    d = d + 1 == kAhead ? 0 : d + 1;
     if constexpr (MODE != kInt8Only) {
       float ss = 0.0f;
 #pragma unroll
@@ -199,7 +249,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
     if constexpr (MODE == kNormOut) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
-        store_slot(static_cast<T*>(a.y) + r * a.ldy, e0 + k * (G * V), a.D, a.vec, pack_slot<T>(v + k * V));
+        store_slot(static_cast<T*>(a.y) + r * a.ldy, e0 + k * (G * V), D, a.vec, pack_slot<T>(v + k * V));
     } else {
       float m = 0.0f;
 #pragma unroll
@@ -209,11 +259,11 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       if (t == 0) a.qscale[r] = scale;
       // a row of zeros, or not finite, is 0 (or NaN) through its scale
       const float steps = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / scale : 0.0f;
-      const int64_t w16 = (a.D + 15) / 16 * 16;
+      const int w16 = (D + 15) / 16 * 16;
       if (off == 0) {  // the slots' bytes lie together in q
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
-          const int64_t e = e0 + k * (G * V);
+          const int e = e0 + k * (G * V);
           if (e >= w16) continue;
           uint32_t b[V / 4];
 #pragma unroll
@@ -226,32 +276,28 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
             *reinterpret_cast<uint32_t*>(a.q + r * a.ldq + e) = b[0];
         }
         if constexpr (CH * G * V < 16 * 64) {  // short rows: the padding may lie past the last slot
-          for (int64_t e = (int64_t)(CH * G + t) * V; e < w16; e += G * V)
+          for (int e = (CH * G + t) * V; e < w16; e += G * V)
             for (int j = 0; j < V; ++j) a.q[r * a.ldq + e + j] = 0;
         }
       } else {  // through shared memory
-        int8_t* qs = qrow_all + (int64_t)grp * w16;
-        if (t < 16 && a.D + t < w16) qs[a.D + t] = 0;
+        int8_t* qs = reinterpret_cast<int8_t*>(norm_smem) + ring_bytes<T, G, CH>(2) + grp * w16;
+        if (t < 16 && D + t < w16) qs[D + t] = 0;
 #pragma unroll
         for (int i = 0; i < CH * V; ++i) {
-          const int64_t e = e0 + (i / V) * (G * V) + i % V;
-          if (e >= 0 && e < a.D) qs[e] = (int8_t)int8_step(v[i], steps);
+          const int e = e0 + (i / V) * (G * V) + i % V;
+          if (e >= 0 && e < D) qs[e] = (int8_t)int8_step(v[i], steps);
         }
         if constexpr (G > 32)
           __syncthreads();
         else
           __syncwarp();
-        for (int64_t i = t; i < w16 / 16; i += G)
+        for (int i = t; i < w16 / 16; i += G)
           reinterpret_cast<uint4*>(a.q + r * a.ldq)[i] = reinterpret_cast<const uint4*>(qs)[i];
         if constexpr (G > 32)
           __syncthreads();
         else
           __syncwarp();
       }
-    }
-    if (!AHEAD && r + step < a.rows) {
-      xs.load(a.x, r + step, a.ldx, e0, G * V, a.D, a.vec);
-      if (a.res) rs.load(a.res, r + step, a.ldr, e0, G * V, a.D, a.vec);
     }
   }
 }
@@ -315,9 +361,8 @@ template <class T, int G, int CH>
 __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_norm_grad_kernel(NormGradArgs a) {
   constexpr int V = 16 / sizeof(T);
   constexpr int R = cta_threads<G>() / G;
-  constexpr bool AHEAD = CH == 1;
   __shared__ __align__(16) float red[2 * (G / 32)];
-  extern __shared__ __align__(16) float dw_row[];  // [D], R > 1 only
+  extern __shared__ __align__(16) uint4 norm_smem[];
   wait_prior_kernel();
   allow_dependent_launch();
   const int t = threadIdx.x % G;
@@ -326,34 +371,38 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
   const int64_t first = (int64_t)blockIdx.x * R + grp;
   int flip = 0;
   const int off = row_off<T>(a.s, first, a.lds, a.vec);
+  const int D = (int)a.D;
+  RowRing<T, G, CH, 3> ring;
+  ring.init(norm_smem, grp, t, off, D, a.vec);
+  const int e0 = ring.e0;
+  auto fetch = [&](int d, int64_t r) {
+    if (r < a.rows) {
+      ring.fetch(d, 0, static_cast<const T*>(a.s) + r * a.lds, r);
+      ring.fetch(d, 1, static_cast<const T*>(a.dy) + r * a.lddy, r);
+      if (a.dso) ring.fetch(d, 2, static_cast<const T*>(a.dso) + r * a.ldo, r);
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) fetch(d, first + d * step);
   float gain[CH * V], dw[CH * V];
 #pragma unroll
-  for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, (int64_t)(k * G + t) * V - off, a.D, gain + k * V);
+  for (int k = 0; k < CH; ++k) load_gain<T>(a.w, a.w_f32, e0 + k * (G * V), D, gain + k * V);
 #pragma unroll
   for (int i = 0; i < CH * V; ++i) dw[i] = 0.0f;
   const float inv_d = 1.0f / (float)a.D;
-  const int64_t e0 = (int64_t)t * V - off;
-  Slots<T, CH> ss, gs, os;
-  float rstd = 0.0f;
-  auto fetch = [&](int64_t r) {
-    ss.load(a.s, r, a.lds, e0, G * V, a.D, a.vec);
-    gs.load(a.dy, r, a.lddy, e0, G * V, a.D, a.vec);
-    if (a.dso) os.load(a.dso, r, a.ldo, e0, G * V, a.D, a.vec);
-    rstd = a.rstd[r];
-  };
-  if (first < a.rows) fetch(first);
+  float rs_next = first < a.rows ? a.rstd[first] : 0.0f;
+  int d = 0;
   for (int64_t r = first; r < a.rows; r += step) {
-    // the current row stays packed: unpacking twice costs fewer registers
-    const Slots<T, CH> cs = ss, cg = gs;
-    Slots<T, CH> co = os;
-    const float rs = rstd;
-    if (AHEAD && r + step < a.rows) fetch(r + step);
+    const float rs = rs_next;
+    if (r + step < a.rows) rs_next = a.rstd[r + step];
+    ring.wait();
     float c = 0.0f;
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float s[V], g[V];
-      unpack16<T>(cs.u[k], s);
-      unpack16<T>(cg.u[k], g);
+      ring.get(d, 0, k, s);
+      ring.get(d, 1, k, g);
 #pragma unroll
       for (int j = 0; j < V; ++j) {
         const float n = s[j] * rs;
@@ -362,18 +411,19 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       }
     }
     c = group_reduce<G, false>(c, red, flip) * inv_d;
+    // read again rather than kept: registers are what bounds the rows in flight
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       float s[V], g[V], o[V];
-      unpack16<T>(cs.u[k], s);
-      unpack16<T>(cg.u[k], g);
-      if (!a.dso) co.u[k] = make_uint4(0u, 0u, 0u, 0u);
-      unpack16<T>(co.u[k], o);
+      ring.get(d, 0, k, s);
+      ring.get(d, 1, k, g);
+      ring.get(d, 2, k, o);  // zero without dsum
 #pragma unroll
       for (int j = 0; j < V; ++j) o[j] = fmaf(rs, fmaf(-(s[j] * rs), c, g[j] * gain[k * V + j]), o[j]);
-      store_slot(static_cast<T*>(a.dx) + r * a.lddx, e0 + k * (G * V), a.D, a.vec, pack_slot<T>(o));
+      store_slot(static_cast<T*>(a.dx) + r * a.lddx, e0 + k * (G * V), D, a.vec, pack_slot<T>(o));
     }
-    if (!AHEAD && r + step < a.rows) fetch(r + step);
+    fetch(d, r + kAhead * step);
+    d = d + 1 == kAhead ? 0 : d + 1;
   }
   if (!a.part) return;
   float* part = a.part + (int64_t)blockIdx.x * a.D;
@@ -384,6 +434,8 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       if (e >= 0 && e < a.D) part[e] = dw[i];
     }
   } else {
+    float* dw_row = reinterpret_cast<float*>(norm_smem);  // the rings are done with
+    __syncthreads();
     for (int64_t e = threadIdx.x; e < a.D; e += blockDim.x) dw_row[e] = 0.0f;
     for (int g = 0; g < R; ++g) {  // the CTA's groups in order: their rows start at different distances
       __syncthreads();
@@ -454,9 +506,9 @@ __global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restric
   if (lane == 0 && c < D) st_elem(dw + c, s);
 }
 
-// Threads per row by the row's slot count: a warp, or a CTA with one slot per
-// thread (two in the longest), so that a thread's 64 registers hold the row
-// and the next one; the memory-pass kernels beyond 2048 slots.
+// Threads per row by the row's slot count: a warp, or a CTA with one or two
+// slots per thread, so that a thread's 64 registers hold its gains and its
+// part of dw; the memory-pass kernels beyond 2048 slots.
 struct NormShape {
   int G, CH;
 };
@@ -466,9 +518,9 @@ NormShape norm_shape(int64_t D, int64_t esize, bool vec) {
   const int64_t n = (D + V - 1) / V + (vec && (D * esize) % 16 != 0 ? 1 : 0);
   if (n <= 32) return {32, 1};
   if (n <= 128) return {128, 1};
-  if (n <= 256) return {256, 1};
-  if (n <= 512) return {512, 1};
-  if (n <= 1024) return {1024, 1};
+  if (n <= 256) return {128, 2};
+  if (n <= 512) return {256, 2};
+  if (n <= 1024) return {512, 2};
   if (n <= 2048) return {1024, 2};
   return {0, 0};
 }
@@ -504,37 +556,61 @@ bool ld_ok(int64_t ld, int64_t rows, int64_t D) {
   return ld >= D && (rows <= 0 || ld <= ((int64_t)1 << 60) / rows);
 }
 
+// More than 48 KB of shared memory has to be asked for, once per device.
+template <class... KArgs, class A>
+cudaError_t launch_rows(void (*kernel)(KArgs...), std::atomic<bool>* asked, int64_t grid, int threads, size_t smem,
+                        cudaStream_t st, const A& a) {
+  if (smem > 40 * 1024) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= kMaxDevices || !asked[dev].load(std::memory_order_acquire)) {
+      e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - 1024);
+      if (e != cudaSuccess) return e;
+      if (dev < kMaxDevices) asked[dev].store(true, std::memory_order_release);
+    }
+  }
+  return launch_dependent(kernel, grid, threads, smem, 1, st, a);
+}
+
+template <class T, int MODE, int G, int CH>
+cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
+  static std::atomic<bool> asked[kMaxDevices] = {};
+  const size_t q = MODE == kNormOut ? 0 : (size_t)(G < 128 ? 128 / G : 1) * (size_t)((a.D + 15) / 16 * 16);
+  return launch_rows(fw_norm_kernel<T, G, CH, MODE>, asked, norm_grid(a.rows, G), cta_threads<G>(),
+                     ring_bytes<T, G, CH>(2) + q, st, a);
+}
+
 template <class T, int MODE>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
   const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
-  const int64_t grid = norm_grid(a.rows, sh.G);
-  cudaError_t e;
-  const int R = sh.G == 32 ? 4 : 1;
-  const size_t smem = MODE == kNormOut ? 0 : (size_t)R * (size_t)((a.D + 15) / 16 * 16);
-  if (sh.G == 32) e = launch_dependent(fw_norm_kernel<T, 32, 1, MODE>, grid, 128, smem, 1, st, a);
-  else if (sh.G == 128) e = launch_dependent(fw_norm_kernel<T, 128, 1, MODE>, grid, 128, smem, 1, st, a);
-  else if (sh.G == 256) e = launch_dependent(fw_norm_kernel<T, 256, 1, MODE>, grid, 256, smem, 1, st, a);
-  else if (sh.G == 512) e = launch_dependent(fw_norm_kernel<T, 512, 1, MODE>, grid, 512, smem, 1, st, a);
-  else if (sh.G == 1024 && sh.CH == 1) e = launch_dependent(fw_norm_kernel<T, 1024, 1, MODE>, grid, 1024, smem, 1, st, a);
-  else if (sh.G == 1024) e = launch_dependent(fw_norm_kernel<T, 1024, 2, MODE>, grid, 1024, smem, 1, st, a);
-  else e = launch_dependent(fw_norm_long_kernel<T, MODE>, grid, 1024, 0, 1, st, a);
-  return e;
+  if (sh.G == 32) return launch_norm<T, MODE, 32, 1>(a, st);
+  if (sh.G == 128 && sh.CH == 1) return launch_norm<T, MODE, 128, 1>(a, st);
+  if (sh.G == 128) return launch_norm<T, MODE, 128, 2>(a, st);
+  if (sh.G == 256) return launch_norm<T, MODE, 256, 2>(a, st);
+  if (sh.G == 512) return launch_norm<T, MODE, 512, 2>(a, st);
+  if (sh.G == 1024) return launch_norm<T, MODE, 1024, 2>(a, st);
+  return launch_dependent(fw_norm_long_kernel<T, MODE>, norm_grid(a.rows, 0), 1024, 0, 1, st, a);
+}
+
+template <class T, int G, int CH>
+cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
+  static std::atomic<bool> asked[kMaxDevices] = {};
+  size_t smem = ring_bytes<T, G, CH>(3);
+  if (G < 128 && smem < (size_t)a.D * 4) smem = (size_t)a.D * 4;
+  return launch_rows(fw_norm_grad_kernel<T, G, CH>, asked, norm_grid(a.rows, G), cta_threads<G>(), smem, st, a);
 }
 
 template <class T>
 cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
   const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
-  const int64_t grid = norm_grid(a.rows, sh.G);
-  cudaError_t e;
-  const size_t smem = sh.G == 32 ? (size_t)a.D * sizeof(float) : 0;
-  if (sh.G == 32) e = launch_dependent(fw_norm_grad_kernel<T, 32, 1>, grid, 128, smem, 1, st, a);
-  else if (sh.G == 128) e = launch_dependent(fw_norm_grad_kernel<T, 128, 1>, grid, 128, smem, 1, st, a);
-  else if (sh.G == 256) e = launch_dependent(fw_norm_grad_kernel<T, 256, 1>, grid, 256, smem, 1, st, a);
-  else if (sh.G == 512) e = launch_dependent(fw_norm_grad_kernel<T, 512, 1>, grid, 512, smem, 1, st, a);
-  else if (sh.G == 1024 && sh.CH == 1) e = launch_dependent(fw_norm_grad_kernel<T, 1024, 1>, grid, 1024, smem, 1, st, a);
-  else if (sh.G == 1024) e = launch_dependent(fw_norm_grad_kernel<T, 1024, 2>, grid, 1024, smem, 1, st, a);
-  else e = launch_dependent(fw_norm_grad_long_kernel<T>, grid, 1024, 0, 1, st, a);
-  return e;
+  if (sh.G == 32) return launch_norm_grad<T, 32, 1>(a, st);
+  if (sh.G == 128 && sh.CH == 1) return launch_norm_grad<T, 128, 1>(a, st);
+  if (sh.G == 128) return launch_norm_grad<T, 128, 2>(a, st);
+  if (sh.G == 256) return launch_norm_grad<T, 256, 2>(a, st);
+  if (sh.G == 512) return launch_norm_grad<T, 512, 2>(a, st);
+  if (sh.G == 1024) return launch_norm_grad<T, 1024, 2>(a, st);
+  return launch_dependent(fw_norm_grad_long_kernel<T>, norm_grid(a.rows, 0), 1024, 0, 1, st, a);
 }
 
 template <int MODE>
