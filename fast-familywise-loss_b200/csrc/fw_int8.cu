@@ -34,15 +34,15 @@ struct Int8Args {
 template <class TO, int SIDE>
 struct Int8Many {
   using Args = Int8Args;
+  static constexpr int COLS = SIDE / 2;  // per epilogue warp
   struct State {
-    float qs, ws[4];
+    float qs, ws[COLS / 32];
   };
   static constexpr TcKind KIND = kTcS8;
   static constexpr bool A_MN = false, B_MN = false;
   static constexpr bool TWO = false, A_MN2 = false;
-  static constexpr int CG = SIDE / 128, BN = SIDE, STAGES = 5, KC = 0, EW = SIDE / 32, A_BOX = 128, AHEAD = 0;
-  static constexpr int COLS = 128;  // per epilogue warp
-  static constexpr uint32_t EPI_BYTES = EW * (sizeof(TO) == 2 ? kStageBytes : 32 * 33 * 4);
+  static constexpr int CG = SIDE / 128, BN = SIDE, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
+  static constexpr uint32_t EPI_BYTES = EW * (sizeof(TO) == 2 ? kStageBytes<COLS> : 32 * 33 * 4);
   struct Plan {
     TileOrder order;
     int first, step;
@@ -79,13 +79,13 @@ struct Int8Many {
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * st.qs * __shfl_sync(kFull, st.ws[c / 32], i);
       if constexpr (sizeof(TO) == 2)
-        stage_block<TO>(reinterpret_cast<uint32_t*>(p.smem), v, p.lane, c);
+        stage_block<TO, COLS>(reinterpret_cast<uint32_t*>(p.smem), v, p.lane, c);
       else
         store_block(reinterpret_cast<float*>(p.smem), v, p.lane, a.N - (t.n0 + s0 + c), a.vec,
                     [&](int i) -> float* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo + c : nullptr; });
     }
     if constexpr (sizeof(TO) == 2)
-      store_staged<TO>(reinterpret_cast<uint32_t*>(p.smem), p.lane, min(COLS, a.N - (t.n0 + s0)),
+      store_staged<TO, COLS>(reinterpret_cast<uint32_t*>(p.smem), p.lane, min(COLS, a.N - (t.n0 + s0)),
                        [&](int i) -> TO* { return i < rows ? out + (int64_t)(r0 + i) * a.ldo : nullptr; });
   }
 };

@@ -480,32 +480,35 @@ __device__ __forceinline__ void store_block(float* sm, const float (&v)[32], int
   __syncwarp();
 }
 
-// A warp's 32 x 128 block of 16-bit values: staged one row per thread, then
+// A warp's 32 x COLS block of 16-bit values: staged one row per thread, then
 // stored row by row.  Rows may start anywhere: the stores are the 16-byte
 // slots of the destination, single elements only at a segment's two ends (32
 // lanes of 2 bytes each would write parts of sectors, at a fifth of the rate).
-constexpr int kStageWords = 65;  // 32-bit words of a row: 64, and one against bank conflicts
-constexpr uint32_t kStageBytes = 32 * kStageWords * 4;
+template <int COLS>
+constexpr int kStageWords = COLS / 2 + 1;  // 32-bit words of a row, and one against bank conflicts
+template <int COLS>
+constexpr uint32_t kStageBytes = 32 * kStageWords<COLS> * 4;
 
-template <class T>
+template <class T, int COLS>
 __device__ __forceinline__ void stage_block(uint32_t* sm, const float (&v)[32], int lane, int c) {
   static_assert(sizeof(T) == 2, "16-bit types");
 #pragma unroll
   for (int i = 0; i < 16; ++i)
-    sm[lane * kStageWords + c / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
+    sm[lane * kStageWords<COLS> + c / 2 + i] = pack2<T>(v[2 * i], v[2 * i + 1]);
 }
 
-// `cols` columns of every row, 16 lanes per row; row_ptr(i) is where column 0
+// `cols` columns of every row, a lane per slot; row_ptr(i) is where column 0
 // of row i goes, or NULL.
-template <class T, class RowPtr>
+template <class T, int COLS, class RowPtr>
 __device__ __forceinline__ void store_staged(const uint32_t* sm, int lane, int cols, RowPtr row_ptr) {
   __syncwarp();
-  const int k = lane & 15;
+  constexpr int LANES = COLS / 8;
+  const int k = lane % LANES;
 #pragma unroll 4
-  for (int i0 = 0; i0 < 32; i0 += 2) {
-    const int i = i0 + (lane >> 4);
+  for (int i0 = 0; i0 < 32; i0 += 32 / LANES) {
+    const int i = i0 + lane / LANES;
     unsigned short* p = reinterpret_cast<unsigned short*>(row_ptr(i));
-    const uint32_t* row = sm + i * kStageWords;
+    const uint32_t* row = sm + i * kStageWords<COLS>;
     // elements before the first slot, slots, elements behind the last
     const int head = min((int)(-(reinterpret_cast<uintptr_t>(p) >> 1) & 7u), cols);
     const int whole = (cols - head) >> 3, tail = head + whole * 8;
@@ -520,8 +523,11 @@ __device__ __forceinline__ void store_staged(const uint32_t* sm, int lane, int c
       }
       *reinterpret_cast<uint4*>(p + e0) = u;
     }
-    const int e = k < 8 ? k : tail + k - 8;  // lanes 0..7: head, 8..15: tail
-    if (p && e < (k < 8 ? head : cols)) p[e] = (unsigned short)(row[e >> 1] >> (16 * (e & 1)));
+#pragma unroll
+    for (int j = k; j < 16; j += LANES) {  // 0..7: head, 8..15: tail
+      const int e = j < 8 ? j : tail + j - 8;
+      if (p && e < (j < 8 ? head : cols)) p[e] = (unsigned short)(row[e >> 1] >> (16 * (e & 1)));
+    }
   }
   __syncwarp();
 }

@@ -514,7 +514,7 @@ struct ProductTile {
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
   static constexpr int CG = 2, BN = kTileN, STAGES = 5, KC = 0, EW = 8, A_BOX = 128, AHEAD = 0;
-  static constexpr uint32_t EPI_BYTES = EW * kStageBytes;
+  static constexpr uint32_t EPI_BYTES = EW * kStageBytes<BN / 2>;
 
   // Tiles: the long ones of dH with vn / 64 / splits stages each, then the
   // short ones of dW with rows / 64, then (last piece, one split) those of dH
@@ -622,12 +622,12 @@ struct ProductTile {
       if (!store) continue;
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = st.zero ? 0.0f : v[i] * st.f;
-      stage_block<T>(sm, v, p.lane, c);
+      stage_block<T, BN / 2>(sm, v, p.lane, c);
     }
     if (!store || cols <= 0) return;
     const int rows = a.V - (a.v0 + r0);  // dW
     T* out = (dh ? static_cast<T*>(a.dhidden) : static_cast<T*>(a.dweight) + (int64_t)(a.v0 + r0) * a.D) + t.n0 + s0;
-    store_staged<T>(sm, p.lane, min(cols, BN / 2), [&](int i) -> T* {
+    store_staged<T, BN / 2>(sm, p.lane, min(cols, BN / 2), [&](int i) -> T* {
       const int r = dh ? __shfl_sync(kFull, st.mine, i) : i < rows ? i : -1;
       return r >= 0 ? out + (int64_t)r * a.D : nullptr;
     });
