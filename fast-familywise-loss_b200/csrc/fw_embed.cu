@@ -505,45 +505,85 @@ __global__ void __launch_bounds__(256, ALIGNED ? 4 : 2) fw_embed_sum_kernel(Embe
 }
 
 // Runs that cross chunks: one warp per chunk that such a run begins in and
-// slab of its row.
+// slab of its row; runs of more than kJoinAlone parts by the eight warps of
+// the CTA, a stretch of parts each (its items are eight chunks of one slab, so
+// that one long run asks for one CTA per slab).
+constexpr int kJoinAlone = 16;
+
 template <class T, bool ALIGNED>
 __global__ void __launch_bounds__(256) fw_embed_join_kernel(EmbedGradArgs a) {
   constexpr int V = 16 / sizeof(T);
+  __shared__ int64_t count[8];  // parts of the run of each warp's item, 0 for none
+  __shared__ float4 stretch[8][V / 4][32];
   wait_prior_kernel();
   allow_dependent_launch();
-  const int lane = threadIdx.x & 31;
-  const int64_t slabs = (a.nslots + 31) / 32, chunks = (a.T + kChunk - 1) / kChunk, work = chunks * slabs;
-  const int64_t nw = (int64_t)gridDim.x * (blockDim.x / 32);
-  for (int64_t i = (int64_t)blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5); i < work; i += nw) {
-    const int64_t c = i / slabs, b = c * kChunk;
-    const int slot = (int)(i % slabs) * 32 + lane;
-    if (b + kChunk >= a.T) continue;
-    const uint32_t key = a.sorted[b + kChunk - 1].x;
-    if (key >= (uint32_t)a.V || a.sorted[b + kChunk].x != key) continue;          // nothing goes on
-    if (a.sorted[b].x == key && b > 0 && a.sorted[b - 1].x == key) continue;  // it began earlier
-    int64_t end = c + 1;  // the last chunk of the run, found 32 chunks at a time
-    for (;;) {
-      const int64_t next = end + 1 + lane;  // does chunk `next` begin with the key?
-      const uint32_t more = __ballot_sync(kFull, next < chunks && a.sorted[next * kChunk].x == key);
-      end += more == kFull ? 32 : __ffs(~more) - 1;
-      if (more != kFull) break;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t slabs = (a.nslots + 31) / 32, chunks = (a.T + kChunk - 1) / kChunk;
+  const int64_t groups = (chunks + 7) / 8, work = groups * slabs;
+  for (int64_t i = blockIdx.x; i < work; i += gridDim.x) {
+    const int64_t c0 = i % groups * 8, c = c0 + w, b = c * kChunk;
+    const int slot = (int)(i / groups) * 32 + lane;
+    int64_t n = 0;
+    if (b + kChunk < a.T) {
+      const uint32_t key = a.sorted[b + kChunk - 1].x;
+      const bool on = key < (uint32_t)a.V && a.sorted[b + kChunk].x == key;
+      const bool earlier = a.sorted[b].x == key && b > 0 && a.sorted[b - 1].x == key;
+      if (on && !earlier) {
+        n = 2;  // its parts, found 32 chunks at a time
+        for (;;) {
+          const int64_t next = c + n + lane;  // does chunk `next` begin with the key?
+          const uint32_t more = __ballot_sync(kFull, next < chunks && a.sorted[next * kChunk].x == key);
+          n += more == kFull ? 32 : __ffs(~more) - 1;
+          if (more != kFull) break;
+        }
+      }
     }
-    float acc[V];
+    // parts from .. to of the run that begins in chunk c, in order
+    auto add = [&](int64_t c, int64_t from, int64_t to, float* acc) {
 #pragma unroll
-    for (int j = 0; j < V; ++j) acc[j] = 0.0f;
-    if (slot < a.nslots) {
+      for (int j = 0; j < V; ++j) acc[j] = 0.0f;
+      if (slot >= a.nslots) return;
 #pragma unroll 8
-      for (int64_t q = c; q <= end; ++q) {
-        const float4* p = reinterpret_cast<const float4*>(a.part + (2 * q + (q == c ? 1 : 0)) * a.pitch + slot * V);
+      for (int64_t q = from; q < to; ++q) {
+        const float4* p = reinterpret_cast<const float4*>(a.part + (2 * (c + q) + (q == 0 ? 1 : 0)) * a.pitch + slot * V);
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
           const float4 x = p[j];
           acc[4 * j] += x.x, acc[4 * j + 1] += x.y, acc[4 * j + 2] += x.z, acc[4 * j + 3] += x.w;
         }
       }
-      T* dst = static_cast<T*>(a.dw) + (int64_t)key * a.D;
-      store_sum<T, ALIGNED>(a, dst, slot_elem<T, ALIGNED>(dst, slot), acc);
+    };
+    auto store = [&](int64_t c, const float* acc) {
+      T* dst = static_cast<T*>(a.dw) + (int64_t)a.sorted[c * kChunk + kChunk - 1].x * a.D;
+      if (slot < a.nslots) store_sum<T, ALIGNED>(a, dst, slot_elem<T, ALIGNED>(dst, slot), acc);
+    };
+    float acc[V];
+    if (n > 0 && n <= kJoinAlone) {
+      add(c, 0, n, acc);
+      store(c, acc);
     }
+    if (lane == 0) count[w] = n;
+    __syncthreads();
+    for (int k = 0; k < 8; ++k) {
+      const int64_t parts = count[k];
+      if (parts <= kJoinAlone) continue;
+      add(c0 + k, parts * w / 8, parts * (w + 1) / 8, acc);
+#pragma unroll
+      for (int j = 0; j < V / 4; ++j)
+        stretch[w][j][lane] = make_float4(acc[4 * j], acc[4 * j + 1], acc[4 * j + 2], acc[4 * j + 3]);
+      __syncthreads();
+      if (w == 0) {
+        for (int q = 1; q < 8; ++q)
+#pragma unroll
+          for (int j = 0; j < V / 4; ++j) {
+            const float4 x = stretch[q][j][lane];
+            acc[4 * j] += x.x, acc[4 * j + 1] += x.y, acc[4 * j + 2] += x.z, acc[4 * j + 3] += x.w;
+          }
+        store(c0 + k, acc);
+      }
+      __syncthreads();
+    }
+    __syncthreads();
   }
 }
 
@@ -677,7 +717,7 @@ cudaError_t launch_embed_grad(EmbedGradArgs a, SortArgs s, const EmbedPlan& p, u
   a.sum_blocks = (int)warps_grid(p.chunks * slabs);
   e = launch_dependent(fw_embed_sum_kernel<T, ALIGNED>, a.sum_blocks + zero, 256, 0, 1, st, a);
   if (e != cudaSuccess) return e;
-  return launch_dependent(fw_embed_join_kernel<T, ALIGNED>, warps_grid(p.chunks * slabs), 256, 0, 1, st, a);
+  return launch_dependent(fw_embed_join_kernel<T, ALIGNED>, warps_grid((p.chunks + 7) / 8 * 8 * slabs), 256, 0, 1, st, a);
 }
 
 template <class T>
