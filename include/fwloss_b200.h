@@ -545,7 +545,8 @@ FWB_API int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const fl
  * fw_xent_backward writes dhidden [B, D] and dweight [V, D] (contiguous,
  * either may be NULL) for grad_output ([B] for FWB_REDUCE_NONE, else one
  * value), the logit gradient formed in pieces of the vocabulary.  Both
- * buffers and the workspaces (fw_xent_workspace bytes) are 16-byte aligned.
+ * buffers and the workspaces (fw_xent_workspace bytes, for the device that is
+ * current: it depends on the SM count) are 16-byte aligned.
  */
 #define FWB_REDUCE_NONE 0
 #define FWB_REDUCE_MEAN 1
