@@ -5,16 +5,25 @@
 //
 // Two layouts of the same product:
 //   many tokens  tokens are the rows of a tile, weight rows its columns: 256 x
-//                256 tiles by two CTAs, bound by the tensor cores, or, where
-//                those are too few for the SMs, 128 x 128 tiles by one;
+//                256 tiles by two CTAs, bound by the tensor cores (4096 x 4096
+//                into 32000 columns: 395 us, 2.7 Pop/s), or, where 128 x 128
+//                tiles by one CTA are no more than the SMs, those (333 x 4096
+//                into 5001: 17.4 us against 20.3; 300 x 4096 into 8000, more
+//                tiles than SMs: 27.1 against 20.0);
 //   few tokens   weight rows are the 128 rows of a tile and the tokens its
-//                16 .. 128 columns: every weight is read once, bound by HBM.
+//                16 .. 128 columns: every weight is read once, bound by HBM
+//                (48 x 4096 into 128256: 95 us, 5.7 TB/s).
 //                The rows that do not make a whole round of tiles are dealt
 //                out evenly over the SMs in steps of 8 (a last round of whole
 //                tiles would leave up to all but one of them idle), loading
 //                only the 32-row boxes they need, and the first weights are brought
 //                into L2 while the kernel before (the norm that makes q) still
-//                runs.
+//                runs.  Past 16 tokens it takes a whole round of tiles, past 64
+//                three (64 x 4096 into 10000: 20.9 us against 16.5 with tiles of
+//                tokens, into 20000: 30.4 against 32.9; 128 tokens into 32000:
+//                37.2 against 35.8, into 128256: 102 against 107).  Columns for
+//                the tokens there are: one token into 128256 86 us, with 128
+//                columns 122.
 #include "fw_tc_gemm.cuh"
 
 namespace fwb200 {
@@ -169,14 +178,15 @@ cudaError_t run_int8_linear(const int8_t* q, int64_t ldq, const int8_t* w, int64
   const int sms = sm_count(), left = a.N % (128 * sms);
   a.per = ((left + sms - 1) / sms + 7) / 8 * 8;
   const int64_t nt = a.N / 128 >= sms ? sms : (left + a.per - 1) / a.per;  // CTAs
+  const int64_t rounds = a.N / 128 / sms;  // of whole tiles of weight rows
   if (a.T <= 16) return run_int8<Int8Few<TO, 16>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  if (a.T <= 32) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  if (a.T <= 64) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  if (a.T <= 128) return run_int8<Int8Few<TO, 128>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
-  const int64_t big = (((int64_t)a.T + 255) / 256) * (((int64_t)a.N + 255) / 256);
-  if (big >= sms / 2) return run_int8<Int8Many<TO, 256>>(q, a.T, ldq, w, a.N, ldw, a, big, st);
+  if (a.T <= 32 && rounds >= 1) return run_int8<Int8Few<TO, 32>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  if (a.T <= 64 && rounds >= 1) return run_int8<Int8Few<TO, 64>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
+  if (a.T <= 128 && rounds >= 3) return run_int8<Int8Few<TO, 128>>(w, a.N, ldw, q, a.T, ldq, a, nt, st);
   const int64_t small = (((int64_t)a.T + 127) / 128) * (((int64_t)a.N + 127) / 128);
-  return run_int8<Int8Many<TO, 128>>(q, a.T, ldq, w, a.N, ldw, a, small, st);
+  if (small <= sms) return run_int8<Int8Many<TO, 128>>(q, a.T, ldq, w, a.N, ldw, a, small, st);
+  const int64_t big = (((int64_t)a.T + 255) / 256) * (((int64_t)a.N + 255) / 256);
+  return run_int8<Int8Many<TO, 256>>(q, a.T, ldq, w, a.N, ldw, a, big, st);
 }
 
 }  // namespace
