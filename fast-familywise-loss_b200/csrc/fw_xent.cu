@@ -509,7 +509,7 @@ struct ProductArgs {
     const float nt = (float)((D + kTileN - 1) / kTileN), k = (float)(piece / 64), mt = (float)row_tiles(head);
     const float rest = dweight ? (float)(piece / kTileM) * (float)short_cost((head->rows + 63) / 64) : 0.0f;
     const float share = fmaxf(nt * (mt * k + rest) / (float)pairs, 16.0f);
-    return min(max_splits, (int)ceilf(k / share - 0.25f));
+    return max(1, min(max_splits, (int)ceilf(k / share - 0.25f)));
   }
 };
 

@@ -43,6 +43,15 @@ def test_loss_and_gradients(B, D, V, dtype):
     check(h, w, y, ("mean", "sum")[B % 2])
 
 
+@pytest.mark.parametrize("B,D,V", [(20000, 1024, 2048), (9000, 2048, 2048), (1300, 1024, 4096), (600, 512, 9000),
+                                   (64, 512, 20000)])
+def test_gradient_of_hidden_whole_and_in_splits(B, D, V):
+    """From rows whose products over V are far shorter than what else a
+    launch holds, to rows whose products are nearly all of it."""
+    h, w, y = data(B, D, V, torch.bfloat16, B + V, ignored=0.1)
+    check(h, w, y)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
 def test_reductions_ignored_rows_and_upstream(dtype, reduction):
