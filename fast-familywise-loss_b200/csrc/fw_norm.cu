@@ -120,12 +120,20 @@ __device__ __forceinline__ float group_reduce(float v, float* buf, int& flip) {
   return v;
 }
 
-// y in steps of the scale, to the nearest, as a byte; `steps` = 1 / scale, 0
-// for a row that has no such step (its y may be NaN).
-__device__ __forceinline__ uint32_t int8_step(float y, float steps) {
-  const float u = steps > 0.0f ? fminf(fmaxf(rintf(y * steps), -127.0f), 127.0f) : 0.0f;
-  return (uint32_t)(int)u & 0xffu;
-}
+// A value in steps of its row's scale, to the nearest, as a byte; 0 for a row
+// that has no such step (its values may be NaN).  1 / scale does not fit fp32
+// for the smallest scales, hence the power of two taken out of it.
+struct Int8Steps {
+  float up, per_step;
+  __device__ __forceinline__ explicit Int8Steps(float scale) {
+    up = scale < 0x1p-100f ? 0x1p100f : 1.0f;
+    per_step = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / (scale * up) : 0.0f;
+  }
+  __device__ __forceinline__ uint32_t operator()(float y) const {
+    const float u = per_step > 0.0f ? fminf(fmaxf(rintf(y * up * per_step), -127.0f), 127.0f) : 0.0f;
+    return (uint32_t)(int)u & 0xffu;
+  }
+};
 
 template <int G>
 __host__ __device__ constexpr int cta_threads() {
@@ -262,7 +270,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       const float scale = m / 127.0f;
       if (t == 0) a.qscale[r] = scale;
       // a row of zeros, or not finite, is 0 (or NaN) through its scale
-      const float steps = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / scale : 0.0f;
+      const Int8Steps steps(scale);
       const int w16 = (D + 15) / 16 * 16;
       if (off == 0) {  // the slots' bytes lie together in q
 #pragma unroll
@@ -272,8 +280,8 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
           uint32_t b[V / 4];
 #pragma unroll
           for (int j = 0; j < V; j += 4)
-            b[j / 4] = int8_step(v[k * V + j], steps) | (int8_step(v[k * V + j + 1], steps) << 8) |
-                       (int8_step(v[k * V + j + 2], steps) << 16) | (int8_step(v[k * V + j + 3], steps) << 24);
+            b[j / 4] = steps(v[k * V + j]) | (steps(v[k * V + j + 1]) << 8) | (steps(v[k * V + j + 2]) << 16) |
+                       (steps(v[k * V + j + 3]) << 24);
           if constexpr (V == 8)
             *reinterpret_cast<uint2*>(a.q + r * a.ldq + e) = make_uint2(b[0], b[1]);
           else
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
 #pragma unroll
         for (int i = 0; i < CH * V; ++i) {
           const int e = e0 + (i / V) * (G * V) + i % V;
-          if (e >= 0 && e < D) qs[e] = (int8_t)int8_step(v[i], steps);
+          if (e >= 0 && e < D) qs[e] = (int8_t)steps(v[i]);
         }
         if constexpr (G > 32)
           __syncthreads();
@@ -348,14 +356,14 @@ __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
       m = group_reduce<1024, true>(m, red, flip);
       const float scale = m / 127.0f;
       if (threadIdx.x == 0) a.qscale[r] = scale;
-      const float steps = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / scale : 0.0f;
+      const Int8Steps steps(scale);
       for (int64_t e = threadIdx.x; e < (a.D + 15) / 16 * 16; e += 1024) {
         float v = 0.0f;
         if (e < a.D) {
           v = elem(e);
           if constexpr (MODE != kInt8Only) v = v * rstd * gain(e);
         }
-        a.q[r * a.ldq + e] = (int8_t)int8_step(v, steps);
+        a.q[r * a.ldq + e] = (int8_t)steps(v);
       }
     }
   }

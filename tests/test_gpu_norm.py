@@ -142,6 +142,23 @@ def check_int8(q, scale, y, D):
     assert not pad.any()
 
 
+@pytest.mark.parametrize("D", [40, 4100, 20000])
+def test_int8_rows_of_the_smallest_values(D):
+    """1 / scale is past fp32's range from scales of 2^-128 down.  Half a step,
+    the fp32 roundings of 127 steps (three of 2^-24), and of the scale itself,
+    which under 2^-126 is a multiple of 2^-149."""
+    g = R.gen(D)
+    x = R.normal((5, D), torch.float32, g)
+    x /= x.abs().amax(-1, keepdim=True)
+    top = torch.tensor([1e-30, 1e-36, 3e-38, 1e-39, 1e-40], device="cuda")
+    x *= top[:, None]
+    q, scale = quantize_rows_int8(x)
+    step = scale.double()[:, None]
+    error = (q.double() * step - x.double()).abs()
+    assert bool((error <= step * (0.5 + 127 * 4 * 2.0 ** -24) + 127 * 2.0 ** -150).all())
+    assert bool((q.abs().amax(-1) == 127).all())
+
+
 def test_gradient_against_differences():
     g = R.gen(11)
     x, r, dy, ds = (R.normal((13, 96), torch.float32, g) for _ in range(4))
