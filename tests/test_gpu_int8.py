@@ -33,6 +33,15 @@ def test_product(T, N, K):
           torch.rand(N, generator=g, device="cuda"), dtype)
 
 
+@pytest.mark.parametrize("T", [1, 16, 17, 32, 33, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("N", [18943, 19000, 60001])
+def test_many_columns(T, N):
+    """Whole rounds of weight tiles, and what is left behind them."""
+    g = R.gen(T + N)
+    check(rows16(T, 300, g), torch.rand(T, generator=g, device="cuda"), rows16(N, 300, g),
+          torch.rand(N, generator=g, device="cuda"), R.FLOATS[N % 3])
+
+
 @pytest.mark.parametrize("dtype", R.FLOATS)
 @pytest.mark.parametrize("T", [3, 300])
 def test_output_types_and_extreme_values(T, dtype):
