@@ -120,18 +120,36 @@ __device__ __forceinline__ float group_reduce(float v, float* buf, int& flip) {
   return v;
 }
 
-// A value in steps of its row's scale, to the nearest, as a byte; 0 for a row
+// Scale of a row whose largest value is m; rounded up where it is subnormal,
+// so that no value is more than 127 steps.
+__device__ __forceinline__ float int8_scale(float m) {
+  const float scale = m / 127.0f;
+  return scale < 0x1p-126f ? __fdiv_ru(m, 127.0f) : scale;
+}
+
+// Values in steps of their row's scale, to the nearest, as bytes; 0 for a row
 // that has no such step (its values may be NaN).  1 / scale does not fit fp32
-// for the smallest scales, hence the power of two taken out of it.
+// for the smallest scales, hence the power of two taken out of it.  The steps
+// are added to 1.5 * 2^23, whose unit is 1: the addition rounds, and the sum's
+// low byte is the integer (a third of the instructions of rounding, clamping and
+// converting: 16384 x 4096 bfloat16 with residual 89 us, alone 40, for 106 and
+// 62; 32000 x 2048 float32 alone 66 for 87, but with residual 159 for 140).
 struct Int8Steps {
   float up, per_step;
+  uint32_t keep;
   __device__ __forceinline__ explicit Int8Steps(float scale) {
+    const bool some = scale > 0.0f && scale < CUDART_INF_F;
     up = scale < 0x1p-100f ? 0x1p100f : 1.0f;
-    per_step = scale > 0.0f && scale < CUDART_INF_F ? 1.0f / (scale * up) : 0.0f;
+    per_step = some ? 1.0f / (scale * up) : 0.0f;
+    keep = some ? 0xffffffffu : 0u;
   }
-  __device__ __forceinline__ uint32_t operator()(float y) const {
-    const float u = per_step > 0.0f ? fminf(fmaxf(rintf(y * up * per_step), -127.0f), 127.0f) : 0.0f;
-    return (uint32_t)(int)u & 0xffu;
+  __device__ __forceinline__ uint32_t word(float y) const {  // low byte
+    return __float_as_uint(fmaf(y * up, per_step, 12582912.0f));
+  }
+  __device__ __forceinline__ int8_t one(float y) const { return (int8_t)(word(y) & keep & 0xffu); }
+  __device__ __forceinline__ uint32_t four(const float* y) const {
+    return __byte_perm(__byte_perm(word(y[0]), word(y[1]), 0x0040), __byte_perm(word(y[2]), word(y[3]), 0x0040), 0x5410) &
+           keep;
   }
 };
 
@@ -267,7 +285,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
 #pragma unroll
       for (int i = 0; i < CH * V; ++i) m = max_nan(m, fabsf(v[i]));  // slots past the row hold 0 * 0
       m = group_reduce<G, true>(m, red, flip);
-      const float scale = m / 127.0f;
+      const float scale = int8_scale(m);
       if (t == 0) a.qscale[r] = scale;
       // a row of zeros, or not finite, is 0 (or NaN) through its scale
       const Int8Steps steps(scale);
@@ -279,9 +297,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
           if (e >= w16) continue;
           uint32_t b[V / 4];
 #pragma unroll
-          for (int j = 0; j < V; j += 4)
-            b[j / 4] = steps(v[k * V + j]) | (steps(v[k * V + j + 1]) << 8) | (steps(v[k * V + j + 2]) << 16) |
-                       (steps(v[k * V + j + 3]) << 24);
+          for (int j = 0; j < V; j += 4) b[j / 4] = steps.four(v + k * V + j);
           if constexpr (V == 8)
             *reinterpret_cast<uint2*>(a.q + r * a.ldq + e) = make_uint2(b[0], b[1]);
           else
@@ -297,7 +313,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
 #pragma unroll
         for (int i = 0; i < CH * V; ++i) {
           const int e = e0 + (i / V) * (G * V) + i % V;
-          if (e >= 0 && e < D) qs[e] = (int8_t)steps(v[i]);
+          if (e >= 0 && e < D) qs[e] = steps.one(v[i]);
         }
         if constexpr (G > 32)
           __syncthreads();
@@ -354,7 +370,7 @@ __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
     }
     if constexpr (MODE != kNormOut) {
       m = group_reduce<1024, true>(m, red, flip);
-      const float scale = m / 127.0f;
+      const float scale = int8_scale(m);
       if (threadIdx.x == 0) a.qscale[r] = scale;
       const Int8Steps steps(scale);
       for (int64_t e = threadIdx.x; e < (a.D + 15) / 16 * 16; e += 1024) {
@@ -363,7 +379,7 @@ __global__ void __launch_bounds__(1024) fw_norm_long_kernel(NormArgs a) {
           v = elem(e);
           if constexpr (MODE != kInt8Only) v = v * rstd * gain(e);
         }
-        a.q[r * a.ldq + e] = (int8_t)steps(v);
+        a.q[r * a.ldq + e] = steps.one(v);
       }
     }
   }
