@@ -41,6 +41,28 @@ def test_rows_and_gradient(T, V, D, dtype):
     check(ids, w, g)
 
 
+@pytest.mark.parametrize("dtype", R.FLOATS)
+@pytest.mark.parametrize("T", [1, 31, 32, 33, 256, 257])
+def test_few_tokens_of_a_large_table(T, dtype):
+    ids, w, g = data(T, 117001, 72, dtype, T, skew=T % 2 == 0)
+    check(ids, w, g)
+
+
+@pytest.mark.parametrize("V,D", [(8192, 1024), (8192, 1025), (131072, 64), (131073, 64)])
+def test_tables_around_the_size_that_is_sorted_for(V, D):
+    ids, w, g = data(200, V, D, torch.float16, V + D)
+    check(ids, w, g, scale=3.0, padding=int(ids[7]))
+
+
+@pytest.mark.parametrize("T", [600, 1100, 9000, 33000])
+def test_runs_of_many_parts(T):
+    """A third of the tokens one row, a third another: parts joined by a warp, and by a CTA."""
+    ids, w, g = data(T, 301, 520, torch.bfloat16, T)
+    ids[torch.randperm(T, generator=R.gen(1), device="cuda")[: T // 3]] = 300
+    ids[torch.randperm(T, generator=R.gen(2), device="cuda")[: T // 3]] = 17
+    check(ids, w, g)
+
+
 @pytest.mark.parametrize("T", [31, 32, 33, 64, 65, 3000, 40000])
 def test_skewed_tokens(T):
     """Runs that end at, before and after a chunk boundary of the sorted order."""
