@@ -25,7 +25,9 @@
 // 1 / B, into everything).  One factor for all rows is applied in fp32 after
 // the sums.  Factors per row are split, g_r = s_r f_r with s_r a power of two:
 // s_r goes into G, f_r in [0.5, 1) multiplies the rows of dH in fp32 and the
-// rows of H that dW is made of.
+// rows of H that dW is made of, which are rounded to their type once more (a
+// term of dW then carries two roundings, of G and of f_r H, as it would if
+// both operands were given in 16 bits).
 //
 // float16 G: exp(z - lse) may be under float16's smallest value, so G is
 // scaled by 2^15 (over the largest s_r), taken out after the sums.
