@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restric
   if (lane == 0 && c < D) st_elem(dw + c, s);
 }
 
-// Threads per row by the row's slot count: a warp, or a CTA with one or two
+// Threads per row by its slots: a warp, or a CTA with one or two
 // slots per thread, so that a thread's 64 registers hold its gains and its
 // part of dw; the memory-pass kernels beyond 2048 slots (2000 x 16000
 // bfloat16, forward and backward: 183 us here, 348 there).
@@ -542,9 +542,14 @@ struct NormShape {
   int G, CH;
 };
 
-NormShape norm_shape(int64_t D, int64_t esize, bool vec) {
-  const int64_t V = 16 / esize;
-  const int64_t n = (D + V - 1) / V + (vec && (D * esize) % 16 != 0 ? 1 : 0);
+// Slots that a row of the matrix covers at most: one more than its elements
+// fill where a row may start inside a slot.
+int64_t row_slots(const void* base, int64_t ld, int64_t D, int64_t esize, bool vec) {
+  const bool inside = vec && (!aligned16(base) || ld * esize % 16 != 0);
+  return (D * esize + 15) / 16 + (inside ? 1 : 0);
+}
+
+NormShape norm_shape(int64_t n) {
   if (n <= 32) return {32, 1};
   if (n <= 128) return {128, 1};
   if (n <= 256) return {128, 2};
@@ -612,7 +617,7 @@ cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
 
 template <class T, int MODE>
 cudaError_t launch_norm(const NormArgs& a, cudaStream_t st) {
-  const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
+  const NormShape sh = norm_shape(row_slots(a.x, a.ldx, a.D, sizeof(T), a.vec));
   if (sh.G == 32) return launch_norm<T, MODE, 32, 1>(a, st);
   if (sh.G == 128 && sh.CH == 1) return launch_norm<T, MODE, 128, 1>(a, st);
   if (sh.G == 128) return launch_norm<T, MODE, 128, 2>(a, st);
@@ -632,7 +637,7 @@ cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
 
 template <class T>
 cudaError_t launch_norm_grad(const NormGradArgs& a, cudaStream_t st) {
-  const NormShape sh = norm_shape(a.D, sizeof(T), a.vec);
+  const NormShape sh = norm_shape(row_slots(a.s, a.lds, a.D, sizeof(T), a.vec));
   if (sh.G == 32) return launch_norm_grad<T, 32, 1>(a, st);
   if (sh.G == 128 && sh.CH == 1) return launch_norm_grad<T, 128, 1>(a, st);
   if (sh.G == 128) return launch_norm_grad<T, 128, 2>(a, st);
@@ -771,7 +776,7 @@ int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy, const 
   a.w_f32 = wdtype == FWB_DTYPE_F32 && dtype != FWB_DTYPE_F32;
   a.vec = same_slots(sum, lds, dy, lddy, es) && same_slots(sum, lds, dx, lddx, es) &&
           (!dsum || same_slots(sum, lds, dsum, ldo, es));
-  const int64_t grid = norm_grid(rows, norm_shape(D, es, a.vec).G);
+  const int64_t grid = norm_grid(rows, norm_shape(row_slots(sum, lds, D, es, a.vec)).G);
   if (dweight && nparts < grid) return FWB_E_CAPACITY;
   cudaError_t e = dtype == FWB_DTYPE_BF16  ? launch_norm_grad<__nv_bfloat16>(a, st)
                   : dtype == FWB_DTYPE_F16 ? launch_norm_grad<__half>(a, st)
