@@ -64,9 +64,11 @@ constexpr int kMaxBins = 1 << kMaxDigitBits;
 constexpr int kDirectTokens = 256;
 constexpr int64_t kDirectElems = (int64_t)1 << 23;  // of the table
 
-// Slots of a row of a contiguous matrix (one more where rows start anywhere).
-__host__ __device__ constexpr int slots_of(int64_t D, int esize) {
-  return (int)((D * esize + 15) / 16 + (D * esize % 16 != 0 ? 1 : 0));
+// Slots that a row of the matrix covers at most: one more than its elements
+// fill where a row may start inside a slot.
+int slots_of(const void* base, int64_t ld, int64_t D, int esize) {
+  const bool inside = !aligned16(base) || ld * esize % 16 != 0;
+  return (int)((D * esize + 15) / 16 + (inside ? 1 : 0));
 }
 
 template <class T>
@@ -756,7 +758,7 @@ int fw_embed_rows(int dtype, const int64_t* ids, int64_t T, const void* weight, 
   const int es = dtype == FWB_DTYPE_F32 ? 4 : 2;
   if (reinterpret_cast<uintptr_t>(weight) % es || reinterpret_cast<uintptr_t>(out) % es) return FWB_E_POINTER;
   EmbedArgs a = {ids, weight, out, T, V, D, ldw, ldo, scale, status, 0, 0};
-  a.nsteps = (slots_of(D, es) + 31) / 32;
+  a.nsteps = (slots_of(out, ldo, D, es) + 31) / 32;
   a.nslabs = (a.nsteps + kSlab - 1) / kSlab;
   const int64_t need = (T * a.nslabs + 7) / 8, cap = (int64_t)sm_count() * 64;
   const int64_t grid = need < cap ? need : cap;
@@ -808,7 +810,7 @@ int fw_embed_grad(int dtype, const int64_t* ids, int64_t T, const void* grad, in
   a.pitch = p.pitch;
   a.padding = padding;
   a.scale = scale;
-  a.nslots = slots_of(D, es);
+  a.nslots = slots_of(dweight, D, D, es);
   a.status = status;
   uint2* other = reinterpret_cast<uint2*>(ws) + T;  // second array of entries, more than kClusterTokens only
   return launch_status(dtype == FWB_DTYPE_BF16  ? launch_embed_grad<__nv_bfloat16>(a, s, p, other, st)
