@@ -30,7 +30,7 @@
 // both operands were given in 16 bits).
 //
 // float16 G: exp(z - lse) may be under float16's smallest value, so G is
-// scaled by 2^15 (over the largest s_r), taken out after the sums.
+// scaled by 2^15 (over the largest finite s_r), taken out after the sums.
 #include "fw_reduce.cuh"
 #include "fw_rowslots.cuh"
 #include "fw_tc_gemm.cuh"
@@ -47,7 +47,7 @@ struct XentHead {
   int32_t rows;    // live rows
   uint32_t done;   // blocks of the joining kernel that have finished
   int32_t status;  // status bits raised inside
-  float top;       // largest s_r of a live row (float16, factors per row)
+  float top;       // largest finite s_r of a live row (float16, factors per row)
 };
 
 struct PackArgs {
@@ -357,10 +357,11 @@ struct Upstream {
   const float* go;  // one per given row, or one
   int per_row, mean, f16;
 
-  // s_r, scaled to the range of the type
+  // s_r, scaled to the range of the type; a factor that is not finite stands for itself
   __device__ float in_g(const XentHead* h, int r) const {
     if (!per_row) return f16 ? kF16Unit : 1.0f;
-    const float s = pow2_above(go[r]);
+    const float g = go[r], s = pow2_above(g);
+    if (!(s < CUDART_INF_F)) return g;
     return f16 && h->top > 0.0f ? s / h->top * kF16Unit : s;
   }
   // f_r; 1 where the factor is in G (0, not finite) or common
@@ -381,13 +382,16 @@ __global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const
   __shared__ float red[32];
   const int rows = head->rows;
   float top = 0.0f;
-  for (int i = threadIdx.x; i < rows; i += 1024) top = max_nan(top, pow2_above(go[row_of[i]]));
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const float s = pow2_above(go[row_of[i]]);
+    if (s < CUDART_INF_F) top = fmaxf(top, s);
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = max_nan(top, __shfl_xor_sync(kFull, top, o));
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = top;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 32; ++i) top = max_nan(top, red[i]);
+    for (int i = 1; i < 32; ++i) top = fmaxf(top, red[i]);
     head->top = top;
   }
 }
