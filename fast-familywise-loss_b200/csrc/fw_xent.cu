@@ -47,7 +47,6 @@ struct XentHead {
   int32_t rows;    // live rows
   uint32_t done;   // blocks of the joining kernel that have finished
   int32_t status;  // status bits raised inside
-  float top;       // largest finite s_r of a live row (float16, factors per row)
 };
 
 struct PackArgs {
@@ -354,15 +353,16 @@ __device__ __forceinline__ float pow2_above(float g) {
 // The upstream gradient: the factors of G's rows (powers of two) and what is
 // left of it.
 struct Upstream {
-  const float* go;  // one per given row, or one
+  const float* go;   // one per given row, or one
+  const float* top;  // largest finite s_r of a live row (float16, factors per row)
   int per_row, mean, f16;
 
   // s_r, scaled to the range of the type; a factor that is not finite stands for itself
-  __device__ float in_g(const XentHead* h, int r) const {
+  __device__ float in_g(int r) const {
     if (!per_row) return f16 ? kF16Unit : 1.0f;
     const float g = go[r], s = pow2_above(g);
     if (!(s < CUDART_INF_F)) return g;
-    return f16 && h->top > 0.0f ? s / h->top * kF16Unit : s;
+    return f16 && *top > 0.0f ? s / *top * kF16Unit : s;
   }
   // f_r; 1 where the factor is in G (0, not finite) or common
   __device__ float rest(int r) const {
@@ -372,13 +372,14 @@ struct Upstream {
   }
   // common factor taken out after the sums
   __device__ float back(const XentHead* h) const {
-    if (per_row) return f16 && h->top > 0.0f ? h->top / kF16Unit : 1.0f;
+    if (per_row) return f16 && *top > 0.0f ? *top / kF16Unit : 1.0f;
     const float g = mean ? go[0] / (float)h->rows : go[0];
     return f16 ? g / kF16Unit : g;
   }
 };
 
-__global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const int32_t* row_of, const float* go) {
+__global__ void __launch_bounds__(1024) fw_xent_top_kernel(const XentHead* head, const int32_t* row_of, const float* go,
+                                                             float* out) {
   __shared__ float red[32];
   const int rows = head->rows;
   float top = 0.0f;
@@ -392,7 +393,7 @@ __global__ void __launch_bounds__(1024) fw_xent_top_kernel(XentHead* head, const
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int i = 1; i < 32; ++i) top = fmaxf(top, red[i]);
-    head->top = top;
+    *out = top;
   }
 }
 
@@ -455,7 +456,7 @@ struct GradTile {
     const bool live = row < a.head->rows;
     st.y = live ? a.label[row] : -2;  // -2: not a live row
     st.lse = live ? a.lse[row] : 0.0f;
-    st.coef = live ? a.up.in_g(a.head, a.row_of[row]) : 0.0f;
+    st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
   }
   template <class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
@@ -701,7 +702,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, zy, loss_pack, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, splits, g, sum, hs, bwd_bytes;
+  int64_t piece, pieces, splits, top, g, sum, hs, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
@@ -727,6 +728,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.piece = up((Vp + p.pieces - 1) / p.pieces, 256);
   p.pieces = (Vp + p.piece - 1) / p.piece;
   at = 0;
+  p.top = at, at += 256;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
   // as many as one row tile could use, 16 stages of K each, within kSumBytes
   p.splits = sm_count() / 2 / ((D + kTileN - 1) / kTileN);
@@ -786,27 +788,29 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
 
 template <class T, TcKind K>
 int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int mean, const float* go,
-                 int per_row, char* state, char* ws, void* dhidden, void* dweight, int32_t* status, cudaStream_t st) {
+                 int per_row, const char* state, char* ws, void* dhidden, void* dweight, int32_t* status, cudaStream_t st) {
   const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
-  XentHead* head = reinterpret_cast<XentHead*>(state);
-  int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
-  int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
+  const XentHead* head = reinterpret_cast<const XentHead*>(state);
+  const int32_t* row_of = reinterpret_cast<const int32_t*>(state + p.row_of);
+  const int32_t* label = reinterpret_cast<const int32_t*>(state + p.label);
   const void* w = p.copy_w ? state + p.wp : weight;
   if (p.copy_w) ldw = p.Dp;
-  const Upstream u = {go, per_row, mean, K == kTcF16};
-  char* hw = state + p.hp;  // dW's operand
+  float* top = reinterpret_cast<float*>(ws + p.top);
+  const Upstream u = {go, top, per_row, mean, K == kTcF16};
+  const char* hw = state + p.hp;  // dW's operand
   if (per_row) {
-    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go);
+    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go, top);
     if (dweight) {
-      hw = ws + p.hs;
+      T* hs = reinterpret_cast<T*>(ws + p.hs);
       const int64_t cap = (int64_t)sm_count() * 8;
       fw_xent_scale_kernel<T><<<(unsigned)(p.Bp < cap ? p.Bp : cap), 256, 0, st>>>(
-          head, row_of, u, reinterpret_cast<const T*>(state + p.hp), reinterpret_cast<T*>(hw), p.Dp);
+          head, row_of, u, reinterpret_cast<const T*>(state + p.hp), hs, p.Dp);
+      hw = ws + p.hs;
     }
     if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
   }
   CUtensorMap mh, mw, mg, wmn, gmn, hmn;
-  char* hp = state + p.hp;
+  const char* hp = state + p.hp;
   char* g = ws + p.g;
   if (!tc_map(&mh, K, hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 128) ||
       !tc_map(&mg, K, g, p.Bp, p.piece, p.piece, 128) || !tc_map(&wmn, K, w, V, D, ldw, 64) ||
@@ -816,7 +820,7 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   float* sum = p.pieces > 1 || p.splits > 1 ? reinterpret_cast<float*>(ws + p.sum) : nullptr;
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
-    const GradArgs ga = {head, label, row_of, reinterpret_cast<float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
+    const GradArgs ga = {head, label, row_of, reinterpret_cast<const float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
                          v0, vn, status};
     if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
     const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
@@ -881,7 +885,7 @@ int fw_xent_forward(int dtype, const void* hidden, int64_t ldh, const void* weig
 }
 
 int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int reduction,
-                     const float* grad_output, void* state, int64_t state_bytes, void* workspace,
+                     const float* grad_output, const void* state, int64_t state_bytes, void* workspace,
                      int64_t workspace_bytes, void* dhidden, void* dweight, int32_t* status, void* stream) {
   if (int rc = xent_check(dtype, B, D, V)) return rc;
   if (reduction < FWB_REDUCE_NONE || reduction > FWB_REDUCE_SUM || ldw < D || ldw > ((int64_t)1 << 38))
@@ -898,7 +902,7 @@ int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int6
   const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
   if (state_bytes < p.state_bytes || workspace_bytes < p.bwd_bytes) return FWB_E_CAPACITY;
   if (!dhidden && !dweight) return FWB_OK;
-  char* s = static_cast<char*>(state);
+  const char* s = static_cast<const char*>(state);
   char* w = static_cast<char*>(workspace);
   const int per_row = reduction == FWB_REDUCE_NONE, mean = reduction == FWB_REDUCE_MEAN;
   return dtype == FWB_DTYPE_BF16

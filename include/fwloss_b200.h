@@ -541,7 +541,8 @@ FWB_API int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const fl
  * FWB_REDUCE_NONE, else one value.
  * `state` (fw_xent_state_bytes, for the same weight pointer and stride) keeps
  * what the gradient needs: packed live rows, their log-sum-exp, and a copy of
- * the weight only if its rows do not start on 16-byte boundaries.
+ * the weight only if its rows do not start on 16-byte boundaries; the gradient
+ * only reads it.
  * fw_xent_backward writes dhidden [B, D] and dweight [V, D] (contiguous,
  * either may be NULL) for grad_output ([B] for FWB_REDUCE_NONE, else one
  * value), the logit gradient formed in pieces of the vocabulary.  Both
@@ -558,7 +559,7 @@ FWB_API int fw_xent_forward(int dtype, const void* hidden, int64_t ldh, const vo
                             int reduction, float* loss, void* state, int64_t state_bytes,
                             void* workspace, int64_t workspace_bytes, int32_t* status, void* stream);
 FWB_API int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V,
-                             int reduction, const float* grad_output, void* state, int64_t state_bytes,
+                             int reduction, const float* grad_output, const void* state, int64_t state_bytes,
                              void* workspace, int64_t workspace_bytes, void* dhidden, void* dweight,
                              int32_t* status, void* stream);
 
