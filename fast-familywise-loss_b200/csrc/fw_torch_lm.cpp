@@ -383,6 +383,12 @@ struct LmHeadCrossEntropy : torch::autograd::Function<LmHeadCrossEntropy> {
     auto go = g[0].detach().contiguous();
     const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
     const int64_t B = a[0], V = w.size(0), D = w.size(1);
+    // A hook may have restored the weight off the 16-byte boundaries it was saved on; the state has no copy of it then.
+    if (fw_xent_state_bytes(B, D, V, w.data_ptr(), ld_of(w)) > state.numel()) {
+      auto c = at::empty({V, (D + 7) / 8 * 8}, w.options()).narrow(1, 0, D);
+      c.copy_(w);
+      w = c;
+    }
     Tensor dh, dw;
     if (want_h) dh = at::empty({B, D}, w.options());
     if (want_w) dw = at::empty({V, D}, w.options());
