@@ -79,6 +79,11 @@ Tensor f32(at::IntArrayRef shape, const Tensor& like) { return at::empty(shape, 
 
 bool recording(const Tensor& t) { return t.requires_grad(); }
 
+// A result without a tangent would drop the operand's silently, whatever the grad mode.
+void no_tangent(const Tensor& t, const char* op) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), op, ": forward-mode differentiation is not implemented");
+}
+
 // The gradients have none of their own: a second derivative raises.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -155,6 +160,7 @@ Tensor embed_tokens(const Tensor& ids, const Tensor& weight, double scale, c10::
   value_check(ids.device() == weight.device(), "embed_tokens: tokens must be on weight's device");
   value_check(!padding || (*padding >= 0 && *padding < weight.size(0)),
               "embed_tokens: padding_idx is outside the table");
+  no_tangent(weight, "embed_tokens");
   const int64_t pad = padding.value_or(-1);
   if (at::GradMode::is_enabled() && recording(weight)) return EmbedTokens::apply(ids, weight, scale, pad, status);
   return embed_rows(ids, weight, scale, status);
@@ -241,6 +247,9 @@ struct RmsNorm : torch::autograd::Function<RmsNorm> {
 
 py::object rms_norm(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual) {
   check_norm(x, weight, eps, residual);
+  no_tangent(x, "rms_norm");
+  no_tangent(weight, "rms_norm");
+  if (residual.has_value()) no_tangent(*residual, "rms_norm");
   if (at::GradMode::is_enabled() &&
       (recording(x) || recording(weight) || (residual.has_value() && recording(*residual)))) {
     auto out = RmsNorm::apply(x, weight, residual, eps);
@@ -418,6 +427,8 @@ Tensor lm_head_cross_entropy(const Tensor& hidden, const Tensor& weight, const T
               "lm_head_cross_entropy: target must have shape [B]");
   value_check(weight.device() == hidden.device() && target.device() == hidden.device(),
               "lm_head_cross_entropy: hidden, weight and target must be on one device");
+  no_tangent(hidden, "lm_head_cross_entropy");
+  no_tangent(weight, "lm_head_cross_entropy");
   if (at::GradMode::is_enabled() && (recording(hidden) || recording(weight)))
     return LmHeadCrossEntropy::apply(hidden, weight, target, ignore_index, reduction, status);
   return xent_forward(hidden, weight, target, ignore_index, reduction, status).loss;
