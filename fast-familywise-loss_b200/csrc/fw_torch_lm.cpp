@@ -166,6 +166,18 @@ Tensor embed_tokens(const Tensor& ids, const Tensor& weight, double scale, c10::
   return embed_rows(ids, weight, scale, status);
 }
 
+Tensor embed_grad_checked(const Tensor& ids, const Tensor& grad, int64_t V, double scale, int64_t padding,
+                          const OptTensor& status) {
+  type_check(grad.is_cuda(), "embed_grad: grad must be a CUDA tensor (this build has no CPU path)");
+  type_check(grad.dim() >= 1 && is_float(grad) && grad.size(-1) >= 1,
+             "embed_grad: grad must be a float32, bfloat16 or float16 tensor [..., D]");
+  type_check(ids.scalar_type() == torch::kLong, "embed_grad: tokens must be an int64 tensor");
+  value_check(ids.device() == grad.device(), "embed_grad: tokens must be on grad's device");
+  value_check(ids.sizes() == grad.sizes().slice(0, grad.dim() - 1), "embed_grad: grad must have the tokens' shape and D");
+  value_check(V >= 1 && padding >= -1 && padding < V, "embed_grad: padding is outside the table (-1: none)");
+  return embed_grad(ids, grad, V, scale, padding, status);
+}
+
 // ---------------------------------------------------------------- norm
 void check_norm(const Tensor& x, const Tensor& weight, double eps, const OptTensor& residual) {
   type_check(x.is_cuda(), "rms_norm: x must be a CUDA tensor (this build has no CPU path)");
@@ -438,7 +450,7 @@ Tensor lm_head_cross_entropy(const Tensor& hidden, const Tensor& weight, const T
 
 void register_lm_operators(pybind11::module_& m) {
   m.def("embed_tokens", &embed_tokens, "rows of a table, scaled (differentiable)");
-  m.def("embed_grad", &embed_grad, "gradient of embed_tokens in the table, deterministic");
+  m.def("embed_grad", &embed_grad_checked, "gradient of embed_tokens in the table, deterministic");
   m.def("rms_norm", &rms_norm, "norm of a residual stream (differentiable)");
   m.def("rms_norm_int8", &rms_norm_int8, "(q, scale[, x + residual])");
   m.def("quantize_rows_int8", &quantize_rows_int8, "(q, scale)");
