@@ -145,7 +145,12 @@ int aux_grid(int64_t rows, int per_block) {
   return (int)(g < 1 ? 1 : g);
 }
 
+std::atomic<int64_t> g_tc_wait_ns{kTcWaitLimitNs};
+
 }  // namespace
+
+uint64_t tc_wait_ns() { return (uint64_t)g_tc_wait_ns.load(std::memory_order_relaxed); }
+
 }  // namespace fwb200
 
 using namespace fwb200;
@@ -153,6 +158,8 @@ using namespace fwb200;
 extern "C" {
 
 const char* fw_version(void) { return "0.1.0"; }
+
+int64_t fw_tc_wait_limit(int64_t ns) { return ns < 0 ? g_tc_wait_ns.load() : g_tc_wait_ns.exchange(ns); }
 
 const char* fw_error_string(int code) {
   switch (code) {
@@ -544,6 +551,7 @@ int fw_lmhead_fused_scan(int dtype, const void* hidden, int64_t B, int64_t D, co
   a.summaries = summaries;
   a.local_idx = local_idx;
   a.status = status;
+  a.wait_ns = tc_wait_ns();
   CUtensorMap tm_h, tm_w;
   if (!make_tile_map_bf16(&tm_h, hidden, B, D, kTcBM) || !make_tile_map_bf16(&tm_w, weight, C, D, kTcBN))
     return FWB_E_LAUNCH;

@@ -85,6 +85,9 @@ cudaError_t launch_dependent(void (*kernel)(KArgs...), int64_t grid, int block, 
 
 }  // namespace
 
+// Limit of the tensor-core kernels' waits (fw_tc_wait_limit).
+uint64_t tc_wait_ns();
+
 // Fused forward(+backward) over rows of element type T with output form OUT
 // (fw_rows.cuh; one explicit instantiation per (T, OUT) in the fw_rows_*.cu
 // translation units).  vec: rows are 16-byte aligned (16-byte accesses).

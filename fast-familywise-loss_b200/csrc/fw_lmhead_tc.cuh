@@ -30,8 +30,8 @@
 // holding them (first NaN), as the other summary producers do.
 //
 // Every mbarrier wait is bounded: on a timeout the kernel sets status bit
-// FWB_STATUS_TIMEOUT and a CTA-wide abort flag, every role leaves its loop,
-// the producer waits (bounded) for the TMA loads it issued to land, the MMA
+// FWB_STATUS_TIMEOUT and a CTA-wide abort flag; once every role has left its
+// loop, the producer waits (bounded) for the TMA loads it issued to land, the MMA
 // warp commits to a drain barrier and waits (bounded) for its issued MMAs,
 // and only then is TMEM released and the CTA allowed to exit.
 #pragma once
@@ -71,6 +71,7 @@ struct TcArgs {
   int32_t* summaries;  // [nchunks, B, kShardHeader + K]
   int32_t* local_idx;  // [nchunks, B, K]
   int32_t* status;
+  uint64_t wait_ns;
 };
 
 // Per-row running state of the epilogue across the tiles of one chunk.
@@ -258,7 +259,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int m0 = (int)(w % a.n_mblocks) * kTcBM;
       for (int64_t n0 = a.col_start[q]; n0 < a.col_start[q + 1]; n0 += kTcBN) {
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status)) goto done;
+          if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status, a.wait_ns)) goto done;
           if (lane == 0) {
             mbar_expect_tx(&full[s], kTcABytes + kTcBBytes);
             tma_load_2d(smA + s * kTcABytes, &tm_hidden, kb * kTcBK, m0, &full[s]);
@@ -280,11 +281,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     for (int64_t w = blockIdx.x; w < nwork; w += gridDim.x) {
       const int q = (int)(w / a.n_mblocks);
       for (int64_t n0 = a.col_start[q]; n0 < a.col_start[q + 1]; n0 += kTcBN) {
-        if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status)) goto done;
+        if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status, a.wait_ns)) goto done;
         tc_fence_after();
         const uint32_t d = tmem + acc * kTcBN;
         for (int kb = 0; kb < nk; ++kb) {
-          if (!mbar_wait(&full[s], ph, abort_flag, a.status)) goto done;
+          if (!mbar_wait(&full[s], ph, abort_flag, a.status, a.wait_ns)) goto done;
           tc_fence_after();
           if (lane == 0) {
             const uint32_t sa = smem_u32(smA + s * kTcABytes);
@@ -322,7 +323,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
       const int64_t yr = row < a.B ? a.y[row] : -1;
       TcRowState st = {-CUDART_INF_F, 0, false, -1, -1};
       for (int64_t n0 = a.col_start[q]; n0 < c1; n0 += kTcBN) {
-        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
+        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status, a.wait_ns)) goto done;
         tc_fence_after();
         for (int cc = 0; cc < kTcBN / 32; ++cc) {
           const int64_t col0 = n0 + 32 * cc;
@@ -348,7 +349,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     }
   }
 done:
+  // Every role has left its loop: one that had finished before another gave up
+  // may still have copies or MMAs in flight.
   __syncwarp();
+  __syncthreads();
   if (*abort_flag && lane == 0) {
     // Aborted: let the copies and MMAs already issued land before the CTA
     // frees its TMEM and shared memory (each wait bounded, kTcDrainLimitNs).

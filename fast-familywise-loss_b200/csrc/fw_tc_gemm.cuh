@@ -25,9 +25,9 @@
 // N; a stage then holds 64 rows of K of as many 64-element column groups as
 // the tile needs).
 //
-// Every wait is bounded; on a timeout all roles leave their loops, the copies
-// and products in flight are waited for (bounded) and TMEM is released, as in
-// the fused LM-head kernel; the CTAs of a pair leave together.
+// Every wait is bounded; on a timeout all roles leave their loops, then the
+// copies and products in flight are waited for (bounded) and TMEM is released,
+// as in the fused LM-head kernel; the CTAs of a pair leave together.
 #pragma once
 
 #include "fw_host.cuh"
@@ -227,7 +227,7 @@ template <class P>
 __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     fw_tc_gemm_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
                       const __grid_constant__ CUtensorMap tm_a2, const __grid_constant__ CUtensorMap tm_b2,
-                      const __grid_constant__ typename P::Args a) {
+                      const __grid_constant__ typename P::Args a, uint64_t wait_ns) {
   constexpr int S = P::STAGES, CG = P::CG;
   constexpr uint32_t kBBytes = GemmSmem<P>::kBBytes;
   constexpr bool kI8 = P::KIND == kTcS8;
@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
       const uint32_t bytes =
           P::A_BOX == 128 ? kGemmABytes : (uint32_t)((t.rows + P::A_BOX - 1) / P::A_BOX * P::A_BOX * kGemmRowBytes);
       for (int kb = 0; kb < t.nk; ++kb) {
-        if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status)) goto done;
+        if (!mbar_wait(&empty[s], ph ^ 1u, abort_flag, a.status, wait_ns)) goto done;
         if (lane == 0) {
           if (rank == 0) mbar_expect_tx(&full[s], CG * (bytes + kBBytes));
           const uint32_t bar = CG == 2 ? in_cta(&full[s], 0) : smem_u32(&full[s]);
@@ -357,11 +357,11 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
         const uint32_t idesc = gemm_idesc(P::KIND, a_mn, P::B_MN, kGemmBM * CG, P::BN);
         const int kc = P::KC == 0 ? max(t.nk, 1) : P::KC;
         for (int k0 = 0; k0 < max(t.nk, 1); k0 += kc) {
-          if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status)) goto done;
+          if (!mbar_wait(&tempty[acc], aph ^ 1u, abort_flag, a.status, wait_ns)) goto done;
           tc_fence_after();
           const uint32_t d = tmem + acc * P::BN;
           for (int kb = k0; kb < min(k0 + kc, t.nk); ++kb) {
-            if (!mbar_wait(&full[s], ph, abort_flag, a.status)) goto done;
+            if (!mbar_wait(&full[s], ph, abort_flag, a.status, wait_ns)) goto done;
             tc_fence_after();
             if (lane == 0) {
               const uint32_t sa = smem_u32(smA + s * kGemmABytes);
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
       typename P::State state{};
       P::begin(a, plan, t, part, state);
       for (int k = 0; k < parts; ++k) {
-        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status)) goto done;
+        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status, wait_ns)) goto done;
         tc_fence_after();
         part.taddr = tmem + (uint32_t)((quad * 32) << 16) + acc * P::BN;
         const uint32_t te = CG == 2 ? in_cta(&tempty[acc], 0) : smem_u32(&tempty[acc]);
@@ -422,7 +422,10 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     }
   }
 done:
+  // Every role has left its loop: one that had finished before another gave up
+  // may still have copies or products in flight.
   __syncwarp();
+  __syncthreads();
   if (*abort_flag && lane == 0) {
     if (warp == 0) {
       if (rank == 0)
@@ -596,7 +599,7 @@ cudaError_t launch_gemm(const CUtensorMap& ma, const CUtensorMap& mb, const type
   const int64_t sms = sm_count() / P::CG * P::CG;
   if (grid > sms) grid = sms;
   return launch_dependent(fw_tc_gemm_kernel<P>, grid, GemmSmem<P>::kThreads, GemmSmem<P>::kBytes, P::CG, st, ma, mb,
-                          ma2 ? *ma2 : ma, mb2 ? *mb2 : mb, a);
+                          ma2 ? *ma2 : ma, mb2 ? *mb2 : mb, a, tc_wait_ns());
 }
 
 }  // namespace

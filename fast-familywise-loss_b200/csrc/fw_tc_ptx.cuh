@@ -9,16 +9,17 @@
 namespace fwb200 {
 
 constexpr int kTcStatusTimeout = 4;
-constexpr uint64_t kTcWaitLimitNs = 2000000000ull;  // 2 s; a tile's MMAs take ~20 us
+constexpr int64_t kTcWaitLimitNs = 2000000000;  // unless set otherwise: 2 s; a tile's MMAs take ~20 us
 constexpr uint64_t kTcDrainLimitNs = 100000000ull;  // 100 ms per drain wait after an abort
 
 // Bounded wait for the phase of the given parity, by a whole warp.  Returns
 // false for every lane (after raising the abort flag and the status bit) on
-// a timeout, or when another role has aborted.
+// a timeout, or when another role has aborted.  A limit of 0 gives up unless
+// the phase is complete already.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
-                                          int32_t* status) {
-  bool ok = mbar_try(bar, parity);
-  if (!ok) {
+                                          int32_t* status, uint64_t limit_ns) {
+  bool ok = limit_ns != 0 ? mbar_try(bar, parity) : mbar_test(bar, parity);
+  if (!ok && limit_ns != 0) {
     const uint64_t t0 = global_ns();
     for (uint32_t i = 1;; ++i) {
       if (mbar_try(bar, parity)) {
@@ -26,7 +27,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
         break;
       }
       if (*abort_flag) break;
-      if ((i & 255u) == 0 && global_ns() - t0 > kTcWaitLimitNs) break;
+      if ((i & 255u) == 0 && global_ns() - t0 > limit_ns) break;
     }
   }
   ok = __all_sync(kFull, ok);

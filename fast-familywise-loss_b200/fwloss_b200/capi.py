@@ -24,6 +24,7 @@ _I64 = ctypes.c_int64
 _SIGS = {
     "fw_version": ([], ctypes.c_char_p),
     "fw_error_string": ([ctypes.c_int], ctypes.c_char_p),
+    "fw_tc_wait_limit": ([ctypes.c_int64], ctypes.c_int64),
     "fw_fused_fwd_bwd": ([_P, _P, _I64, _I64, _I64, ctypes.c_float, _P, _P, _P, _P, _P, _P], ctypes.c_int),
     "fw_forward_mask": ([_P, _P, _I64, _I64, _I64, _P, _P, _P, _P, _P, _P], ctypes.c_int),
     "fw_backward_mask": ([_P, _P, _P, _I64, _I64, ctypes.c_float, _P, _P, _P], ctypes.c_int),

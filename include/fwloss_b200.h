@@ -58,10 +58,20 @@ extern "C" {
 
 #define FWB_STATUS_LABEL_RANGE 1   /* some label y[r] is outside [0, C)          */
 #define FWB_STATUS_NONFINITE 2     /* some row maximum is NaN or +-inf           */
-#define FWB_STATUS_TIMEOUT 4       /* a bounded wait gave up (fused LM-head kernel, staged streaming tiles, cross-GPU loss sum) */
+#define FWB_STATUS_TIMEOUT 4       /* a bounded wait gave up (tensor-core kernels, staged streaming tiles, cross-GPU loss sum) */
 
 /* Library version, "major.minor.patch". */
 FWB_API const char* fw_version(void);
+
+/*
+ * Longest wait inside the tensor-core kernels (fused LM-head scan, 8-bit output
+ * layer, softmax cross entropy) that this process launches from now on, in
+ * nanoseconds of wall clock; 2 s at the start.  A wait that passes it gives up
+ * (FWB_STATUS_TIMEOUT).  Raise it where GPUs are time-sliced: a preempted
+ * kernel's clock runs on.  0 gives up at the first wait that is not over
+ * already; a negative value changes nothing.  Returns the limit before.
+ */
+FWB_API int64_t fw_tc_wait_limit(int64_t ns);
 
 /* Human-readable text for an FWB_* return code. */
 FWB_API const char* fw_error_string(int code);
