@@ -75,7 +75,7 @@ struct Int8Many {
 #pragma unroll
     for (int k = 0; k < COLS / 32; ++k) st.ws[k] = col + 32 * k < a.N ? a.ws[col + 32 * k] : 0.0f;
   }
-  template <class Done>
+  template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
                                   Done done) {
     const int r0 = t.m0 + p.row, rows = a.T - r0, s0 = p.share * COLS;
@@ -83,10 +83,11 @@ struct Int8Many {
 #pragma unroll
     for (int c = 0; c < COLS; c += 32) {
       float v[32];
-      tmem_ld32(p.taddr + s0 + c, v);
+      if constexpr (!LOST) tmem_ld32(p.taddr + s0 + c, v);
       if (c + 32 == COLS) done();
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] = (float)__float_as_int(v[i]) * st.qs * __shfl_sync(kFull, st.ws[c / 32], i);
+      for (int i = 0; i < 32; ++i)
+        v[i] = LOST ? CUDART_NAN_F : (float)__float_as_int(v[i]) * st.qs * __shfl_sync(kFull, st.ws[c / 32], i);
       if constexpr (sizeof(TO) == 2)
         stage_block<TO, COLS>(reinterpret_cast<uint32_t*>(p.smem), v, p.lane, c);
       else
@@ -137,7 +138,7 @@ struct Int8Few {
 #pragma unroll
     for (int k = 0; k < (NT + 31) / 32; ++k) st.qs[k] = k * 32 + p.lane < a.T ? a.qs[k * 32 + p.lane] : 0.0f;
   }
-  template <class Done>
+  template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
                                   Done done) {
     const int n = t.m0 + p.row + p.lane;
@@ -147,15 +148,18 @@ struct Int8Few {
 #pragma unroll
     for (int c = 0; c < NT; c += STEP) {
       float v[STEP];
-      if constexpr (STEP == 32)
+      if constexpr (LOST) {
+      } else if constexpr (STEP == 32) {
         tmem_ld32(p.taddr + c, v);
-      else
+      } else {
         tmem_ld16(p.taddr + c, v);
+      }
       if (c + STEP == NT) done();
 #pragma unroll
       for (int i = 0; i < STEP; ++i) {
         const int tok = c + i;
-        const float x = (float)__float_as_int(v[i]) * __shfl_sync(kFull, st.qs[tok / 32], tok % 32) * st.ws;
+        const float x =
+            LOST ? CUDART_NAN_F : (float)__float_as_int(v[i]) * __shfl_sync(kFull, st.qs[tok / 32], tok % 32) * st.ws;
         if (mine && tok < a.T) st_elem(out + (int64_t)tok * a.ldo, x);
       }
     }

@@ -27,7 +27,8 @@
 //
 // Every wait is bounded; on a timeout all roles leave their loops, then the
 // copies and products in flight are waited for (bounded) and TMEM is released,
-// as in the fused LM-head kernel; the CTAs of a pair leave together.
+// as in the fused LM-head kernel; the CTAs of a pair leave together.  The
+// epilogue writes NaN for the tiles it could not finish.
 #pragma once
 
 #include "fw_host.cuh"
@@ -210,9 +211,12 @@ struct TcPart {
 //   struct State     what an epilogue thread keeps over a tile's parts
 //   begin(args, plan, tile, part, state)  before the tile's products are done:
 //                    loads that the epilogue would wait for
-//   epilogue(args, plan, tile, part, state, k, parts, done): part k of the
-//                    tile's `parts`; done() hands the accumulator back once
-//                    its last column has been read.
+//   epilogue<LOST>(args, plan, tile, part, state, k, parts, done): part k of
+//                    the tile's `parts`; done() hands the accumulator back once
+//                    its last column has been read.  LOST: there is no
+//                    accumulator, a wait gave up; what the tile would have
+//                    given is written as NaN (nothing, where the operator
+//                    tells by its own status word).
 template <class P>
 struct GemmSmem {
   static constexpr uint32_t kBRows = P::BN / P::CG;
@@ -400,16 +404,17 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     part.lane = lane;
     part.share = (warp - 2) >> 2;
     part.smem = smE + (warp - 2) * (P::EPI_BYTES / P::EW);
-    for (int it = 0; P::get(a, plan, it, &t); ++it) {
+    int it = 0;
+    for (; P::get(a, plan, it, &t); ++it) {
       const int parts = P::KC == 0 ? 1 : max((t.nk + P::KC - 1) / (P::KC == 0 ? 1 : P::KC), 1);
       typename P::State state{};
       P::begin(a, plan, t, part, state);
       for (int k = 0; k < parts; ++k) {
-        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status, wait_ns)) goto done;
+        if (!mbar_wait(&tfull[acc], aph, abort_flag, a.status, wait_ns)) goto lost;
         tc_fence_after();
         part.taddr = tmem + (uint32_t)((quad * 32) << 16) + acc * P::BN;
         const uint32_t te = CG == 2 ? in_cta(&tempty[acc], 0) : smem_u32(&tempty[acc]);
-        P::epilogue(a, plan, t, part, state, k, parts, [te, lane] {
+        P::template epilogue<false>(a, plan, t, part, state, k, parts, [te, lane] {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive_at(te);
@@ -419,6 +424,13 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
           aph ^= 1u;
         }
       }
+    }
+    goto done;
+  lost:  // this tile and those behind it
+    for (; P::get(a, plan, it, &t); ++it) {
+      typename P::State state{};
+      P::begin(a, plan, t, part, state);
+      P::template epilogue<true>(a, plan, t, part, state, 0, 1, [] {});
     }
   }
 done:

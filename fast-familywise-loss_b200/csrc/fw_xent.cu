@@ -229,9 +229,10 @@ struct LseTile {
   __device__ static void begin(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st) {
     st.y = a.label[t.m0 + p.row + p.lane];
   }
-  template <class Done>
+  template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int k,
                                   int parts, Done done) {
+    if constexpr (LOST) return;  // the status word in the state makes every loss NaN
 #pragma unroll
     for (int c = 0; c < kLseCols; c += 16) {
       float v[16];
@@ -458,7 +459,7 @@ struct GradTile {
     st.lse = live ? a.lse[row] : 0.0f;
     st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
   }
-  template <class Done>
+  template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
                                   Done done) {
     const int row = t.m0 + p.row + p.lane, y = st.y;
@@ -467,12 +468,12 @@ struct GradTile {
     T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (t.n0 - a.v0);
     for (int c = p.share * (BN / 2); c < (p.share + 1) * (BN / 2); c += 32) {
       float v[32];
-      tmem_ld32(p.taddr + c, v);
+      if constexpr (!LOST) tmem_ld32(p.taddr + c, v);
       if (c + 32 == (p.share + 1) * (BN / 2)) done();
       const int valid = live ? min(32, a.V - (t.n0 + c)) : 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float q = exp2_hw((v[i] - lse) * kLog2e);
+        float q = LOST ? CUDART_NAN_F : exp2_hw((v[i] - lse) * kLog2e);
         if (t.n0 + c + i == y) q -= 1.0f;
         v[i] = i < valid ? q * coef : 0.0f;
       }
@@ -606,7 +607,7 @@ struct ProductTile {
     st.zero = t.nk == 0 || (dh && row >= a.head->rows);
     st.f = st.zero ? 0.0f : dh ? plan.back * a.up.rest(st.mine) : plan.back;
   }
-  template <class Done>
+  template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st, int,
                                   int, Done done) {
     uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
@@ -619,7 +620,12 @@ struct ProductTile {
     float* sum = summed ? a.sum + ((int64_t)t.rows * a.Bp + r0 + p.lane) * a.lds + t.n0 + s0 : nullptr;
     for (int c = 0; c < BN / 2; c += 32) {
       float v[32];
-      tmem_ld32(p.taddr + s0 + c, v);
+      if constexpr (LOST) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = CUDART_NAN_F;
+      } else {
+        tmem_ld32(p.taddr + s0 + c, v);
+      }
       if (c + 32 == BN / 2) done();
       if (c >= cols) continue;
       if (summed) {  // this thread's own row of the sum so far; lds is D rounded up to 32

@@ -24,7 +24,8 @@ def lm_head_cross_entropy(hidden, weight, target, reduction="mean", ignore_index
     whose target is ignore_index take no part, whatever hidden holds there:
     loss 0 under "none", gradient 0, and the mean is over the other rows (NaN
     if there is none).  Any other target outside [0, V) makes its row's loss
-    and gradient NaN.  `status`, if given, is an int32 CUDA tensor whose first
+    and gradient NaN, and so does an on-chip wait that gave up for what it was
+    for.  `status`, if given, is an int32 CUDA tensor whose first
     word receives FWB_STATUS_* flags (target out of range, non-finite row, a
     wait that gave up)."""
     mode = _REDUCTIONS.get(reduction)

@@ -26,6 +26,7 @@ def int8_linear(q, q_scale, weight, weight_scale, out_dtype=torch.bfloat16, stat
     weight [N, K] int8 with weight_scale [N] (scales fp32); K at most 131071.
 
     Rows of q and weight that do not start on 16-byte boundaries are copied
-    first, at every call: lay a weight out with quantize_rows_int8.  `status`,
-    if given, receives FWB_STATUS_TIMEOUT if an on-chip wait gave up."""
+    first, at every call: lay a weight out with quantize_rows_int8.  Where an
+    on-chip wait gave up, the logits it was for are NaN; `status`, if given,
+    receives FWB_STATUS_TIMEOUT."""
     return ext().int8_linear(q, q_scale, weight, weight_scale, out_dtype, status)

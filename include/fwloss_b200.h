@@ -535,7 +535,9 @@ FWB_API int fw_rms_norm_grad(int dtype, int wdtype, const void* dy, int64_t lddy
  * out[t, n] = (sum_k q[t, k] * wq[n, k]) * q_scale[t] * w_scale[n]: the sum is
  * an exact 32-bit integer (hence K <= FWB_INT8_MAX_K), the result is rounded
  * once to out_dtype.  Rows of q and wq start on 16-byte boundaries (ldq and
- * ldw multiples of 16); columns from K on are not read as values.
+ * ldw multiples of 16); columns from K on are not read as values.  Where a wait
+ * gave up (FWB_STATUS_TIMEOUT) the results it was for are NaN, as they are in
+ * the cross entropy below.
  */
 #define FWB_INT8_MAX_K 131071
 FWB_API int fw_int8_linear(int out_dtype, const int8_t* q, int64_t ldq, const float* q_scale,
