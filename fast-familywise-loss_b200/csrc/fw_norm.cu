@@ -290,6 +290,7 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
       // a row of zeros, or not finite, is 0 (or NaN) through its scale
       const Int8Steps steps(scale);
       const int w16 = (D + 15) / 16 * 16;
+      static_assert(CH * G * V % 16 == 0, "the slots cover the row's padding");
       if (off == 0) {  // the slots' bytes lie together in q
 #pragma unroll
         for (int k = 0; k < CH; ++k) {
@@ -302,10 +303,6 @@ __global__ void __launch_bounds__(cta_threads<G>(), 1024 / cta_threads<G>()) fw_
             *reinterpret_cast<uint2*>(a.q + r * a.ldq + e) = make_uint2(b[0], b[1]);
           else
             *reinterpret_cast<uint32_t*>(a.q + r * a.ldq + e) = b[0];
-        }
-        if constexpr (CH * G * V < 16 * 64) {  // short rows: the padding may lie past the last slot
-          for (int e = (CH * G + t) * V; e < w16; e += G * V)
-            for (int j = 0; j < V; ++j) a.q[r * a.ldq + e + j] = 0;
         }
       } else {  // through shared memory
         int8_t* qs = reinterpret_cast<int8_t*>(norm_smem) + ring_bytes<T, G, CH>(2) + grp * w16;

@@ -21,24 +21,6 @@ __device__ __forceinline__ uint4 ld_global16(const void* p) {
 }
 
 template <class T>
-__device__ __forceinline__ uint4 load_slot(const T* row, int64_t e0, int64_t D, bool vec) {
-  constexpr int V = 16 / sizeof(T);
-  if (vec && e0 >= 0 && e0 + V <= D) return ld_stream16(row + e0);
-  uint32_t w[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-  for (int j = 0; j < V; ++j) {
-    const int64_t e = e0 + j;
-    if (e >= 0 && e < D) {
-      if constexpr (sizeof(T) == 4)
-        w[j] = __float_as_uint(row[e]);
-      else
-        w[j >> 1] |= (uint32_t)*reinterpret_cast<const unsigned short*>(row + e) << (16 * (j & 1));
-    }
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-template <class T>
 __device__ __forceinline__ void store_slot(T* row, int64_t e0, int64_t D, bool vec, const uint4& u) {
   constexpr int V = 16 / sizeof(T);
   if (vec && e0 >= 0 && e0 + V <= D) {
