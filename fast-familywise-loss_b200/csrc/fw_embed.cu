@@ -456,7 +456,7 @@ __device__ __forceinline__ void sum_chunk(const EmbedGradArgs& a, const Span<T>&
       if (!ALIGNED)
         e0 -= dst_off(static_cast<const T*>(a.dw) + (int64_t)__shfl_sync(kFull, ent.x, (i0 + i) & 31) * a.D);
       u[i] = i0 + i >= live || e0 >= a.D ? make_uint4(0u, 0u, 0u, 0u)
-             : ALIGNED                   ? ld_stream16(row + e0)
+             : ALIGNED                   ? ld_global16_once(row + e0)
                                          : load_slot_shifted(row, e0, span);
     }
 #pragma unroll
@@ -632,7 +632,7 @@ __global__ void __launch_bounds__(256) fw_embed_direct_kernel(EmbedGradArgs a) {
       for (; hit != 0u; hit &= hit - 1u) {
         const T* row = static_cast<const T*>(a.g) + (int64_t)(t0 + __ffs(hit) - 1) * a.ldg;
         float x[V];
-        unpack16<T>(ALIGNED ? ld_stream16(row + e0) : load_slot_shifted(row, e0, span), x);
+        unpack16<T>(ALIGNED ? ld_global16_once(row + e0) : load_slot_shifted(row, e0, span), x);
 #pragma unroll
         for (int j = 0; j < V; ++j) acc[j] += x[j];
       }

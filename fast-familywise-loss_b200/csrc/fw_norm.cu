@@ -509,8 +509,7 @@ __global__ void __launch_bounds__(1024) fw_norm_grad_long_kernel(NormGradArgs a)
 // dw[e] = sum over the parts, in a fixed order: 32 columns per CTA, each of
 // its 32 warps adds every 32nd part.
 template <class T>
-__global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* __restrict__ part, int64_t n, int64_t D,
-                                                          T* __restrict__ dw) {
+__global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* part, int64_t n, int64_t D, T* dw) {
   __shared__ float sm[32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t e = (int64_t)blockIdx.x * 32 + lane;

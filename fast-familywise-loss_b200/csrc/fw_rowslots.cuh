@@ -14,9 +14,25 @@
 
 namespace fwb200 {
 
+// 16 bytes of global memory.  Not the non-coherent form, which wants memory
+// that nobody writes while the kernel runs: a programmatic dependent has
+// started while the kernel before it still writes what it will read.
 __device__ __forceinline__ uint4 ld_global16(const void* p) {
   uint4 r;
-  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  asm volatile("ld.global.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p)
+               : "memory");
+  return r;
+}
+
+// The same for what is read once.
+__device__ __forceinline__ uint4 ld_global16_once(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p)
+               : "memory");
   return r;
 }
 
