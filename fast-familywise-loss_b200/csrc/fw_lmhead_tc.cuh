@@ -278,6 +278,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
   } else if (warp == 1) {
     // --------------------------------------------- MMA issuer (lane 0 issues)
     uint32_t s = 0, ph = 0, acc = 0, aph = 0;
+    if (gives_up(a.wait_ns, abort_flag, a.status)) goto done;
     for (int64_t w = blockIdx.x; w < nwork; w += gridDim.x) {
       const int q = (int)(w / a.n_mblocks);
       for (int64_t n0 = a.col_start[q]; n0 < a.col_start[q + 1]; n0 += kTcBN) {

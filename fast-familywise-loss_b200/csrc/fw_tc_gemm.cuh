@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(GemmSmem<P>::kThreads, 1)
     }
   } else if (warp == 1) {
     uint32_t s = 0, ph = 0, acc = 0, aph = 0;
+    if (gives_up(wait_ns, abort_flag, a.status)) goto done;
     if (rank == 0) {
       for (int it = 0; P::get(a, plan, it, &t); ++it) {
         const bool a_mn = P::TWO && t.kind ? P::A_MN2 : P::A_MN;

@@ -14,12 +14,11 @@ constexpr uint64_t kTcDrainLimitNs = 100000000ull;  // 100 ms per drain wait aft
 
 // Bounded wait for the phase of the given parity, by a whole warp.  Returns
 // false for every lane (after raising the abort flag and the status bit) on
-// a timeout, or when another role has aborted.  A limit of 0 gives up unless
-// the phase is complete already.
+// a timeout, or when another role has aborted.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag,
                                           int32_t* status, uint64_t limit_ns) {
-  bool ok = limit_ns != 0 ? mbar_try(bar, parity) : mbar_test(bar, parity);
-  if (!ok && limit_ns != 0) {
+  bool ok = mbar_try(bar, parity);
+  if (!ok) {
     const uint64_t t0 = global_ns();
     for (uint32_t i = 1;; ++i) {
       if (mbar_try(bar, parity)) {
@@ -36,6 +35,18 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     *abort_flag = 1;
   }
   return ok;
+}
+
+// A limit of 0 stands for a wait that has run out: the MMA issuer asks here,
+// once, and gives up before its first (inside every wait the question would
+// cost 1 to 4 % of a large product).
+__device__ __forceinline__ bool gives_up(uint64_t limit_ns, volatile int* abort_flag, int32_t* status) {
+  if (limit_ns != 0) return false;
+  if ((threadIdx.x & 31) == 0) {
+    raise_status(status, kTcStatusTimeout);
+    *abort_flag = 1;
+  }
+  return true;
 }
 
 // Abort path, one thread: waits (at most kTcDrainLimitNs) for the phase of

@@ -68,8 +68,8 @@ FWB_API const char* fw_version(void);
  * layer, softmax cross entropy) that this process launches from now on, in
  * nanoseconds of wall clock; 2 s at the start.  A wait that passes it gives up
  * (FWB_STATUS_TIMEOUT).  Raise it where GPUs are time-sliced: a preempted
- * kernel's clock runs on.  0 gives up at the first wait that is not over
- * already; a negative value changes nothing.  Returns the limit before.
+ * kernel's clock runs on.  0 makes every launch give up at once, to see what a
+ * program does then; a negative value changes nothing.  Returns the limit before.
  */
 FWB_API int64_t fw_tc_wait_limit(int64_t ns);
 

@@ -1,6 +1,6 @@
-"""Waits inside the tensor-core kernels that give up: the limit is set so that
-every wait that is not over already does, the kernels report it, and nothing of
-theirs is left behind for the launches after them."""
+"""Waits inside the tensor-core kernels that give up: with the limit at 0 the
+matrix issuers do at once and everybody else when nothing comes; the kernels
+report it, and nothing of theirs is left behind for the launches after them."""
 import contextlib
 
 import pytest
