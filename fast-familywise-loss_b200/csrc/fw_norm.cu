@@ -4,7 +4,7 @@
 //
 //   s = x + residual, rounded to the stream's type      (s = x without one)
 //   y = s * rstd * w,   rstd = 1 / sqrt(mean(s^2) + eps)
-//   q = rint(y / scale), scale = max|y| / 127           (8-bit form)
+//   q = y / scale to the nearest, scale = max|y| / 127  (8-bit form)
 //
 // s is defined as the stored, rounded sum, so the gradient (which reads the
 // stored stream) is the gradient of exactly this function:
@@ -27,7 +27,7 @@
 // fixed order by a second kernel.
 //
 // Forward and backward with a residual, 16384 x 4096 bfloat16 (1.07 GB): 193
-// us, 5.6 TB/s; without the copies ahead 202.  8001 x 7001 (rows at every
+// to 201 us, 5.3 to 5.6 TB/s; without the copies ahead 202 where it takes 193.  8001 x 7001 (rows at every
 // alignment): 174 us, 5.2 TB/s, without them 570.
 #include <cuda_runtime.h>
 
@@ -129,11 +129,14 @@ __device__ __forceinline__ float int8_scale(float m) {
 
 // Values in steps of their row's scale, to the nearest, as bytes; 0 for a row
 // that has no such step (its values may be NaN).  1 / scale does not fit fp32
-// for the smallest scales, hence the power of two taken out of it.  The steps
-// are added to 1.5 * 2^23, whose unit is 1: the addition rounds, and the sum's
-// low byte is the integer (a third of the instructions of rounding, clamping and
-// converting: 16384 x 4096 bfloat16 with residual 89 us, alone 40, for 106 and
-// 62; 32000 x 2048 float32 alone 66 for 87, but with residual 159 for 140).
+// for the smallest scales, hence the power of two taken out of it.  Its
+// rounding moves a value by less than 2^-17 of a step, so one that close to
+// the middle between two steps may take either.  The steps are added to 1.5 *
+// 2^23, whose unit is 1: the addition rounds, and the sum's low byte is the
+// integer (a third of the instructions of rounding, clamping and converting:
+// norm of 16384 x 4096 bfloat16 with residual 95 us, alone 65, the rows
+// themselves 47, for 113, 88 and 69; of 32000 x 2048 float32 162, 94 and 73, for
+// 158, 114 and 94; of 8000 x 8192 float32 with residual 297 for 348).
 struct Int8Steps {
   float up, per_step;
   uint32_t keep;
@@ -532,8 +535,11 @@ __global__ void __launch_bounds__(1024) fw_norm_dw_kernel(const float* part, int
 
 // Threads per row by its slots: a warp, or a CTA with one or two
 // slots per thread, so that a thread's 64 registers hold its gains and its
-// part of dw; the memory-pass kernels beyond 2048 slots (2000 x 16000
-// bfloat16, forward and backward: 183 us here, 348 there).
+// part of dw; the memory-pass kernels beyond 2048 slots.  With 1024 threads
+// one CTA fills an SM and nothing covers its barriers, and the gradient's 64
+// registers spill a few: 2000 x 16000 bfloat16 takes 76 us forward and 122
+// backward, where the bytes take 39 each way; the memory passes, for 2000 x
+// 17000, 102 and 286.
 struct NormShape {
   int G, CH;
 };

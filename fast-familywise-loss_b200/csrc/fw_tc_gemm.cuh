@@ -144,7 +144,8 @@ struct TcTile {
 };
 
 // Division of n < 2^31 by a divisor met again and again: a multiplication and
-// a shift.  The multiplier is floor(2^32 (2^s - d) / d) + 1 for the first
+// a shift (Granlund and Montgomery, Division by Invariant Integers using
+// Multiplication, 1994).  The multiplier is floor(2^32 (2^s - d) / d) + 1 for the first
 // 2^s >= d; n < 2^31 leaves room for one more, so the quotient may be a rounded
 // one (a 64-bit integer division here costs a short kernel half a microsecond).
 struct FastDiv {

@@ -16,7 +16,7 @@ from ._native import ext
 
 def quantize_rows_int8(x):
     """(q int8 [R, D], scale fp32 [R]) with x[r] = q[r] * scale[r] to within
-    half a step, scale = max|x[r]| / 127.  q's rows start on 16-byte
+    half a step (and fp32's rounding), scale = max|x[r]| / 127.  q's rows start on 16-byte
     boundaries (its row stride is D rounded up to 16)."""
     return ext().quantize_rows_int8(x)
 

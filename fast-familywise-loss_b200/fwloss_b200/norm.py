@@ -28,8 +28,8 @@ def rms_norm_int8(x, weight, eps=1e-6, residual=None):
     int8_linear: (q int8 [..., D], scale fp32 [...]) with norm = q * scale, and
     x + residual as a third result where `residual` is given.
 
-    scale = max|norm| / 127 of the row, q rounded to the nearest (ties to
-    even).  A row of zeros has scale 0; a row that is not finite has that scale
+    scale = max|norm| / 127 of the row, q = norm / scale to the nearest (by the
+    fp32 reciprocal: within 2^-17 of the middle between two steps, either).  A row of zeros has scale 0; a row that is not finite has that scale
     and q = 0, so that what is computed from it is NaN.  For serving: not
     differentiable."""
     return ext().rms_norm_int8(x, weight, eps, residual)

@@ -505,8 +505,9 @@ FWB_API int fw_rms_norm(int dtype, int wdtype, const void* x, int64_t ldx, const
                         int64_t lds, void* y, int64_t ldy, float* rstd, void* stream);
 
 /*
- * The same norm with an 8-bit output: q = rint(y / scale[r]) with
- * scale[r] = max|y| / 127.  Rows of q start on 16-byte boundaries: ldq is a
+ * The same norm with an 8-bit output: q = y / scale[r] to the nearest integer,
+ * scale[r] = max|y| / 127 (by the fp32 reciprocal of scale[r]: a quotient
+ * within 2^-17 of the middle between two integers may take either).  Rows of q start on 16-byte boundaries: ldq is a
  * multiple of 16 and at least D rounded up to 16; the columns from D up to
  * that are set to 0.  A row whose largest value is 0 or not finite gives
  * q = 0 and that scale.
