@@ -77,8 +77,9 @@ def build_lib(force=False, verbose=False):
 
 
 def build_ext(force=False):
-    srcs = [os.path.join(CSRC, f) for f in ("fw_torch_binding.cpp", "fw_torch_lm.cpp")]
-    deps = srcs + [os.path.join(INCLUDE, "fwloss_b200.h"), LIB]
+    srcs = [os.path.join(CSRC, f) for f in ("fw_torch_binding.cpp", "fw_torch_lm.cpp", "fw_torch_score.cpp")]
+    headers = [os.path.join(CSRC, "fw_torch_lm.h"), os.path.join(INCLUDE, "fwloss_b200.h")]
+    deps = srcs + headers + [LIB]
     if not force and not _stale(EXT, deps):
         return EXT
     from concurrent.futures import ThreadPoolExecutor
@@ -92,10 +93,10 @@ def build_ext(force=False):
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     os.makedirs(BUILD_DIR, exist_ok=True)
     objs = [os.path.join(BUILD_DIR, os.path.basename(s)[:-4] + ".o") for s in srcs]
-    todo = [(s, o) for s, o in zip(srcs, objs) if force or _stale(o, [s, os.path.join(INCLUDE, "fwloss_b200.h")])]
+    todo = [(s, o) for s, o in zip(srcs, objs) if force or _stale(o, [s] + headers)]
     flags = ["-O2", "-std=c++17", "-fPIC", "-DTORCH_EXTENSION_NAME=fw_radix_cuda", "-DTORCH_API_INCLUDE_EXTENSION_H",
              f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-Wno-deprecated-declarations"] + [f"-I{p}" for p in incs]
-    with ThreadPoolExecutor(max_workers=2) as ex:
+    with ThreadPoolExecutor(max_workers=len(srcs)) as ex:
         list(ex.map(lambda so: subprocess.run(["g++", *flags, "-c", so[0], "-o", so[1]], check=True), todo))
     cmd = ["g++", "-shared", "-o", EXT + ".tmp", *objs]
     cmd += [f"-L{p}" for p in libdirs] + [f"-Wl,-rpath,{p}" for p in libdirs]

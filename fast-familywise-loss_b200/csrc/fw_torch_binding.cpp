@@ -662,7 +662,8 @@ void segment_grad_weight(torch::Tensor hidden, torch::Tensor sorted_keys, torch:
            "fw_segment_grad_weight");
 }
 
-void register_lm_operators(pybind11::module_& m);  // fw_torch_lm.cpp
+void register_lm_operators(pybind11::module_& m);     // fw_torch_lm.cpp
+void register_score_operators(pybind11::module_& m);  // fw_torch_score.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "B200 (sm_100a) Familywise loss: drop-in for the fw_radix_cuda module";
@@ -709,5 +710,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("gathered"), py::arg("rank"), py::arg("col_start"), py::arg("z_local"), py::arg("targets"),
         py::arg("grad_scale"), py::arg("grad"), py::arg("local_idx"), py::arg("status") = py::none());
   register_lm_operators(m);
+  register_score_operators(m);
   m.def("version", []() { return std::string(fw_version()); });
 }

@@ -576,6 +576,30 @@ FWB_API int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t
                              void* workspace, int64_t workspace_bytes, void* dhidden, void* dweight,
                              int32_t* status, void* stream);
 
+/*
+ * Log probabilities of given tokens from logits [B, V] (row stride ld), at a
+ * temperature T with inv_t = 1 / T: logp[r] = log softmax(logits[r] / T)[y[r]]
+ * and entropy[r] of that distribution, both fp32; for k > 0 (at most
+ * FWB_TOP_MAX and V) also the k likeliest columns, top_ids[r * k + i] with
+ * their log probabilities top_logp, the likeliest first, equal logits by the
+ * lowest column.  Columns of -inf have probability 0.  A row with
+ * y = ignore_index is not read: 0 everywhere, top_ids -1.  Any other y outside
+ * [0, V) (FWB_STATUS_LABEL_RANGE), and a row whose largest logit is not finite
+ * (FWB_STATUS_NONFINITE), give NaN and -1.
+ * `state` (fp32 [B, 4], 16-byte aligned, may be NULL) keeps what the gradient
+ * needs besides the logits; fw_token_log_probs_grad writes all of grad [B, V]
+ * (row stride ldg, of the logits' type) for the upstream gradients dlogp and
+ * dentropy (fp32 [B]; NULL: none), 0 in ignored rows.
+ */
+#define FWB_TOP_MAX 32
+FWB_API int fw_token_log_probs(int dtype, const void* logits, int64_t ld, const int64_t* y, int64_t B,
+                               int64_t V, float inv_t, int64_t ignore_index, int k, float* logp,
+                               float* entropy, float* top_logp, int64_t* top_ids, float* state,
+                               int32_t* status, void* stream);
+FWB_API int fw_token_log_probs_grad(int dtype, const void* logits, int64_t ld, int64_t B, int64_t V,
+                                    float inv_t, const float* state, const float* dlogp,
+                                    const float* dentropy, void* grad, int64_t ldg, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
