@@ -1,8 +1,12 @@
-// Torch front of the operators that score tokens: checks, outputs, the current
+// Torch front of the operators that score tokens and end a training step: checks, outputs, the current
 // stream and the autograd nodes, as in fw_torch_lm.cpp.
 #include "fw_torch_lm.h"
 
+#include <ATen/MemoryOverlap.h>
+
+#include <algorithm>
 #include <cmath>
+#include <string>
 
 namespace {
 
@@ -92,9 +96,152 @@ py::object token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t k
   return py::make_tuple(s.logp, s.entropy, s.top_logp, s.top_ids);
 }
 
+// ---------------------------------------------------------------- gradient norm and clipping
+struct List {
+  std::vector<Tensor> held;  // what the pointers are to: the tensors, or dense copies
+  std::vector<const void*> in;
+  std::vector<void*> out;
+  std::vector<int64_t> numel;
+  std::vector<int32_t> types, out_types;
+};
+
+bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
+
+void check_grads(const std::vector<Tensor>& grads, const char* op) {
+  const auto say = [op](const char* what) { return std::string(op) + ": " + what; };
+  value_check(!grads.empty(), say("no tensors").c_str());
+  for (const auto& t : grads) {
+    type_check(t.is_cuda(), say("gradients must be CUDA tensors (this build has no CPU path)").c_str());
+    type_check(t.layout() == torch::kStrided && is_float(t),
+               say("gradients must be dense float32, bfloat16 or float16 tensors").c_str());
+    value_check(t.device() == grads[0].device(), say("gradients must be on one device").c_str());
+    no_tangent(t, op);
+  }
+}
+
+void check_max_norm(double max_norm) {
+  value_check(max_norm >= 0.0 && !std::isnan(max_norm), "clip_grad_norm_: max_norm must not be negative");
+}
+
+Tensor norm_workspace(const std::vector<Tensor>& grads, int64_t* n) {
+  *n = fw_grad_norm_workspace((int64_t)grads.size());
+  return bytes(*n, grads[0]);
+}
+
+Tensor grad_norm(const std::vector<Tensor>& grads, const OptTensor& status) {
+  check_grads(grads, "grad_norm");
+  for (const auto& t : grads)
+    value_check(!(at::GradMode::is_enabled() && t.requires_grad()),
+                "grad_norm: not differentiable; pass gradients (p.grad), or detach");
+  at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  List l;
+  for (const auto& t : grads) {
+    l.held.push_back(dense(t) ? t : t.contiguous());
+    l.in.push_back(l.held.back().data_ptr());
+    l.numel.push_back(t.numel());
+    l.types.push_back(code(t));
+  }
+  int64_t nw;
+  auto ws = norm_workspace(grads, &nw);
+  auto norm = f32({}, grads[0]);
+  ok(fw_grad_norm((int64_t)grads.size(), l.in.data(), l.numel.data(), l.types.data(), ws.data_ptr(), nw,
+                  norm.data_ptr<float>(), status_of(status, grads[0]), stream()),
+     "fw_grad_norm");
+  return norm;
+}
+
+// Written ranges must not overlap each other, nor a range that is read for another tensor.
+void check_overlaps(const List& l) {
+  struct Range {
+    uintptr_t lo, hi;
+    bool written;
+  };
+  std::vector<Range> ranges;
+  const auto size = [](int32_t type) { return type == FWB_DTYPE_F32 ? 4 : 2; };
+  bool sorted = true;
+  const auto add = [&](const void* p, int64_t bytes, bool written) {
+    const auto lo = reinterpret_cast<uintptr_t>(p);
+    if (!ranges.empty() && ranges.back().lo > lo) sorted = false;
+    ranges.push_back({lo, lo + (uintptr_t)bytes, written});
+  };
+  for (size_t i = 0; i < l.in.size(); ++i) {
+    if (l.numel[i] == 0) continue;
+    add(l.out[i], l.numel[i] * size(l.out_types[i]), true);
+    if (l.in[i] != l.out[i] || l.types[i] != l.out_types[i]) add(l.in[i], l.numel[i] * size(l.types[i]), false);
+  }
+  if (!sorted) std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
+  uintptr_t written = 0, read = 0;  // ends of the ranges so far
+  for (const auto& r : ranges) {
+    value_check(r.lo >= written && (!r.written || r.lo >= read),
+                "clip_grad_norm_: tensors that are written overlap others (the same tensor twice?)");
+    (r.written ? written : read) = std::max(r.written ? written : read, r.hi);
+  }
+}
+
+Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const c10::optional<std::vector<Tensor>>& out,
+                       const OptTensor& norm_in, const OptTensor& status) {
+  check_grads(grads, "clip_grad_norm_");
+  check_max_norm(max_norm);
+  const auto& dest = out.has_value() ? *out : grads;
+  value_check(dest.size() == grads.size(), "clip_grad_norm_: out must have a tensor for every gradient");
+  for (size_t i = 0; i < dest.size(); ++i) {
+    const auto& t = dest[i];
+    value_check(!t.requires_grad(), "clip_grad_norm_: written tensors must not require grad (pass p.grad, not p)");
+    if (!out.has_value()) continue;
+    type_check(t.is_cuda() && t.layout() == torch::kStrided && is_float(t),
+               "clip_grad_norm_: out must hold dense float32, bfloat16 or float16 CUDA tensors");
+    value_check(t.device() == grads[0].device() && t.sizes() == grads[i].sizes(),
+                "clip_grad_norm_: out must have the gradients' shapes and device");
+  }
+  if (norm_in.has_value())
+    value_check(norm_in->device() == grads[0].device() && norm_in->scalar_type() == torch::kFloat32 && norm_in->numel() == 1,
+                "clip_grad_norm_: norm must be one float32 value on the gradients' device");
+  at::NoGradGuard no_grad;
+  const c10::cuda::CUDAGuard guard(grads[0].device());
+  List l;
+  std::vector<std::pair<Tensor, Tensor>> back;  // results that are copied to where they belong
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const auto &g = grads[i], &d = dest[i];
+    Tensor from = dense(g) ? g : g.contiguous(), to = d;
+    if (!dense(d) || (d.strides() != from.strides() && !(d.is_contiguous() && from.is_contiguous()))) {
+      // an element of `to` is where it is in `from`
+      to = out.has_value() ? at::empty_strided(from.sizes(), from.strides(), d.options()) : from;
+      back.emplace_back(d, to);
+    }
+    l.held.push_back(from);
+    l.held.push_back(to);
+    l.in.push_back(from.data_ptr());
+    l.out.push_back(to.data_ptr());
+    l.numel.push_back(g.numel());
+    l.types.push_back(code(from));
+    l.out_types.push_back(code(to));
+  }
+  for (const auto& b : back) at::assert_no_internal_overlap(b.first);
+  check_overlaps(l);
+  int64_t nw = 0;
+  Tensor ws, norm;
+  if (norm_in.has_value()) {
+    norm = *norm_in;
+  } else {
+    ws = norm_workspace(grads, &nw);
+    norm = f32({}, grads[0]);
+  }
+  ok(fw_grad_clip((int64_t)grads.size(), l.in.data(), l.out.data(), l.numel.data(), l.types.data(), l.out_types.data(),
+                  (float)max_norm, norm_in.has_value() ? norm.data_ptr<float>() : nullptr,
+                  ws.defined() ? ws.data_ptr() : nullptr, nw, norm.data_ptr<float>(), status_of(status, grads[0]), stream()),
+     "fw_grad_clip");
+  for (const auto& b : back) b.first.copy_(b.second);
+  for (const auto& t : dest)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 }  // namespace
 
 void register_score_operators(pybind11::module_& m) {
   m.def("token_log_probs", &token_log_probs,
         "(logp, entropy[, top_logp, top_ids]) from logits (differentiable in the first two)");
+  m.def("grad_norm", &grad_norm, "global norm of many tensors");
+  m.def("clip_grad_norm_", &clip_grad_norm_, "gradients clipped to a global norm, in place or into others; the norm");
 }

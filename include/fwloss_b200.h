@@ -600,6 +600,32 @@ FWB_API int fw_token_log_probs_grad(int dtype, const void* logits, int64_t ld, i
                                     float inv_t, const float* state, const float* dlogp,
                                     const float* dentropy, void* grad, int64_t ldg, void* stream);
 
+/*
+ * Global norm of n tensors, norm = sqrt(sum of all elements' squares), and the
+ * tensors scaled to it, out[i] = grads[i] * min(1, max_norm / norm).  grads,
+ * out, numel, dtypes and out_dtypes are host arrays of n entries; a tensor is
+ * numel[i] contiguous elements at an address aligned to its type; at most 2^24
+ * tensors of 2^43 elements together.  The sums are fp64 past 32 elements, in a
+ * fixed order; the products fp32, rounded once to out_dtypes[i].  out[i] may be
+ * grads[i] (nothing is written then where the factor is 1, if that is so of all
+ * tensors); other overlaps are not allowed, and nothing checks for them.  A norm
+ * that is not finite scales by what the formula gives (0 for infinity, else
+ * NaN) and sets FWB_STATUS_NONFINITE.  The workspace (16-byte aligned,
+ * fw_grad_norm_workspace bytes for the device that is current, which has to be
+ * the one the call runs on) holds partial sums.
+ * fw_grad_clip takes the norm from norm_in, one value on the device, if that
+ * is given (norm, status and the workspace are not used then), else computes
+ * it and writes it to norm.
+ */
+FWB_API int64_t fw_grad_norm_workspace(int64_t n);
+FWB_API int fw_grad_norm(int64_t n, const void* const* grads, const int64_t* numel, const int32_t* dtypes,
+                         void* workspace, int64_t workspace_bytes, float* norm, int32_t* status,
+                         void* stream);
+FWB_API int fw_grad_clip(int64_t n, const void* const* grads, void* const* out, const int64_t* numel,
+                         const int32_t* dtypes, const int32_t* out_dtypes, float max_norm,
+                         const float* norm_in, void* workspace, int64_t workspace_bytes, float* norm,
+                         int32_t* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
