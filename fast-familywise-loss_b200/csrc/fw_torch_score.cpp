@@ -10,6 +10,12 @@
 
 namespace {
 
+// A temperature whose reciprocal fp32 holds.
+bool fits(double temperature) {
+  return temperature > 0.0 && std::isfinite((float)temperature) && std::isfinite((float)(1.0 / temperature)) &&
+         (float)(1.0 / temperature) > 0.0f;
+}
+
 // ---------------------------------------------------------------- log probabilities from logits
 struct Scores {
   Tensor logp, entropy, top_logp, top_ids, state;
@@ -82,8 +88,7 @@ py::object token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t k
               "token_log_probs: tokens must have the logits' leading shape");
   value_check(k >= 0 && k <= FWB_TOP_MAX && k <= logits.size(-1),
               "token_log_probs: top_k must be between 0 and 32, and at most V");
-  value_check(temperature > 0.0 && std::isfinite((float)temperature) && std::isfinite((float)(1.0 / temperature)) &&
-                  (float)(1.0 / temperature) > 0.0f,
+  value_check(fits(temperature),
               "token_log_probs: temperature must be positive and finite, and so must its reciprocal");
   no_tangent(logits, "token_log_probs");
   if (at::GradMode::is_enabled() && recording(logits)) {
@@ -94,6 +99,99 @@ py::object token_log_probs(const Tensor& logits, const Tensor& tokens, int64_t k
   auto s = score_forward(logits, tokens, k, temperature, ignore_index, status, false);
   if (k == 0) return py::make_tuple(s.logp, s.entropy);
   return py::make_tuple(s.logp, s.entropy, s.top_logp, s.top_ids);
+}
+
+// ---------------------------------------------------------------- log probabilities of an output layer
+struct HeadScores {
+  Tensor logp, entropy, state;
+};
+
+HeadScores head_forward(const Tensor& hidden, const Tensor& weight, const Tensor& tokens, double temperature,
+                        int64_t ignore_index, const OptTensor& status) {
+  const c10::cuda::CUDAGuard guard(hidden.device());
+  auto h = rows_of(hidden), w = rows_of(weight);
+  auto y = tokens.contiguous();
+  const int64_t B = h.size(0), D = h.size(1), V = w.size(0);
+  HeadScores out;
+  out.logp = f32({B}, h);
+  out.entropy = f32({B}, h);
+  const int64_t ns = fw_lm_head_log_probs_state(B, D, V, w.data_ptr(), ld_of(w));
+  const int64_t nw = fw_lm_head_log_probs_workspace(B, D, V, 0);
+  out.state = bytes(ns, h);
+  auto ws = bytes(nw, h);
+  ok(fw_lm_head_log_probs(code(h), h.data_ptr(), ld_of(h), w.data_ptr(), ld_of(w), y.data_ptr<int64_t>(), B, D, V,
+                          (float)(1.0 / temperature), ignore_index, out.logp.data_ptr<float>(),
+                          out.entropy.data_ptr<float>(), out.state.data_ptr(), ns, ws.data_ptr(), nw,
+                          status_of(status, h), stream()),
+     "fw_lm_head_log_probs");
+  return out;
+}
+
+struct LmHeadLogProbs : torch::autograd::Function<LmHeadLogProbs> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& hidden, const Tensor& weight, const Tensor& tokens,
+                               double temperature, int64_t ignore_index, const OptTensor& status) {
+    ctx->set_materialize_grads(false);
+    auto s = head_forward(hidden, weight, tokens, temperature, ignore_index, status);
+    ctx->save_for_backward({weight, s.state});
+    keep_status(ctx, status);
+    ctx->saved_data["rows"] = c10::IValue(hidden.size(0));
+    ctx->saved_data["temperature"] = c10::IValue(temperature);
+    return {s.logp, s.entropy};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    if (!g[0].defined() && !g[1].defined()) return variable_list(6);
+    const auto saved = ctx->get_saved_variables();
+    const c10::cuda::CUDAGuard guard(saved[0].device());
+    auto w = rows_of(saved[0].detach());
+    const Tensor& state = saved[1];
+    const Tensor dlogp = upstream(g[0]), dentropy = upstream(g[1]);
+    const bool want_h = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1);
+    const int64_t B = ctx->saved_data["rows"].toInt(), V = w.size(0), D = w.size(1);
+    // A hook may have restored the weight off the 16-byte boundaries it was saved on; the state has no copy of it then.
+    if (fw_lm_head_log_probs_state(B, D, V, w.data_ptr(), ld_of(w)) > state.numel()) {
+      auto c = at::empty({V, (D + 7) / 8 * 8}, w.options()).narrow(1, 0, D);
+      c.copy_(w);
+      w = c;
+    }
+    Tensor dh, dw;
+    if (want_h) dh = at::empty({B, D}, w.options());
+    if (want_w) dw = at::empty({V, D}, w.options());
+    const int64_t nw = fw_lm_head_log_probs_workspace(B, D, V, 1);
+    auto ws = bytes(nw, w);
+    const OptTensor status = kept_status(ctx);
+    ok(fw_lm_head_log_probs_grad(code(w), w.data_ptr(), ld_of(w), B, D, V,
+                                 (float)(1.0 / ctx->saved_data["temperature"].toDouble()), floats(dlogp),
+                                 floats(dentropy), state.data_ptr(), state.numel(), ws.data_ptr(), nw,
+                                 want_h ? dh.data_ptr() : nullptr, want_w ? dw.data_ptr() : nullptr,
+                                 status_of(status, w), stream()),
+       "fw_lm_head_log_probs_grad");
+    return once({dh, dw, Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+py::tuple lm_head_log_probs(const Tensor& hidden, const Tensor& weight, const Tensor& tokens, double temperature,
+                            int64_t ignore_index, const OptTensor& status) {
+  type_check(hidden.is_cuda() && weight.is_cuda(),
+             "lm_head_log_probs: hidden and weight must be CUDA tensors (this build has no CPU path)");
+  type_check(hidden.dim() == 2 && weight.dim() == 2 && weight.numel() > 0,
+             "lm_head_log_probs: hidden [B, D] and weight [V, D] must be matrices");
+  type_check(hidden.scalar_type() == weight.scalar_type() &&
+                 (hidden.scalar_type() == torch::kBFloat16 || hidden.scalar_type() == torch::kHalf),
+             "lm_head_log_probs: hidden and weight must both be bfloat16 or both float16");
+  value_check(hidden.size(1) == weight.size(1), "lm_head_log_probs: hidden and weight disagree on D");
+  type_check(tokens.scalar_type() == torch::kLong, "lm_head_log_probs: tokens must be int64");
+  value_check(tokens.dim() == 1 && tokens.size(0) == hidden.size(0), "lm_head_log_probs: tokens must have shape [B]");
+  value_check(weight.device() == hidden.device() && tokens.device() == hidden.device(),
+              "lm_head_log_probs: hidden, weight and tokens must be on one device");
+  value_check(fits(temperature), "lm_head_log_probs: temperature must be positive and finite, and so must its reciprocal");
+  no_tangent(hidden, "lm_head_log_probs");
+  no_tangent(weight, "lm_head_log_probs");
+  if (at::GradMode::is_enabled() && (recording(hidden) || recording(weight))) {
+    auto out = LmHeadLogProbs::apply(hidden, weight, tokens, temperature, ignore_index, status);
+    return py::make_tuple(out[0], out[1]);
+  }
+  auto s = head_forward(hidden, weight, tokens, temperature, ignore_index, status);
+  return py::make_tuple(s.logp, s.entropy);
 }
 
 // ---------------------------------------------------------------- gradient norm and clipping
@@ -242,6 +340,7 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
 void register_score_operators(pybind11::module_& m) {
   m.def("token_log_probs", &token_log_probs,
         "(logp, entropy[, top_logp, top_ids]) from logits (differentiable in the first two)");
+  m.def("lm_head_log_probs", &lm_head_log_probs, "(logp, entropy) of an output layer (differentiable)");
   m.def("grad_norm", &grad_norm, "global norm of many tensors");
   m.def("clip_grad_norm_", &clip_grad_norm_, "gradients clipped to a global norm, in place or into others; the norm");
 }

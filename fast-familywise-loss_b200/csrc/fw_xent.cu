@@ -35,6 +35,17 @@
 //
 // float16 G: exp(z - lse) may be under float16's smallest value, so G is
 // scaled by 2^15 (over the largest finite s_r), taken out after the sums.
+//
+// Log probabilities with entropies take the same kernels (BOTH below).  With a
+// temperature T and t = (z - max z) / T the tiles keep sum exp(t) t as well,
+// from which the entropy is h_r = log S - (sum exp(t) t) / S, two positive
+// terms, and with upstream factors a of logp and b of the entropy the logit
+// gradient is, with l = log p,
+//   T G_rj = a_r (1[j = y(r)] - p_rj) - b_r p_rj (l_rj + h_r),
+// its factor per row max(|a_r|, |b_r|), split as above.  |p (l + h)| is at most
+// (log V) / 4 + 0.3, under 5.2, hence 2^13 in the place of 2^15 for float16.
+#include <cmath>
+
 #include "fw_reduce.cuh"
 #include "fw_rowslots.cuh"
 #include "fw_tc_gemm.cuh"
@@ -43,7 +54,9 @@ namespace fwb200 {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kF16Unit = 32768.0f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kF16Unit = 32768.0f, kF16UnitBoth = 8192.0f;
+constexpr float kExpFloor = -200.0f;  // 2^kExpFloor is 0 in fp32; keeps 0 * t finite
 constexpr int kPackThreads = 256;
 
 // Device words at the start of the state.
@@ -61,6 +74,7 @@ struct PackArgs {
   int32_t* row_of;   // [Bp] packed -> given row (behind the live ones the ignored ones, then -1)
   int32_t* label;    // [Bp] -1: outside [0, V)
   float* loss_rows;  // zero for ignored rows, per given row; may be NULL
+  float* more_rows;  // the same
   XentHead* head;
   int32_t* status;
   int per_cta;
@@ -122,6 +136,7 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
         a.label[dst] = alive && ok ? (int32_t)y : -1;
         if (alive && !ok) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
         if (!alive && r < a.B && a.loss_rows) a.loss_rows[r] = 0.0f;
+        if (!alive && r < a.B && a.more_rows) a.more_rows[r] = 0.0f;
       }
       if (dst >= rows_up) continue;
       T* out = static_cast<T*>(a.hp) + dst * a.Dp;
@@ -198,6 +213,8 @@ struct LseArgs {
   int64_t Bp;
   int V, D;
   int32_t* status;
+  float* part_t;  // BOTH: sum of 2^t t, t = (z - maximum) c
+  float c;        // BOTH: log2(e) / T
 };
 
 // The accumulator is taken over every kLseStages stages of K and added up in
@@ -208,7 +225,7 @@ struct LseArgs {
 constexpr int kLseStages = 8;
 constexpr int kLseCols = 128;  // columns of a tile per epilogue thread: they stay in its registers
 
-template <TcKind K>
+template <TcKind K, bool BOTH>
 struct LseTile {
   using Args = LseArgs;
   struct State {
@@ -250,7 +267,7 @@ struct LseTile {
     const int n0 = t.n0 + p.share * kLseCols;
     const int y = st.y - n0;
     const int valid = a.V - n0;
-    float m = -CUDART_INF_F, s = 0.0f;
+    float m = -CUDART_INF_F, s = 0.0f, u = 0.0f;
 #pragma unroll
     for (int i = 0; i < kLseCols; ++i) {
       if (i >= valid) st.z[i] = -CUDART_INF_F;
@@ -258,11 +275,21 @@ struct LseTile {
       m = max_nan(m, st.z[i]);
     }
     if (m != -CUDART_INF_F) {  // a NaN maximum, or +inf, makes the sum NaN
-      float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f}, u2[2] = {0.0f, 0.0f};
 #pragma unroll
-      for (int i = 0; i < kLseCols; ++i) s4[i & 3] += exp2_hw((st.z[i] - m) * kLog2e);
+      for (int i = 0; i < kLseCols; ++i) {
+        if constexpr (BOTH) {
+          const float t2 = fmaxf((st.z[i] - m) * a.c, kExpFloor), e = exp2_hw(t2);
+          s4[i & 3] += e;
+          u2[i & 1] = fmaf(e, t2, u2[i & 1]);
+        } else {
+          s4[i & 3] += exp2_hw((st.z[i] - m) * kLog2e);
+        }
+      }
       s = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+      u = u2[0] + u2[1];
     }
+    if constexpr (BOTH) a.part_t[(int64_t)(n0 / kLseCols) * a.Bp + row] = u;
     a.part[(int64_t)(n0 / kLseCols) * a.Bp + row] = make_float2(m, s);
   }
 };
@@ -280,9 +307,73 @@ struct JoinArgs {
   int ntiles;
   int reduction;
   int32_t* status;
+  const float* part_t;           // BOTH, which writes logp in the place of the loss
+  float *entropy, *entropy_pack;  // per given row, packed
+  float inv_t;
 };
 
 constexpr int kJoinWarps = 32;
+
+// Maximum and sums of BOTH, relative to another maximum (not under it).
+__device__ __forceinline__ void raise_sums(float m, float to, float c, float* s, float* u) {
+  const float d = fmaxf((m - to) * c, kExpFloor), f = exp2f(d);
+  *u = f * fmaf(d, *s, *u);
+  *s *= f;
+}
+
+// As fw_xent_join_kernel, for log probabilities and entropies.
+__global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_both_kernel(JoinArgs a) {
+  __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32], su[kJoinWarps][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  wait_prior_kernel();
+  const int rows = a.head->rows;
+  const int row = blockIdx.x * 32 + lane;
+  const float c = a.inv_t * kLog2e;
+  float m = -CUDART_INF_F, s = 0.0f, u = 0.0f;
+  if (row < rows) {
+#pragma unroll 4
+    for (int t = w; t < a.ntiles; t += kJoinWarps) {
+      float2 p = a.part[(int64_t)t * a.Bp + row];
+      float pu = a.part_t[(int64_t)t * a.Bp + row];
+      const float to = max_nan(m, p.x);
+      if (to == -CUDART_INF_F) continue;
+      if (m != -CUDART_INF_F) raise_sums(m, to, c, &s, &u);
+      if (p.x != -CUDART_INF_F) {
+        raise_sums(p.x, to, c, &p.y, &pu);
+        s += p.y;
+        u += pu;
+      }
+      m = to;
+    }
+  }
+  sm[w][lane] = m;
+  ss[w][lane] = s;
+  su[w][lane] = u;
+  __syncthreads();
+  if (w != 0 || row >= rows) return;
+  float M = sm[0][lane];
+#pragma unroll
+  for (int i = 1; i < kJoinWarps; ++i) M = max_nan(M, sm[i][lane]);
+  float S = 0.0f, U = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < kJoinWarps; ++i) {
+    if (sm[i][lane] == -CUDART_INF_F) continue;
+    s = ss[i][lane], u = su[i][lane];
+    raise_sums(sm[i][lane], M, c, &s, &u);
+    S += s;
+    U += u;
+  }
+  const bool label = a.label[row] >= 0, ok = label && a.head->status == 0 && fabsf(M) < CUDART_INF_F;
+  if (lane == 0 && a.head->status != 0) raise_status(a.status, a.head->status);
+  if (label && !(fabsf(M) < CUDART_INF_F)) raise_status(a.status, FWB_STATUS_NONFINITE);
+  const float log_s = logf(S), nan = CUDART_NAN_F;
+  const int to = a.row_of[row];
+  const float h = ok ? log_s - U * kLn2 / S : nan;
+  a.lse[row] = ok ? fmaf(M, a.inv_t, log_s) : nan;
+  a.entropy_pack[row] = h;
+  a.entropy[to] = h;
+  a.loss[to] = ok ? (a.zy[row] - M) * a.inv_t - log_s : nan;
+}
 
 // 32 rows per CTA, the tiles' pairs split over its warps; the last CTA to
 // finish adds the losses in a fixed order.
@@ -361,35 +452,51 @@ struct Upstream {
   const float* go;   // one per given row, or one
   const float* top;  // largest finite s_r of a live row (float16, factors per row)
   int per_row, mean, f16;
+  int both;             // go is logp's, either may be NULL
+  const float* go_ent;  // the entropy's
+  float inv_t;
 
+  // g_r
+  __device__ float factor(int r) const {
+    return both ? max_nan(go ? fabsf(go[r]) : 0.0f, go_ent ? fabsf(go_ent[r]) : 0.0f) : go[r];
+  }
+  __device__ float unit() const { return both ? kF16UnitBoth : kF16Unit; }
   // s_r, scaled to the range of the type; a factor that is not finite stands for itself
   __device__ float in_g(int r) const {
     if (!per_row) return f16 ? kF16Unit : 1.0f;
-    const float g = go[r], s = pow2_above(g);
+    const float g = factor(r), s = pow2_above(g);
     if (!(s < CUDART_INF_F)) return g;
-    return f16 && *top > 0.0f ? s / *top * kF16Unit : s;
+    return f16 && *top > 0.0f ? s / *top * unit() : s;
+  }
+  // -a_r / g_r and -b_r / g_r; NaN where g_r is not finite
+  __device__ float2 shares(int r) const {
+    const float g = factor(r);
+    if (g == 0.0f) return make_float2(0.0f, 0.0f);
+    if (!(g < CUDART_INF_F)) return make_float2(CUDART_NAN_F, CUDART_NAN_F);
+    return make_float2(go ? -go[r] / g : 0.0f, go_ent ? -go_ent[r] / g : 0.0f);
   }
   // f_r; 1 where the factor is in G (0, not finite) or common
   __device__ float rest(int r) const {
     if (!per_row) return 1.0f;
-    const float g = go[r], s = pow2_above(g);
+    const float g = factor(r), s = pow2_above(g);
     return s > 0.0f && s < CUDART_INF_F ? g / s : 1.0f;
   }
   // common factor taken out after the sums
   __device__ float back(const XentHead* h) const {
+    if (both) return f16 && *top > 0.0f ? *top / kF16UnitBoth * inv_t : inv_t;
     if (per_row) return f16 && *top > 0.0f ? *top / kF16Unit : 1.0f;
     const float g = mean ? go[0] / (float)h->rows : go[0];
     return f16 ? g / kF16Unit : g;
   }
 };
 
-__global__ void __launch_bounds__(1024) fw_xent_top_kernel(const XentHead* head, const int32_t* row_of, const float* go,
+__global__ void __launch_bounds__(1024) fw_xent_top_kernel(const XentHead* head, const int32_t* row_of, Upstream up,
                                                              float* out) {
   __shared__ float red[32];
   const int rows = head->rows;
   float top = 0.0f;
   for (int i = threadIdx.x; i < rows; i += 1024) {
-    const float s = pow2_above(go[row_of[i]]);
+    const float s = pow2_above(up.factor(row_of[i]));
     if (s < CUDART_INF_F) top = fmaxf(top, s);
   }
 #pragma unroll
@@ -432,14 +539,17 @@ struct GradArgs {
   int V, D;
   int v0, vn;  // first column of the piece, its columns rounded up to 256
   int32_t* status;
+  const float* entropy;  // BOTH: packed
 };
 
-template <class T, TcKind K>
+template <class T, TcKind K, bool BOTH>
 struct GradTile {
   using Args = GradArgs;
   struct State {
     float lse, coef;
     int y;
+    float h;        // BOTH: the row's entropy,
+    float2 shares;  // its factors over g_r
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
@@ -462,6 +572,10 @@ struct GradTile {
     st.y = live ? a.label[row] : -2;  // -2: not a live row
     st.lse = live ? a.lse[row] : 0.0f;
     st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
+    if constexpr (BOTH) {
+      st.h = live ? a.entropy[row] : 0.0f;
+      st.shares = live ? a.up.shares(a.row_of[row]) : make_float2(0.0f, 0.0f);
+    }
   }
   template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
@@ -477,8 +591,17 @@ struct GradTile {
       const int valid = live ? min(32, a.V - (t.n0 + c)) : 0;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        float q = LOST ? CUDART_NAN_F : exp2_hw((v[i] - lse) * kLog2e);
-        if (t.n0 + c + i == y) q -= 1.0f;
+        float q;
+        if constexpr (LOST) {
+          q = CUDART_NAN_F;
+        } else if constexpr (BOTH) {  // of a bad row lse and h are NaN, and so is q
+          const float l = fmaxf(fmaf(v[i], a.up.inv_t, -lse), kExpFloor * kLn2), p = exp2_hw(l * kLog2e);
+          q = p * fmaf(st.shares.y, l + st.h, st.shares.x);
+          if (t.n0 + c + i == y) q -= st.shares.x;
+        } else {
+          q = exp2_hw((v[i] - lse) * kLog2e);
+          if (t.n0 + c + i == y) q -= 1.0f;
+        }
         v[i] = i < valid ? q * coef : 0.0f;
       }
 #pragma unroll
@@ -708,14 +831,14 @@ struct XentPlan {
   int64_t Bp, Dp;
   bool copy_w;
   // state: what backward needs
-  int64_t row_of, label, lse, hp, wp, state_bytes;
+  int64_t row_of, label, lse, entropy, hp, wp, state_bytes;
   // forward workspace
-  int64_t part, zy, loss_pack, fwd_bytes;
+  int64_t part, part_t, zy, loss_pack, fwd_bytes;
   // backward workspace
   int64_t piece, pieces, splits, top, g, sum, hs, bwd_bytes;
 };
 
-XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
+XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = false) {
   XentPlan p = {};
   p.Bp = up(B, 256);
   p.Dp = up(D, 8);
@@ -724,11 +847,13 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w) {
   p.row_of = at, at += up(4 * p.Bp, 256);
   p.label = at, at += up(4 * p.Bp, 256);
   p.lse = at, at += up(4 * p.Bp, 256);
+  p.entropy = at, at += both ? up(4 * p.Bp, 256) : 0;
   p.hp = at, at += up(2 * p.Bp * p.Dp, 256);
   p.wp = at, at += copy_w ? up(2 * V * p.Dp, 256) : 0;
   p.state_bytes = at;
   at = 0;
   p.part = at, at += up(8 * p.Bp * up(V, kTileN) / kLseCols, 256);
+  p.part_t = at, at += both ? up(4 * p.Bp * up(V, kTileN) / kLseCols, 256) : 0;
   p.zy = at, at += up(4 * p.Bp, 256);
   p.loss_pack = at, at += up(4 * p.Bp, 256);
   p.fwd_bytes = at;
@@ -762,17 +887,19 @@ int xent_check(int dtype, int64_t B, int64_t D, int64_t V) {
 // Rows that a TMA tile load can read in place.
 bool tma_rows(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
 
-template <class T, TcKind K>
+// BOTH: log probabilities in the place of losses, FWB_REDUCE_NONE.
+template <class T, TcKind K, bool BOTH>
 int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* y, int64_t B,
-                int64_t D, int64_t V, int64_t ignore, int reduction, float* loss, char* state, char* ws,
-                int32_t* status, cudaStream_t st) {
-  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+                int64_t D, int64_t V, int64_t ignore, int reduction, float* loss, float* entropy, float inv_t,
+                char* state, char* ws, int32_t* status, cudaStream_t st) {
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw), BOTH);
   XentHead* head = reinterpret_cast<XentHead*>(state);
   int32_t* row_of = reinterpret_cast<int32_t*>(state + p.row_of);
   int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
   const int64_t per_cta = (p.Bp + 4 * sm_count() - 1) / (4 * sm_count());
   PackArgs pk = {hidden, y, B, p.Bp, D, p.Dp, ldh, V, ignore, state + p.hp, row_of, label,
-                 reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, (int)(per_cta < 8 ? 8 : per_cta)};
+                 reduction == FWB_REDUCE_NONE ? loss : nullptr, BOTH ? entropy : nullptr, head, status,
+                 (int)(per_cta < 8 ? 8 : per_cta)};
   if (launch_dependent(fw_xent_pack_kernel<T>, (p.Bp + pk.per_cta - 1) / pk.per_cta, kPackThreads, 0, 1, st, pk) !=
       cudaSuccess)
     return FWB_E_LAUNCH;
@@ -788,28 +915,30 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   CUtensorMap mh, mw;
   if (!tc_map(&mh, K, state + p.hp, p.Bp, D, p.Dp, 128) || !tc_map(&mw, K, w, V, D, ldw, 128)) return FWB_E_LAUNCH;
   LseArgs la = {head, label, reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.zy), p.Bp, (int)V,
-                (int)D, &head->status};
+                (int)D, &head->status, reinterpret_cast<float*>(ws + p.part_t), inv_t * kLog2e};
   const int64_t nt = (V + 255) / 256;
-  if (launch_gemm<LseTile<K>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
+  if (launch_gemm<LseTile<K, BOTH>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
   JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
-                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + kLseCols - 1) / kLseCols), reduction, status};
-  return launch_status(launch_dependent(fw_xent_join_kernel, p.Bp / 32, kJoinWarps * 32, 0, 1, st, ja));
+                 reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + kLseCols - 1) / kLseCols), reduction, status,
+                 la.part_t, entropy, reinterpret_cast<float*>(state + p.entropy), inv_t};
+  return launch_status(launch_dependent(BOTH ? fw_xent_join_both_kernel : fw_xent_join_kernel, p.Bp / 32, kJoinWarps * 32, 0, 1, st, ja));
 }
 
-template <class T, TcKind K>
+template <class T, TcKind K, bool BOTH>
 int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int mean, const float* go,
-                 int per_row, const char* state, char* ws, void* dhidden, void* dweight, int32_t* status, cudaStream_t st) {
-  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw));
+                 const float* go_ent, float inv_t, int per_row, const char* state, char* ws, void* dhidden, void* dweight,
+                 int32_t* status, cudaStream_t st) {
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw), BOTH);
   const XentHead* head = reinterpret_cast<const XentHead*>(state);
   const int32_t* row_of = reinterpret_cast<const int32_t*>(state + p.row_of);
   const int32_t* label = reinterpret_cast<const int32_t*>(state + p.label);
   const void* w = p.copy_w ? state + p.wp : weight;
   if (p.copy_w) ldw = p.Dp;
   float* top = reinterpret_cast<float*>(ws + p.top);
-  const Upstream u = {go, top, per_row, mean, K == kTcF16};
+  const Upstream u = {go, top, per_row, mean, K == kTcF16, BOTH, go_ent, inv_t};
   const char* hw = state + p.hp;  // dW's operand
   if (per_row) {
-    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, go, top);
+    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, u, top);
     if (dweight) {
       T* hs = reinterpret_cast<T*>(ws + p.hs);
       const int64_t cap = (int64_t)sm_count() * 8;
@@ -831,8 +960,8 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
     const GradArgs ga = {head, label, row_of, reinterpret_cast<const float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
-                         v0, vn, status};
-    if (launch_gemm<GradTile<T, K>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
+                         v0, vn, status, reinterpret_cast<const float*>(state + p.entropy)};
+    if (launch_gemm<GradTile<T, K, BOTH>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
     const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
     const int64_t pairs = sm_count() / 2;
     const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
@@ -888,10 +1017,11 @@ int fw_xent_forward(int dtype, const void* hidden, int64_t ldh, const void* weig
   }
   char* s = static_cast<char*>(state);
   char* w = static_cast<char*>(workspace);
-  return dtype == FWB_DTYPE_BF16 ? run_forward<__nv_bfloat16, kTcBf16>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index,
-                                                                       reduction, loss, s, w, status, st)
-                                 : run_forward<__half, kTcF16>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index,
-                                                               reduction, loss, s, w, status, st);
+  return dtype == FWB_DTYPE_BF16
+             ? run_forward<__nv_bfloat16, kTcBf16, false>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index, reduction,
+                                                          loss, nullptr, 1.0f, s, w, status, st)
+             : run_forward<__half, kTcF16, false>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index, reduction, loss,
+                                                  nullptr, 1.0f, s, w, status, st);
 }
 
 int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, int reduction,
@@ -916,10 +1046,73 @@ int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int6
   char* w = static_cast<char*>(workspace);
   const int per_row = reduction == FWB_REDUCE_NONE, mean = reduction == FWB_REDUCE_MEAN;
   return dtype == FWB_DTYPE_BF16
-             ? run_backward<__nv_bfloat16, kTcBf16>(weight, ldw, B, D, V, mean, grad_output, per_row, s, w, dhidden,
-                                                    dweight, status, st)
-             : run_backward<__half, kTcF16>(weight, ldw, B, D, V, mean, grad_output, per_row, s, w, dhidden, dweight,
-                                            status, st);
+             ? run_backward<__nv_bfloat16, kTcBf16, false>(weight, ldw, B, D, V, mean, grad_output, nullptr, 1.0f, per_row,
+                                                           s, w, dhidden, dweight, status, st)
+             : run_backward<__half, kTcF16, false>(weight, ldw, B, D, V, mean, grad_output, nullptr, 1.0f, per_row, s, w,
+                                                   dhidden, dweight, status, st);
+}
+
+int64_t fw_lm_head_log_probs_state(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw) {
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
+  return xent_plan(B, D, V, !tma_rows(weight, ldw), true).state_bytes;
+}
+
+int64_t fw_lm_head_log_probs_workspace(int64_t B, int64_t D, int64_t V, int backward) {
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
+  const XentPlan p = xent_plan(B, D, V, false, true);
+  return backward ? p.bwd_bytes : p.fwd_bytes;
+}
+
+int fw_lm_head_log_probs(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw, const int64_t* y,
+                         int64_t B, int64_t D, int64_t V, float inv_t, int64_t ignore_index, float* logp, float* entropy,
+                         void* state, int64_t state_bytes, void* workspace, int64_t workspace_bytes, int32_t* status,
+                         void* stream) {
+  if (int rc = xent_check(dtype, B, D, V)) return rc;
+  if (ldh < D || ldw < D || ldh > ((int64_t)1 << 38) || ldw > ((int64_t)1 << 38)) return FWB_E_SHAPE;
+  if (!(inv_t > 0.0f) || !std::isfinite(inv_t)) return FWB_E_SHAPE;
+  if (!weight || !state || !workspace) return FWB_E_POINTER;
+  if (B > 0 && (!hidden || !y || !logp || !entropy)) return FWB_E_POINTER;
+  if (reinterpret_cast<uintptr_t>(hidden) % 2 || reinterpret_cast<uintptr_t>(weight) % 2 || !aligned16(state) ||
+      !aligned16(workspace))
+    return FWB_E_POINTER;
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw), true);
+  if (state_bytes < p.state_bytes || workspace_bytes < p.fwd_bytes) return FWB_E_CAPACITY;
+  if (B == 0) return FWB_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  char* s = static_cast<char*>(state);
+  char* w = static_cast<char*>(workspace);
+  return dtype == FWB_DTYPE_BF16
+             ? run_forward<__nv_bfloat16, kTcBf16, true>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index,
+                                                         FWB_REDUCE_NONE, logp, entropy, inv_t, s, w, status, st)
+             : run_forward<__half, kTcF16, true>(hidden, ldh, weight, ldw, y, B, D, V, ignore_index, FWB_REDUCE_NONE,
+                                                 logp, entropy, inv_t, s, w, status, st);
+}
+
+int fw_lm_head_log_probs_grad(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t V, float inv_t,
+                              const float* dlogp, const float* dentropy, const void* state, int64_t state_bytes,
+                              void* workspace, int64_t workspace_bytes, void* dhidden, void* dweight, int32_t* status,
+                              void* stream) {
+  if (int rc = xent_check(dtype, B, D, V)) return rc;
+  if (ldw < D || ldw > ((int64_t)1 << 38) || !(inv_t > 0.0f) || !std::isfinite(inv_t)) return FWB_E_SHAPE;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (B == 0) {
+    if (dweight && cudaMemsetAsync(dweight, 0, (size_t)(2 * V * D), st) != cudaSuccess) return FWB_E_LAUNCH;
+    return FWB_OK;
+  }
+  if (!weight || !state || !workspace) return FWB_E_POINTER;
+  if (reinterpret_cast<uintptr_t>(weight) % 2 || reinterpret_cast<uintptr_t>(dhidden) % 2 ||
+      reinterpret_cast<uintptr_t>(dweight) % 2 || !aligned16(state) || !aligned16(workspace))
+    return FWB_E_POINTER;
+  const XentPlan p = xent_plan(B, D, V, !tma_rows(weight, ldw), true);
+  if (state_bytes < p.state_bytes || workspace_bytes < p.bwd_bytes) return FWB_E_CAPACITY;
+  if (!dhidden && !dweight) return FWB_OK;
+  const char* s = static_cast<const char*>(state);
+  char* w = static_cast<char*>(workspace);
+  return dtype == FWB_DTYPE_BF16
+             ? run_backward<__nv_bfloat16, kTcBf16, true>(weight, ldw, B, D, V, 0, dlogp, dentropy, inv_t, 1, s, w,
+                                                          dhidden, dweight, status, st)
+             : run_backward<__half, kTcF16, true>(weight, ldw, B, D, V, 0, dlogp, dentropy, inv_t, 1, s, w, dhidden,
+                                                  dweight, status, st);
 }
 
 }  // extern "C"

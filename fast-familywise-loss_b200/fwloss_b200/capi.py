@@ -95,6 +95,12 @@ _SIGS["fw_xent_backward"] = ([_C_INT, _P, _I64, _I64, _I64, _I64, _C_INT, _P, _P
                              _C_INT)
 _SIGS["fw_token_log_probs"] = ([_C_INT, _P, _I64, _P, _I64, _I64, _F32, _I64, _C_INT, _P, _P, _P, _P, _P, _P, _P], _C_INT)
 _SIGS["fw_token_log_probs_grad"] = ([_C_INT, _P, _I64, _I64, _I64, _F32, _P, _P, _P, _P, _I64, _P], _C_INT)
+_SIGS["fw_lm_head_log_probs_state"] = ([_I64, _I64, _I64, _P, _I64], _I64)
+_SIGS["fw_lm_head_log_probs_workspace"] = ([_I64, _I64, _I64, _C_INT], _I64)
+_SIGS["fw_lm_head_log_probs"] = ([_C_INT, _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _F32, _I64, _P, _P, _P, _I64, _P, _I64,
+                                  _P, _P], _C_INT)
+_SIGS["fw_lm_head_log_probs_grad"] = ([_C_INT, _P, _I64, _I64, _I64, _I64, _F32, _P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P],
+                                      _C_INT)
 _SIGS["fw_grad_norm_workspace"] = ([_I64], _I64)
 _SIGS["fw_grad_norm"] = ([_I64, _P, _P, _P, _P, _I64, _P, _P, _P], _C_INT)
 _SIGS["fw_grad_clip"] = ([_I64, _P, _P, _P, _P, _P, _F32, _P, _P, _I64, _P, _P, _P], _C_INT)

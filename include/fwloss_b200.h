@@ -601,6 +601,30 @@ FWB_API int fw_token_log_probs_grad(int dtype, const void* logits, int64_t ld, i
                                     const float* dentropy, void* grad, int64_t ldg, void* stream);
 
 /*
+ * Log probabilities and entropies (fp32 [B]) of logits = hidden [B, D] x
+ * weight [V, D]^T at a temperature T, inv_t = 1 / T, without storing the
+ * logits: what fw_token_log_probs gives for them, with its rules for
+ * ignore_index, tokens out of range and rows that are not finite, and with the
+ * operands, state and workspaces of fw_xent_forward.
+ * fw_lm_head_log_probs_grad writes dhidden [B, D] and dweight [V, D]
+ * (contiguous, either may be NULL) for the upstream gradients dlogp and
+ * dentropy (fp32 [B]; NULL: none); a factor that is not finite makes its row of
+ * dhidden and all of dweight NaN.
+ */
+FWB_API int64_t fw_lm_head_log_probs_state(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw);
+FWB_API int64_t fw_lm_head_log_probs_workspace(int64_t B, int64_t D, int64_t V, int backward);
+FWB_API int fw_lm_head_log_probs(int dtype, const void* hidden, int64_t ldh, const void* weight, int64_t ldw,
+                                 const int64_t* y, int64_t B, int64_t D, int64_t V, float inv_t,
+                                 int64_t ignore_index, float* logp, float* entropy, void* state,
+                                 int64_t state_bytes, void* workspace, int64_t workspace_bytes,
+                                 int32_t* status, void* stream);
+FWB_API int fw_lm_head_log_probs_grad(int dtype, const void* weight, int64_t ldw, int64_t B, int64_t D,
+                                      int64_t V, float inv_t, const float* dlogp, const float* dentropy,
+                                      const void* state, int64_t state_bytes, void* workspace,
+                                      int64_t workspace_bytes, void* dhidden, void* dweight,
+                                      int32_t* status, void* stream);
+
+/*
  * Global norm of n tensors, norm = sqrt(sum of all elements' squares), and the
  * tensors scaled to it, out[i] = grads[i] * min(1, max_norm / norm).  grads,
  * out, numel, dtypes and out_dtypes are host arrays of n entries; a tensor is
