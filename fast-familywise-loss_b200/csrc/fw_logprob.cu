@@ -20,10 +20,14 @@
 // whole warps, and the elements that reach the bound are ranked.  Elements are
 // ordered by 64-bit keys (value, then lowest column first), all different, so
 // ties need no case of their own.
+#include <cooperative_groups.h>
+
 #include <cmath>
 
 #include "fw_host.cuh"
 #include "fw_rowslots.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace fwb200 {
 namespace {
@@ -97,6 +101,30 @@ __device__ __forceinline__ uint4 load_slot_row(const T* row, int e0, int V) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Sums of a thread, kept relative to its running maximum.
+template <class T>
+struct Running {
+  Sums q;
+  __device__ __forceinline__ Running() { q = {-CUDART_INF_F, 0.0f, 0.0f}; }
+  __device__ __forceinline__ void raise(float to, float c) { q.raise(to, c); }
+  template <int N>
+  __device__ __forceinline__ void add(const uint4 (&x)[N], float c) {
+    constexpr int VN = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float z[VN];
+      unpack16<T>(x[i], z);
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const float t = fmaxf((z[j] - q.m) * c, kFloor), e = exp2_ftz(t);
+        q.s += e;
+        q.u = fmaf(e, t, q.u);
+      }
+    }
+  }
+  __device__ __forceinline__ Sums result(float) const { return q; }
+};
+
 // Descending over the lanes.
 __device__ __forceinline__ uint64_t warp_sort(uint64_t x, int lane) {
 #pragma unroll
@@ -122,48 +150,161 @@ __device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b, int lane)
   return x;
 }
 
+constexpr int kFound = 256;  // keys that reach the bound, before the slower way is taken
+
 template <int NW>
 struct TopShared {
-  uint64_t first[NW * 32];  // each thread's largest key
-  uint64_t held[NW][64];    // keys that reach the bound, per warp
-  uint64_t best[32];        // the CTA's largest, descending
+  static constexpr int NT = NW * 32, NG = NT < 64 ? NT : 64;  // threads; groups of NT / NG neighbours
+  uint64_t first[NT];     // each thread's largest key, 0 without elements
+  uint64_t group[NG];     // the largest of each group
+  uint64_t found[kFound];
+  uint64_t held[NW][64];  // the slower way: keys that reach the bound, per warp
+  uint64_t best[32];      // the CTA's k largest, descending, 0 where there are fewer
   uint64_t bound;
-  int count[NW];
+  int count[NW], n, n_who;
+  uint16_t who[NT];       // threads whose largest key reaches the bound
 };
 
-// Largest bound that at least k of the keys reach, to the point where no more
-// than 2 k do; 0 if there are fewer than k.  One warp.
-template <int NT>
-__device__ __forceinline__ uint64_t top_bound(const uint64_t* keys, int k, int lane) {
-  uint64_t mine[NT / 32], t = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) mine[i] = keys[i * 32 + lane];
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t up = t | (1ull << bit);
-    int n = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) n += mine[i] >= up;
-    n = __reduce_add_sync(kFull, n);
-    if (n < k) continue;
-    t = up;
-    if (n <= 2 * k) break;
+// A CTA's part of a row: slots [k0, k1), of which [lo, hi) are whole.
+template <class T>
+struct Segment {
+  const T* row;
+  int off, V, k0, k1, lo, hi;
+  __device__ __forceinline__ int element(int k) const { return k * (16 / (int)sizeof(T)) - off; }
+  __device__ __forceinline__ uint4 load(int k) const {
+    return k >= lo && k < hi ? ld_global16_once(row + element(k)) : load_slot_row(row, element(k), V);
   }
-  return t;
+};
+
+// The bound: the k-th largest of the groups' keys (0 if there are not so many),
+// which k different elements reach.  top.bound is 0 before.
+template <int NW>
+__device__ __forceinline__ void top_bound(TopShared<NW>& top, int k) {
+  using S = TopShared<NW>;
+  constexpr int P = S::NT / S::NG, M = S::NG / P;  // threads per key, keys each compares with
+  const int mine = threadIdx.x / P, from = (threadIdx.x % P) * M;
+  const uint64_t own = top.group[mine];
+  int rank = 0;
+#pragma unroll
+  for (int i = 0; i < M; ++i) rank += top.group[from + i] > own;
+#pragma unroll
+  for (int o = 1; o < P; o <<= 1) rank += __shfl_xor_sync(kFull, rank, o);
+  if (rank == k - 1) top.bound = own;  // without elements (0) several may write the same
 }
 
-// One row per CTA of NW warps.
-template <class T, int NW, bool TOP>
-__global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 16) fw_logprob_kernel(ScoreArgs a) {
+// Leaves the k largest keys of the segment in top.best.  top.first and the
+// bound are there; top.n and top.n_who are 0.
+template <class T, int NW>
+__device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg, int k) {
+  constexpr int VN = 16 / sizeof(T), NT = NW * 32;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const uint64_t bound = top.bound, first = top.first[tid];
+  const bool in = first != 0 && first >= bound;
+  const uint32_t all = __ballot_sync(kFull, in);
+  int base = 0;
+  if (lane == 0 && all) base = atomicAdd(&top.n_who, __popc(all));
+  base = __shfl_sync(kFull, base, 0);
+  if (in) top.who[base + __popc(all & ((1u << lane) - 1u))] = (uint16_t)tid;
+  if (tid < 32) top.best[tid] = 0;
+  __syncthreads();
+  const int each = (seg.k1 - seg.k0 + NT - 1) / NT, work = top.n_who * each;
+  for (int i0 = tid; i0 < work; i0 += 2 * NT) {
+    uint4 x[2];
+    int e0[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int i = i0 + b * NT, t = i / each, kk = i < work ? seg.k0 + top.who[t] + (i - t * each) * NT : seg.k1;
+      x[b] = kk < seg.k1 ? seg.load(kk) : neg_inf_slot<T>();
+      e0[b] = kk < seg.k1 ? seg.element(kk) : seg.V;
+    }
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      float z[VN];
+      unpack16<T>(x[b], z);
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const int e = e0[b] + j;
+        const uint64_t key = rank_key(z[j], e);
+        if (key >= bound && e >= 0 && e < seg.V) {
+          const int at = atomicAdd(&top.n, 1);
+          if (at < kFound) top.found[at] = key;
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = top.n;
+  if (n <= kFound) {
+    for (int i = tid; i < n; i += NT) {
+      const uint64_t own = top.found[i];
+      int rank = 0;
+      for (int o = 0; o < n; ++o) rank += top.found[o] > own;
+      if (rank < k) top.best[rank] = own;
+    }
+    __syncthreads();
+    return;
+  }
+  // The slower way, for rows whose largest elements lie with few threads: each warp keeps the 32 largest of what it
+  // has seen in order, one per lane, and raises its own bound by them.
+  uint64_t mine = bound, list = 0;
+  uint64_t* held = top.held[w];
+  int have = 0;  // keys in the buffer
+  const auto drain = [&] {
+    __syncwarp();
+    uint64_t x = lane < have ? held[lane] : 0;
+    list = warp_merge(list, warp_sort(x, lane), lane);
+    if (lane + 32 < have) x = held[lane + 32];
+    __syncwarp();
+    if (lane + 32 < have) held[lane] = x;
+    have = max(have - 32, 0);
+    const uint64_t kth = __shfl_sync(kFull, list, k - 1);
+    mine = kth > mine ? kth : mine;
+    __syncwarp();
+  };
+  for (int t = w; t < top.n_who; t += NW) {
+    for (int k0 = seg.k0 + top.who[t]; k0 < seg.k1; k0 += NT * 32) {
+      const int kk = k0 + lane * NT;
+      float z[VN];
+      unpack16<T>(kk < seg.k1 ? seg.load(kk) : neg_inf_slot<T>(), z);
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const int e = seg.element(kk) + j;
+        const uint64_t key = rank_key(z[j], e);
+        const bool reaches = kk < seg.k1 && e >= 0 && e < seg.V && key >= mine;
+        const uint32_t who = __ballot_sync(kFull, reaches);
+        if (!who) continue;
+        if (reaches) held[have + __popc(who & ((1u << lane) - 1u))] = key;
+        have += __popc(who);
+        if (have > 32) drain();
+      }
+    }
+  }
+  drain();
+  held[lane] = list;
+  __syncthreads();
+  const uint64_t own = held[lane];
+  int rank = 0;
+  for (int g = 0; g < NW; ++g)
+    for (int i = 0; i < 32; ++i) rank += top.held[g][i] > own;
+  if (own != 0 && rank < k) top.best[rank] = own;
+  __syncthreads();
+}
+
+// One row per cluster of CL CTAs of NW warps, each taking an equal part of it.
+template <class T, int NW, bool TOP, int CL>
+__global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_logprob_kernel(ScoreArgs a) {
   constexpr int VN = 16 / sizeof(T), NT = NW * 32;
   __shared__ Sums part[NW];
-  __shared__ float2 row_stat;
+  __shared__ Sums whole;  // of this CTA
   __shared__ TopShared<TOP ? NW : 1> top;
   wait_prior_kernel();
   allow_dependent_launch();
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int64_t r = blockIdx.x;
+  const int64_t r = blockIdx.x / CL;
+  const int rank = CL > 1 ? (int)(blockIdx.x % CL) : 0;
   const int64_t y = a.y[r];
   if (y == a.ignore) {
+    if (rank != 0) return;
     if (tid == 0) {
       a.logp[r] = 0.0f;
       a.entropy[r] = 0.0f;
@@ -176,22 +317,28 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 16) fw_lo
     return;
   }
   const T* row = static_cast<const T*>(a.z) + r * a.ld;
-  const int V = a.V;
-  const int off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
-  const int slots = (int)(((int64_t)off + V + VN - 1) / VN);
-  const int lo = off ? 1 : 0, hi = (int)(((int64_t)off + V) / VN);  // whole slots
+  const bool label = y >= 0 && y < a.V;
+  const float zy = tid == 0 && label ? Elem<T>::to_f(row[y]) : 0.0f;
+  Segment<T> seg;
+  seg.row = row;
+  seg.V = a.V;
+  seg.off = (int)((reinterpret_cast<uintptr_t>(row) & 15u) / sizeof(T));
+  const int slots = (int)(((int64_t)seg.off + a.V + VN - 1) / VN);
+  seg.k0 = (int)((int64_t)slots * rank / CL);
+  seg.k1 = (int)((int64_t)slots * (rank + 1) / CL);
+  seg.lo = seg.off ? 1 : 0;
+  seg.hi = (int)(((int64_t)seg.off + a.V) / VN);
   const float c = a.inv_t * kLog2e;
-  Sums q = {-CUDART_INF_F, 0.0f, 0.0f};
-  int at = tid;  // slot where the maximum first stood
-  for (int k0 = tid; k0 < slots; k0 += NT * kBatch) {
+  Running<T> run;
+  int at = seg.k0 + tid;  // slot where the maximum first stood
+  for (int k0 = seg.k0 + tid; k0 < seg.k1; k0 += NT * kBatch) {
     uint4 x[kBatch];
-    if (k0 >= lo && k0 + (kBatch - 1) * NT < hi) {
+    if (k0 >= seg.lo && k0 + (kBatch - 1) * NT < min(seg.hi, seg.k1)) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) x[i] = ld_global16_once(row + ((k0 + i * NT) * VN - off));
+      for (int i = 0; i < kBatch; ++i) x[i] = ld_global16_once(row + seg.element(k0 + i * NT));
     } else {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i)
-        x[i] = k0 + i * NT < slots ? load_slot_row(row, (k0 + i * NT) * VN - off, V) : neg_inf_slot<T>();
+      for (int i = 0; i < kBatch; ++i) x[i] = k0 + i * NT < seg.k1 ? seg.load(k0 + i * NT) : neg_inf_slot<T>();
     }
     float sm[kBatch], bm = -CUDART_INF_F;
 #pragma unroll
@@ -199,137 +346,125 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 16) fw_lo
       sm[i] = slot_max_nan<T>(x[i]);
       bm = max_nan(bm, sm[i]);
     }
-    if (!(bm <= q.m)) {
-      const float to = max_nan(q.m, bm);
-      q.raise(to, c);
+    if (!(bm <= run.q.m)) {
+      const float to = max_nan(run.q.m, bm);
+      run.raise(to, c);
       if (TOP) {
 #pragma unroll
         for (int i = kBatch - 1; i >= 0; --i)
           if (sm[i] == to) at = k0 + i * NT;
       }
     }
-    if (q.m == -CUDART_INF_F) continue;
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      float z[VN];
-      unpack16<T>(x[i], z);
-#pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const float t = fmaxf((z[j] - q.m) * c, kFloor), e = exp2_ftz(t);
-        q.s += e;
-        q.u = fmaf(e, t, q.u);
-      }
-    }
+    if (run.q.m != -CUDART_INF_F) run.add(x, c);
   }
-  if constexpr (TOP) {
-    uint64_t first = 0;  // a thread without elements
-    if (tid < slots) {
-      float z[VN];
-      const int e0 = at * VN - off;
-      unpack16<T>(load_slot_row(row, e0, V), z);
-#pragma unroll
-      for (int j = VN - 1; j >= 0; --j)
-        if (z[j] == q.m && e0 + j >= 0 && e0 + j < V) first = rank_key(z[j], e0 + j);
-    }
-    top.first[tid] = first;
-  }
+  uint4 x_at = make_uint4(0u, 0u, 0u, 0u);
+  if (TOP && seg.k0 + tid < seg.k1) x_at = seg.load(at);  // used behind the sums
+  Sums q = run.result(c);
+  const float m_thread = q.m;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
     q.join(p, c);
   }
   if (lane == 0) part[w] = q;
-  __syncthreads();
-  if (tid == 0) {
-    for (int i = 1; i < NW; ++i) q.join(part[i], c);
-    const bool label = y >= 0 && y < V, finite = fabsf(q.m) < CUDART_INF_F;
-    const float nan = CUDART_NAN_F;
-    float m = nan, logs = nan, h = nan, logp = nan;
-    if (label && finite) {
-      m = q.m;
-      logs = logf(q.s);
-      h = logs - q.u * kLn2 / q.s;
-      logp = (Elem<T>::to_f(row[y]) - m) * a.inv_t - logs;
+  if constexpr (TOP) {
+    uint64_t first = 0;
+    if (seg.k0 + tid < seg.k1) {
+      float z[VN];
+      const int e0 = seg.element(at);
+      unpack16<T>(x_at, z);
+#pragma unroll
+      for (int j = VN - 1; j >= 0; --j)
+        if (z[j] == m_thread && e0 + j >= 0 && e0 + j < a.V) first = rank_key(z[j], e0 + j);
     }
+    top.first[tid] = first;
+#pragma unroll
+    for (int o = 1; o < NT / TopShared<NW>::NG; o <<= 1) {
+      const uint64_t other = __shfl_xor_sync(kFull, first, o);
+      first = other > first ? other : first;
+    }
+    top.group[tid / (NT / TopShared<NW>::NG)] = first;
+    if (tid == 0) {
+      top.bound = 0;
+      top.n = 0;
+      top.n_who = 0;
+    }
+  }
+  __syncthreads();
+  if (w == 0) {
+    q = lane < NW ? part[lane] : Sums{-CUDART_INF_F, 0.0f, 0.0f};
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) {
+      const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
+      q.join(p, c);
+    }
+    if (lane == 0) whole = q;
+  }
+  if constexpr (TOP) {
+    top_bound(top, a.k);
+    __syncthreads();
+    top_of<T, NW>(top, seg, a.k);
+  }
+  float m = CUDART_NAN_F, logs = CUDART_NAN_F, h = CUDART_NAN_F, logp = CUDART_NAN_F;
+  const auto finish = [&] {  // of the row, from q; one thread or several
+    if (!label || !(fabsf(q.m) < CUDART_INF_F)) return;
+    m = q.m;
+    logs = logf(q.s);
+    h = logs - q.u * kLn2 / q.s;
+    logp = (zy - m) * a.inv_t - logs;
+  };
+  const auto give = [&] {
     if (!label) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
-    if (!finite) raise_status(a.status, FWB_STATUS_NONFINITE);
+    if (!(fabsf(q.m) < CUDART_INF_F)) raise_status(a.status, FWB_STATUS_NONFINITE);
     a.logp[r] = logp;
     a.entropy[r] = h;
     if (a.state) a.state[r] = make_float4(m, logs, h, __int_as_float(label ? (int)y : -1));
-    row_stat = make_float2(m, logs);
-  }
-  if constexpr (TOP) {
-    if (w == NW - 1) {
-      const uint64_t b = top_bound<NT>(top.first, a.k, lane);
-      if (lane == 0) top.bound = b;
+  };
+  const auto give_top = [&](uint64_t key, int i) {
+    const bool bad = isnan(m);
+    a.top_logp[r * a.k + i] = bad ? CUDART_NAN_F : (key_value((uint32_t)(key >> 32)) - m) * a.inv_t - logs;
+    a.top_ids[r * a.k + i] = bad ? -1 : (int64_t)(uint32_t)~(uint32_t)key;
+  };
+  if constexpr (CL == 1) {
+    if (w == 0) {
+      if (TOP) q = whole;  // written by this warp, or before the barriers of top_of
+      finish();
+      if (tid == 0) give();
+      if (TOP && lane < a.k) give_top(top.best[lane], lane);
     }
-    __syncthreads();
-    // `list`: the warp's 32 largest so far, once its buffer has overflowed; they raise its own bound, not the
-    // one by which all warps share out the threads
-    const uint64_t common = top.bound;
-    uint64_t bound = common, list = 0;
-    uint64_t* held = top.held[w];
-    int n = 0;  // keys in the buffer
-    bool full = false;
-    const auto drain = [&] {
-      __syncwarp();
-      uint64_t x = lane < n ? held[lane] : 0;
-      list = warp_merge(list, warp_sort(x, lane), lane);
-      if (lane + 32 < n) x = held[lane + 32];
-      __syncwarp();
-      if (lane + 32 < n) held[lane] = x;
-      n = max(n - 32, 0);
-      full = true;
-      __syncwarp();
-    };
-    int turn = 0;
-    for (int g = 0; g < NW; ++g) {
-      const uint64_t f = top.first[g * 32 + lane];
-      // a bound of 0 stands for all of the row: threads without elements have none
-      uint32_t who = __ballot_sync(kFull, f >= common && f != 0);
-      for (; who; who &= who - 1) {
-        if (turn++ % NW != w) continue;
-        const int t = g * 32 + __ffs(who) - 1;
-        for (int k0 = t; k0 < slots; k0 += NT * 32) {
-          const int k = k0 + lane * NT;
-          float z[VN];
-          unpack16<T>(k < slots ? load_slot_row(row, k * VN - off, V) : neg_inf_slot<T>(), z);
+  } else {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (rank == 0) {
+      if (w == 0) {
+        q = lane < CL ? *cluster.map_shared_rank(&whole, lane % CL) : Sums{-CUDART_INF_F, 0.0f, 0.0f};
 #pragma unroll
-          for (int j = 0; j < VN; ++j) {
-            const int e = k * VN - off + j;
-            const uint64_t key = k < slots && e >= 0 && e < V ? rank_key(z[j], e) : 0;
-            const bool in = key != 0 && key >= bound;
-            const uint32_t all = __ballot_sync(kFull, in);
-            if (!all) continue;
-            if (in) held[n + __popc(all & ((1u << lane) - 1u))] = key;
-            n += __popc(all);
-            if (n > 32) {
-              drain();
-              const uint64_t kth = __shfl_sync(kFull, list, a.k - 1);
-              bound = kth > bound ? kth : bound;
-            }
-          }
+        for (int o = CL / 2; o > 0; o >>= 1) {
+          const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
+          q.join(p, c);
+        }
+        q = {__shfl_sync(kFull, q.m, 0), __shfl_sync(kFull, q.s, 0), __shfl_sync(kFull, q.u, 0)};
+        finish();
+        if (tid == 0) {
+          give();
+          part[0] = {m, logs, 0.0f};
         }
       }
+      if constexpr (TOP) {
+        static_assert(CL * 32 <= NT, "a key per thread");
+        uint64_t own = 0;
+        if (tid < CL * 32) own = cluster.map_shared_rank(&top, w)->best[lane];
+        if (tid < CL * 32) top.found[tid] = own;
+        __syncthreads();
+        m = part[0].m;
+        logs = part[0].s;
+        int i = 0;
+#pragma unroll 8
+        for (int o = 0; o < CL * 32; ++o) i += top.found[o] > own;
+        if (own != 0 && i < a.k) give_top(own, i);
+      }
     }
-    if (full) {
-      drain();
-      held[lane] = list;
-      n = __popc(__ballot_sync(kFull, list != 0));
-    }
-    if (lane == 0) top.count[w] = n;
-    __syncthreads();
-    const bool mine = lane < top.count[w];
-    const uint64_t own = mine ? held[lane] : 0;
-    int rank = 0;
-    for (int g = 0; g < NW; ++g)
-      for (int i = 0, ng = top.count[g]; i < ng; ++i) rank += top.held[g][i] > own;
-    if (mine && rank < a.k) {
-      const float2 st = row_stat;
-      const bool bad = isnan(st.x);
-      a.top_logp[r * a.k + rank] = bad ? CUDART_NAN_F : (key_value((uint32_t)(own >> 32)) - st.x) * a.inv_t - st.y;
-      a.top_ids[r * a.k + rank] = bad ? -1 : (int64_t)(uint32_t)~(uint32_t)own;
-    }
+    cluster.sync();  // rank 0 has read the others' shared memory
   }
 }
 
@@ -401,18 +536,23 @@ int score_check(int dtype, int64_t B, int64_t V, int64_t ld, float inv_t) {
 
 bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to != 0; }
 
-template <class T, int NW>
+template <class T, int NW, int CL>
 int launch_score(const ScoreArgs& a, cudaStream_t st) {
-  return launch_status(a.k > 0 ? launch_dependent(fw_logprob_kernel<T, NW, true>, a.B, NW * 32, 0, 1, st, a)
-                               : launch_dependent(fw_logprob_kernel<T, NW, false>, a.B, NW * 32, 0, 1, st, a));
+  return launch_status(a.k > 0
+                           ? launch_dependent(fw_logprob_kernel<T, NW, true, CL>, a.B * CL, NW * 32, 0, CL, st, a)
+                           : launch_dependent(fw_logprob_kernel<T, NW, false, CL>, a.B * CL, NW * 32, 0, CL, st, a));
 }
 
 template <class T>
 int run_score(const ScoreArgs& a, cudaStream_t st) {
-  const int slots = a.V / (16 / (int)sizeof(T));
-  if (slots <= 256) return launch_score<T, 1>(a, st);
-  if (slots <= 2048) return launch_score<T, 4>(a, st);
-  return launch_score<T, 8>(a, st);
+  const int64_t slots = a.V / (16 / (int)sizeof(T)), ctas = (int64_t)sm_count() * 4;
+  if (slots <= 256) return launch_score<T, 1, 1>(a, st);
+  // few long rows: in parts of at least 512 slots, as long as all parts run at once
+  if (slots >= 8 * 512 && a.B * 8 <= ctas) return launch_score<T, 8, 8>(a, st);
+  if (slots >= 4 * 512 && a.B * 4 <= ctas) return launch_score<T, 8, 4>(a, st);
+  if (slots >= 2 * 512 && a.B * 2 <= ctas) return launch_score<T, 8, 2>(a, st);
+  if (slots <= 2048) return launch_score<T, 4, 1>(a, st);
+  return launch_score<T, 8, 1>(a, st);
 }
 
 template <class T>
