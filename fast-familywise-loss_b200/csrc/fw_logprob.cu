@@ -67,12 +67,18 @@ struct Sums {
     }
     m = to;
   }
-  __device__ __forceinline__ void join(Sums o, float c) {
-    const float to = max_nan(m, o.m);
+  // Of every N neighbouring lanes, in all of them.
+  template <int N>
+  __device__ __forceinline__ void join_lanes(float c) {
+    float to = m;
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) to = max_nan(to, __shfl_xor_sync(kFull, to, o));
     raise(to, c);
-    o.raise(to, c);
-    s += o.s;
-    u += o.u;
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(kFull, s, o);
+      u += __shfl_xor_sync(kFull, u, o);
+    }
   }
 };
 
@@ -207,18 +213,20 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   if (in) top.who[base + __popc(all & ((1u << lane) - 1u))] = (uint16_t)tid;
   if (tid < 32) top.best[tid] = 0;
   __syncthreads();
+  const float least = bound ? key_value((uint32_t)(bound >> 32)) : -CUDART_INF_F;
   const int each = (seg.k1 - seg.k0 + NT - 1) / NT, work = top.n_who * each;
-  for (int i0 = tid; i0 < work; i0 += 2 * NT) {
-    uint4 x[2];
-    int e0[2];
+  for (int i0 = tid; i0 < work; i0 += kBatch * NT) {
+    uint4 x[kBatch];
+    int e0[kBatch];
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBatch; ++b) {
       const int i = i0 + b * NT, t = i / each, kk = i < work ? seg.k0 + top.who[t] + (i - t * each) * NT : seg.k1;
       x[b] = kk < seg.k1 ? seg.load(kk) : neg_inf_slot<T>();
       e0[b] = kk < seg.k1 ? seg.element(kk) : seg.V;
     }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < kBatch; ++b) {
+      if (!(slot_max_nan<T>(x[b]) >= least)) continue;
       float z[VN];
       unpack16<T>(x[b], z);
 #pragma unroll
@@ -330,7 +338,8 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
   seg.hi = (int)(((int64_t)seg.off + a.V) / VN);
   const float c = a.inv_t * kLog2e;
   Running<T> run;
-  int at = seg.k0 + tid;  // slot where the maximum first stood
+  int at = seg.k0 + tid;  // slot where the maximum first stood,
+  uint4 x_at = make_uint4(0u, 0u, 0u, 0u);  // and that slot
   for (int k0 = seg.k0 + tid; k0 < seg.k1; k0 += NT * kBatch) {
     uint4 x[kBatch];
     if (k0 >= seg.lo && k0 + (kBatch - 1) * NT < min(seg.hi, seg.k1)) {
@@ -352,24 +361,22 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
       if (TOP) {
 #pragma unroll
         for (int i = kBatch - 1; i >= 0; --i)
-          if (sm[i] == to) at = k0 + i * NT;
+          if (sm[i] == to) {
+            at = k0 + i * NT;
+            x_at = x[i];
+          }
       }
     }
     if (run.q.m != -CUDART_INF_F) run.add(x, c);
   }
-  uint4 x_at = make_uint4(0u, 0u, 0u, 0u);
-  if (TOP && seg.k0 + tid < seg.k1) x_at = seg.load(at);  // used behind the sums
   Sums q = run.result(c);
   const float m_thread = q.m;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
-    q.join(p, c);
-  }
+  q.join_lanes<32>(c);
   if (lane == 0) part[w] = q;
   if constexpr (TOP) {
     uint64_t first = 0;
     if (seg.k0 + tid < seg.k1) {
+      if (m_thread == -CUDART_INF_F) x_at = neg_inf_slot<T>();  // no slot raised it: the first
       float z[VN];
       const int e0 = seg.element(at);
       unpack16<T>(x_at, z);
@@ -393,11 +400,7 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
   __syncthreads();
   if (w == 0) {
     q = lane < NW ? part[lane] : Sums{-CUDART_INF_F, 0.0f, 0.0f};
-#pragma unroll
-    for (int o = NW / 2; o > 0; o >>= 1) {
-      const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
-      q.join(p, c);
-    }
+    q.join_lanes<NW>(c);
     if (lane == 0) whole = q;
   }
   if constexpr (TOP) {
@@ -437,13 +440,8 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
     cluster.sync();
     if (rank == 0) {
       if (w == 0) {
-        q = lane < CL ? *cluster.map_shared_rank(&whole, lane % CL) : Sums{-CUDART_INF_F, 0.0f, 0.0f};
-#pragma unroll
-        for (int o = CL / 2; o > 0; o >>= 1) {
-          const Sums p = {__shfl_xor_sync(kFull, q.m, o), __shfl_xor_sync(kFull, q.s, o), __shfl_xor_sync(kFull, q.u, o)};
-          q.join(p, c);
-        }
-        q = {__shfl_sync(kFull, q.m, 0), __shfl_sync(kFull, q.s, 0), __shfl_sync(kFull, q.u, 0)};
+        q = *cluster.map_shared_rank(&whole, lane % CL);
+        q.join_lanes<CL>(c);
         finish();
         if (tid == 0) {
           give();
@@ -451,17 +449,20 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
         }
       }
       if constexpr (TOP) {
-        static_assert(CL * 32 <= NT, "a key per thread");
+        static_assert(CL * 32 <= NT && CL * 32 <= kFound, "a key per thread");
         uint64_t own = 0;
-        if (tid < CL * 32) own = cluster.map_shared_rank(&top, w)->best[lane];
-        if (tid < CL * 32) top.found[tid] = own;
+        if (w < CL && lane < a.k) {
+          own = cluster.map_shared_rank(&top, w)->best[lane];
+          top.found[w * a.k + lane] = own;
+        }
         __syncthreads();
         m = part[0].m;
         logs = part[0].s;
-        int i = 0;
-#pragma unroll 8
-        for (int o = 0; o < CL * 32; ++o) i += top.found[o] > own;
-        if (own != 0 && i < a.k) give_top(own, i);
+        if (own != 0) {
+          int i = 0;
+          for (int o = 0; o < CL * a.k; ++o) i += top.found[o] > own;
+          if (i < a.k) give_top(own, i);
+        }
       }
     }
     cluster.sync();  // rank 0 has read the others' shared memory
