@@ -13,13 +13,13 @@
 // writes theirs.
 //
 // The k likeliest columns come without a second pass over the row.  Every
-// thread also knows where its maximum first stood; the k-th largest of these
-// maxima is a bound that k different elements reach, so whatever is among the
-// row's k largest is not under it, and lies with the few threads (about k)
-// whose maximum is not under it.  Their slots are read again, from L2, by
-// whole warps, and the elements that reach the bound are ranked.  Elements are
-// ordered by 64-bit keys (value, then lowest column first), all different, so
-// ties need no case of their own.
+// thread also knows its largest element; the k-th largest of these (taken over
+// up to 64 groups of threads) is a bound that k different elements reach, so
+// whatever is among the row's k largest reaches it too, and lies with the few
+// threads (k and some) whose largest element does.  Their slots are read again,
+// from L2, by whole warps, and the elements that reach the bound are ranked by
+// 64-bit keys (value, then lowest column first), all different, so ties need no
+// case of their own.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -107,28 +107,135 @@ __device__ __forceinline__ uint4 load_slot_row(const T* row, int e0, int V) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Sums of a thread, kept relative to its running maximum.
+// Two floats in one register pair, for the packed fp32 instructions.
+struct Pair {
+  uint64_t v;
+  __device__ __forceinline__ static Pair of(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(lo), "f"(hi));
+    return p;
+  }
+  __device__ __forceinline__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+};
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+  Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+
+// Both halves raised to `floor`, a pair of finite values.
+template <class T>
+__device__ __forceinline__ uint32_t floor2(uint32_t x, uint32_t floor) {
+  uint32_t r;
+  if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(floor));
+  else
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(floor));
+  return r;
+}
+// -2^100 in bfloat16; the lowest finite float16
+template <class T>
+constexpr uint32_t kFloor2 = std::is_same<T, __nv_bfloat16>::value ? 0xf180f180u : 0xfbfffbffu;
+template <class T>
+constexpr float kFloor16 = std::is_same<T, __nv_bfloat16>::value ? -1.2676506e30f : -65504.0f;
+
+// A thread's maximum, and its sums of 2^t and 2^t t relative to a reference,
+// which is not moved before the maximum has passed it by 8 powers of two (a
+// maximum of a few elements is passed all the time, and moving costs as much
+// as three elements).  With r2 = fl(ref c), t = fma(z, c, -r2) is rounded once,
+// and off = r2 - ref c is what t is away from (z - ref) c.  Where r2 is large,
+// off could be, too, and t is (z - ref) c.
+// Elements that are -inf or far down are raised so that 0 * t is finite: t
+// itself, or in pairs the 16-bit elements, if their floor is 200 powers of two
+// under the reference.  Pairs take 4.5 instructions an element with the
+// maximum, single ones 8 (4096 x 32000 bfloat16: 43 and 55 us; HBM takes 40).
 template <class T>
 struct Running {
-  Sums q;
-  __device__ __forceinline__ Running() { q = {-CUDART_INF_F, 0.0f, 0.0f}; }
-  __device__ __forceinline__ void raise(float to, float c) { q.raise(to, c); }
+  float m, ref, r2, off, lim;
+  bool pairs;
+  Pair s, u;
+  __device__ __forceinline__ Running() {
+    m = ref = lim = -CUDART_INF_F;
+    r2 = off = 0.0f;
+    pairs = false;
+    s = u = Pair::of(0.0f, 0.0f);
+  }
+  __device__ __forceinline__ void move(float to, float c) {  // to >= ref, or NaN
+    const float n2 = to * c;
+    bool fits = fabsf(n2) < 1048576.0f;  // |off| < 2^-4
+    if constexpr (sizeof(T) == 2) fits = fits && n2 - kFloor16<T> * c >= 200.0f && kFloor16<T> * c > -1e38f;
+    const float n_off = fits ? fmaf(-to, c, n2) : 0.0f;
+    if (ref != -CUDART_INF_F) {
+      const float d = fmaxf((ref - to) * c + (off - n_off), kFloor), f = exp2_ftz(d);
+      const float2 a = s.get(), b = u.get();
+      u = Pair::of(f * fmaf(d, a.x, b.x), f * fmaf(d, a.y, b.y));
+      s = Pair::of(f * a.x, f * a.y);
+    }
+    ref = to, r2 = n2, off = n_off, pairs = fits;
+    lim = fits ? to + 8.0f / c : to;
+  }
   template <int N>
   __device__ __forceinline__ void add(const uint4 (&x)[N], float c) {
     constexpr int VN = 16 / sizeof(T);
+    if (pairs) {
+      const Pair c2 = Pair::of(c, c), back = Pair::of(-r2, -r2);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float z[VN];
-      unpack16<T>(x[i], z);
+      for (int i = 0; i < N; ++i) {
+        uint4 v = x[i];
+        if constexpr (sizeof(T) == 2)
+          v = make_uint4(floor2<T>(v.x, kFloor2<T>), floor2<T>(v.y, kFloor2<T>), floor2<T>(v.z, kFloor2<T>),
+                         floor2<T>(v.w, kFloor2<T>));
+        float z[VN];
+        unpack16<T>(v, z);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const float t = fmaxf((z[j] - q.m) * c, kFloor), e = exp2_ftz(t);
-        q.s += e;
-        q.u = fmaf(e, t, q.u);
+        for (int j = 0; j < VN; j += 2) {
+          Pair t = fma2(Pair::of(z[j], z[j + 1]), c2, back);
+          float2 f = t.get();
+          if constexpr (sizeof(T) == 4) {
+            f = make_float2(fmaxf(f.x, kFloor), fmaxf(f.y, kFloor));
+            t = Pair::of(f.x, f.y);
+          }
+          const Pair e = Pair::of(exp2_ftz(f.x), exp2_ftz(f.y));
+          s = add2(s, e);
+          u = fma2(e, t, u);
+        }
       }
+    } else {
+      float2 a = s.get(), b = u.get();
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float z[VN];
+        unpack16<T>(x[i], z);
+#pragma unroll
+        for (int j = 0; j < VN; ++j) {
+          const float t = fmaxf((z[j] - ref) * c, kFloor), e = exp2_ftz(t);
+          (j & 1 ? a.y : a.x) += e;
+          (j & 1 ? b.y : b.x) = fmaf(e, t, j & 1 ? b.y : b.x);
+        }
+      }
+      s = Pair::of(a.x, a.y);
+      u = Pair::of(b.x, b.y);
     }
   }
-  __device__ __forceinline__ Sums result(float) const { return q; }
+  __device__ __forceinline__ Sums result(float c) const {  // relative to the maximum
+    const float2 a = s.get(), b = u.get();
+    Sums q = {m, a.x + a.y, b.x + b.y};
+    if (ref != -CUDART_INF_F) {
+      const float d = fmaxf((ref - m) * c + off, kFloor), f = exp2_ftz(d);
+      q.u = f * fmaf(d, q.s, q.u);
+      q.s *= f;
+    }
+    return q;
+  }
 };
 
 // Descending over the lanes.
@@ -161,14 +268,13 @@ constexpr int kFound = 256;  // keys that reach the bound, before the slower way
 template <int NW>
 struct TopShared {
   static constexpr int NT = NW * 32, NG = NT < 64 ? NT : 64;  // threads; groups of NT / NG neighbours
-  uint64_t first[NT];     // each thread's largest key, 0 without elements
-  uint64_t group[NG];     // the largest of each group
+  float group[NG];        // the largest element of each group
   uint64_t found[kFound];
   uint64_t held[NW][64];  // the slower way: keys that reach the bound, per warp
   uint64_t best[32];      // the CTA's k largest, descending, 0 where there are fewer
-  uint64_t bound;
-  int count[NW], n, n_who;
-  uint16_t who[NT];       // threads whose largest key reaches the bound
+  float bound;
+  int n, n_who;
+  uint16_t who[NT];       // threads whose largest element reaches the bound
 };
 
 // A CTA's part of a row: slots [k0, k1), of which [lo, hi) are whole.
@@ -182,30 +288,37 @@ struct Segment {
   }
 };
 
-// The bound: the k-th largest of the groups' keys (0 if there are not so many),
-// which k different elements reach.  top.bound is 0 before.
+// The bound: the k-th largest of the groups' largest elements, which k
+// different elements reach.  top.bound is -inf before.
 template <int NW>
 __device__ __forceinline__ void top_bound(TopShared<NW>& top, int k) {
   using S = TopShared<NW>;
-  constexpr int P = S::NT / S::NG, M = S::NG / P;  // threads per key, keys each compares with
-  const int mine = threadIdx.x / P, from = (threadIdx.x % P) * M;
-  const uint64_t own = top.group[mine];
-  int rank = 0;
+  constexpr int P = S::NT / S::NG, M = S::NG / P;  // threads per group, groups each compares with
+  const float own = top.group[threadIdx.x / P];
+  int above = 0, reach = 0;  // groups above this one; not under it
 #pragma unroll
-  for (int i = 0; i < M; ++i) rank += top.group[from + i] > own;
+  for (int i = 0; i < M; ++i) {
+    const float o = top.group[(threadIdx.x % P) + i * P];
+    above += o > own;
+    reach += o >= own;
+  }
 #pragma unroll
-  for (int o = 1; o < P; o <<= 1) rank += __shfl_xor_sync(kFull, rank, o);
-  if (rank == k - 1) top.bound = own;  // without elements (0) several may write the same
+  for (int o = 1; o < P; o <<= 1) {
+    above += __shfl_xor_sync(kFull, above, o);
+    reach += __shfl_xor_sync(kFull, reach, o);
+  }
+  if (above < k && reach >= k) top.bound = own;  // equal ones all write it
 }
 
-// Leaves the k largest keys of the segment in top.best.  top.first and the
-// bound are there; top.n and top.n_who are 0.
+// Leaves the k largest keys of the segment in top.best.  `largest` is this
+// thread's largest element, the bound is there, top.n and top.n_who are 0.
 template <class T, int NW>
-__device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg, int k) {
+__device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg, float largest, int k) {
   constexpr int VN = 16 / sizeof(T), NT = NW * 32;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const uint64_t bound = top.bound, first = top.first[tid];
-  const bool in = first != 0 && first >= bound;
+  const float least = top.bound;
+  const uint64_t bound = (uint64_t)sort_key(least) << 32;
+  const bool in = seg.k0 + tid < seg.k1 && largest >= least;
   const uint32_t all = __ballot_sync(kFull, in);
   int base = 0;
   if (lane == 0 && all) base = atomicAdd(&top.n_who, __popc(all));
@@ -213,29 +326,29 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   if (in) top.who[base + __popc(all & ((1u << lane) - 1u))] = (uint16_t)tid;
   if (tid < 32) top.best[tid] = 0;
   __syncthreads();
-  const float least = bound ? key_value((uint32_t)(bound >> 32)) : -CUDART_INF_F;
-  const int each = (seg.k1 - seg.k0 + NT - 1) / NT, work = top.n_who * each;
-  for (int i0 = tid; i0 < work; i0 += kBatch * NT) {
-    uint4 x[kBatch];
-    int e0[kBatch];
+  // a warp per thread of the list, its slots over the lanes, four such loads in flight
+  const int n_who = top.n_who;
+  for (int t0 = w; t0 < n_who; t0 += kBatch * NW) {
+    for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
+      uint4 x[kBatch];
+      int kk[kBatch];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b * NT, t = i / each, kk = i < work ? seg.k0 + top.who[t] + (i - t * each) * NT : seg.k1;
-      x[b] = kk < seg.k1 ? seg.load(kk) : neg_inf_slot<T>();
-      e0[b] = kk < seg.k1 ? seg.element(kk) : seg.V;
-    }
+      for (int b = 0; b < kBatch; ++b) {
+        kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
+        if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
+      }
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      if (!(slot_max_nan<T>(x[b]) >= least)) continue;
-      float z[VN];
-      unpack16<T>(x[b], z);
+      for (int b = 0; b < kBatch; ++b) {
+        if (kk[b] >= seg.k1 || !(slot_max_nan<T>(x[b]) >= least)) continue;
+        float z[VN];
+        unpack16<T>(x[b], z);
 #pragma unroll
-      for (int j = 0; j < VN; ++j) {
-        const int e = e0[b] + j;
-        const uint64_t key = rank_key(z[j], e);
-        if (key >= bound && e >= 0 && e < seg.V) {
-          const int at = atomicAdd(&top.n, 1);
-          if (at < kFound) top.found[at] = key;
+        for (int j = 0; j < VN; ++j) {
+          const int e = seg.element(kk[b]) + j;
+          if (z[j] >= least && e >= 0 && e < seg.V) {
+            const int at = atomicAdd(&top.n, 1);
+            if (at < kFound) top.found[at] = rank_key(z[j], e);
+          }
         }
       }
     }
@@ -338,8 +451,6 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
   seg.hi = (int)(((int64_t)seg.off + a.V) / VN);
   const float c = a.inv_t * kLog2e;
   Running<T> run;
-  int at = seg.k0 + tid;  // slot where the maximum first stood,
-  uint4 x_at = make_uint4(0u, 0u, 0u, 0u);  // and that slot
   for (int k0 = seg.k0 + tid; k0 < seg.k1; k0 += NT * kBatch) {
     uint4 x[kBatch];
     if (k0 >= seg.lo && k0 + (kBatch - 1) * NT < min(seg.hi, seg.k1)) {
@@ -349,50 +460,24 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) x[i] = k0 + i * NT < seg.k1 ? seg.load(k0 + i * NT) : neg_inf_slot<T>();
     }
-    float sm[kBatch], bm = -CUDART_INF_F;
+    float bm = -CUDART_INF_F;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      sm[i] = slot_max_nan<T>(x[i]);
-      bm = max_nan(bm, sm[i]);
-    }
-    if (!(bm <= run.q.m)) {
-      const float to = max_nan(run.q.m, bm);
-      run.raise(to, c);
-      if (TOP) {
-#pragma unroll
-        for (int i = kBatch - 1; i >= 0; --i)
-          if (sm[i] == to) {
-            at = k0 + i * NT;
-            x_at = x[i];
-          }
-      }
-    }
-    if (run.q.m != -CUDART_INF_F) run.add(x, c);
+    for (int i = 0; i < kBatch; ++i) bm = max_nan(bm, slot_max_nan<T>(x[i]));
+    run.m = max_nan(run.m, bm);
+    if (!(bm <= run.lim)) run.move(run.m, c);
+    if (run.ref != -CUDART_INF_F) run.add(x, c);
   }
   Sums q = run.result(c);
   const float m_thread = q.m;
   q.join_lanes<32>(c);
   if (lane == 0) part[w] = q;
   if constexpr (TOP) {
-    uint64_t first = 0;
-    if (seg.k0 + tid < seg.k1) {
-      if (m_thread == -CUDART_INF_F) x_at = neg_inf_slot<T>();  // no slot raised it: the first
-      float z[VN];
-      const int e0 = seg.element(at);
-      unpack16<T>(x_at, z);
+    float g = m_thread;
 #pragma unroll
-      for (int j = VN - 1; j >= 0; --j)
-        if (z[j] == m_thread && e0 + j >= 0 && e0 + j < a.V) first = rank_key(z[j], e0 + j);
-    }
-    top.first[tid] = first;
-#pragma unroll
-    for (int o = 1; o < NT / TopShared<NW>::NG; o <<= 1) {
-      const uint64_t other = __shfl_xor_sync(kFull, first, o);
-      first = other > first ? other : first;
-    }
-    top.group[tid / (NT / TopShared<NW>::NG)] = first;
+    for (int o = 1; o < NT / TopShared<NW>::NG; o <<= 1) g = fmaxf(g, __shfl_xor_sync(kFull, g, o));
+    top.group[tid / (NT / TopShared<NW>::NG)] = g;
     if (tid == 0) {
-      top.bound = 0;
+      top.bound = -CUDART_INF_F;
       top.n = 0;
       top.n_who = 0;
     }
@@ -406,7 +491,7 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
   if constexpr (TOP) {
     top_bound(top, a.k);
     __syncthreads();
-    top_of<T, NW>(top, seg, a.k);
+    top_of<T, NW>(top, seg, m_thread, a.k);
   }
   float m = CUDART_NAN_F, logs = CUDART_NAN_F, h = CUDART_NAN_F, logp = CUDART_NAN_F;
   const auto finish = [&] {  // of the row, from q; one thread or several
