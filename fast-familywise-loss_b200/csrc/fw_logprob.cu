@@ -263,6 +263,16 @@ __device__ __forceinline__ uint64_t warp_merge(uint64_t a, uint64_t b, int lane)
   return x;
 }
 
+// The threads of a row's group: a CTA, or one of its warps.
+template <int NW>
+__device__ __forceinline__ void group_sync() {
+  if constexpr (NW == 1)
+    __syncwarp();
+  else
+    __syncthreads();
+}
+constexpr int kWarpRows = 8;  // rows per CTA, a warp each, of the short ones
+
 constexpr int kFound = 256;  // keys that reach the bound, before the slower way is taken
 
 template <int NW>
@@ -294,11 +304,12 @@ template <int NW>
 __device__ __forceinline__ void top_bound(TopShared<NW>& top, int k) {
   using S = TopShared<NW>;
   constexpr int P = S::NT / S::NG, M = S::NG / P;  // threads per group, groups each compares with
-  const float own = top.group[threadIdx.x / P];
+  const int tid = threadIdx.x % S::NT;
+  const float own = top.group[tid / P];
   int above = 0, reach = 0;  // groups above this one; not under it
 #pragma unroll
   for (int i = 0; i < M; ++i) {
-    const float o = top.group[(threadIdx.x % P) + i * P];
+    const float o = top.group[(tid % P) + i * P];
     above += o > own;
     reach += o >= own;
   }
@@ -315,45 +326,58 @@ __device__ __forceinline__ void top_bound(TopShared<NW>& top, int k) {
 template <class T, int NW>
 __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg, float largest, int k) {
   constexpr int VN = 16 / sizeof(T), NT = NW * 32;
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int tid = threadIdx.x % NT, lane = tid & 31, w = tid >> 5;
   const float least = top.bound;
   const uint64_t bound = (uint64_t)sort_key(least) << 32;
   const bool in = seg.k0 + tid < seg.k1 && largest >= least;
+  const auto look = [&](const uint4& x, int kk) {
+    if (!(slot_max_nan<T>(x) >= least)) return;
+    float z[VN];
+    unpack16<T>(x, z);
+#pragma unroll
+    for (int j = 0; j < VN; ++j) {
+      const int e = seg.element(kk) + j;
+      if (z[j] >= least && e >= 0 && e < seg.V) {
+        const int at = atomicAdd(&top.n, 1);
+        if (at < kFound) top.found[at] = rank_key(z[j], e);
+      }
+    }
+  };
   const uint32_t all = __ballot_sync(kFull, in);
   int base = 0;
   if (lane == 0 && all) base = atomicAdd(&top.n_who, __popc(all));
   base = __shfl_sync(kFull, base, 0);
   if (in) top.who[base + __popc(all & ((1u << lane) - 1u))] = (uint16_t)tid;
   if (tid < 32) top.best[tid] = 0;
-  __syncthreads();
-  // a warp per thread of the list, its slots over the lanes, four such loads in flight
+  group_sync<NW>();
   const int n_who = top.n_who;
-  for (int t0 = w; t0 < n_who; t0 += kBatch * NW) {
-    for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
+  if (seg.k1 - seg.k0 <= kBatch * NT) {  // few slots each: every thread its own
+    if (in) {
       uint4 x[kBatch];
-      int kk[kBatch];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
-        if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
-      }
+      for (int b = 0; b < kBatch; ++b)
+        if (seg.k0 + tid + b * NT < seg.k1) x[b] = seg.load(seg.k0 + tid + b * NT);
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        if (kk[b] >= seg.k1 || !(slot_max_nan<T>(x[b]) >= least)) continue;
-        float z[VN];
-        unpack16<T>(x[b], z);
+      for (int b = 0; b < kBatch; ++b)
+        if (seg.k0 + tid + b * NT < seg.k1) look(x[b], seg.k0 + tid + b * NT);
+    }
+  } else {  // a warp per thread of the list, its slots over the lanes, kBatch such loads in flight
+    for (int t0 = w; t0 < n_who; t0 += kBatch * NW) {
+      for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
+        uint4 x[kBatch];
+        int kk[kBatch];
 #pragma unroll
-        for (int j = 0; j < VN; ++j) {
-          const int e = seg.element(kk[b]) + j;
-          if (z[j] >= least && e >= 0 && e < seg.V) {
-            const int at = atomicAdd(&top.n, 1);
-            if (at < kFound) top.found[at] = rank_key(z[j], e);
-          }
+        for (int b = 0; b < kBatch; ++b) {
+          kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
+          if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
         }
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+          if (kk[b] < seg.k1) look(x[b], kk[b]);
       }
     }
   }
-  __syncthreads();
+  group_sync<NW>();
   const int n = top.n;
   if (n <= kFound) {
     for (int i = tid; i < n; i += NT) {
@@ -362,7 +386,7 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
       for (int o = 0; o < n; ++o) rank += top.found[o] > own;
       if (rank < k) top.best[rank] = own;
     }
-    __syncthreads();
+    group_sync<NW>();
     return;
   }
   // The slower way, for rows whose largest elements lie with few threads: each warp keeps the 32 largest of what it
@@ -402,26 +426,32 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   }
   drain();
   held[lane] = list;
-  __syncthreads();
+  group_sync<NW>();
   const uint64_t own = held[lane];
   int rank = 0;
   for (int g = 0; g < NW; ++g)
     for (int i = 0; i < 32; ++i) rank += top.held[g][i] > own;
   if (own != 0 && rank < k) top.best[rank] = own;
-  __syncthreads();
+  group_sync<NW>();
 }
 
-// One row per cluster of CL CTAs of NW warps, each taking an equal part of it.
+// One row per cluster of CL CTAs of NW warps, each taking an equal part of it;
+// or, for NW = 1, one row per warp of a CTA.
 template <class T, int NW, bool TOP, int CL>
-__global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_logprob_kernel(ScoreArgs a) {
+__global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 3) fw_logprob_kernel(ScoreArgs a) {
   constexpr int VN = 16 / sizeof(T), NT = NW * 32;
-  __shared__ Sums part[NW];
-  __shared__ Sums whole;  // of this CTA
-  __shared__ TopShared<TOP ? NW : 1> top;
+  constexpr int R = NW == 1 ? kWarpRows : 1;
+  __shared__ Sums parts[R][NW];
+  __shared__ Sums whole;  // of this CTA, for its cluster
+  __shared__ TopShared<TOP ? NW : 1> tops[TOP ? R : 1];
   wait_prior_kernel();
   allow_dependent_launch();
-  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
-  const int64_t r = blockIdx.x / CL;
+  const int group = R > 1 ? threadIdx.x / NT : 0;
+  const int tid = threadIdx.x % NT, lane = tid & 31, w = tid >> 5;
+  const int64_t r = (int64_t)blockIdx.x * R / CL + group;
+  if (r >= a.B) return;
+  Sums(&part)[NW] = parts[group];
+  TopShared<TOP ? NW : 1>& top = tops[TOP ? group : 0];
   const int rank = CL > 1 ? (int)(blockIdx.x % CL) : 0;
   const int64_t y = a.y[r];
   if (y == a.ignore) {
@@ -482,15 +512,15 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
       top.n_who = 0;
     }
   }
-  __syncthreads();
+  group_sync<NW>();
   if (w == 0) {
     q = lane < NW ? part[lane] : Sums{-CUDART_INF_F, 0.0f, 0.0f};
     q.join_lanes<NW>(c);
-    if (lane == 0) whole = q;
+    if (CL > 1 && lane == 0) whole = q;
   }
   if constexpr (TOP) {
     top_bound(top, a.k);
-    __syncthreads();
+    group_sync<NW>();
     top_of<T, NW>(top, seg, m_thread, a.k);
   }
   float m = CUDART_NAN_F, logs = CUDART_NAN_F, h = CUDART_NAN_F, logp = CUDART_NAN_F;
@@ -515,7 +545,7 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
   };
   if constexpr (CL == 1) {
     if (w == 0) {
-      if (TOP) q = whole;  // written by this warp, or before the barriers of top_of
+      q = {__shfl_sync(kFull, q.m, 0), __shfl_sync(kFull, q.s, 0), __shfl_sync(kFull, q.u, 0)};
       finish();
       if (tid == 0) give();
       if (TOP && lane < a.k) give_top(top.best[lane], lane);
@@ -540,7 +570,7 @@ __global__ void __launch_bounds__(NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 24) fw_lo
           own = cluster.map_shared_rank(&top, w)->best[lane];
           top.found[w * a.k + lane] = own;
         }
-        __syncthreads();
+        group_sync<NW>();
         m = part[0].m;
         logs = part[0].s;
         if (own != 0) {
@@ -624,9 +654,10 @@ bool misaligned(const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p
 
 template <class T, int NW, int CL>
 int launch_score(const ScoreArgs& a, cudaStream_t st) {
-  return launch_status(a.k > 0
-                           ? launch_dependent(fw_logprob_kernel<T, NW, true, CL>, a.B * CL, NW * 32, 0, CL, st, a)
-                           : launch_dependent(fw_logprob_kernel<T, NW, false, CL>, a.B * CL, NW * 32, 0, CL, st, a));
+  const int64_t grid = NW == 1 ? (a.B + kWarpRows - 1) / kWarpRows : a.B * CL;
+  const int threads = NW == 1 ? kWarpRows * 32 : NW * 32;
+  return launch_status(a.k > 0 ? launch_dependent(fw_logprob_kernel<T, NW, true, CL>, grid, threads, 0, CL, st, a)
+                               : launch_dependent(fw_logprob_kernel<T, NW, false, CL>, grid, threads, 0, CL, st, a));
 }
 
 template <class T>
