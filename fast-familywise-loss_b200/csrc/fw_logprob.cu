@@ -588,56 +588,104 @@ __global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 
 struct ScoreGradArgs {
   const void* z;
   int64_t B, ld, ldg;
-  int V, units;  // units of kGradSlots slots per row
+  int V, parts;  // CTAs per row
   float inv_t;
   const float4* state;
   const float *dlogp, *dentropy;  // either may be NULL: zero
   void* grad;
 };
 
-constexpr int kGradSlots = 32 * kBatch;  // a warp's step
+// 16-byte slots in flight per thread, and CTAs of 256 threads per SM.  4096 x
+// 32000, float32 and bfloat16, with 2 and 8: 171 and 88 us; 4 and 4: 167 and
+// 90; 4 and 5: 167 and 86; 8 and 3: 163 and 91.
+constexpr int kGradBatch = 4, kGradCtas = 5;
 
-// One warp per kGradSlots slots of the gradient's rows.
-template <class T>
-__global__ void __launch_bounds__(256, 4) fw_logprob_grad_kernel(ScoreGradArgs a) {
-  constexpr int VN = 16 / sizeof(T);
+// What a row's elements are worked out from, in powers of two:
+//   l = log2 p = fma(z, c, -r2) + shift, or (z - m) c + shift where r2 is large
+//   d = -2^l (h l + g)
+struct RowGrad {
+  float m, c, r2, shift, g, h;
+  bool live, fits;
+};
+
+// Rows in `parts` parts, a CTA each, or (NW = 1) a row per warp.
+template <class T, int NW>
+__global__ void __launch_bounds__(256, kGradCtas) fw_logprob_grad_kernel(ScoreGradArgs a) {
+  constexpr int VN = 16 / sizeof(T), NT = NW * 32, N = kGradBatch;
   wait_prior_kernel();
   allow_dependent_launch();
-  const int lane = threadIdx.x & 31;
-  const int64_t work = a.B * a.units, step = (int64_t)gridDim.x * 8;
-  const Span<T> span(a.z, a.B, a.ld, a.V);
-  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < work; i += step) {
-    const int64_t r = i / a.units;
-    const T* row = static_cast<const T*>(a.z) + r * a.ld;
-    T* out = static_cast<T*>(a.grad) + r * a.ldg;
-    const int off = (int)((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
-    const int e0 = (int)((i - r * a.units) * kGradSlots + lane) * VN - off;
-    const float4 st = a.state[r];
-    const int y = __float_as_int(st.w);
-    const bool live = y != -2;
-    uint4 x[kBatch];
+  const int tid = threadIdx.x % NT;
+  const int64_t r = NW == 1 ? (int64_t)blockIdx.x * 8 + threadIdx.x / 32 : blockIdx.x / a.parts;
+  if (r >= a.B) return;
+  const int part = NW == 1 ? 0 : (int)(blockIdx.x - r * a.parts);
+  const T* row = static_cast<const T*>(a.z) + r * a.ld;
+  T* out = static_cast<T*>(a.grad) + r * a.ldg;
+  const int V = a.V;
+  const int off = (int)((reinterpret_cast<uintptr_t>(out) & 15u) / sizeof(T));
+  const int slots = (int)(((int64_t)off + V + VN - 1) / VN);
+  const int k1 = (int)((int64_t)slots * (part + 1) / a.parts);
+  // where the gradient's whole slots are whole slots of the logits
+  const bool same = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15u) == 0;
+  const int lo = same ? (off ? 1 : 0) : k1, hi = min(k1, (int)(((int64_t)off + V) / VN));
+  const Span<T> span(a.z, a.B, a.ld, V);
+
+  const float4 st = a.state[r];
+  const int y = __float_as_int(st.w);
+  RowGrad q;
+  q.live = y != -2;
+  q.m = st.x;
+  q.c = a.inv_t * kLog2e;
+  q.r2 = q.m * q.c;
+  q.fits = fabsf(q.r2) < 1048576.0f;
+  q.shift = -st.y * kLog2e + (q.fits ? fmaf(-q.m, q.c, q.r2) : 0.0f);
+  const float g = a.dlogp ? a.dlogp[r] * a.inv_t : 0.0f, h = a.dentropy ? a.dentropy[r] * a.inv_t : 0.0f;
+  q.h = -h * kLn2;
+  q.g = a.dentropy ? -fmaf(h, st.z, g) : -g;
+  if (isnan(st.x)) q.g = CUDART_NAN_F;
+
+  for (int k0 = (int)((int64_t)slots * part / a.parts) + tid; k0 < k1; k0 += NT * N) {
+    uint4 x[N];
+    if (!q.live) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int e = e0 + b * 32 * VN;
-      x[b] = make_uint4(0u, 0u, 0u, 0u);
-      if (live && e < a.V) x[b] = load_slot_shifted(row, e, span);
+      for (int i = 0; i < N; ++i)
+        if (k0 + i * NT < k1) store_slot(out, (int64_t)(k0 + i * NT) * VN - off, (int64_t)V, true, make_uint4(0u, 0u, 0u, 0u));
+      continue;
     }
-    const float g = a.dlogp ? a.dlogp[r] * a.inv_t : 0.0f, h = a.dentropy ? a.dentropy[r] * a.inv_t : 0.0f;
+    const bool whole = k0 >= lo && k0 + (N - 1) * NT < hi;
+    if (whole) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int e = e0 + b * 32 * VN;
-      if (e >= a.V) continue;
+      for (int i = 0; i < N; ++i) x[i] = ld_global16_once(row + ((k0 + i * NT) * VN - off));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = k0 + i * NT < k1 ? load_slot_shifted(row, (k0 + i * NT) * VN - off, span) : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = (k0 + i * NT) * VN - off;
       float z[VN];
-      unpack16<T>(x[b], z);
+      unpack16<T>(x[i], z);
 #pragma unroll
       for (int j = 0; j < VN; ++j) {
         // an element outside the row may be anything; it is not stored
-        const float l = fmaxf((z[j] - st.x) * a.inv_t - st.y, kFloor);
-        float d = -exp2_ftz(l * kLog2e) * (a.dentropy ? fmaf(h, l + st.z, g) : g);
-        if (e + j == y) d += g;
-        z[j] = live ? (isnan(st.x) ? CUDART_NAN_F : d) : 0.0f;
+        float l = q.fits ? fmaf(z[j], q.c, -q.r2) : (z[j] - q.m) * q.c;
+        l = fmaxf(l + q.shift, kFloor);
+        z[j] = exp2_ftz(l) * fmaf(q.h, l, q.g);
       }
-      store_slot(out, (int64_t)e, (int64_t)a.V, true, pack_slot<T>(z));
+      if ((unsigned)(y - e) < (unsigned)VN) {
+#pragma unroll
+        for (int j = 0; j < VN; ++j)
+          if (e + j == y) z[j] += g;
+      }
+      x[i] = pack_slot<T>(z);
+    }
+    if (whole) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(out + ((k0 + i * NT) * VN - off)) = x[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (k0 + i * NT < k1) store_slot(out, (int64_t)(k0 + i * NT) * VN - off, (int64_t)V, true, x[i]);
     }
   }
 }
@@ -675,9 +723,12 @@ int run_score(const ScoreArgs& a, cudaStream_t st) {
 template <class T>
 int run_score_grad(ScoreGradArgs a, cudaStream_t st) {
   const int64_t slots = a.V / (16 / (int)sizeof(T)) + 2;  // whatever the row's start
-  a.units = (int)((slots + kGradSlots - 1) / kGradSlots);
-  const int64_t need = (a.B * a.units + 7) / 8, cap = (int64_t)sm_count() * 48;
-  return launch_status(launch_dependent(fw_logprob_grad_kernel<T>, need < cap ? need : cap, 256, 0, 1, st, a));
+  a.parts = 1;
+  if (slots <= 256) return launch_status(launch_dependent(fw_logprob_grad_kernel<T, 1>, (a.B + 7) / 8, 256, 0, 1, st, a));
+  // parts of no less than one step of a CTA, as many as run at once
+  const int64_t most = (slots + 256 * kGradBatch - 1) / (256 * kGradBatch), want = (int64_t)sm_count() * kGradCtas / a.B;
+  a.parts = (int)(want < 1 ? 1 : want < most ? want : most);
+  return launch_status(launch_dependent(fw_logprob_grad_kernel<T, 8>, a.B * a.parts, 256, 0, 1, st, a));
 }
 
 }  // namespace
