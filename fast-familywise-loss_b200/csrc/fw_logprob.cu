@@ -708,10 +708,16 @@ int launch_score(const ScoreArgs& a, cudaStream_t st) {
                                : launch_dependent(fw_logprob_kernel<T, NW, false, CL>, grid, threads, 0, CL, st, a));
 }
 
+// Rows of one warp each: up to 256 slots, or 512 where there are warps' worth
+// of rows on every SM.  4096 x 4000 bfloat16 (500 slots) by warps and by CTAs:
+// gradient 16.8 and 25.0 us, 5 alternatives 20.4 and 23.6; 512 such rows: 7.8
+// and 6.3, 10.1 and 6.6; 4096 x 8000: 29 and 26, 29 and 29.
+bool by_warps(int64_t slots, int64_t B) { return slots <= (B >= (int64_t)sm_count() * 16 ? 512 : 256); }
+
 template <class T>
 int run_score(const ScoreArgs& a, cudaStream_t st) {
   const int64_t slots = a.V / (16 / (int)sizeof(T)), ctas = (int64_t)sm_count() * 4;
-  if (slots <= 256) return launch_score<T, 1, 1>(a, st);
+  if (by_warps(slots, a.B)) return launch_score<T, 1, 1>(a, st);
   // few long rows: in parts of at least 512 slots, as long as all parts run at once
   if (slots >= 8 * 512 && a.B * 8 <= ctas) return launch_score<T, 8, 8>(a, st);
   if (slots >= 4 * 512 && a.B * 4 <= ctas) return launch_score<T, 8, 4>(a, st);
@@ -724,7 +730,8 @@ template <class T>
 int run_score_grad(ScoreGradArgs a, cudaStream_t st) {
   const int64_t slots = a.V / (16 / (int)sizeof(T)) + 2;  // whatever the row's start
   a.parts = 1;
-  if (slots <= 256) return launch_status(launch_dependent(fw_logprob_grad_kernel<T, 1>, (a.B + 7) / 8, 256, 0, 1, st, a));
+  if (by_warps(slots, a.B))
+    return launch_status(launch_dependent(fw_logprob_grad_kernel<T, 1>, (a.B + 7) / 8, 256, 0, 1, st, a));
   // parts of no less than one step of a CTA, as many as run at once
   const int64_t most = (slots + 256 * kGradBatch - 1) / (256 * kGradBatch), want = (int64_t)sm_count() * kGradCtas / a.B;
   a.parts = (int)(want < 1 ? 1 : want < most ? want : most);
