@@ -28,7 +28,7 @@ constexpr float kLost = 8.0779357e-28f;  // 2^-90: squares under 2^-149 are gone
 
 // Tensors of one launch.  Tile t of the launch is in the tensor i with
 // first[i] <= t < first[i + 1]; groups of 8 elements start where the written
-// tensor (the read one, for the norm) is aligned to 16 bytes.
+// tensor (the read one, for the norm) is aligned to their size, 16 or 32 bytes.
 template <int N>
 struct Table {
   int n, tiles;
@@ -40,19 +40,34 @@ struct Table {
 };
 
 __device__ __forceinline__ int groups_off(const void* p, int type) {  // elements before p's first group boundary
-  return (int)((reinterpret_cast<uintptr_t>(p) & 15u) >> (type == FWB_DTYPE_F32 ? 2 : 1));
+  const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+  return type == FWB_DTYPE_F32 ? (int)(a & 31u) >> 2 : (int)(a & 15u) >> 1;
 }
 
 template <class T>
 constexpr int kParts = sizeof(T) / 2;  // 16-byte slots per group
 
+// A group at an aligned address, by one access: whole sectors of 32 bytes.
+__device__ __forceinline__ void load_whole(uint4 (&u)[1], const void* p) { u[0] = ld_global16_once(p); }
+__device__ __forceinline__ void load_whole(uint4 (&u)[2], const void* p) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0].x), "=r"(u[0].y), "=r"(u[0].z), "=r"(u[0].w), "=r"(u[1].x), "=r"(u[1].y), "=r"(u[1].z), "=r"(u[1].w)
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store_whole(void* p, const uint4 (&u)[1]) { *static_cast<uint4*>(p) = u[0]; }
+__device__ __forceinline__ void store_whole(void* p, const uint4 (&u)[2]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0].x), "r"(u[0].y), "r"(u[0].z),
+               "r"(u[0].w), "r"(u[1].x), "r"(u[1].y), "r"(u[1].z), "r"(u[1].w)
+               : "memory");
+}
+
 // Elements e .. e + 8 of x, which may start anywhere; outside [0, n) as zero.
 template <class T>
 __device__ __forceinline__ void load_group(uint4 (&u)[kParts<T>], const T* x, int64_t e, int64_t n) {
   constexpr int V = 16 / sizeof(T);
-  if (e >= 0 && e + 8 <= n && (reinterpret_cast<uintptr_t>(x + e) & 15u) == 0) {
-#pragma unroll
-    for (int i = 0; i < kParts<T>; ++i) u[i] = ld_global16_once(x + e + i * V);
+  if (e >= 0 && e + 8 <= n && (reinterpret_cast<uintptr_t>(x + e) & (8 * sizeof(T) - 1)) == 0) {
+    load_whole(u, x + e);
   } else {
 #pragma unroll
     for (int i = 0; i < kParts<T>; ++i) u[i] = load_elems(x + e + i * V, x, x + n);
@@ -173,10 +188,15 @@ __device__ __forceinline__ void tile_scale(const TI* x, TO* y, int64_t e0, int64
     for (int i = 0; i < kParts<TI>; ++i) unpack16<TI>(u[g][i], v + i * (16 / (int)sizeof(TI)));
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] *= f;
+    constexpr int V = 16 / sizeof(TO);
+    uint4 o[kParts<TO>];
 #pragma unroll
-    for (int i = 0; i < kParts<TO>; ++i) {
-      constexpr int V = 16 / sizeof(TO);
-      store_slot(y, e + i * V, n, true, pack_slot<TO>(v + i * V));
+    for (int i = 0; i < kParts<TO>; ++i) o[i] = pack_slot<TO>(v + i * V);
+    if (e >= 0 && e + 8 <= n) {
+      store_whole(y + e, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kParts<TO>; ++i) store_slot(y, e + i * V, n, false, o[i]);
     }
   }
 }
@@ -260,7 +280,8 @@ int64_t fill(const Tensors& t, int64_t at, Table<N>* out) {
     if (t.numel[at] == 0) continue;
     const bool w = t.out != nullptr;
     const int type = w ? t.type_out[at] : t.type_in[at];
-    const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(w ? t.out[at] : t.in[at]) & 15u) / type_size(type);
+    const int size = type_size(type);
+    const int64_t off = (int64_t)(reinterpret_cast<uintptr_t>(w ? t.out[at] : t.in[at]) & (uintptr_t)(8 * size - 1)) / size;
     const int64_t more = (t.numel[at] + off + kTile - 1) / kTile;
     const int i = out->n++;
     out->in[i] = t.in[at];

@@ -196,23 +196,34 @@ py::tuple lm_head_log_probs(const Tensor& hidden, const Tensor& weight, const Te
 
 // ---------------------------------------------------------------- gradient norm and clipping
 struct List {
-  std::vector<Tensor> held;  // what the pointers are to: the tensors, or dense copies
+  std::vector<Tensor> held;  // copies that the pointers are to
   std::vector<const void*> in;
   std::vector<void*> out;
   std::vector<int64_t> numel;
   std::vector<int32_t> types, out_types;
+  explicit List(size_t n) {
+    in.reserve(n);
+    out.reserve(n);
+    numel.reserve(n);
+    types.reserve(n);
+    out_types.reserve(n);
+  }
 };
 
 bool dense(const Tensor& t) { return t.is_non_overlapping_and_dense(); }
 
+[[noreturn]] void refuse_type(const char* op, const char* what) { throw py::type_error(std::string(op) + ": " + what); }
+
+[[noreturn]] void refuse(const char* op, const char* what) { throw py::value_error(std::string(op) + ": " + what); }
+
 void check_grads(const std::vector<Tensor>& grads, const char* op) {
-  const auto say = [op](const char* what) { return std::string(op) + ": " + what; };
-  value_check(!grads.empty(), say("no tensors").c_str());
+  if (grads.empty()) refuse(op, "no tensors");
+  const auto device = grads[0].device();
   for (const auto& t : grads) {
-    type_check(t.is_cuda(), say("gradients must be CUDA tensors (this build has no CPU path)").c_str());
-    type_check(t.layout() == torch::kStrided && is_float(t),
-               say("gradients must be dense float32, bfloat16 or float16 tensors").c_str());
-    value_check(t.device() == grads[0].device(), say("gradients must be on one device").c_str());
+    if (!t.is_cuda()) refuse_type(op, "gradients must be CUDA tensors (this build has no CPU path)");
+    if (t.layout() != torch::kStrided || !is_float(t))
+      refuse_type(op, "gradients must be dense float32, bfloat16 or float16 tensors");
+    if (t.device() != device) refuse(op, "gradients must be on one device");
     no_tangent(t, op);
   }
 }
@@ -233,10 +244,11 @@ Tensor grad_norm(const std::vector<Tensor>& grads, const OptTensor& status) {
                 "grad_norm: not differentiable; pass gradients (p.grad), or detach");
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(grads[0].device());
-  List l;
+  List l(grads.size());
   for (const auto& t : grads) {
-    l.held.push_back(dense(t) ? t : t.contiguous());
-    l.in.push_back(l.held.back().data_ptr());
+    const bool as_is = dense(t);
+    if (!as_is) l.held.push_back(t.contiguous());
+    l.in.push_back(as_is ? t.data_ptr() : l.held.back().data_ptr());
     l.numel.push_back(t.numel());
     l.types.push_back(code(t));
   }
@@ -297,23 +309,27 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
                 "clip_grad_norm_: norm must be one float32 value on the gradients' device");
   at::NoGradGuard no_grad;
   const c10::cuda::CUDAGuard guard(grads[0].device());
-  List l;
+  List l(grads.size());
   std::vector<std::pair<Tensor, Tensor>> back;  // results that are copied to where they belong
   for (size_t i = 0; i < grads.size(); ++i) {
     const auto &g = grads[i], &d = dest[i];
-    Tensor from = dense(g) ? g : g.contiguous(), to = d;
-    if (!dense(d) || (d.strides() != from.strides() && !(d.is_contiguous() && from.is_contiguous()))) {
-      // an element of `to` is where it is in `from`
-      to = out.has_value() ? at::empty_strided(from.sizes(), from.strides(), d.options()) : from;
-      back.emplace_back(d, to);
+    l.numel.push_back(g.numel());
+    l.types.push_back(code(g));
+    l.out_types.push_back(code(d));
+    if (dense(g) && (!out.has_value() || (dense(d) && (d.strides() == g.strides() || (d.is_contiguous() && g.is_contiguous()))))) {
+      l.in.push_back(g.data_ptr());
+      l.out.push_back(d.data_ptr());
+      continue;
     }
+    const Tensor from = dense(g) ? g : g.contiguous();
+    Tensor to = out.has_value() ? d : from;
+    if (!dense(to) || (to.strides() != from.strides() && !(to.is_contiguous() && from.is_contiguous())))
+      to = at::empty_strided(from.sizes(), from.strides(), d.options());  // an element is where it is in `from`
+    if (!to.is_same(d)) back.emplace_back(d, to);
     l.held.push_back(from);
     l.held.push_back(to);
     l.in.push_back(from.data_ptr());
     l.out.push_back(to.data_ptr());
-    l.numel.push_back(g.numel());
-    l.types.push_back(code(from));
-    l.out_types.push_back(code(to));
   }
   for (const auto& b : back) at::assert_no_internal_overlap(b.first);
   check_overlaps(l);
