@@ -321,6 +321,16 @@ __device__ __forceinline__ void top_bound(TopShared<NW>& top, int k) {
   if (above < k && reach >= k) top.bound = own;  // equal ones all write it
 }
 
+// How many of n keys are above `own`.
+__device__ __forceinline__ int keys_above(const uint64_t* keys, int n, uint64_t own) {
+  int above = 0, i = 0;
+  for (; i + 8 <= n; i += 8)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) above += keys[i + j] > own;
+  for (; i < n; ++i) above += keys[i] > own;
+  return above;
+}
+
 // Leaves the k largest keys of the segment in top.best.  `largest` is this
 // thread's largest element, the bound is there, top.n and top.n_who are 0.
 template <class T, int NW>
@@ -382,8 +392,7 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   if (n <= kFound) {
     for (int i = tid; i < n; i += NT) {
       const uint64_t own = top.found[i];
-      int rank = 0;
-      for (int o = 0; o < n; ++o) rank += top.found[o] > own;
+      const int rank = keys_above(top.found, n, own);
       if (rank < k) top.best[rank] = own;
     }
     group_sync<NW>();
@@ -429,8 +438,7 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   group_sync<NW>();
   const uint64_t own = held[lane];
   int rank = 0;
-  for (int g = 0; g < NW; ++g)
-    for (int i = 0; i < 32; ++i) rank += top.held[g][i] > own;
+  for (int g = 0; g < NW; ++g) rank += keys_above(top.held[g], 32, own);
   if (own != 0 && rank < k) top.best[rank] = own;
   group_sync<NW>();
 }
@@ -574,8 +582,7 @@ __global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 
         m = part[0].m;
         logs = part[0].s;
         if (own != 0) {
-          int i = 0;
-          for (int o = 0; o < CL * a.k; ++o) i += top.found[o] > own;
+          const int i = keys_above(top.found, CL * a.k, own);
           if (i < a.k) give_top(own, i);
         }
       }
