@@ -35,7 +35,14 @@ namespace {
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -200.0f;  // 2^kFloor is 0 in fp32; keeps 0 * t finite
-constexpr int kBatch = 4;          // slots in flight per thread
+// Slots in flight per thread, and CTAs of 256 threads per SM.  4096 x 32000
+// without and with 5 alternatives, float32: 4 slots and 4 CTAs 82 and 97 us, 4
+// and 5 80 and 93, 8 and 4 77 and 93; bfloat16: 52 and 66, 48 and 60, 48 and 68.
+template <class T>
+constexpr int kBatch = sizeof(T) == 4 ? 8 : 4;
+template <class T, int CL>
+constexpr int kCtas = sizeof(T) == 2 && CL == 1 ? 5 : 4;
+constexpr int kAgain = 4;  // slots in flight per thread where they are read again
 
 struct ScoreArgs {
   const void* z;
@@ -157,7 +164,7 @@ constexpr float kFloor16 = std::is_same<T, __nv_bfloat16>::value ? -1.2676506e30
 // Elements that are -inf or far down are raised so that 0 * t is finite: t
 // itself, or in pairs the 16-bit elements, if their floor is 200 powers of two
 // under the reference.  Pairs take 4.5 instructions an element with the
-// maximum, single ones 8 (4096 x 32000 bfloat16: 43 and 55 us; HBM takes 40).
+// maximum, single ones 8 (4096 x 32000 bfloat16: 51 and 55 us).
 template <class T>
 struct Running {
   float m, ref, r2, off, lim;
@@ -361,28 +368,28 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   if (tid < 32) top.best[tid] = 0;
   group_sync<NW>();
   const int n_who = top.n_who;
-  if (seg.k1 - seg.k0 <= kBatch * NT) {  // few slots each: every thread its own
+  if (seg.k1 - seg.k0 <= kAgain * NT) {  // few slots each: every thread its own
     if (in) {
-      uint4 x[kBatch];
+      uint4 x[kAgain];
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
+      for (int b = 0; b < kAgain; ++b)
         if (seg.k0 + tid + b * NT < seg.k1) x[b] = seg.load(seg.k0 + tid + b * NT);
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b)
+      for (int b = 0; b < kAgain; ++b)
         if (seg.k0 + tid + b * NT < seg.k1) look(x[b], seg.k0 + tid + b * NT);
     }
-  } else {  // a warp per thread of the list, its slots over the lanes, kBatch such loads in flight
-    for (int t0 = w; t0 < n_who; t0 += kBatch * NW) {
+  } else {  // a warp per thread of the list, its slots over the lanes, kAgain such loads in flight
+    for (int t0 = w; t0 < n_who; t0 += kAgain * NW) {
       for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
-        uint4 x[kBatch];
-        int kk[kBatch];
+        uint4 x[kAgain];
+        int kk[kAgain];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
+        for (int b = 0; b < kAgain; ++b) {
           kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
           if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
         }
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b)
+        for (int b = 0; b < kAgain; ++b)
           if (kk[b] < seg.k1) look(x[b], kk[b]);
       }
     }
@@ -446,8 +453,8 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
 // One row per cluster of CL CTAs of NW warps, each taking an equal part of it;
 // or, for NW = 1, one row per warp of a CTA.
 template <class T, int NW, bool TOP, int CL>
-__global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 4 : NW == 4 ? 8 : 3) fw_logprob_kernel(ScoreArgs a) {
-  constexpr int VN = 16 / sizeof(T), NT = NW * 32;
+__global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? kCtas<T, CL> : NW == 4 ? 8 : 3) fw_logprob_kernel(ScoreArgs a) {
+  constexpr int VN = 16 / sizeof(T), NT = NW * 32, N = kBatch<T>;
   constexpr int R = NW == 1 ? kWarpRows : 1;
   __shared__ Sums parts[R][NW];
   __shared__ Sums whole;  // of this CTA, for its cluster
@@ -489,18 +496,18 @@ __global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 
   seg.hi = (int)(((int64_t)seg.off + a.V) / VN);
   const float c = a.inv_t * kLog2e;
   Running<T> run;
-  for (int k0 = seg.k0 + tid; k0 < seg.k1; k0 += NT * kBatch) {
-    uint4 x[kBatch];
-    if (k0 >= seg.lo && k0 + (kBatch - 1) * NT < min(seg.hi, seg.k1)) {
+  for (int k0 = seg.k0 + tid; k0 < seg.k1; k0 += NT * N) {
+    uint4 x[N];
+    if (k0 >= seg.lo && k0 + (N - 1) * NT < min(seg.hi, seg.k1)) {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) x[i] = ld_global16_once(row + seg.element(k0 + i * NT));
+      for (int i = 0; i < N; ++i) x[i] = ld_global16_once(row + seg.element(k0 + i * NT));
     } else {
 #pragma unroll
-      for (int i = 0; i < kBatch; ++i) x[i] = k0 + i * NT < seg.k1 ? seg.load(k0 + i * NT) : neg_inf_slot<T>();
+      for (int i = 0; i < N; ++i) x[i] = k0 + i * NT < seg.k1 ? seg.load(k0 + i * NT) : neg_inf_slot<T>();
     }
     float bm = -CUDART_INF_F;
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) bm = max_nan(bm, slot_max_nan<T>(x[i]));
+    for (int i = 0; i < N; ++i) bm = max_nan(bm, slot_max_nan<T>(x[i]));
     run.m = max_nan(run.m, bm);
     if (!(bm <= run.lim)) run.move(run.m, c);
     if (run.ref != -CUDART_INF_F) run.add(x, c);
