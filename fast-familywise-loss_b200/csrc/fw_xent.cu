@@ -41,9 +41,15 @@
 // from which the entropy is h_r = log S - (sum exp(t) t) / S, two positive
 // terms, and with upstream factors a of logp and b of the entropy the logit
 // gradient is, with l = log p,
-//   T G_rj = a_r (1[j = y(r)] - p_rj) - b_r p_rj (l_rj + h_r),
-// its factor per row max(|a_r|, |b_r|), split as above.  |p (l + h)| is at most
-// (log V) / 4 + 0.3, under 5.2, hence 2^13 in the place of 2^15 for float16.
+//   T G_rj = a_r (1[j = y(r)] - p_rj) - b_r p_rj (l_rj + h_r).
+// Its factors are in G whole: they have no common power of two to be split off
+// where a and b differ, and a row of H is then rounded no further.  What the
+// rounding takes from the label's entry, which would show in a whole row of dH,
+// is kept in fp32 and added to dH as that much of the label's row of W.  The
+// error of dW is 1.4 times that of a form in 32 bits rounded at the end (each of
+// its largest terms carries one rounding), dH's 1.0 to 1.1 times.
+// |p (l + h)| is at most (log V) / 4 + 0.3, under 5.2, hence 2^13 in the place
+// of 2^15 for float16.
 #include <cmath>
 
 #include "fw_reduce.cuh"
@@ -456,29 +462,27 @@ struct Upstream {
   const float* go_ent;  // the entropy's
   float inv_t;
 
-  // g_r
+  // g_r; of BOTH the larger of the two
   __device__ float factor(int r) const {
     return both ? max_nan(go ? fabsf(go[r]) : 0.0f, go_ent ? fabsf(go_ent[r]) : 0.0f) : go[r];
   }
-  __device__ float unit() const { return both ? kF16UnitBoth : kF16Unit; }
   // s_r, scaled to the range of the type; a factor that is not finite stands for itself
   __device__ float in_g(int r) const {
     if (!per_row) return f16 ? kF16Unit : 1.0f;
-    const float g = factor(r), s = pow2_above(g);
+    const float g = go[r], s = pow2_above(g);
     if (!(s < CUDART_INF_F)) return g;
-    return f16 && *top > 0.0f ? s / *top * unit() : s;
+    return f16 && *top > 0.0f ? s / *top * kF16Unit : s;
   }
-  // -a_r / g_r and -b_r / g_r; NaN where g_r is not finite
-  __device__ float2 shares(int r) const {
-    const float g = factor(r);
-    if (g == 0.0f) return make_float2(0.0f, 0.0f);
-    if (!(g < CUDART_INF_F)) return make_float2(CUDART_NAN_F, CUDART_NAN_F);
-    return make_float2(go ? -go[r] / g : 0.0f, go_ent ? -go_ent[r] / g : 0.0f);
+  // BOTH: -a_r and -b_r, scaled to the range of the type; NaN where either is not finite
+  __device__ float2 in_g_both(int r) const {
+    if (!(factor(r) < CUDART_INF_F)) return make_float2(CUDART_NAN_F, CUDART_NAN_F);
+    const float a = go ? -go[r] : 0.0f, b = go_ent ? -go_ent[r] : 0.0f;
+    return f16 && *top > 0.0f ? make_float2(a / *top * kF16UnitBoth, b / *top * kF16UnitBoth) : make_float2(a, b);
   }
-  // f_r; 1 where the factor is in G (0, not finite) or common
+  // f_r; 1 where the factor is in G (0, not finite, BOTH) or common
   __device__ float rest(int r) const {
-    if (!per_row) return 1.0f;
-    const float g = factor(r), s = pow2_above(g);
+    if (!per_row || both) return 1.0f;
+    const float g = go[r], s = pow2_above(g);
     return s > 0.0f && s < CUDART_INF_F ? g / s : 1.0f;
   }
   // common factor taken out after the sums
@@ -540,6 +544,7 @@ struct GradArgs {
   int v0, vn;  // first column of the piece, its columns rounded up to 256
   int32_t* status;
   const float* entropy;  // BOTH: packed
+  float* label_rest;     // BOTH: what rounding took from the label's entry, packed
 };
 
 template <class T, TcKind K, bool BOTH>
@@ -548,8 +553,8 @@ struct GradTile {
   struct State {
     float lse, coef;
     int y;
-    float h;        // BOTH: the row's entropy,
-    float2 shares;  // its factors over g_r
+    float h;      // BOTH: the row's entropy,
+    float2 both;  // and its factors
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
@@ -571,10 +576,12 @@ struct GradTile {
     const bool live = row < a.head->rows;
     st.y = live ? a.label[row] : -2;  // -2: not a live row
     st.lse = live ? a.lse[row] : 0.0f;
-    st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
     if constexpr (BOTH) {
+      st.coef = 1.0f;
       st.h = live ? a.entropy[row] : 0.0f;
-      st.shares = live ? a.up.shares(a.row_of[row]) : make_float2(0.0f, 0.0f);
+      st.both = live ? a.up.in_g_both(a.row_of[row]) : make_float2(0.0f, 0.0f);
+    } else {
+      st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
     }
   }
   template <bool LOST, class Done>
@@ -596,8 +603,11 @@ struct GradTile {
           q = CUDART_NAN_F;
         } else if constexpr (BOTH) {  // of a bad row lse and h are NaN, and so is q
           const float l = fmaxf(fmaf(v[i], a.up.inv_t, -lse), kExpFloor * kLn2), p = exp2_hw(l * kLog2e);
-          q = p * fmaf(st.shares.y, l + st.h, st.shares.x);
-          if (t.n0 + c + i == y) q -= st.shares.x;
+          q = p * fmaf(st.both.y, l + st.h, st.both.x);
+          if (t.n0 + c + i == y) {
+            q -= st.both.x;
+            a.label_rest[row] = q - Elem<T>::to_f(Elem<T>::from_f(q));
+          }
         } else {
           q = exp2_hw((v[i] - lse) * kLog2e);
           if (t.n0 + c + i == y) q -= 1.0f;
@@ -635,6 +645,21 @@ struct ProductArgs {
   int max_splits;  // sums there is room for
   int pairs;       // CTA pairs of the launch
   int32_t* status;
+  // BOTH: dH takes label_rest of the label's row of the weight
+  const float* label_rest;
+  const int32_t* label;
+  const void* w;
+  int64_t ldw;
+
+  // 8 columns of it from c on, times `by`, added to v
+  template <class T>
+  __device__ void add_label(int y, int c, float by, float* v) const {
+    const T* p = static_cast<const T*>(w) + (int64_t)y * ldw + c;
+    float x[8];
+    unpack16<T>(c + 8 <= D ? ld_global16(p) : load_elems(p, p, p + (D - c)), x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = fmaf(by, x[i], v[i]);
+  }
 
   __device__ int v_tiles() const { return dweight ? (min(vn, V - v0) + kTileM - 1) / kTileM : 0; }
   // The same for every piece (whole ones are taken to reckon with).
@@ -648,13 +673,15 @@ struct ProductArgs {
   }
 };
 
-template <class T, TcKind K>
+template <class T, TcKind K, bool BOTH>
 struct ProductTile {
   using Args = ProductArgs;
   struct State {
     int mine;  // dH: the given row of this lane's row
     float f;   // its factor
     bool zero;
+    float rest;  // BOTH: its label_rest, 0 without a label
+    int label;
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
@@ -733,6 +760,10 @@ struct ProductTile {
     st.mine = dh ? a.row_of[row] : -1;
     st.zero = t.nk == 0 || (dh && row >= a.head->rows);
     st.f = st.zero ? 0.0f : dh ? plan.back * a.up.rest(st.mine) : plan.back;
+    if constexpr (BOTH) {
+      st.label = dh && !st.zero ? a.label[row] : -1;
+      st.rest = st.label >= 0 ? a.label_rest[row] : 0.0f;
+    }
   }
   template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st, int,
@@ -770,6 +801,13 @@ struct ProductTile {
         }
       }
       if (!store) continue;
+      if constexpr (BOTH && !LOST) {
+        if (st.rest != 0.0f) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8)
+            if (c + i < cols) a.template add_label<T>(st.label, t.n0 + s0 + c + i, st.rest, v + i);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = st.zero ? 0.0f : v[i] * st.f;
       stage_block<T, BN / 2>(sm, v, p.lane, c);
@@ -785,7 +823,7 @@ struct ProductTile {
 };
 
 // dH from the sums of its splits; one warp per row and 128 columns.
-template <class T>
+template <class T, bool BOTH>
 __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
   wait_prior_kernel();
   allow_dependent_launch();
@@ -805,6 +843,17 @@ __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
       for (int q = 0; q < splits; ++q) {
         const float4 x = *reinterpret_cast<const float4*>(a.sum + ((int64_t)q * a.Bp + r) * a.lds + c);
         v.x += x.x, v.y += x.y, v.z += x.z, v.w += x.w;
+      }
+      if constexpr (BOTH) {
+        const int y = a.label[r];
+        if (y >= 0) {
+          const float by = a.label_rest[r];
+          const T* w = static_cast<const T*>(a.w) + (int64_t)y * a.ldw + c;
+          v.x = fmaf(by, ld_elem(w), v.x);
+          if (c + 1 < a.D) v.y = fmaf(by, ld_elem(w + 1), v.y);
+          if (c + 2 < a.D) v.z = fmaf(by, ld_elem(w + 2), v.z);
+          if (c + 3 < a.D) v.w = fmaf(by, ld_elem(w + 3), v.w);
+        }
       }
       const float f = back * a.up.rest(to);
       v.x *= f, v.y *= f, v.z *= f, v.w *= f;
@@ -835,7 +884,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, part_t, zy, loss_pack, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, splits, top, g, sum, hs, bwd_bytes;
+  int64_t piece, pieces, splits, top, label_rest, g, sum, hs, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = false) {
@@ -864,6 +913,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = fal
   p.pieces = (Vp + p.piece - 1) / p.piece;
   at = 0;
   p.top = at, at += 256;
+  p.label_rest = at, at += both ? up(4 * p.Bp, 256) : 0;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
   // as many as one row tile could use, 16 stages of K each, within kSumBytes
   p.splits = sm_count() / 2 / ((D + kTileN - 1) / kTileN);
@@ -872,7 +922,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = fal
   if (p.splits > p.piece / 64 / 16) p.splits = p.piece / 64 / 16;
   if (p.splits < 1) p.splits = 1;
   p.sum = at, at += p.pieces > 1 || p.splits > 1 ? up(4 * p.splits * p.Bp * up(D, 32), 256) : 0;
-  p.hs = at, at += up(2 * p.Bp * p.Dp, 256);  // factors per row
+  p.hs = at, at += both ? 0 : up(2 * p.Bp * p.Dp, 256);  // factors per row
   p.bwd_bytes = at;
   return p;
 }
@@ -939,7 +989,7 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   const char* hw = state + p.hp;  // dW's operand
   if (per_row) {
     if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, u, top);
-    if (dweight) {
+    if (dweight && !BOTH) {
       T* hs = reinterpret_cast<T*>(ws + p.hs);
       const int64_t cap = (int64_t)sm_count() * 8;
       fw_xent_scale_kernel<T><<<(unsigned)(p.Bp < cap ? p.Bp : cap), 256, 0, st>>>(
@@ -960,17 +1010,18 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   for (int64_t i = 0; i < p.pieces; ++i) {
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
     const GradArgs ga = {head, label, row_of, reinterpret_cast<const float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
-                         v0, vn, status, reinterpret_cast<const float*>(state + p.entropy)};
+                         v0, vn, status, reinterpret_cast<const float*>(state + p.entropy),
+                         reinterpret_cast<float*>(ws + p.label_rest)};
     if (launch_gemm<GradTile<T, K, BOTH>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
     const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
     const int64_t pairs = sm_count() / 2;
     const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
                             i == 0, i == p.pieces - 1, (int)p.piece, (int)p.splits,
-                            (int)(tiles < pairs ? tiles : pairs), status};
-    if (launch_gemm<ProductTile<T, K>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
+                            (int)(tiles < pairs ? tiles : pairs), status, ga.label_rest, label, w, ldw};
+    if (launch_gemm<ProductTile<T, K, BOTH>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
     if (dhidden && pa.last && p.splits > 1) {
       const int64_t need = (p.Bp * ((D + 127) / 128) + 7) / 8, cap = (int64_t)sm_count() * 16;
-      if (launch_dependent(fw_xent_dhidden_kernel<T>, need < cap ? need : cap, 256, 0, 1, st, pa) != cudaSuccess)
+      if (launch_dependent(fw_xent_dhidden_kernel<T, BOTH>, need < cap ? need : cap, 256, 0, 1, st, pa) != cudaSuccess)
         return FWB_E_LAUNCH;
     }
   }

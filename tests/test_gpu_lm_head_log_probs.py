@@ -4,10 +4,9 @@ against the 64-bit definition.
 Logits: products of 16-bit numbers are exact in fp32, and D additions with
 truncation are off by 2 * E32 of the absolute terms each at most (e_z); what
 follows from logits that are off so is score_ref's.  A logit gradient is rounded
-once to the operands' type; dweight's other operand, hidden times the factor's
-part in [0.5, 1), once more; both sums are truncating fp32 additions.  float16's
-logit gradient may be under its range: half of 2^-24 over 2^13, of the largest
-factor's next power of two.
+once to the operands' type (for dhidden the label's entry is not); both sums are
+truncating fp32 additions.  float16's logit gradient may be under its range:
+half of 2^-24 over 2^13, of the largest factor's next power of two.
 """
 import ctypes
 
@@ -47,7 +46,7 @@ def reference(hidden, weight, tokens, temperature=1.0, a=None, b=None, ignore=-1
     eG = torch.where(live[:, None], eG, torch.zeros_like(eG))
     dh, dw = G @ w, G.t() @ h
     e_dh = eG @ w.abs() + (G.abs() @ w.abs()) * (2 * V + 8) * R.E32 + R.rounded(dh, dtype)
-    e_dw = eG.t() @ h.abs() + (G.abs().t() @ h.abs()) * ((2 * B + 8) * R.E32 + R.U[dtype] * (1 + R.U[dtype])) + R.rounded(dw, dtype)
+    e_dw = eG.t() @ h.abs() + (G.abs().t() @ h.abs()) * (2 * B + 8) * R.E32 + R.rounded(dw, dtype)
     return r, (dh, e_dh), (dw, e_dw)
 
 
