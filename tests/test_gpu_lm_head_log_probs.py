@@ -167,6 +167,38 @@ def test_upstream_factors(value, dtype):
     R.within(got[0][rest], dh[0][rest], dh[1][rest], "other rows")
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,D,V", [(700, 300, 1), (700, 300, 40), (900, 100, 3000), (513, 136, 700)])
+def test_labels_met_again_and_again(B, D, V, dtype):
+    """More rows than a list of finds holds with labels of one 32 rows of the weight, and with one label."""
+    g = R.gen(B + V)
+    h, w = R.normal((B, D), dtype, g), R.normal((V, D), dtype, g, D ** -0.5)
+    y = torch.randint(0, min(V, 45), (B,), generator=g, device="cuda") + (V - min(V, 45))
+    check(h, w, y)
+    y[: B // 2] = V // 2
+    y[::7] = -100
+    check(h, w, y, kind="logp")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rounding_of_the_labels_entry_is_made_good(dtype):
+    """A label's gradient is the one large entry of its row; both products have to come out as if it were not rounded:
+    within the rounding of the result and a twentieth of the entry's."""
+    g = R.gen(21)
+    h, w = R.normal((64, 64), dtype, g, 1e-3), R.normal((4096, 64), dtype, g)  # probabilities of 2^-12 each
+    y = torch.randperm(4096, generator=g, device="cuda")[:64]
+    hh, ww = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    a = torch.rand(64, generator=g, device="cuda") + 1.0
+    dh, dw = torch.autograd.grad(fw.lm_head_log_probs(hh, ww, y)[0], (hh, ww), a)
+    _, (eh, _), (ew, _) = reference(h, w, y, 1.0, a)
+    term = a.double()[:, None] * w[y].double().abs()
+    # the other 4095 entries are 2^-12 of the label's, each rounded: their sum of absolute terms is under w's largest
+    R.within(dh, eh, R.rounded(eh, dtype) + term * R.U[dtype] / 20 + R.U[dtype] * 2.0 ** -12 * 64 * 5 * a[:, None] * 2, "dhidden")
+    got, want = dw[y], ew[y]
+    R.within(got, want, R.rounded(want, dtype) + a[:, None].double() * h.double().abs() * R.U[dtype] / 20
+             + R.U[dtype] * 2.0 ** -12 * 64 * 5e-3 * 2, "dweight")
+
+
 def test_equal_to_the_loss():
     """-logp is lm_head_cross_entropy's loss, both within their bounds of one value; and the entropy's share is apart."""
     g = R.gen(7)
