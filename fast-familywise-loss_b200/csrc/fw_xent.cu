@@ -678,6 +678,7 @@ struct ProductArgs {
 template <class T, TcKind K, bool BOTH>
 struct ProductTile {
   using Args = ProductArgs;
+  static constexpr int kHeld = BOTH ? 8 : 1;
   struct State {
     int mine;  // dH: the given row of this lane's row
     float f;   // its factor
@@ -685,6 +686,8 @@ struct ProductTile {
     float rest;  // BOTH: its label_rest, 0 without a label
     int label;
     int found, seen;  // BOTH, dW: entries of the warp's list, packed rows looked at for it
+    uint2 h[kHeld];   // of few finds: 4 columns of their rows of H per lane,
+    float by[kHeld];  // and label_rest
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
@@ -767,17 +770,33 @@ struct ProductTile {
       st.label = dh && !st.zero ? a.label[row] : -1;
       st.rest = st.label >= 0 ? a.label_rest[row] : 0.0f;
       st.found = st.seen = 0;
-      if (!dh) st.found = find(a, list_of(p), p.lane, a.v0 + t.m0 + p.row, &st.seen);
+      if (!dh) {
+        st.found = find(a, list_of(p), p.lane, a.v0 + t.m0 + p.row, &st.seen);
+        if (held(a, st)) {
+          const int c = t.n0 + p.share * (BN / 2) + 4 * p.lane;
+#pragma unroll
+          for (int i = 0; i < kHeld; ++i) {
+            if (i >= st.found) break;
+            const int64_t r = list_of(p)[i * kWords] >> 5;
+            st.h[i] = make_uint2(0u, 0u);
+            if (c < a.ldh) st.h[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.hp) + r * a.ldh + c);
+            st.by[i] = a.label_rest[r];
+          }
+        }
+      }
     }
   }
+  // Few finds: their rows of H come while the products run.
+  __device__ static bool held(const Args& a, const State& st) { return st.found <= kHeld && st.seen >= a.head->rows; }
 
   // BOTH: dW's rows take label_rest times the rows of H that have them as
   // labels.  A warp owns 32 rows v, looks through the labels for them while the
   // tile's products run, and keeps up to 32 finds (packed row, v), in the order
-  // of the rows, in the spare word of its staging rows; where there are more it
-  // takes them 32 by 32, again for every 16 columns.  The sum of the finds is
-  // formed 16 columns at a time, a lane each, in the last words of the staging
-  // rows, which are written last.  (4014 live rows, 128256 x 4096 bfloat16: the
+  // of the rows, in the spare word of its staging rows.  Up to kHeld finds have
+  // their rows of H loaded meanwhile, four columns a lane.  More are summed 16
+  // columns at a time, a lane each, in the last words of the staging rows, which
+  // are written last; and where there are more than 32 they are looked for again
+  // for every 16 columns, 32 by 32.  (4014 live rows, 128256 x 4096 bfloat16: the
   // error of dW 1.4 to 1.0 times that of a form in 32 bits rounded once.)
   static constexpr int kWords = kStageWords<BN / 2>;
   __device__ static uint32_t* list_of(const TcPart& p) { return reinterpret_cast<uint32_t*>(p.smem) + kWords - 1; }
@@ -809,6 +828,24 @@ struct ProductTile {
     }
     __syncwarp();
     return n;
+  }
+  // The same from what the lanes hold: columns c .. c + 32 of the warp's 128.
+  __device__ static void add_held(const TcPart& p, const State& st, int c, float* v) {
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (i >= st.found) break;
+      const bool mine = p.lane == (int)(list_of(p)[i * kWords] & 31u);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {  // columns 4 j .. 4 j + 4 are lane (c / 4 + j)'s
+        const uint32_t lo = __shfl_sync(kFull, st.h[i].x, c / 4 + j), hi = __shfl_sync(kFull, st.h[i].y, c / 4 + j);
+        if (mine) {
+          v[4 * j] = fmaf(st.by[i], Elem<T>::bits_to_f(lo & 0xffffu), v[4 * j]);
+          v[4 * j + 1] = fmaf(st.by[i], Elem<T>::bits_to_f(lo >> 16), v[4 * j + 1]);
+          v[4 * j + 2] = fmaf(st.by[i], Elem<T>::bits_to_f(hi & 0xffffu), v[4 * j + 2]);
+          v[4 * j + 3] = fmaf(st.by[i], Elem<T>::bits_to_f(hi >> 16), v[4 * j + 3]);
+        }
+      }
+    }
   }
   // v += the finds' sum for columns c .. c + 16 of the matrix.
   __device__ static void add_found(const Args& a, const TcPart& p, State& st, int v0, int c, float* v) {
@@ -891,7 +928,9 @@ struct ProductTile {
           for (int i = 0; i < 32; i += 8)
             if (c + i < cols) a.template add_label<T>(st.label, t.n0 + s0 + c + i, st.rest, v + i);
         }
-        if (!dh && (st.found > 0 || st.seen < a.head->rows)) {
+        if (!dh && held(a, st)) {
+          add_held(p, st, c, v);
+        } else if (!dh) {
           add_found(a, p, st, a.v0 + r0, t.n0 + s0 + c, v);
           add_found(a, p, st, a.v0 + r0, t.n0 + s0 + c + 16, v + 16);
         }
