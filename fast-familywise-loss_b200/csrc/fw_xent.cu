@@ -54,6 +54,7 @@
 
 #include "fw_reduce.cuh"
 #include "fw_rowslots.cuh"
+#include "fw_sort.cuh"
 #include "fw_tc_gemm.cuh"
 
 namespace fwb200 {
@@ -80,10 +81,10 @@ struct PackArgs {
   int32_t* row_of;   // [Bp] packed -> given row (behind the live ones the ignored ones, then -1)
   int32_t* label;    // [Bp] -1: outside [0, V)
   float* loss_rows;  // zero for ignored rows, per given row; may be NULL
-  float* more_rows;  // the same
   XentHead* head;
   int32_t* status;
   int per_cta;
+  float* more_rows;  // sorted: the same, entropies
 };
 
 // Every CTA counts the live rows before its own by reading all labels, so
@@ -142,7 +143,6 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
         a.label[dst] = alive && ok ? (int32_t)y : -1;
         if (alive && !ok) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
         if (!alive && r < a.B && a.loss_rows) a.loss_rows[r] = 0.0f;
-        if (!alive && r < a.B && a.more_rows) a.more_rows[r] = 0.0f;
       }
       if (dst >= rows_up) continue;
       T* out = static_cast<T*>(a.hp) + dst * a.Dp;
@@ -151,6 +151,97 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_kernel(PackArgs a) 
         *reinterpret_cast<uint4*>(out + e) = alive ? load_slot_shifted(in, (int)e, span) : make_uint4(0u, 0u, 0u, 0u);
     }
     before += __popc(live);
+  }
+}
+
+// As fw_xent_pack_kernel, the live rows in the order of their labels, equal ones
+// by position, those outside [0, V) last: the product finds the rows of a label
+// next to each other.  Up to kCountRows rows every CTA counts what comes before
+// its own (4096 rows: 1 us more than counting the live ones; 8192: 6); more are
+// sorted first, and `sorted` has them (key V: out of range, V + 1: ignored).
+constexpr int64_t kCountRows = 8192;
+
+template <class T>
+__global__ void __launch_bounds__(kPackThreads) fw_xent_pack_sorted_kernel(PackArgs a, const uint2* sorted) {
+  __shared__ int red[10][kPackThreads / 32];
+  constexpr int V = 16 / sizeof(T);
+  wait_prior_kernel();
+  allow_dependent_launch();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * a.per_cta;
+  const Span<T> span(a.hidden, a.B, a.ldh, a.D);
+  const auto key_of = [&](int64_t y, int64_t i) {  // of a live row
+    return ((uint64_t)(y >= 0 && y < a.V ? (uint32_t)y : 0xffffffffu) << 32) | (uint64_t)i;
+  };
+  const auto put = [&](int64_t dst, int64_t r, bool live, int64_t y, int64_t rows_up) {  // one warp
+    if (lane == 0) {
+      const bool ok = y >= 0 && y < a.V;
+      a.row_of[dst] = r < a.B ? (int32_t)r : -1;
+      a.label[dst] = live && ok ? (int32_t)y : -1;
+      if (live && !ok) raise_status(a.status, FWB_STATUS_LABEL_RANGE);
+      if (!live && r < a.B) a.loss_rows[r] = a.more_rows[r] = 0.0f;
+    }
+    if (dst >= rows_up) return;
+    T* out = static_cast<T*>(a.hp) + dst * a.Dp;
+    const T* in = static_cast<const T*>(a.hidden) + (live ? r : 0) * a.ldh;
+    for (int64_t e = (int64_t)lane * V; e < a.Dp; e += 32 * V)
+      *reinterpret_cast<uint4*>(out + e) = live ? load_slot_shifted(in, (int)e, span) : make_uint4(0u, 0u, 0u, 0u);
+  };
+  if (sorted) {
+    int64_t lo = 0, hi = a.B;  // live rows: up to the first ignored one
+    while (lo < hi) {
+      const int64_t mid = (lo + hi) / 2;
+      if (sorted[mid].x <= (uint32_t)a.V)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.head = {(int32_t)lo, 0u, 0};
+    for (int64_t i = r0 + w; i < r0 + a.per_cta && i < a.Bp; i += kPackThreads / 32) {
+      const uint2 e = i < a.B ? sorted[i] : make_uint2((uint32_t)a.V + 1u, (uint32_t)i);
+      put(i, e.y, i < lo, e.x < (uint32_t)a.V ? (int64_t)e.x : -1, (lo + 255) / 256 * 256);
+    }
+    return;
+  }
+  for (int g0 = 0; g0 < a.per_cta; g0 += 8) {  // 8 rows, a warp each
+    uint64_t key[8];
+    int n[10] = {};  // live rows before each in the order of labels; all; before the first by position
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t r = r0 + g0 + k, y = r < a.B ? a.y[r] : a.ignore;
+      key[k] = y != a.ignore ? key_of(y, r) : 0u;
+    }
+    for (int64_t i = threadIdx.x; i < a.B; i += kPackThreads) {
+      const int64_t y = a.y[i];
+      if (y == a.ignore) continue;
+      const uint64_t own = key_of(y, i);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) n[k] += own < key[k];
+      n[8] += 1;
+      n[9] += i < r0 + g0;
+    }
+#pragma unroll
+    for (int k = 0; k < 10; ++k) {
+      n[k] = __reduce_add_sync(kFull, n[k]);
+      if (lane == 0) red[k][w] = n[k];
+    }
+    __syncthreads();
+    int rank = 0, total = 0, before = 0;  // of this warp's row
+#pragma unroll
+    for (int i = 0; i < kPackThreads / 32; ++i) {
+      rank += red[w][i];
+      total += red[8][i];
+      before += red[9][i];
+    }
+    if (g0 == 0 && blockIdx.x == 0 && threadIdx.x == 0) *a.head = {total, 0u, 0};
+    const int64_t r = r0 + g0 + w, y = r < a.B ? a.y[r] : a.ignore;
+    const bool live = y != a.ignore;
+    for (int k = 0; k < w; ++k) {
+      const int64_t q = r0 + g0 + k;
+      before += q < a.B && a.y[q] != a.ignore;
+    }
+    if (g0 + w < a.per_cta && r < a.Bp) put(live ? rank : total + (r - before), r, live, y, ((int64_t)total + 255) / 256 * 256);
+    __syncthreads();
   }
 }
 
@@ -678,16 +769,13 @@ struct ProductArgs {
 template <class T, TcKind K, bool BOTH>
 struct ProductTile {
   using Args = ProductArgs;
-  static constexpr int kHeld = BOTH ? 8 : 1;
   struct State {
     int mine;  // dH: the given row of this lane's row
     float f;   // its factor
     bool zero;
     float rest;  // BOTH: its label_rest, 0 without a label
     int label;
-    int found, seen;  // BOTH, dW: entries of the warp's list, packed rows looked at for it
-    uint2 h[kHeld];   // of few finds: 4 columns of their rows of H per lane,
-    float by[kHeld];  // and label_rest
+    bool any;  // BOTH, dW: there are such rows for one of the warp's 32
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
@@ -769,121 +857,74 @@ struct ProductTile {
     if constexpr (BOTH) {
       st.label = dh && !st.zero ? a.label[row] : -1;
       st.rest = st.label >= 0 ? a.label_rest[row] : 0.0f;
-      st.found = st.seen = 0;
-      if (!dh) {
-        st.found = find(a, list_of(p), p.lane, a.v0 + t.m0 + p.row, &st.seen);
-        if (held(a, st)) {
-          const int c = t.n0 + p.share * (BN / 2) + 4 * p.lane;
-#pragma unroll
-          for (int i = 0; i < kHeld; ++i) {
-            if (i >= st.found) break;
-            const int64_t r = list_of(p)[i * kWords] >> 5;
-            st.h[i] = make_uint2(0u, 0u);
-            if (c < a.ldh) st.h[i] = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.hp) + r * a.ldh + c);
-            st.by[i] = a.label_rest[r];
-          }
-        }
-      }
+      st.any = !dh && add_rows(a, p, a.v0 + t.m0 + p.row, t.n0 + p.share * (BN / 2));
     }
   }
-  // Few finds: their rows of H come while the products run.
-  __device__ static bool held(const Args& a, const State& st) { return st.found <= kHeld && st.seen >= a.head->rows; }
 
   // BOTH: dW's rows take label_rest times the rows of H that have them as
-  // labels.  A warp owns 32 rows v, looks through the labels for them while the
-  // tile's products run, and keeps up to 32 finds (packed row, v), in the order
-  // of the rows, in the spare word of its staging rows.  Up to kHeld finds have
-  // their rows of H loaded meanwhile, four columns a lane.  More are summed 16
-  // columns at a time, a lane each, in the last words of the staging rows, which
-  // are written last; and where there are more than 32 they are looked for again
-  // for every 16 columns, 32 by 32.  (4014 live rows, 128256 x 4096 bfloat16: the
-  // error of dW 1.4 to 1.0 times that of a form in 32 bits rounded once.)
-  static constexpr int kWords = kStageWords<BN / 2>;
-  __device__ static uint32_t* list_of(const TcPart& p) { return reinterpret_cast<uint32_t*>(p.smem) + kWords - 1; }
-  __device__ static int find(const Args& a, uint32_t* list, int lane, int v0, int* seen) {
-    const int rows = a.head->rows;
-    int n = 0;
-    __syncwarp();
-    while (*seen < rows) {
-      int d[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const int r = *seen + 32 * k + lane;
-        d[k] = r < rows ? a.label[r] - v0 : -1;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const bool in = (unsigned)d[k] < 32u;
-        const uint32_t all = __ballot_sync(kFull, in);
-        if (all) {
-          if (n + __popc(all) > 32) {
-            __syncwarp();
-            return n;
-          }
-          if (in) list[(n + __popc(all & ((1u << lane) - 1u))) * kWords] = ((uint32_t)(*seen + lane) << 5) | (uint32_t)d[k];
-          n += __popc(all);
-        }
-        *seen += 32;
-      }
-    }
-    __syncwarp();
-    return n;
-  }
-  // The same from what the lanes hold: columns c .. c + 32 of the warp's 128.
-  __device__ static void add_held(const TcPart& p, const State& st, int c, float* v) {
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      if (i >= st.found) break;
-      const bool mine = p.lane == (int)(list_of(p)[i * kWords] & 31u);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {  // columns 4 j .. 4 j + 4 are lane (c / 4 + j)'s
-        const uint32_t lo = __shfl_sync(kFull, st.h[i].x, c / 4 + j), hi = __shfl_sync(kFull, st.h[i].y, c / 4 + j);
-        if (mine) {
-          v[4 * j] = fmaf(st.by[i], Elem<T>::bits_to_f(lo & 0xffffu), v[4 * j]);
-          v[4 * j + 1] = fmaf(st.by[i], Elem<T>::bits_to_f(lo >> 16), v[4 * j + 1]);
-          v[4 * j + 2] = fmaf(st.by[i], Elem<T>::bits_to_f(hi & 0xffffu), v[4 * j + 2]);
-          v[4 * j + 3] = fmaf(st.by[i], Elem<T>::bits_to_f(hi >> 16), v[4 * j + 3]);
-        }
-      }
-    }
-  }
-  // v += the finds' sum for columns c .. c + 16 of the matrix.
-  __device__ static void add_found(const Args& a, const TcPart& p, State& st, int v0, int c, float* v) {
-    uint32_t* list = list_of(p);
-    float* sum = reinterpret_cast<float*>(p.smem) + kWords - 17;
+  // labels.  Packed rows are in the order of their labels, so those of a warp's
+  // 32 rows are next to each other.  While the tile's products run, the warp
+  // adds them up, four columns a lane, and leaves each sum in the staging row
+  // that the epilogue takes it from before it writes there: in bfloat16, whose
+  // range is that of the sums, and whose rounding is of a part that is itself
+  // what a rounding left.  (4014 live rows, 128256 x 4096 bfloat16: the error of
+  // dW 1.4 to 1.0 times that of a form in 32 bits rounded once.)
+  __device__ static bool add_rows(const Args& a, const TcPart& p, int v0, int c0) {
     const int rows = a.head->rows, lane = p.lane;
-    const bool again = st.seen < rows;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sum[lane * kWords + i] = 0.0f;
+    const int from = first_at(a.label, rows, (uint32_t)v0, lane), to = first_at(a.label, rows, (uint32_t)v0 + 32u, lane);
+    if (from == to) return false;
+    uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
+    constexpr int kWords = kStageWords<BN / 2>;
+    for (int i = lane; i < 32 * kWords; i += 32) sm[i] = 0u;
     __syncwarp();
-    const T* h = static_cast<const T*>(a.hp) + c + lane;
-    const bool mine = lane < 16 && c + lane < a.D;
-    for (;;) {
-      for (int i0 = 0; i0 < st.found; i0 += 8) {
-        float x[8];
-        int d[8];
+    const int c = c0 + 4 * lane;
+    const T* h = static_cast<const T*>(a.hp) + c;
+    float x[4] = {};
+    int run = a.label[from];
+    const auto give = [&] {
+      sm[(run - v0) * kWords + 2 * lane] = pack2<__nv_bfloat16>(x[0], x[1]);
+      sm[(run - v0) * kWords + 2 * lane + 1] = pack2<__nv_bfloat16>(x[2], x[3]);
+    };
+    for (int r0 = from; r0 < to; r0 += 8) {
+      uint2 u[8];
+      float by[8];
+      int y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t e = i0 + i < st.found ? list[(i0 + i) * kWords] : 0u;
-          d[i] = (int)(e & 31u);
-          x[i] = mine && i0 + i < st.found ? a.label_rest[e >> 5] * ld_elem(h + (int64_t)(e >> 5) * a.ldh) : 0.0f;
-        }
-        if (mine) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) sum[d[i] * kWords + lane] += x[i];
-        }
+      for (int i = 0; i < 8; ++i) {
+        const int r = min(r0 + i, to - 1);
+        y[i] = a.label[r];
+        by[i] = a.label_rest[r];
+        u[i] = c < a.ldh ? *reinterpret_cast<const uint2*>(h + (int64_t)r * a.ldh) : make_uint2(0u, 0u);
       }
-      if (st.seen >= rows) break;
-      st.found = find(a, list, lane, v0, &st.seen);
-    }
-    if (again) {  // from the first ones on for the next columns
-      st.seen = 0;
-      st.found = find(a, list, lane, v0, &st.seen);
-    }
-    __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] += sum[lane * kWords + i];
+      for (int i = 0; i < 8; ++i) {
+        if (r0 + i >= to) break;
+        if (y[i] != run) {
+          give();
+          run = y[i];
+          x[0] = x[1] = x[2] = x[3] = 0.0f;
+        }
+        x[0] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x & 0xffffu), x[0]);
+        x[1] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x >> 16), x[1]);
+        x[2] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y & 0xffffu), x[2]);
+        x[3] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y >> 16), x[3]);
+      }
+    }
+    give();
     __syncwarp();
+    return true;
+  }
+  // First of the packed rows, in the order of their labels, whose label is at least v: 33 parts a step.
+  __device__ static int first_at(const int32_t* label, int rows, uint32_t v, int lane) {
+    int lo = 0, hi = rows;  // labels before lo are under v, those from hi on are not
+    while (lo < hi) {
+      const int step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step - 1;
+      const bool under = at < hi && (uint32_t)label[at] < v;
+      const int n = __popc(__ballot_sync(kFull, under));  // the first n of them
+      if (n < 32) hi = min(hi, lo + (n + 1) * step - 1);
+      lo += n * step;
+    }
+    return lo;
   }
 
   template <bool LOST, class Done>
@@ -928,11 +969,13 @@ struct ProductTile {
           for (int i = 0; i < 32; i += 8)
             if (c + i < cols) a.template add_label<T>(st.label, t.n0 + s0 + c + i, st.rest, v + i);
         }
-        if (!dh && held(a, st)) {
-          add_held(p, st, c, v);
-        } else if (!dh) {
-          add_found(a, p, st, a.v0 + r0, t.n0 + s0 + c, v);
-          add_found(a, p, st, a.v0 + r0, t.n0 + s0 + c + 16, v + 16);
+        if (st.any) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint32_t u = sm[p.lane * kStageWords<BN / 2> + c / 2 + i];
+            v[2 * i] += __uint_as_float(u << 16);
+            v[2 * i + 1] += __uint_as_float(u & 0xffff0000u);
+          }
         }
       }
 #pragma unroll
@@ -1009,7 +1052,7 @@ struct XentPlan {
   // state: what backward needs
   int64_t row_of, label, lse, entropy, hp, wp, state_bytes;
   // forward workspace
-  int64_t part, part_t, zy, loss_pack, fwd_bytes;
+  int64_t part, part_t, zy, loss_pack, sorted, hist, fwd_bytes;
   // backward workspace
   int64_t piece, pieces, splits, top, label_rest, g, sum, hs, bwd_bytes;
 };
@@ -1032,6 +1075,12 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = fal
   p.part_t = at, at += both ? up(4 * p.Bp * up(V, kTileN) / kLseCols, 256) : 0;
   p.zy = at, at += up(4 * p.Bp, 256);
   p.loss_pack = at, at += up(4 * p.Bp, 256);
+  if (both && B > kCountRows) {
+    int passes, bits;
+    sort_digits(V + 1, &passes, &bits);
+    p.sorted = at, at += up(16 * B, 256);
+    p.hist = at, at += up((B + kSortTile - 1) / kSortTile * ((int64_t)4 << bits), 256);
+  }
   p.fwd_bytes = at;
   const int64_t Vp = up(V, 256);
   p.pieces = (2 * p.Bp * Vp + kPieceBytes - 1) / kPieceBytes;
@@ -1075,11 +1124,26 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   int32_t* label = reinterpret_cast<int32_t*>(state + p.label);
   const int64_t per_cta = (p.Bp + 4 * sm_count() - 1) / (4 * sm_count());
   PackArgs pk = {hidden, y, B, p.Bp, D, p.Dp, ldh, V, ignore, state + p.hp, row_of, label,
-                 reduction == FWB_REDUCE_NONE ? loss : nullptr, BOTH ? entropy : nullptr, head, status,
-                 (int)(per_cta < 8 ? 8 : per_cta)};
-  if (launch_dependent(fw_xent_pack_kernel<T>, (p.Bp + pk.per_cta - 1) / pk.per_cta, kPackThreads, 0, 1, st, pk) !=
-      cudaSuccess)
-    return FWB_E_LAUNCH;
+                 reduction == FWB_REDUCE_NONE ? loss : nullptr, head, status, (int)(per_cta < 8 ? 8 : per_cta), entropy};
+  const int64_t ctas = (p.Bp + pk.per_cta - 1) / pk.per_cta;
+  if constexpr (BOTH) {
+    const uint2* sorted = nullptr;
+    if (B > kCountRows) {
+      SortArgs s = {};
+      s.ids = y, s.T = B, s.V = V, s.padding = ignore, s.tail = 1;
+      s.hist = reinterpret_cast<uint32_t*>(ws + p.hist);
+      s.tiles = (int)((B + kSortTile - 1) / kSortTile);
+      int passes;
+      sort_digits(V + 1, &passes, &s.bits);
+      uint2* ent = reinterpret_cast<uint2*>(ws + p.sorted);
+      sorted = sort_launch(s, ent, ent + B, passes, st);
+      if (cudaGetLastError() != cudaSuccess) return FWB_E_LAUNCH;
+    }
+    if (launch_dependent(fw_xent_pack_sorted_kernel<T>, ctas, kPackThreads, 0, 1, st, pk, sorted) != cudaSuccess)
+      return FWB_E_LAUNCH;
+  } else {
+    if (launch_dependent(fw_xent_pack_kernel<T>, ctas, kPackThreads, 0, 1, st, pk) != cudaSuccess) return FWB_E_LAUNCH;
+  }
   const void* w = weight;
   if (p.copy_w) {
     const int64_t need = (V * ((p.Dp + 1023) / 1024) + 7) / 8, cap = (int64_t)sm_count() * 16;

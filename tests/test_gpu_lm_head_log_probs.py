@@ -170,7 +170,7 @@ def test_upstream_factors(value, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,D,V", [(700, 300, 1), (700, 300, 40), (900, 100, 3000), (513, 136, 700)])
 def test_labels_met_again_and_again(B, D, V, dtype):
-    """More rows than a list of finds holds with labels of one 32 rows of the weight, and with one label."""
+    """Many rows with labels of one 32 rows of the weight, and with one label."""
     g = R.gen(B + V)
     h, w = R.normal((B, D), dtype, g), R.normal((V, D), dtype, g, D ** -0.5)
     y = torch.randint(0, min(V, 45), (B,), generator=g, device="cuda") + (V - min(V, 45))
@@ -178,6 +178,28 @@ def test_labels_met_again_and_again(B, D, V, dtype):
     y[: B // 2] = V // 2
     y[::7] = -100
     check(h, w, y, kind="logp")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,V", [(8192, 300), (8193, 300), (20011, 3), (40000, 511), (9000, 512)])
+def test_many_rows(B, V, dtype):
+    """Rows counted and rows sorted into the order of their labels; ignored rows and bad labels among them."""
+    g = R.gen(B + V)
+    h, w = R.normal((B, 40), dtype, g), R.normal((V, 40), dtype, g, 0.3)
+    y = tokens_for(B, V, g, 0.2)
+    check(h, w, y)
+    bad = torch.randint(0, B, (5,), generator=g, device="cuda")
+    y[bad] = torch.tensor([V, -1, V + 7, 1 << 40, -(1 << 50)], device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    hh, ww = h.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    out = fw.lm_head_log_probs(hh, ww, y, status=status)
+    assert int(status) == 1
+    r, (dh, e_dh), _ = reference(h, w, y, 1.0, torch.ones(B, device="cuda"))
+    R.within(out[0], r["logp"], r["e_logp"], "logp")
+    R.within(out[1], r["entropy"], r["e_entropy"], "entropy")
+    got = torch.autograd.grad(out[0].sum(), (hh, ww))
+    R.within(got[0], dh, e_dh, "dhidden")
+    assert got[1].isnan().all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
