@@ -184,8 +184,17 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_sorted_kernel(PackA
     if (dst >= rows_up) return;
     T* out = static_cast<T*>(a.hp) + dst * a.Dp;
     const T* in = static_cast<const T*>(a.hidden) + (live ? r : 0) * a.ldh;
-    for (int64_t e = (int64_t)lane * V; e < a.Dp; e += 32 * V)
-      *reinterpret_cast<uint4*>(out + e) = live ? load_slot_shifted(in, (int)e, span) : make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t e0 = (int64_t)lane * V; e0 < a.Dp; e0 += 4 * 32 * V) {
+      uint4 x[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t e = e0 + k * 32 * V;
+        x[k] = live && e < a.Dp ? load_slot_shifted(in, (int)e, span) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (e0 + k * 32 * V < a.Dp) *reinterpret_cast<uint4*>(out + e0 + k * 32 * V) = x[k];
+    }
   };
   if (sorted) {
     int64_t lo = 0, hi = a.B;  // live rows: up to the first ignored one
@@ -211,14 +220,20 @@ __global__ void __launch_bounds__(kPackThreads) fw_xent_pack_sorted_kernel(PackA
       const int64_t r = r0 + g0 + k, y = r < a.B ? a.y[r] : a.ignore;
       key[k] = y != a.ignore ? key_of(y, r) : 0u;
     }
-    for (int64_t i = threadIdx.x; i < a.B; i += kPackThreads) {
-      const int64_t y = a.y[i];
-      if (y == a.ignore) continue;
-      const uint64_t own = key_of(y, i);
+    for (int64_t i0 = threadIdx.x; i0 < a.B; i0 += 4 * kPackThreads) {
+      int64_t y[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) n[k] += own < key[k];
-      n[8] += 1;
-      n[9] += i < r0 + g0;
+      for (int q = 0; q < 4; ++q) y[q] = i0 + q * kPackThreads < a.B ? a.y[i0 + q * kPackThreads] : a.ignore;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t i = i0 + q * kPackThreads;
+        const bool live = y[q] != a.ignore;
+        const uint64_t own = live ? key_of(y[q], i) : ~0ull;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) n[k] += own < key[k];
+        n[8] += live;
+        n[9] += live && i < r0 + g0;
+      }
     }
 #pragma unroll
     for (int k = 0; k < 10; ++k) {
@@ -420,7 +435,7 @@ __device__ __forceinline__ void raise_sums(float m, float to, float c, float* s,
 
 // As fw_xent_join_kernel, for log probabilities and entropies.
 __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_both_kernel(JoinArgs a) {
-  __shared__ float sm[kJoinWarps][32], ss[kJoinWarps][32], su[kJoinWarps][32];
+  __shared__ float sm[kJoinWarps][33], ss[kJoinWarps][33], su[kJoinWarps][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   wait_prior_kernel();
   const int rows = a.head->rows;
@@ -447,29 +462,29 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_both_kernel(Join
   ss[w][lane] = s;
   su[w][lane] = u;
   __syncthreads();
-  if (w != 0 || row >= rows) return;
-  float M = sm[0][lane];
+  // a warp per row, a lane per part
+  const int mine = blockIdx.x * 32 + w;
+  if (mine >= rows) return;
+  m = sm[lane][w], s = ss[lane][w], u = su[lane][w];
+  const float M = warp_max_nan(m);
+  if (m != -CUDART_INF_F) raise_sums(m, M, c, &s, &u);
 #pragma unroll
-  for (int i = 1; i < kJoinWarps; ++i) M = max_nan(M, sm[i][lane]);
-  float S = 0.0f, U = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < kJoinWarps; ++i) {
-    if (sm[i][lane] == -CUDART_INF_F) continue;
-    s = ss[i][lane], u = su[i][lane];
-    raise_sums(sm[i][lane], M, c, &s, &u);
-    S += s;
-    U += u;
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(kFull, s, o);
+    u += __shfl_xor_sync(kFull, u, o);
   }
-  const bool label = a.label[row] >= 0, ok = label && a.head->status == 0 && fabsf(M) < CUDART_INF_F;
-  if (lane == 0 && a.head->status != 0) raise_status(a.status, a.head->status);
+  if (lane != 0) return;
+  const float S = s, U = u;
+  const bool label = a.label[mine] >= 0, ok = label && a.head->status == 0 && fabsf(M) < CUDART_INF_F;
+  if (w == 0 && a.head->status != 0) raise_status(a.status, a.head->status);
   if (label && !(fabsf(M) < CUDART_INF_F)) raise_status(a.status, FWB_STATUS_NONFINITE);
   const float log_s = logf(S), nan = CUDART_NAN_F;
-  const int to = a.row_of[row];
+  const int to = a.row_of[mine];
   const float h = ok ? log_s - U * kLn2 / S : nan;
-  a.lse[row] = ok ? fmaf(M, a.inv_t, log_s) : nan;
-  a.entropy_pack[row] = h;
+  a.lse[mine] = ok ? fmaf(M, a.inv_t, log_s) : nan;
+  a.entropy_pack[mine] = h;
   a.entropy[to] = h;
-  a.loss[to] = ok ? (a.zy[row] - M) * a.inv_t - log_s : nan;
+  a.loss[to] = ok ? (a.zy[mine] - M) * a.inv_t - log_s : nan;
 }
 
 // 32 rows per CTA, the tiles' pairs split over its warps; the last CTA to
@@ -588,6 +603,8 @@ struct Upstream {
 __global__ void __launch_bounds__(1024) fw_xent_top_kernel(const XentHead* head, const int32_t* row_of, Upstream up,
                                                              float* out) {
   __shared__ float red[32];
+  wait_prior_kernel();
+  allow_dependent_launch();
   const int rows = head->rows;
   float top = 0.0f;
   for (int i = threadIdx.x; i < rows; i += 1024) {
@@ -1179,7 +1196,8 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
   const Upstream u = {go, top, per_row, mean, K == kTcF16, BOTH, go_ent, inv_t};
   const char* hw = state + p.hp;  // dW's operand
   if (per_row) {
-    if (u.f16) fw_xent_top_kernel<<<1, 1024, 0, st>>>(head, row_of, u, top);
+    if (u.f16 && launch_dependent(fw_xent_top_kernel, 1, 1024, 0, 1, st, head, row_of, u, top) != cudaSuccess)
+      return FWB_E_LAUNCH;
     if (dweight && !BOTH) {
       T* hs = reinterpret_cast<T*>(ws + p.hs);
       const int64_t cap = (int64_t)sm_count() * 8;
