@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(256, kGradCtas) fw_logprob_grad_kernel(ScoreGr
 int score_check(int dtype, int64_t B, int64_t V, int64_t ld, float inv_t) {
   if (dtype != FWB_DTYPE_F32 && dtype != FWB_DTYPE_BF16 && dtype != FWB_DTYPE_F16) return FWB_E_DTYPE;
   if (B < 0 || V < 1 || ld < V || B > (1 << 28) || V > (1 << 28) || ld > ((int64_t)1 << 32)) return FWB_E_SHAPE;
-  if (!(inv_t > 0.0f) || !std::isfinite(inv_t)) return FWB_E_SHAPE;
+  if (!(inv_t > 0.0f) || !std::isfinite(inv_t * kLog2e)) return FWB_E_SHAPE;
   return FWB_OK;
 }
 

@@ -10,9 +10,9 @@
 
 namespace {
 
-// A temperature whose reciprocal fp32 holds.
+// A temperature whose reciprocal fp32 holds, with some room above.
 bool fits(double temperature) {
-  return temperature > 0.0 && std::isfinite((float)temperature) && std::isfinite((float)(1.0 / temperature)) &&
+  return temperature > 0.0 && std::isfinite((float)temperature) && std::isfinite(1.5f * (float)(1.0 / temperature)) &&
          (float)(1.0 / temperature) > 0.0f;
 }
 

@@ -257,7 +257,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             f(*bad)
     for kw in ({"top_k": 33}, {"top_k": -1}, {"top_k": 31}, {"temperature": 0.0}, {"temperature": -1.0},
-               {"temperature": float("nan")}, {"temperature": float("inf")}, {"temperature": 1e-40}):
+               {"temperature": float("nan")}, {"temperature": float("inf")}, {"temperature": 1e-40}, {"temperature": 3.2e-39}):
         with pytest.raises(ValueError):
             f(z, y, **kw)
     with pytest.raises(RuntimeError):

@@ -36,7 +36,7 @@ def test_token_log_probs_arguments():
 
     assert fwd(dtype=3) == DTYPE
     for bad in (dict(ld=7), dict(B=-1), dict(V=0), dict(V=1 << 29, ld=1 << 29), dict(B=1 << 29), dict(it=0.0), dict(it=-1.0),
-                dict(it=float("nan")), dict(it=float("inf")), dict(k=-1), dict(k=9)):
+                dict(it=float("nan")), dict(it=float("inf")), dict(it=3e38), dict(k=-1), dict(k=9)):
         assert fwd(**bad) == SHAPE, bad
     assert fwd(V=100, ld=100, k=33) == CAPACITY
     for bad in (dict(z=P), dict(y=P), dict(logp=P), dict(ent=P), dict(tl=P), dict(ti=P), dict(z=ODD), dict(state=OFF)):
@@ -67,7 +67,7 @@ def test_lm_head_log_probs_arguments():
         return f(dtype, h, ldh, w, ldw, y, B, 8, 10, it, -100, logp, ent, state, n, ws, m, P, P)
 
     assert fwd(dtype=0) == DTYPE
-    for bad in (dict(ldh=7), dict(ldw=7), dict(it=0.0), dict(it=float("inf")), dict(B=-1)):
+    for bad in (dict(ldh=7), dict(ldw=7), dict(it=0.0), dict(it=float("inf")), dict(it=3e38), dict(B=-1), dict(B=(1 << 24) + 1)):
         assert fwd(**bad) == SHAPE, bad
     for bad in (dict(h=P), dict(w=P), dict(y=P), dict(logp=P), dict(ent=P), dict(state=P), dict(ws=P), dict(w=ODD, n=1 << 20),
                 dict(state=OFF), dict(ws=OFF)):
