@@ -3,7 +3,9 @@
 //
 // Bound by HBM: the norm reads every element once; scaling reads them again
 // (from L2, where they fit: the second kernel walks each CTA's part backwards,
-// so that what was read last is read first) and writes them.  The tensors'
+// so that what was read last is read first) and writes them.  2.9 GB of bfloat16
+// scaled into copies: 1.42 ms, 6.2 TB/s of the 8.8 GB moved; 267 MB of bfloat16
+// into float32 187 us; the norm alone of 308 MB 50 us, 6.2 TB/s.  The tensors'
 // addresses travel in the kernels' arguments, so nothing is copied to the
 // device and a captured graph holds them.
 //
@@ -23,6 +25,10 @@ namespace {
 
 constexpr int kTile = 8192;  // elements: 4 groups of 8 per thread
 constexpr int kThreads = 256;
+// CTAs per SM of the norm and of the scaling.  3 GB of bfloat16: norm 423 us with
+// 4, 411 with 5; norm and scaled copy 1453 and 1487 (1416 with 4 and stores that
+// leave L2 first).
+constexpr int kNormCtas = 5, kScaleCtas = 4;
 constexpr int kGroups = kTile / 8 / kThreads;
 constexpr float kLost = 8.0779357e-28f;  // 2^-90: squares under 2^-149 are gone, 2^-59 of this
 
@@ -55,9 +61,10 @@ __device__ __forceinline__ void load_whole(uint4 (&u)[2], const void* p) {
                : "l"(p)
                : "memory");
 }
-__device__ __forceinline__ void store_whole(void* p, const uint4 (&u)[1]) { *static_cast<uint4*>(p) = u[0]; }
+// What is stored is not read again here, what was loaded may be.
+__device__ __forceinline__ void store_whole(void* p, const uint4 (&u)[1]) { __stcs(static_cast<uint4*>(p), u[0]); }
 __device__ __forceinline__ void store_whole(void* p, const uint4 (&u)[2]) {
-  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0].x), "r"(u[0].y), "r"(u[0].z),
+  asm volatile("st.global.L2::evict_first.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(u[0].x), "r"(u[0].y), "r"(u[0].z),
                "r"(u[0].w), "r"(u[1].x), "r"(u[1].y), "r"(u[1].z), "r"(u[1].w)
                : "memory");
 }
@@ -136,7 +143,7 @@ __device__ __forceinline__ double block_sum(double d) {
 }
 
 template <int N>
-__global__ void __launch_bounds__(kThreads, 4) fw_grad_squares_kernel(const __grid_constant__ Table<N> t, double* part) {
+__global__ void __launch_bounds__(kThreads, kNormCtas) fw_grad_squares_kernel(const __grid_constant__ Table<N> t, double* part) {
   wait_prior_kernel();
   allow_dependent_launch();
   const int lo = (int)((int64_t)t.tiles * blockIdx.x / gridDim.x), hi = (int)((int64_t)t.tiles * (blockIdx.x + 1) / gridDim.x);
@@ -214,7 +221,7 @@ __device__ __forceinline__ void tile_scale_to(const TI* x, void* y, int type, in
 // `part` NULL: the norm is *norm_in.  `inplace`: nothing is written where the
 // factor is 1.
 template <int N>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, kScaleCtas)
     fw_grad_scale_kernel(const __grid_constant__ Table<N> t, const double* part, int parts, const float* norm_in,
                          float max_norm, int inplace, float* norm, int32_t* status) {
   wait_prior_kernel();
@@ -269,7 +276,7 @@ int check_tensors(const Tensors& t) {
   return FWB_OK;
 }
 
-int64_t max_ctas() { return (int64_t)sm_count() * 4; }
+int64_t norm_ctas() { return (int64_t)sm_count() * kNormCtas; }
 
 // Fills a launch's table from tensor `at` on and returns the tensor behind it.
 template <int N>
@@ -298,12 +305,11 @@ int64_t fill(const Tensors& t, int64_t at, Table<N>* out) {
 }
 
 template <int N, class Launch>
-int for_tables(const Tensors& t, Launch&& launch) {
+int for_tables(const Tensors& t, int64_t cap, Launch&& launch) {
   Table<N> table;
   for (int64_t at = 0; at < t.n;) {
     at = fill(t, at, &table);
     if (table.n == 0) break;
-    const int64_t cap = max_ctas();
     if (launch(table, table.tiles < cap ? table.tiles : cap) != cudaSuccess) return FWB_E_LAUNCH;
   }
   return FWB_OK;
@@ -312,7 +318,7 @@ int for_tables(const Tensors& t, Launch&& launch) {
 template <int N>
 int run_squares(const Tensors& t, double* part, int* parts, cudaStream_t st) {
   *parts = 0;
-  return for_tables<N>(t, [&](const Table<N>& table, int64_t grid) {
+  return for_tables<N>(t, norm_ctas(), [&](const Table<N>& table, int64_t grid) {
     const cudaError_t e = launch_dependent(fw_grad_squares_kernel<N>, grid, kThreads, 0, 1, st, table, part + *parts);
     *parts += (int)grid;
     return e;
@@ -325,7 +331,7 @@ int run_scale(const Tensors& t, const double* part, int parts, const float* norm
   bool inplace = true;
   for (int64_t i = 0; i < t.n; ++i)
     if (t.numel[i] > 0 && (t.in[i] != t.out[i] || t.type_in[i] != t.type_out[i])) inplace = false;
-  return for_tables<N>(t, [&](const Table<N>& table, int64_t grid) {
+  return for_tables<N>(t, (int64_t)sm_count() * kScaleCtas, [&](const Table<N>& table, int64_t grid) {
     const cudaError_t e = launch_dependent(fw_grad_scale_kernel<N>, grid, kThreads, 0, 1, st, table, part, parts, norm_in,
                                            max_norm, (int)inplace, norm, status);
     norm = nullptr;  // given by the first launch
@@ -333,7 +339,7 @@ int run_scale(const Tensors& t, const double* part, int parts, const float* norm
   });
 }
 
-int64_t squares_bytes(int64_t n) { return 8 * max_ctas() * ((n + kFew - 1) / kFew); }
+int64_t squares_bytes(int64_t n) { return 8 * norm_ctas() * ((n + kFew - 1) / kFew); }
 
 bool nothing(const Tensors& t) {
   for (int64_t i = 0; i < t.n; ++i)
