@@ -76,8 +76,9 @@ __device__ __forceinline__ void load_group(uint4 (&u)[kParts<T>], const T* x, in
   if (e >= 0 && e + 8 <= n && (reinterpret_cast<uintptr_t>(x + e) & (8 * sizeof(T) - 1)) == 0) {
     load_whole(u, x + e);
   } else {
+    const Span<T> span(x, 1, n, n);
 #pragma unroll
-    for (int i = 0; i < kParts<T>; ++i) u[i] = load_elems(x + e + i * V, x, x + n);
+    for (int i = 0; i < kParts<T>; ++i) u[i] = load_slot_shifted(x + e + i * V, 0, span);
   }
 }
 
