@@ -430,7 +430,7 @@ constexpr int kJoinWarps = 32;
 
 // Maximum and sums of BOTH, relative to another maximum (not under it).
 __device__ __forceinline__ void raise_sums(float m, float to, float c, float* s, float* u) {
-  const float d = fmaxf((m - to) * c, kExpFloor), f = exp2f(d);
+  const float d = fmaxf((m - to) * c, kExpFloor), f = exp2_hw(d);
   *u = f * fmaf(d, *s, *u);
   *s *= f;
 }
@@ -445,17 +445,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_both_kernel(Join
   const float c = a.inv_t * kLog2e;
   float m = -CUDART_INF_F, s = 0.0f, u = 0.0f;
   if (row < rows) {
-#pragma unroll 4
-    for (int t = w; t < a.ntiles; t += kJoinWarps) {
-      float2 p = a.part[(int64_t)t * a.Bp + row];
-      float pu = a.part_t[(int64_t)t * a.Bp + row];
-      const float to = max_nan(m, p.x);
+    constexpr int N = 8;  // parts in flight, joined by their largest maximum
+    for (int t0 = w; t0 < a.ntiles; t0 += N * kJoinWarps) {
+      float2 p[N];
+      float pu[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int t = t0 + i * kJoinWarps;
+        p[i] = t < a.ntiles ? a.part[(int64_t)t * a.Bp + row] : make_float2(-CUDART_INF_F, 0.0f);
+        pu[i] = t < a.ntiles ? a.part_t[(int64_t)t * a.Bp + row] : 0.0f;
+      }
+      float to = m;
+#pragma unroll
+      for (int i = 0; i < N; ++i) to = max_nan(to, p[i].x);
       if (to == -CUDART_INF_F) continue;
       if (m != -CUDART_INF_F) raise_sums(m, to, c, &s, &u);
-      if (p.x != -CUDART_INF_F) {
-        raise_sums(p.x, to, c, &p.y, &pu);
-        s += p.y;
-        u += pu;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (p[i].x == -CUDART_INF_F) continue;
+        raise_sums(p[i].x, to, c, &p[i].y, &pu[i]);
+        s += p[i].y;
+        u += pu[i];
       }
       m = to;
     }
