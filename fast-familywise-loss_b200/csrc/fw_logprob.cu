@@ -591,7 +591,9 @@ __global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? 
         group_sync<NW>();
         m = part[0].m;
         logs = part[0].s;
-        if (own != 0) {
+        if (isnan(m)) {  // a bad row need not have given k keys
+          if (tid < a.k) give_top(0, tid);
+        } else if (own != 0) {
           const int i = keys_above(top.found, CL * a.k, own);
           if (i < a.k) give_top(own, i);
         }

@@ -298,6 +298,54 @@ def test_nodes():
         fw.lm_head_log_probs(fwd.make_dual(h.detach(), torch.ones_like(h)), w, y)
 
 
+def test_weight_restored_with_other_strides():
+    """A saved-tensor hook may bring the weight back off the 16-byte boundaries it was saved on."""
+    g = R.gen(30)
+    h = R.normal((70, 64), torch.bfloat16, g).requires_grad_(True)
+    w = R.normal((300, 64), torch.bfloat16, g, 0.3).requires_grad_(True)
+    y = tokens_for(70, 300, g, 0.1)
+    up = torch.randn(70, device="cuda")
+
+    def off(t):
+        if t.dim() != 2:
+            return t
+        store = torch.empty(t.shape[0], t.shape[1] + 3, dtype=t.dtype, device="cuda")
+        store[:, 1:-2] = t
+        return store[:, 1:-2]
+
+    want = torch.autograd.grad(fw.lm_head_log_probs(h, w, y), (h, w), (up, up))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, off):
+        out = fw.lm_head_log_probs(h, w, y)
+        got = torch.autograd.grad(out, (h, w), (up, up))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
+def test_gradients_on_two_streams():
+    """Two gradients of one retained graph at once, and another forward beside them."""
+    g = R.gen(31)
+    h = R.normal((600, 128), torch.bfloat16, g).requires_grad_(True)
+    w = R.normal((4000, 128), torch.bfloat16, g, 0.2).requires_grad_(True)
+    y = tokens_for(600, 4000, g, 0.1)
+    up = torch.randn(600, device="cuda")
+    out = fw.lm_head_log_probs(h, w, y)
+    want = torch.autograd.grad(out, (h, w), (up, up), retain_graph=True)
+    torch.cuda.synchronize()
+    streams, held = [torch.cuda.Stream() for _ in range(3)], []
+    for _ in range(4):
+        for s in streams[:2]:
+            with torch.cuda.stream(s):
+                held.append(torch.autograd.grad(out, (h, w), (up, up), retain_graph=True))
+        with torch.cuda.stream(streams[2]):
+            again = fw.lm_head_log_probs(h, w, y)
+    torch.cuda.synchronize()
+    for got in held:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+    for a, b in zip(again, out):
+        assert torch.equal(a.detach(), b.detach())
+
+
 def test_refusals():
     h, w = torch.zeros(4, 8, device="cuda", dtype=torch.bfloat16), torch.zeros(9, 8, device="cuda", dtype=torch.bfloat16)
     y = torch.zeros(4, dtype=torch.int64, device="cuda")

@@ -142,8 +142,10 @@ def test_leading_shapes():
     assert torch.equal(d.reshape(24, 99), torch.autograd.grad(flat[0], z, up.reshape(24))[0].reshape(24, 99))
     one = fw.token_log_probs(z[1, 2], y[1, 2])
     assert one[0].shape == () and torch.equal(one[0], out[0][1, 2]) and torch.equal(one[1], out[1][1, 2])
-    none = fw.token_log_probs(torch.zeros(0, 9, device="cuda", requires_grad=True), torch.zeros(0, dtype=torch.int64, device="cuda"), 3)
+    x = torch.zeros(0, 9, device="cuda", requires_grad=True)
+    none = fw.token_log_probs(x, torch.zeros(0, dtype=torch.int64, device="cuda"), 3)
     assert [tuple(t.shape) for t in none] == [(0,), (0,), (0, 3), (0, 3)]
+    assert torch.autograd.grad(none[0].sum(), x)[0].shape == (0, 9)
 
 
 @pytest.mark.parametrize("dtype", R.FLOATS)
@@ -167,6 +169,44 @@ def test_rows_that_are_not_finite(dtype):
     assert int(status) == 0
     out = fw.token_log_probs(z, y)
     assert float(out[0][3]) == NEG and bool(torch.isfinite(out[1][3]))
+
+
+@pytest.mark.parametrize("dtype", R.FLOATS)
+@pytest.mark.parametrize("V", [40000, 9000, 2100])
+def test_bad_rows_of_few_long_ones(V, dtype):
+    """Rows split over CTAs: every alternative of a bad one is written, whatever was there."""
+    g = R.gen(V)
+    z = R.normal((7, V), dtype, g)
+    z[0, V // 2], z[1, 0], z[2] = float("nan"), float("inf"), NEG
+    z[3, :] = float("nan")
+    z[4, 20:] = NEG  # fewer than 32 columns left
+    y = torch.tensor([0, 1, 2, 3, 5, -100, V], device="cuda")
+    for _ in range(3):
+        torch.full((7, 32), 777, dtype=torch.int64, device="cuda")  # what freed memory holds
+        torch.full((7, 32), 777.0, device="cuda")
+        check(z, y, k=32, grads=("both",))
+
+
+def test_offsets_past_2_31_elements():
+    if torch.cuda.get_device_properties(0).total_memory < 60e9:
+        pytest.skip("needs 20 GB of device memory")
+    B, V, last = 17000, 131072, 7
+    z = torch.zeros(B, V, dtype=torch.bfloat16, device="cuda")
+    tail = R.normal((last, V), torch.bfloat16, R.gen(2), 2.0)
+    z[-last:] = tail
+    y = torch.full((B,), -100, device="cuda")
+    y[-last:] = tokens_for(last, V, R.gen(3))
+    x, xt = z.requires_grad_(True), tail.clone().requires_grad_(True)
+    up = torch.ones(B, device="cuda")
+    out, ref = fw.token_log_probs(x, y, top_k=4), fw.token_log_probs(xt, y[-last:], top_k=4)
+    bound = S.rows(tail.double(), y[-last:], 1.0)
+    for i, e in ((0, "e_logp"), (1, "e_entropy")):  # few rows take another way through them
+        R.within(out[i][-last:], ref[i].double(), 2 * bound[e])
+    assert torch.equal(out[3][-last:], ref[3])
+    (d,) = torch.autograd.grad(out[0], x, up)
+    want, e = S.logit_grad(bound, up[-last:])
+    R.within(d[-last:], want, S.grad_bound(want, e, torch.bfloat16))
+    assert not d[: 100].any() and not d[B // 2: B // 2 + 100].any()
 
 
 @pytest.mark.parametrize("dtype", R.FLOATS)
