@@ -7,9 +7,8 @@
 // with upstream factors g of logp and h of H.  Both terms of H are positive, so
 // nothing cancels; exp(t) t is 0 where exp(t) is (masked columns are -inf).
 //
-// One pass over the row: every thread keeps a maximum and both sums relative
-// to it, and rescales them in the rare batch of slots that raises it.  Bound by
-// HBM: the forward reads the logits once, the gradient reads them again and
+// One pass over the row: every thread keeps its maximum, and both sums relative
+// to a reference near it, which moves in few batches of slots.  Bound by HBM: the forward reads the logits once, the gradient reads them again and
 // writes theirs.  4096 x 32000: forward float32 77 us (6.8 TB/s), bfloat16 48
 // (5.5: the exponentials beside it), with 5 alternatives 88 and 60, gradient 167
 // and 86 (6.1 to 6.3 TB/s).  Few rows are bound by latency: 48 x 128256 bfloat16
@@ -21,8 +20,9 @@
 // whatever is among the row's k largest reaches it too, and lies with the few
 // threads (k and some) whose largest element does.  Their slots are read again,
 // from L2, by whole warps, and the elements that reach the bound are ranked by
-// 64-bit keys (value, then lowest column first), all different, so ties need no
-// case of their own.
+// 64-bit keys (value, then lowest column first), all different.  Where that
+// would be very many, because the bound's value is a mask's, those above it and
+// the first k of that value are enough.
 #include <cooperative_groups.h>
 
 #include <cmath>
@@ -40,7 +40,7 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFloor = -200.0f;  // 2^kFloor is 0 in fp32; keeps 0 * t finite
 // Slots in flight per thread, and CTAs of 256 threads per SM.  4096 x 32000
 // without and with 5 alternatives, float32: 4 slots and 4 CTAs 82 and 97 us, 4
-// and 5 80 and 93, 8 and 4 77 and 93; bfloat16: 52 and 66, 48 and 60, 48 and 68.
+// and 5 80 and 93, 8 and 4 77 and 88; bfloat16: 52 and 66, 48 and 60, 48 and 68.
 template <class T>
 constexpr int kBatch = sizeof(T) == 4 ? 8 : 4;
 template <class T, int CL>
@@ -293,7 +293,7 @@ struct TopShared {
   uint64_t held[NW][64];  // the slower way: keys that reach the bound, per warp
   uint64_t best[32];      // the CTA's k largest, descending, 0 where there are fewer
   float bound;
-  int n, n_who;
+  int n, n_who, count[NW];
   uint16_t who[NT];       // threads whose largest element reaches the bound
 };
 
@@ -350,14 +350,15 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   const float least = top.bound;
   const uint64_t bound = (uint64_t)sort_key(least) << 32;
   const bool in = seg.k0 + tid < seg.k1 && largest >= least;
-  const auto look = [&](const uint4& x, int kk) {
+  const auto look = [&](const uint4& x, int kk, bool above) {
     if (!(slot_max_nan<T>(x) >= least)) return;
+    if (*const_cast<volatile int*>(&top.n) > kFound) return;  // the list has overflowed already
     float z[VN];
     unpack16<T>(x, z);
 #pragma unroll
     for (int j = 0; j < VN; ++j) {
       const int e = seg.element(kk) + j;
-      if (z[j] >= least && e >= 0 && e < seg.V) {
+      if ((above ? z[j] > least : z[j] >= least) && e >= 0 && e < seg.V) {
         const int at = atomicAdd(&top.n, 1);
         if (at < kFound) top.found[at] = rank_key(z[j], e);
       }
@@ -370,45 +371,97 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
   if (in) top.who[base + __popc(all & ((1u << lane) - 1u))] = (uint16_t)tid;
   if (tid < 32) top.best[tid] = 0;
   group_sync<NW>();
-  const int n_who = top.n_who;
-  if (seg.k1 - seg.k0 <= kAgain * NT) {  // few slots each: every thread its own
-    if (in) {
-      uint4 x[kAgain];
-#pragma unroll
-      for (int b = 0; b < kAgain; ++b)
-        if (seg.k0 + tid + b * NT < seg.k1) x[b] = seg.load(seg.k0 + tid + b * NT);
-#pragma unroll
-      for (int b = 0; b < kAgain; ++b)
-        if (seg.k0 + tid + b * NT < seg.k1) look(x[b], seg.k0 + tid + b * NT);
-    }
-  } else {  // a warp per thread of the list, its slots over the lanes, kAgain such loads in flight
-    for (int t0 = w; t0 < n_who; t0 += kAgain * NW) {
-      for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
-        uint4 x[kAgain];
-        int kk[kAgain];
-#pragma unroll
-        for (int b = 0; b < kAgain; ++b) {
-          kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
-          if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
-        }
-#pragma unroll
-        for (int b = 0; b < kAgain; ++b)
-          if (kk[b] < seg.k1) look(x[b], kk[b]);
-      }
-    }
-  }
-  group_sync<NW>();
-  const int n = top.n;
-  if (n <= kFound) {
+  const auto overflow = [&] { return *const_cast<volatile int*>(&top.n) > kFound; };
+  const auto rank_found = [&](int n) {
     for (int i = tid; i < n; i += NT) {
       const uint64_t own = top.found[i];
       const int rank = keys_above(top.found, n, own);
       if (rank < k) top.best[rank] = own;
     }
     group_sync<NW>();
+  };
+  const int n_who = top.n_who;
+  // More than half of the threads reach the bound where the elements at it are many of one value: a mask's, say.
+  bool many = NW > 1 && n_who > NT / 2;
+  if (!many) {
+    if (seg.k1 - seg.k0 <= kAgain * NT) {  // few slots each: every thread its own
+      if (in) {
+        uint4 x[kAgain];
+#pragma unroll
+        for (int b = 0; b < kAgain; ++b)
+          if (seg.k0 + tid + b * NT < seg.k1) x[b] = seg.load(seg.k0 + tid + b * NT);
+#pragma unroll
+        for (int b = 0; b < kAgain; ++b)
+          if (seg.k0 + tid + b * NT < seg.k1) look(x[b], seg.k0 + tid + b * NT, false);
+      }
+    } else {  // a warp per thread of the list, its slots over the lanes, kAgain such loads in flight
+      for (int t0 = w; t0 < n_who && !overflow(); t0 += kAgain * NW) {
+        for (int s0 = lane * NT; s0 < seg.k1 - seg.k0; s0 += 32 * NT) {
+          uint4 x[kAgain];
+          int kk[kAgain];
+#pragma unroll
+          for (int b = 0; b < kAgain; ++b) {
+            kk[b] = t0 + b * NW < n_who ? seg.k0 + top.who[t0 + b * NW] + s0 : seg.k1;
+            if (kk[b] < seg.k1) x[b] = seg.load(kk[b]);
+          }
+#pragma unroll
+          for (int b = 0; b < kAgain; ++b)
+            if (kk[b] < seg.k1) look(x[b], kk[b], false);
+        }
+      }
+    }
+    group_sync<NW>();
+    const int n = top.n;
+    if (n <= kFound) {
+      rank_found(n);
+      return;
+    }
+    group_sync<NW>();
+    if (tid == 0) top.n = 0;
+    group_sync<NW>();
+  }
+  // Many elements reach the bound.  If few are above it, those and the first k at it will do, which are looked for
+  // from the start of the segment.
+  if (largest > least) {
+    for (int kk = seg.k0 + tid; kk < seg.k1 && !overflow(); kk += NT) look(seg.load(kk), kk, true);
+  }
+  group_sync<NW>();
+  const int above = top.n;
+  if (above <= kFound - 32) {
+    int at = 0;  // elements at the bound so far
+    for (int base = seg.k0; base < seg.k1 && at < k; base += NT) {
+      const int kk = base + tid;
+      float z[VN];
+      unpack16<T>(kk < seg.k1 ? seg.load(kk) : neg_inf_slot<T>(), z);
+      uint32_t here = 0u;
+#pragma unroll
+      for (int j = 0; j < VN; ++j) {
+        const int e = seg.element(kk) + j;
+        here |= (z[j] == least && kk < seg.k1 && e >= 0 && e < seg.V ? 1u : 0u) << j;
+      }
+      int before = __popc(here);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFull, before, o);
+        if (lane >= o) before += u;
+      }
+      if (lane == 31) top.count[w] = before;
+      group_sync<NW>();
+      before += at - __popc(here);
+#pragma unroll
+      for (int i = 0; i < NW; ++i) {
+        before += i < w ? top.count[i] : 0;
+        at += top.count[i];
+      }
+      for (; here && before < k; here &= here - 1u, ++before)
+        top.found[above + before] = rank_key(least, seg.element(kk) + __ffs(here) - 1);
+      group_sync<NW>();
+    }
+    rank_found(above + min(at, k));
     return;
   }
-  // The slower way, for rows whose largest elements lie with few threads: each warp keeps the 32 largest of what it
+  // The slower way, for rows whose largest elements lie with few threads (4096 x 32000 rising float32: 249 us, 98
+  // for rows without an order): each warp keeps the 32 largest of what it
   // has seen in order, one per lane, and raises its own bound by them.
   uint64_t mine = bound, list = 0;
   uint64_t* held = top.held[w];

@@ -187,6 +187,25 @@ def test_bad_rows_of_few_long_ones(V, dtype):
         check(z, y, k=32, grads=("both",))
 
 
+@pytest.mark.parametrize("dtype", R.FLOATS)
+@pytest.mark.parametrize("B,V", [(9, 900), (9, 5001), (5, 40000), (700, 9001), (2400, 3500)])
+def test_masks(B, V, dtype):
+    """Most columns of one value: -inf, the type's lowest, one between the others; few or many columns above it."""
+    g = R.gen(B + V)
+    rows = []
+    for i in range(9):
+        z = R.normal((V,), dtype, g, 2.0)
+        mask = (NEG, torch.finfo(dtype).min, -1.0)[i % 3]
+        keep = torch.rand(V, generator=g, device="cuda") < (3 / V, 40 / V, 0.3)[i // 3]
+        keep[int(torch.randint(0, V, (1,), generator=g, device="cuda"))] = True
+        rows.append(torch.where(keep, z, torch.full_like(z, mask)))
+    rows[0][: V // 2] = -50.0  # the mask begins late
+    z = torch.stack([rows[i % 9] for i in range(B)])
+    y = z.argmax(1)
+    for k in (1, 5, 32):
+        check(z, y, k=k, grads=("both",) if k == 5 else ())
+
+
 def test_offsets_past_2_31_elements():
     if torch.cuda.get_device_properties(0).total_memory < 60e9:
         pytest.skip("needs 20 GB of device memory")
