@@ -771,8 +771,13 @@ struct ProductArgs {
   const int32_t* label;
   const void* w;
   int64_t ldw;
-  const void* hp;  // and dW that of the rows of H with this label
+  // and dW that of the rows of H with this label: their sum is in the row of
+  // `sums` with the number of the first of them, first_row[v - v0] (-1: none)
+  const void* hp;
   int64_t ldh;
+  __nv_bfloat16* sums;
+  int64_t lds2;
+  int32_t* first_row;
 
   // 8 columns of it from c on, times `by`, added to v
   template <class T>
@@ -805,7 +810,7 @@ struct ProductTile {
     bool zero;
     float rest;  // BOTH: its label_rest, 0 without a label
     int label;
-    bool any;  // BOTH, dW: there are such rows for one of the warp's 32
+    bool any;  // BOTH, dW: there are sums for one of the warp's 32 rows
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, A_MN2 = true, B_MN = true, TWO = true;
@@ -887,74 +892,42 @@ struct ProductTile {
     if constexpr (BOTH) {
       st.label = dh && !st.zero ? a.label[row] : -1;
       st.rest = st.label >= 0 ? a.label_rest[row] : 0.0f;
-      st.any = !dh && add_rows(a, p, a.v0 + t.m0 + p.row, t.n0 + p.share * (BN / 2));
+      st.any = !dh && fetch(a, p, t.m0 + p.row, t.n0 + p.share * (BN / 2));
     }
   }
 
-  // BOTH: dW's rows take label_rest times the rows of H that have them as
-  // labels.  Packed rows are in the order of their labels, so those of a warp's
-  // 32 rows are next to each other.  While the tile's products run, the warp
-  // adds them up, four columns a lane, and leaves each sum in the staging row
-  // that the epilogue takes it from before it writes there: in bfloat16, whose
-  // range is that of the sums, and whose rounding is of a part that is itself
-  // what a rounding left.  (4014 live rows, 128256 x 4096 bfloat16: the error of
-  // dW 1.4 to 1.0 times that of a form in 32 bits rounded once.)
-  __device__ static bool add_rows(const Args& a, const TcPart& p, int v0, int c0) {
-    const int rows = a.head->rows, lane = p.lane;
-    const int from = first_at(a.label, rows, (uint32_t)v0, lane), to = first_at(a.label, rows, (uint32_t)v0 + 32u, lane);
-    if (from == to) return false;
+  // BOTH: dW's rows take what is in `sums`.  While the tile's products run, the
+  // warp leaves its rows' in the staging rows that the epilogue takes them from
+  // before it writes there.  (Loads wait here behind the operands' copies, some
+  // 5000 clocks, so that many are in flight and none depends on another.)
+  __device__ static bool fetch(const Args& a, const TcPart& p, int v, int c0) {
+    if (c0 >= a.D) return false;
+    const int first = a.first_row[v + p.lane];
+    uint32_t who = __ballot_sync(kFull, first >= 0);
+    if (who == 0u) return false;
     uint32_t* sm = reinterpret_cast<uint32_t*>(p.smem);
     constexpr int kWords = kStageWords<BN / 2>;
-    for (int i = lane; i < 32 * kWords; i += 32) sm[i] = 0u;
+    for (int i = p.lane; i < 32 * kWords; i += 32) sm[i] = 0u;
     __syncwarp();
-    const int c = c0 + 4 * lane;
-    const T* h = static_cast<const T*>(a.hp) + c;
-    float x[4] = {};
-    int run = a.label[from];
-    const auto give = [&] {
-      sm[(run - v0) * kWords + 2 * lane] = pack2<__nv_bfloat16>(x[0], x[1]);
-      sm[(run - v0) * kWords + 2 * lane + 1] = pack2<__nv_bfloat16>(x[2], x[3]);
-    };
-    for (int r0 = from; r0 < to; r0 += 8) {
-      uint2 u[8];
-      float by[8];
-      int y[8];
+    while (who) {
+      uint2 u[16];
+      int to[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = min(r0 + i, to - 1);
-        y[i] = a.label[r];
-        by[i] = a.label_rest[r];
-        u[i] = c < a.ldh ? *reinterpret_cast<const uint2*>(h + (int64_t)r * a.ldh) : make_uint2(0u, 0u);
+      for (int i = 0; i < 16; ++i) {
+        to[i] = __ffs(who) - 1;  // -1: no more
+        who &= who - 1;
+        const int64_t row = __shfl_sync(kFull, first, to[i] & 31);
+        if (to[i] >= 0) u[i] = *reinterpret_cast<const uint2*>(a.sums + row * a.lds2 + c0 + 4 * p.lane);
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r0 + i >= to) break;
-        if (y[i] != run) {
-          give();
-          run = y[i];
-          x[0] = x[1] = x[2] = x[3] = 0.0f;
+      for (int i = 0; i < 16; ++i)
+        if (to[i] >= 0) {
+          sm[to[i] * kWords + 2 * p.lane] = u[i].x;
+          sm[to[i] * kWords + 2 * p.lane + 1] = u[i].y;
         }
-        x[0] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x & 0xffffu), x[0]);
-        x[1] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x >> 16), x[1]);
-        x[2] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y & 0xffffu), x[2]);
-        x[3] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y >> 16), x[3]);
-      }
     }
-    give();
     __syncwarp();
     return true;
-  }
-  // First of the packed rows, in the order of their labels, whose label is at least v: 33 parts a step.
-  __device__ static int first_at(const int32_t* label, int rows, uint32_t v, int lane) {
-    int lo = 0, hi = rows;  // labels before lo are under v, those from hi on are not
-    while (lo < hi) {
-      const int step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step - 1;
-      const bool under = at < hi && (uint32_t)label[at] < v;
-      const int n = __popc(__ballot_sync(kFull, under));  // the first n of them
-      if (n < 32) hi = min(hi, lo + (n + 1) * step - 1);
-      lo += n * step;
-    }
-    return lo;
   }
 
   template <bool LOST, class Done>
@@ -1022,6 +995,119 @@ struct ProductTile {
   }
 };
 
+// First of the packed rows, in the order of their labels, whose label is at least v: 33 parts a step, by a warp.
+__device__ __forceinline__ int first_at(const int32_t* label, int rows, uint32_t v, int lane) {
+  int lo = 0, hi = rows;  // labels before lo are under v, those from hi on are not
+  while (lo < hi) {
+    const int step = (hi - lo + 32) / 33, at = lo + (lane + 1) * step - 1;
+    const bool under = at < hi && (uint32_t)label[at] < v;
+    const int n = __popc(__ballot_sync(kFull, under));  // the first n of them
+    if (n < 32) hi = min(hi, lo + (n + 1) * step - 1);
+    lo += n * step;
+  }
+  return lo;
+}
+
+// BOTH: label_rest times the rows of H, summed over the rows of every label:
+// what rounding took from dW's largest terms (bfloat16 has the range of the
+// sums, and rounds what is itself the rest of a rounding).  Packed rows are in
+// the order of their labels, so a label's are next to each other.  A CTA takes
+// the labels that begin in 32 rows, and 128 columns: those that end there a warp
+// each, the one that may go on beyond (the commonest tokens are those of a tenth
+// of the rows) all its warps, if it is long.  The grid's last CTAs look for the
+// first row of every v of the piece.  (Summed by the warps of the product's
+// tiles instead: labels that fall off as 1 / rank, 1609 live rows, 32000 x 2048
+// bfloat16, gradient 828 us, so 623; 65536 x 256 into 1000 3719 and 658.)
+template <class T>
+__global__ void __launch_bounds__(256) fw_xent_labels_kernel(ProductArgs a) {
+  __shared__ float4 part[8][32];
+  wait_prior_kernel();
+  allow_dependent_launch();
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int rows = a.head->rows, slabs = (a.D + 127) / 128, summing = a.Bp / 32 * slabs;
+  if ((int)blockIdx.x >= summing) {
+    const int i = ((int)blockIdx.x - summing) * 256 + threadIdx.x;
+    if (i >= a.vn) return;
+    const uint32_t v = (uint32_t)(a.v0 + i);
+    int lo = 0, hi = rows;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if ((uint32_t)a.label[mid] < v)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    a.first_row[i] = lo < rows && (uint32_t)a.label[lo] == v ? lo : -1;
+    return;
+  }
+  const int r0 = (int)blockIdx.x / slabs * 32, c = (int)blockIdx.x % slabs * 128 + 4 * lane;
+  if (r0 >= rows) return;
+  const int n = min(32, rows - r0);
+  const int y = lane < n ? a.label[r0 + lane] : -1, before = r0 + lane > 0 && lane < n ? a.label[r0 + lane - 1] : -2;
+  const uint32_t starts = __ballot_sync(kFull, lane < n && y != before);
+  if (starts == 0u) return;
+  const T* h = static_cast<const T*>(a.hp) + c;
+  // rows from .. to into x
+  const auto add = [&](int from, int to, float (&x)[4]) {
+    for (int r = from; r < to; r += 8) {
+      uint2 u[8];
+      float by[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t q = min(r + i, to - 1);
+        by[i] = a.label_rest[q];
+        u[i] = c < a.ldh ? *reinterpret_cast<const uint2*>(h + q * a.ldh) : make_uint2(0u, 0u);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r + i >= to) break;
+        x[0] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x & 0xffffu), x[0]);
+        x[1] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x >> 16), x[1]);
+        x[2] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y & 0xffffu), x[2]);
+        x[3] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y >> 16), x[3]);
+      }
+    }
+  };
+  const auto give = [&](int row, const float (&x)[4]) {
+    *reinterpret_cast<uint2*>(a.sums + (int64_t)row * a.lds2 + c) =
+        make_uint2(pack2<__nv_bfloat16>(x[0], x[1]), pack2<__nv_bfloat16>(x[2], x[3]));
+  };
+  const auto wanted = [&](int at) {  // its label is of this piece
+    const int v = __shfl_sync(kFull, y, at);
+    return v >= a.v0 && v < a.v0 + a.vn;
+  };
+  const int last = 31 - __clz((int)starts), turn = __popc(starts) - 1;
+  int i = 0;
+  for (uint32_t s = starts & ~(1u << last); s; s &= s - 1u, ++i) {
+    const int at = __ffs(s) - 1, end = __ffs(starts & ~((2u << at) - 1u)) - 1;
+    if (i % 8 != w || !wanted(at)) continue;
+    float x[4] = {};
+    add(r0 + at, r0 + end, x);
+    give(r0 + at, x);
+  }
+  if (!wanted(last)) return;
+  const int from = r0 + last, yl = __shfl_sync(kFull, y, last);
+  int to = r0 + n;
+  if (to < rows && a.label[to] == yl) to = first_at(a.label, rows, (uint32_t)yl + 1u, lane);
+  float x[4] = {};
+  if (to - from <= 32) {
+    if (turn % 8 != w) return;
+    add(from, to, x);
+    give(from, x);
+    return;
+  }
+  add(from + (int)((int64_t)(to - from) * w / 8), from + (int)((int64_t)(to - from) * (w + 1) / 8), x);
+  part[w][lane] = make_float4(x[0], x[1], x[2], x[3]);
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int q = 1; q < 8; ++q) {
+    const float4 o = part[q][lane];
+    x[0] += o.x, x[1] += o.y, x[2] += o.z, x[3] += o.w;
+  }
+  give(from, x);
+}
+
 // dH from the sums of its splits; one warp per row and 128 columns.
 template <class T, bool BOTH>
 __global__ void __launch_bounds__(256) fw_xent_dhidden_kernel(ProductArgs a) {
@@ -1084,7 +1170,7 @@ struct XentPlan {
   // forward workspace
   int64_t part, part_t, zy, loss_pack, sorted, hist, fwd_bytes;
   // backward workspace
-  int64_t piece, pieces, splits, top, label_rest, g, sum, hs, bwd_bytes;
+  int64_t piece, pieces, splits, top, label_rest, sums, first, g, sum, hs, bwd_bytes;
 };
 
 XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = false) {
@@ -1120,6 +1206,8 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = fal
   at = 0;
   p.top = at, at += 256;
   p.label_rest = at, at += both ? up(4 * p.Bp, 256) : 0;
+  p.sums = at, at += both ? up(2 * p.Bp * up(D, 128), 256) : 0;
+  p.first = at, at += both ? up(4 * p.piece, 256) : 0;
   p.g = at, at += up(2 * p.Bp * p.piece, 256);
   // as many as one row tile could use, 16 stages of K each, within kSumBytes
   p.splits = sm_count() / 2 / ((D + kTileN - 1) / kTileN);
@@ -1240,7 +1328,12 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
     const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
                             i == 0, i == p.pieces - 1, (int)p.piece, (int)p.splits,
                             (int)(tiles < pairs ? tiles : pairs), status, ga.label_rest, label, w, ldw,
-                            hp, p.Dp};
+                            hp, p.Dp, reinterpret_cast<__nv_bfloat16*>(ws + p.sums), up(D, 128),
+                            reinterpret_cast<int32_t*>(ws + p.first)};
+    if (BOTH && dweight) {
+      const int64_t ctas = p.Bp / 32 * ((D + 127) / 128) + vn / 256;
+      if (launch_dependent(fw_xent_labels_kernel<T>, ctas, 256, 0, 1, st, pa) != cudaSuccess) return FWB_E_LAUNCH;
+    }
     if (launch_gemm<ProductTile<T, K, BOTH>>(mg, wmn, pa, tiles, st, &gmn, &hmn) != cudaSuccess) return FWB_E_LAUNCH;
     if (dhidden && pa.last && p.splits > 1) {
       const int64_t need = (p.Bp * ((D + 127) / 128) + 7) / 8, cap = (int64_t)sm_count() * 16;
@@ -1328,18 +1421,17 @@ int fw_xent_backward(int dtype, const void* weight, int64_t ldw, int64_t B, int6
 
 static int head_check(int dtype, int64_t B, int64_t D, int64_t V, float inv_t) {
   if (int rc = xent_check(dtype, B, D, V)) return rc;
-  // an epilogue that walks all rows of one label has to end well within the other roles' waits
-  if (B > (1 << 24) || !(inv_t > 0.0f) || !std::isfinite(inv_t * kLog2e)) return FWB_E_SHAPE;
+  if (!(inv_t > 0.0f) || !std::isfinite(inv_t * kLog2e)) return FWB_E_SHAPE;
   return FWB_OK;
 }
 
 int64_t fw_lm_head_log_probs_state(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw) {
-  if (head_check(FWB_DTYPE_BF16, B, D, V, 1.0f) != FWB_OK) return 0;
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
   return xent_plan(B, D, V, !tma_rows(weight, ldw), true).state_bytes;
 }
 
 int64_t fw_lm_head_log_probs_workspace(int64_t B, int64_t D, int64_t V, int backward) {
-  if (head_check(FWB_DTYPE_BF16, B, D, V, 1.0f) != FWB_OK) return 0;
+  if (xent_check(FWB_DTYPE_BF16, B, D, V) != FWB_OK) return 0;
   const XentPlan p = xent_plan(B, D, V, false, true);
   return backward ? p.bwd_bytes : p.fwd_bytes;
 }

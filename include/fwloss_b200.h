@@ -601,8 +601,8 @@ FWB_API int fw_token_log_probs_grad(int dtype, const void* logits, int64_t ld, i
                                     const float* dentropy, void* grad, int64_t ldg, void* stream);
 
 /*
- * Log probabilities and entropies (fp32 [B], B <= 2^24) of logits = hidden
- * [B, D] x weight [V, D]^T at a temperature T, inv_t = 1 / T, without storing the
+ * Log probabilities and entropies (fp32 [B]) of logits = hidden [B, D] x
+ * weight [V, D]^T at a temperature T, inv_t = 1 / T, without storing the
  * logits: what fw_token_log_probs gives for them, with its rules for
  * ignore_index, tokens out of range and rows that are not finite, and with the
  * operands, state and workspaces of fw_xent_forward.

@@ -181,6 +181,21 @@ def test_labels_met_again_and_again(B, D, V, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,D,V", [(1000, 300, 2000), (3000, 129, 70), (2500, 64, 40000)])
+def test_common_labels(B, D, V, dtype):
+    """Labels that fall off as 1 / rank, runs of one label from 1 to a third of the rows, starting anywhere; one piece
+    of the vocabulary and several."""
+    g = R.gen(B)
+    h, w = R.normal((B, D), dtype, g), R.normal((V, D), dtype, g, D ** -0.5)
+    u = torch.rand(B, generator=g, device="cuda", dtype=torch.float64)
+    y = ((V + 1.0) ** u - 1.0).long().clamp_(0, V - 1)
+    check(h, w, y)
+    y[: B // 3] = V - 1
+    y[torch.rand(B, generator=g, device="cuda") < 0.1] = -100
+    check(h, w, y, temperature=1.3, kind="logp")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("B,V", [(8192, 300), (8193, 300), (20011, 3), (40000, 511), (9000, 512)])
 def test_many_rows(B, V, dtype):
     """Rows counted and rows sorted into the order of their labels; ignored rows and bad labels among them."""

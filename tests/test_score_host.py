@@ -67,7 +67,7 @@ def test_lm_head_log_probs_arguments():
         return f(dtype, h, ldh, w, ldw, y, B, 8, 10, it, -100, logp, ent, state, n, ws, m, P, P)
 
     assert fwd(dtype=0) == DTYPE
-    for bad in (dict(ldh=7), dict(ldw=7), dict(it=0.0), dict(it=float("inf")), dict(it=3e38), dict(B=-1), dict(B=(1 << 24) + 1)):
+    for bad in (dict(ldh=7), dict(ldw=7), dict(it=0.0), dict(it=float("inf")), dict(it=3e38), dict(B=-1), dict(B=(1 << 26) + 1)):
         assert fwd(**bad) == SHAPE, bad
     for bad in (dict(h=P), dict(w=P), dict(y=P), dict(logp=P), dict(ent=P), dict(state=P), dict(ws=P), dict(w=ODD, n=1 << 20),
                 dict(state=OFF), dict(ws=OFF)):
