@@ -1012,9 +1012,9 @@ __device__ __forceinline__ int first_at(const int32_t* label, int rows, uint32_t
 // what rounding took from dW's largest terms (bfloat16 has the range of the
 // sums, and rounds what is itself the rest of a rounding).  Packed rows are in
 // the order of their labels, so a label's are next to each other.  A CTA takes
-// the labels that begin in 32 rows, and 128 columns: those that end there a warp
-// each, the one that may go on beyond (the commonest tokens are those of a tenth
-// of the rows) all its warps, if it is long.  The grid's last CTAs look for the
+// the labels that begin in 32 rows, and 128 columns: a warp those that begin in
+// four of the rows, all warps the one that may go on beyond the 32, if it is long
+// (the commonest tokens are those of a tenth of the rows).  The grid's last CTAs look for the
 // first row of every v of the piece.  (Summed by the warps of the product's
 // tiles instead: labels that fall off as 1 / rank, 1609 live rows, 32000 x 2048
 // bfloat16, gradient 828 us, so 623; 65536 x 256 into 1000 3719 and 658.)
@@ -1047,25 +1047,25 @@ __global__ void __launch_bounds__(256) fw_xent_labels_kernel(ProductArgs a) {
   const uint32_t starts = __ballot_sync(kFull, lane < n && y != before);
   if (starts == 0u) return;
   const T* h = static_cast<const T*>(a.hp) + c;
-  // rows from .. to into x
-  const auto add = [&](int from, int to, float (&x)[4]) {
+  const auto load = [&](int64_t row, float& by, uint2& u) {
+    by = a.label_rest[row];
+    u = c < a.ldh ? *reinterpret_cast<const uint2*>(h + row * a.ldh) : make_uint2(0u, 0u);
+  };
+  const auto add_row = [&](float by, uint2 u, float (&x)[4]) {
+    x[0] = fmaf(by, Elem<T>::bits_to_f(u.x & 0xffffu), x[0]);
+    x[1] = fmaf(by, Elem<T>::bits_to_f(u.x >> 16), x[1]);
+    x[2] = fmaf(by, Elem<T>::bits_to_f(u.y & 0xffffu), x[2]);
+    x[3] = fmaf(by, Elem<T>::bits_to_f(u.y >> 16), x[3]);
+  };
+  const auto add = [&](int from, int to, float (&x)[4]) {  // rows from .. to
     for (int r = from; r < to; r += 8) {
       uint2 u[8];
       float by[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int64_t q = min(r + i, to - 1);
-        by[i] = a.label_rest[q];
-        u[i] = c < a.ldh ? *reinterpret_cast<const uint2*>(h + q * a.ldh) : make_uint2(0u, 0u);
-      }
+      for (int i = 0; i < 8; ++i) load(min(r + i, to - 1), by[i], u[i]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (r + i >= to) break;
-        x[0] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x & 0xffffu), x[0]);
-        x[1] = fmaf(by[i], Elem<T>::bits_to_f(u[i].x >> 16), x[1]);
-        x[2] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y & 0xffffu), x[2]);
-        x[3] = fmaf(by[i], Elem<T>::bits_to_f(u[i].y >> 16), x[3]);
-      }
+      for (int i = 0; i < 8; ++i)
+        if (r + i < to) add_row(by[i], u[i], x);
     }
   };
   const auto give = [&](int row, const float (&x)[4]) {
@@ -1076,14 +1076,28 @@ __global__ void __launch_bounds__(256) fw_xent_labels_kernel(ProductArgs a) {
     const int v = __shfl_sync(kFull, y, at);
     return v >= a.v0 && v < a.v0 + a.vn;
   };
-  const int last = 31 - __clz((int)starts), turn = __popc(starts) - 1;
-  int i = 0;
-  for (uint32_t s = starts & ~(1u << last); s; s &= s - 1u, ++i) {
-    const int at = __ffs(s) - 1, end = __ffs(starts & ~((2u << at) - 1u)) - 1;
-    if (i % 8 != w || !wanted(at)) continue;
+  const int last = 31 - __clz((int)starts);
+  if (const uint32_t mine = starts & (0xfu << 4 * w) & ~(1u << last)) {  // labels that begin in the warp's 4 rows
+    int at = __ffs(mine) - 1;
+    const int end = __ffs(starts & ~((2u << (31 - __clz((int)mine))) - 1u)) - 1;
     float x[4] = {};
-    add(r0 + at, r0 + end, x);
-    give(r0 + at, x);
+    for (int r = at; r < end; r += 8) {
+      uint2 u[8];
+      float by[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) load(r0 + min(r + i, end - 1), by[i], u[i]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        if (r + i >= end) break;
+        if (r + i != at && (starts >> (r + i) & 1u)) {
+          if (wanted(at)) give(r0 + at, x);
+          at = r + i;
+          x[0] = x[1] = x[2] = x[3] = 0.0f;
+        }
+        add_row(by[i], u[i], x);
+      }
+    }
+    if (wanted(at)) give(r0 + at, x);
   }
   if (!wanted(last)) return;
   const int from = r0 + last, yl = __shfl_sync(kFull, y, last);
@@ -1091,7 +1105,7 @@ __global__ void __launch_bounds__(256) fw_xent_labels_kernel(ProductArgs a) {
   if (to < rows && a.label[to] == yl) to = first_at(a.label, rows, (uint32_t)yl + 1u, lane);
   float x[4] = {};
   if (to - from <= 32) {
-    if (turn % 8 != w) return;
+    if (last / 4 != w) return;
     add(from, to, x);
     give(from, x);
     return;
