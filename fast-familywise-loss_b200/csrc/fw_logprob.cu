@@ -12,7 +12,7 @@
 // writes theirs.  4096 x 32000: forward float32 77 us (6.8 TB/s), bfloat16 48
 // (5.5: the exponentials beside it), with 5 alternatives 88 and 60, gradient 167
 // and 86 (6.1 to 6.3 TB/s).  Few rows are bound by latency: 48 x 128256 bfloat16
-// 7.8 us, with 20 alternatives 14.
+// 6.3 us, with 20 alternatives 10.7.
 //
 // The k likeliest columns come without a second pass over the row.  Every
 // thread also knows its largest element; the k-th largest of these (taken over
@@ -41,10 +41,13 @@ constexpr float kFloor = -200.0f;  // 2^kFloor is 0 in fp32; keeps 0 * t finite
 // Slots in flight per thread, and CTAs of 256 threads per SM.  4096 x 32000
 // without and with 5 alternatives, float32: 4 slots and 4 CTAs 82 and 97 us, 4
 // and 5 80 and 93, 8 and 4 77 and 88; bfloat16: 52 and 66, 48 and 60, 48 and 68.
-template <class T>
-constexpr int kBatch = sizeof(T) == 4 ? 8 : 4;
+// Rows split over CTAs, 48 x 128256 bfloat16 without and with 20 alternatives: 4
+// and 4 7.7 and 14.7, 8 and 4 7.8 and 14.7, 8 and 3 7.2 and 13.4.
 template <class T, int CL>
-constexpr int kCtas = sizeof(T) == 2 && CL == 1 ? 5 : 4;
+constexpr int kBatch = sizeof(T) == 4 || CL > 1 ? 8 : 4;
+constexpr int kSplitCtas = 3;
+template <class T, int CL>
+constexpr int kCtas = CL > 1 ? kSplitCtas : sizeof(T) == 2 ? 5 : 4;
 constexpr int kAgain = 4;  // slots in flight per thread where they are read again
 
 struct ScoreArgs {
@@ -510,7 +513,7 @@ __device__ __forceinline__ void top_of(TopShared<NW>& top, const Segment<T>& seg
 // or, for NW = 1, one row per warp of a CTA.
 template <class T, int NW, bool TOP, int CL>
 __global__ void __launch_bounds__(NW == 1 ? kWarpRows * 32 : NW * 32, NW == 8 ? kCtas<T, CL> : NW == 4 ? 8 : 3) fw_logprob_kernel(ScoreArgs a) {
-  constexpr int VN = 16 / sizeof(T), NT = NW * 32, N = kBatch<T>;
+  constexpr int VN = 16 / sizeof(T), NT = NW * 32, N = kBatch<T, CL>;
   constexpr int R = NW == 1 ? kWarpRows : 1;
   __shared__ Sums parts[R][NW];
   __shared__ Sums whole;  // of this CTA, for its cluster
@@ -788,12 +791,18 @@ bool by_warps(int64_t slots, int64_t B) { return slots <= (B >= (int64_t)sm_coun
 
 template <class T>
 int run_score(const ScoreArgs& a, cudaStream_t st) {
-  const int64_t slots = a.V / (16 / (int)sizeof(T)), ctas = (int64_t)sm_count() * 4;
+  const int64_t slots = a.V / (16 / (int)sizeof(T)), ctas = (int64_t)sm_count() * kSplitCtas;
   if (by_warps(slots, a.B)) return launch_score<T, 1, 1>(a, st);
-  // few long rows: in parts of at least 512 slots, as long as all parts run at once
-  if (slots >= 8 * 512 && a.B * 8 <= ctas) return launch_score<T, 8, 8>(a, st);
-  if (slots >= 4 * 512 && a.B * 4 <= ctas) return launch_score<T, 8, 4>(a, st);
-  if (slots >= 2 * 512 && a.B * 2 <= ctas) return launch_score<T, 8, 2>(a, st);
+  // Few long rows: split until a CTA has one round of loads (2048 slots), as long as all parts run at once; for more
+  // than 8 alternatives over 4 CTAs at most, since each gives its k to be ranked again.  128256 bfloat16 in 1, 2, 4, 8
+  // parts, 16 rows without and with 20 alternatives: 11.2, 6.7, 4.7, 4.3 and 14.5, 10.7, 8.6, 9.2 us; 48 rows 17.7, 8.6,
+  // 6.8, 6.3 and 21.1, 12.4, 10.6, 12.6; 128 rows 19.0, 13.6, 14.5, 16.3 and 23.5, 18.6, 22.4, 31.8; 32000 float32 (8000
+  // slots), 1 row: 4.5, 4.0, 3.2, 3.0 and (5 alternatives) 6.2, 6.1, 5.3, 5.7.
+  int parts = 1;
+  while (parts < (a.k > 8 ? 4 : 8) && slots > parts * 2048 && a.B * parts * 2 <= ctas) parts *= 2;
+  if (parts == 8) return launch_score<T, 8, 8>(a, st);
+  if (parts == 4) return launch_score<T, 8, 4>(a, st);
+  if (parts == 2) return launch_score<T, 8, 2>(a, st);
   if (slots <= 2048) return launch_score<T, 4, 1>(a, st);
   return launch_score<T, 8, 1>(a, st);
 }
