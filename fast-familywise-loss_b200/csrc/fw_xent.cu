@@ -415,7 +415,7 @@ struct JoinArgs {
   const float* zy;
   const int32_t* label;
   const int32_t* row_of;
-  float* lse;        // [Bp], packed
+  float* lse;        // [Bp], packed; BOTH: maximum
   float* loss_pack;  // [Bp], packed
   float* loss;       // [B] (reduction none) or one value
   int64_t Bp;
@@ -424,6 +424,7 @@ struct JoinArgs {
   int32_t* status;
   const float* part_t;           // BOTH, which writes logp in the place of the loss
   float *entropy, *entropy_pack;  // per given row, packed
+  float* log_s;                   // BOTH: log S, packed
   float inv_t;
 };
 
@@ -494,7 +495,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) fw_xent_join_both_kernel(Join
   const float log_s = logf(S), nan = CUDART_NAN_F;
   const int to = a.row_of[mine];
   const float h = ok ? log_s - U * kLn2 / S : nan;
-  a.lse[mine] = ok ? fmaf(M, a.inv_t, log_s) : nan;
+  a.lse[mine] = ok ? M : nan;
+  a.log_s[mine] = ok ? log_s : nan;
   a.entropy_pack[mine] = h;
   a.entropy[to] = h;
   a.loss[to] = ok ? (a.zy[mine] - M) * a.inv_t - log_s : nan;
@@ -592,11 +594,11 @@ struct Upstream {
     if (!(s < CUDART_INF_F)) return g;
     return f16 && *top > 0.0f ? s / *top * kF16Unit : s;
   }
-  // BOTH: -a_r and -b_r, scaled to the range of the type; NaN where either is not finite
-  __device__ float2 in_g_both(int r) const {
-    if (!(factor(r) < CUDART_INF_F)) return make_float2(CUDART_NAN_F, CUDART_NAN_F);
-    const float a = go ? -go[r] : 0.0f, b = go_ent ? -go_ent[r] : 0.0f;
-    return f16 && *top > 0.0f ? make_float2(a / *top * kF16UnitBoth, b / *top * kF16UnitBoth) : make_float2(a, b);
+  // BOTH: -a_r and -b_r, scaled to the range of the type (float16: by kF16UnitBoth / top); NaN where either is not finite
+  __device__ float top_both() const { return f16 && *top > 0.0f ? *top : 0.0f; }
+  __device__ float2 in_g_both(float a, float b, float top) const {
+    if (!(fabsf(a) < CUDART_INF_F && fabsf(b) < CUDART_INF_F)) return make_float2(CUDART_NAN_F, CUDART_NAN_F);
+    return top > 0.0f ? make_float2(-a / top * kF16UnitBoth, -b / top * kF16UnitBoth) : make_float2(-a, -b);
   }
   // f_r; 1 where the factor is in G (0, not finite, BOTH) or common
   __device__ float rest(int r) const {
@@ -665,17 +667,16 @@ struct GradArgs {
   int v0, vn;  // first column of the piece, its columns rounded up to 256
   int32_t* status;
   const float* entropy;  // BOTH: packed
+  const float* log_s;    // BOTH: log S, packed; `lse` has the maxima
   float* label_rest;     // BOTH: what rounding took from the label's entry, packed
 };
 
-template <class T, TcKind K, bool BOTH>
+template <class T, TcKind K>
 struct GradTile {
   using Args = GradArgs;
   struct State {
     float lse, coef;
     int y;
-    float h;      // BOTH: the row's entropy,
-    float2 both;  // and its factors
   };
   static constexpr TcKind KIND = K;
   static constexpr bool A_MN = false, B_MN = false;
@@ -697,13 +698,7 @@ struct GradTile {
     const bool live = row < a.head->rows;
     st.y = live ? a.label[row] : -2;  // -2: not a live row
     st.lse = live ? a.lse[row] : 0.0f;
-    if constexpr (BOTH) {
-      st.coef = 1.0f;
-      st.h = live ? a.entropy[row] : 0.0f;
-      st.both = live ? a.up.in_g_both(a.row_of[row]) : make_float2(0.0f, 0.0f);
-    } else {
-      st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
-    }
+    st.coef = live ? a.up.in_g(a.row_of[row]) : 0.0f;
   }
   template <bool LOST, class Done>
   __device__ static void epilogue(const Args& a, const Plan&, const TcTile& t, const TcPart& p, State& st, int, int,
@@ -722,13 +717,6 @@ struct GradTile {
         float q;
         if constexpr (LOST) {
           q = CUDART_NAN_F;
-        } else if constexpr (BOTH) {  // of a bad row lse and h are NaN, and so is q
-          const float l = fmaxf(fmaf(v[i], a.up.inv_t, -lse), kExpFloor * kLn2), p = exp2_hw(l * kLog2e);
-          q = p * fmaf(st.both.y, l + st.h, st.both.x);
-          if (t.n0 + c + i == y) {
-            q -= st.both.x;
-            a.label_rest[row] = q - Elem<T>::to_f(Elem<T>::from_f(q));
-          }
         } else {
           q = exp2_hw((v[i] - lse) * kLog2e);
           if (t.n0 + c + i == y) q -= 1.0f;
@@ -737,6 +725,117 @@ struct GradTile {
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) *reinterpret_cast<uint4*>(g + c + 8 * i) = pack_slot<T>(v + 8 * i);
+    }
+  }
+};
+
+// BOTH: with l = (z - max z) / T - log S, and the maximum and log S apart: M / T
+// + log S in one number would be off by half an ulp of M / T, by 2e-5 at T = 0.1
+// and 2e-3 at T = 1e-3 where the winning logit is 50.
+// A sum over all of K in the accumulator (KC 0) shrinks a logit more than the
+// forward's does (kLseStages), by up to D / 8 ulps of its terms, which T
+// divides too: of a winning logit of 50, D = 2048, a probability of 1 came out
+// 2e-4 too small at T = 1, 2 % at T = 0.01.  That is under the rounding of G down
+// to kLowT.  At lower temperatures z is made as in the forward: the same bits, of
+// which the maximum is one, and the probabilities add up to 1 within fp32's
+// rounding whatever T is.  Parts are short, and the epilogue of a tile's last one
+// is then waited for: 1609 live rows, 32000 x 2048 float16 172 and 217 us, 4014
+// rows, 128256 x 4096 bfloat16 3.32 and 3.96 ms.
+// Nothing in `begin` waits: a row's factors, which are behind row_of, are asked
+// for after the first part, and worked out after the last (with parts: 226 us
+// where the labels' entries are looked at one by one, 217 all at once).
+constexpr float kLowT = 0.5f;
+
+template <class T, TcKind K, bool LOW>
+struct GradBothTile {
+  using Args = GradArgs;
+  static constexpr int COLS = 128;  // of a tile per epilogue thread
+  struct State {
+    int y, row;      // -2: not a live row; the given row
+    float m, log_s, h;
+    float lo, en;    // the upstream factors
+    float z[COLS] = {};  // the logits so far
+  };
+  static constexpr TcKind KIND = K;
+  static constexpr bool A_MN = false, B_MN = false;
+  static constexpr bool TWO = false, A_MN2 = false;
+  static constexpr int CG = 2, BN = kTileN, STAGES = 7, KC = LOW ? kLseStages : 0, EW = 4 * BN / COLS, A_BOX = 128, AHEAD = 0;
+  static constexpr uint32_t EPI_BYTES = 0;
+  struct Plan {
+    TurnPlan turn;
+    int rows;
+    float top;  // of the factors, float16
+  };
+  __device__ static void plan(const Args& a, int group, int groups, Plan* p) {
+    p->turn.set(row_tiles(a.head), a.vn / BN, group, groups);
+    p->rows = a.head->rows;
+    p->top = a.up.top_both();
+  }
+  __device__ static bool get(const Args& a, const Plan& p, int i, TcTile* t) {
+    int m, n;
+    if (!p.turn.get(i, &m, &n)) return false;
+    *t = {m * kTileM, a.v0 + n * BN, 0, 0, (a.D + 63) / 64, 128, 0};
+    return true;
+  }
+  __device__ static void begin(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st) {
+    const int row = t.m0 + p.row + p.lane;
+    st.y = -2;
+    st.row = -1;
+    st.m = st.log_s = st.h = st.lo = st.en = 0.0f;
+    if (row < plan.rows) {
+      st.y = a.label[row];
+      st.row = a.row_of[row];
+      st.m = a.lse[row];
+      st.log_s = a.log_s[row];
+      st.h = a.entropy[row];
+    }
+  }
+  template <bool LOST, class Done>
+  __device__ static void epilogue(const Args& a, const Plan& plan, const TcTile& t, const TcPart& p, State& st, int k,
+                                  int parts, Done done) {
+    const int row = t.m0 + p.row + p.lane, n0 = t.n0 + p.share * COLS;
+    if constexpr (!LOST) {
+#pragma unroll
+      for (int c = 0; c < COLS; c += 16) {
+        float v[16];
+        tmem_ld16(p.taddr + p.share * COLS + c, v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st.z[c + i] += v[i];
+      }
+      done();
+      if (k == 0 && st.row >= 0) {
+        if (a.up.go) st.lo = a.up.go[st.row];
+        if (a.up.go_ent) st.en = a.up.go_ent[st.row];
+      }
+      if (k < parts - 1) return;
+    }
+    T* g = static_cast<T*>(a.g) + (int64_t)row * a.ldg + (n0 - a.v0);
+    const float2 f = a.up.in_g_both(st.lo, st.en, plan.top);
+    const int y = st.y - n0, valid = st.y != -2 ? a.V - n0 : 0;
+    const auto entry = [&](float z) {  // of a bad row m, log_s and h are NaN, and so is what comes of them
+      const float l = fmaxf(fmaf(z - st.m, a.up.inv_t, -st.log_s), kExpFloor * kLn2);
+      return exp2_hw(l * kLog2e) * fmaf(f.y, l + st.h, f.x);
+    };
+    float zy = 0.0f;
+#pragma unroll
+    for (int c = 0; c < COLS; c += 8) {
+      if (!LOST && (unsigned)(y - c) < 8u) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) zy = c + i == y ? st.z[c + i] : zy;
+      }
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        v[i] = LOST ? CUDART_NAN_F : entry(st.z[c + i]);
+        v[i] = c + i < valid ? v[i] : 0.0f;
+      }
+      *reinterpret_cast<uint4*>(g + c) = pack_slot<T>(v);
+    }
+    if (!LOST && (unsigned)y < (unsigned)COLS) {
+      const float q = entry(zy) - f.x;
+      const T r = Elem<T>::from_f(q);
+      g[y] = r;
+      a.label_rest[row] = q - Elem<T>::to_f(r);
     }
   }
 };
@@ -1180,7 +1279,7 @@ struct XentPlan {
   int64_t Bp, Dp;
   bool copy_w;
   // state: what backward needs
-  int64_t row_of, label, lse, entropy, hp, wp, state_bytes;
+  int64_t row_of, label, lse, entropy, log_s, hp, wp, state_bytes;
   // forward workspace
   int64_t part, part_t, zy, loss_pack, sorted, hist, fwd_bytes;
   // backward workspace
@@ -1197,6 +1296,7 @@ XentPlan xent_plan(int64_t B, int64_t D, int64_t V, bool copy_w, bool both = fal
   p.label = at, at += up(4 * p.Bp, 256);
   p.lse = at, at += up(4 * p.Bp, 256);
   p.entropy = at, at += both ? up(4 * p.Bp, 256) : 0;
+  p.log_s = at, at += both ? up(4 * p.Bp, 256) : 0;
   p.hp = at, at += up(2 * p.Bp * p.Dp, 256);
   p.wp = at, at += copy_w ? up(2 * V * p.Dp, 256) : 0;
   p.state_bytes = at;
@@ -1293,7 +1393,7 @@ int run_forward(const void* hidden, int64_t ldh, const void* weight, int64_t ldw
   if (launch_gemm<LseTile<K, BOTH>>(mh, mw, la, (p.Bp / 256) * nt, st) != cudaSuccess) return FWB_E_LAUNCH;
   JoinArgs ja = {head, la.part, la.zy, label, row_of, reinterpret_cast<float*>(state + p.lse),
                  reinterpret_cast<float*>(ws + p.loss_pack), loss, p.Bp, (int)((V + kLseCols - 1) / kLseCols), reduction, status,
-                 la.part_t, entropy, reinterpret_cast<float*>(state + p.entropy), inv_t};
+                 la.part_t, entropy, reinterpret_cast<float*>(state + p.entropy), reinterpret_cast<float*>(state + p.log_s), inv_t};
   return launch_status(launch_dependent(BOTH ? fw_xent_join_both_kernel : fw_xent_join_kernel, p.Bp / 32, kJoinWarps * 32, 0, 1, st, ja));
 }
 
@@ -1335,8 +1435,17 @@ int run_backward(const void* weight, int64_t ldw, int64_t B, int64_t D, int64_t 
     const int v0 = (int)(i * p.piece), vn = (int)(Vp - v0 < p.piece ? Vp - v0 : p.piece);
     const GradArgs ga = {head, label, row_of, reinterpret_cast<const float*>(state + p.lse), u, g, p.piece, (int)V, (int)D,
                          v0, vn, status, reinterpret_cast<const float*>(state + p.entropy),
+                         reinterpret_cast<const float*>(state + p.log_s),
                          reinterpret_cast<float*>(ws + p.label_rest)};
-    if (launch_gemm<GradTile<T, K, BOTH>>(mh, mw, ga, mb * (vn / 256), st) != cudaSuccess) return FWB_E_LAUNCH;
+    const int64_t logit_tiles = mb * (vn / 256);
+    cudaError_t e;
+    if constexpr (!BOTH)
+      e = launch_gemm<GradTile<T, K>>(mh, mw, ga, logit_tiles, st);
+    else if (inv_t > 1.0f / kLowT)
+      e = launch_gemm<GradBothTile<T, K, true>>(mh, mw, ga, logit_tiles, st);
+    else
+      e = launch_gemm<GradBothTile<T, K, false>>(mh, mw, ga, logit_tiles, st);
+    if (e != cudaSuccess) return FWB_E_LAUNCH;
     const int64_t tiles = (dhidden ? mb * nd * p.splits : 0) + (dweight ? vn / 256 * nd : 0);
     const int64_t pairs = sm_count() / 2;
     const ProductArgs pa = {head, row_of, u, sum, dhidden, dweight, (int)p.Bp, (int)V, (int)D, (int)up(D, 32), v0, vn,
