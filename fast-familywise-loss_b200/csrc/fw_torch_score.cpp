@@ -289,6 +289,88 @@ void check_overlaps(const List& l) {
   }
 }
 
+// A tensor's memory: `lo` and what dims [stride, size] reach from there, in bytes, elements of `size`.
+struct Memory {
+  int64_t lo, hi, size;
+  c10::SmallVector<std::pair<int64_t, int64_t>, 4> dims;
+  explicit Memory(const Tensor& t) : lo((int64_t)reinterpret_cast<uintptr_t>(t.data_ptr())), size((int64_t)t.element_size()) {
+    if (dense(t)) {
+      dims.push_back({size, t.numel()});
+    } else {
+      for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1 && t.stride(d) > 0) dims.push_back({t.stride(d) * size, t.size(d)});
+    }
+    hi = lo + size;
+    for (const auto& d : dims) hi += d.first * (d.second - 1);
+  }
+};
+
+// Whether two tensors have a byte in common.  Their elements are at lo + sum of stride * i: looked for is a set of
+// indices whose distance is under an element's size, from the largest stride down, where a stride that both have counts
+// as one with their difference as index; of every index only those values are tried from which the smaller strides
+// reach.  Interleaved views take a few steps; where strides have nothing to do with each other it may be very many, and
+// tensors that are not told apart in 2^16 steps count as overlapping.
+bool meet(const Memory& a, const Memory& b) {
+  if (a.lo >= b.hi || b.lo >= a.hi) return false;
+  struct Step {
+    int64_t stride, least, most;  // of the index
+    int64_t under, over;          // what the strides behind it add at least and at most
+  };
+  c10::SmallVector<Step, 8> steps;
+  const auto add = [&](int64_t stride, int64_t least, int64_t most) {
+    for (auto& s : steps)
+      if (s.stride == stride) {
+        s.least += least, s.most += most;
+        return;
+      }
+    steps.push_back({stride, least, most, 0, 0});
+  };
+  for (const auto& d : a.dims) add(d.first, 0, d.second - 1);
+  for (const auto& d : b.dims) add(d.first, 1 - d.second, 0);
+  std::sort(steps.begin(), steps.end(), [](const Step& x, const Step& y) { return x.stride > y.stride; });
+  for (size_t i = steps.size(); i-- > 1;) {
+    steps[i - 1].under = steps[i].under + steps[i].stride * steps[i].least;
+    steps[i - 1].over = steps[i].over + steps[i].stride * steps[i].most;
+  }
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0 ? 1 : 0); };
+  int left = 1 << 16;
+  const auto search = [&](auto&& self, size_t i, int64_t at) -> bool {  // at: a's place less b's, so far
+    if (i == steps.size()) return at > -a.size && at < b.size;
+    const Step& s = steps[i];
+    const int64_t first = std::max(s.least, -floor_div(at + s.over + a.size - 1, s.stride));
+    const int64_t last = std::min(s.most, floor_div(b.size - 1 - at - s.under, s.stride));
+    for (int64_t k = first; k <= last; ++k)
+      if (--left <= 0 || self(self, i + 1, at + s.stride * k)) return true;
+    return false;
+  };
+  return search(search, 0, a.lo - b.lo);
+}
+
+// The same for results that are copied to where they belong (`back`), by their own memory.
+void check_copied(const std::vector<Tensor>& grads, const std::vector<Tensor>& dest, const std::vector<bool>& copied) {
+  struct Range {
+    Memory memory;
+    size_t tensor;
+    bool written, copied;
+  };
+  std::vector<Range> ranges;
+  ranges.reserve(2 * grads.size());
+  for (size_t i = 0; i < grads.size(); ++i) {
+    if (grads[i].numel() == 0) continue;
+    ranges.push_back({Memory(dest[i]), i, true, (bool)copied[i]});
+    if (!grads[i].is_same(dest[i])) ranges.push_back({Memory(grads[i]), i, false, false});
+  }
+  std::sort(ranges.begin(), ranges.end(), [](const Range& x, const Range& y) { return x.memory.lo < y.memory.lo; });
+  std::vector<const Range*> open;  // those that reach the present one's start
+  for (const auto& r : ranges) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Range* o) { return o->memory.hi <= r.memory.lo; }), open.end());
+    for (const Range* o : open)
+      if (o->tensor != r.tensor && (o->copied || r.copied) && meet(o->memory, r.memory))
+        refuse("clip_grad_norm_", "tensors that are written overlap others (the same tensor twice?)");
+    open.push_back(&r);
+  }
+}
+
 Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const c10::optional<std::vector<Tensor>>& out,
                        const OptTensor& norm_in, const OptTensor& status) {
   check_grads(grads, "clip_grad_norm_");
@@ -311,6 +393,7 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
   const c10::cuda::CUDAGuard guard(grads[0].device());
   List l(grads.size());
   std::vector<std::pair<Tensor, Tensor>> back;  // results that are copied to where they belong
+  std::vector<bool> copied(grads.size());
   for (size_t i = 0; i < grads.size(); ++i) {
     const auto &g = grads[i], &d = dest[i];
     l.numel.push_back(g.numel());
@@ -325,7 +408,10 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
     Tensor to = out.has_value() ? d : from;
     if (!dense(to) || (to.strides() != from.strides() && !(to.is_contiguous() && from.is_contiguous())))
       to = at::empty_strided(from.sizes(), from.strides(), d.options());  // an element is where it is in `from`
-    if (!to.is_same(d)) back.emplace_back(d, to);
+    if (!to.is_same(d)) {
+      back.emplace_back(d, to);
+      copied[i] = true;
+    }
     l.held.push_back(from);
     l.held.push_back(to);
     l.in.push_back(from.data_ptr());
@@ -333,6 +419,7 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
   }
   for (const auto& b : back) at::assert_no_internal_overlap(b.first);
   check_overlaps(l);
+  if (!back.empty()) check_copied(grads, dest, copied);
   int64_t nw = 0;
   Tensor ws, norm;
   if (norm_in.has_value()) {
