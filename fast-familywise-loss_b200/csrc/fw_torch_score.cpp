@@ -420,6 +420,11 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
   for (const auto& b : back) at::assert_no_internal_overlap(b.first);
   check_overlaps(l);
   if (!back.empty()) check_copied(grads, dest, copied);
+  if (norm_in.has_value()) {  // every CTA reads it, while others have begun to write
+    const Memory at(*norm_in);
+    for (const auto& t : dest)
+      value_check(t.numel() == 0 || !meet(at, Memory(t)), "clip_grad_norm_: norm must not lie in a tensor that is written");
+  }
   int64_t nw = 0;
   Tensor ws, norm;
   if (norm_in.has_value()) {

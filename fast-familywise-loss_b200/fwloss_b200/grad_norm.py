@@ -47,8 +47,9 @@ def clip_grad_norm_(grads, max_norm, out=None, norm=None, status=None):
     where `out` has a tensor for each of them (same shapes, any of the three
     types), which then holds the products, rounded once.  Tensors that are
     written must not overlap others, nor require grad: pass p.grad, not p.
-    `norm`, a float32 CUDA tensor of one value, is taken for the global norm
-    instead of the tensors' own, and returned.  A norm that is not finite gives
+    `norm`, a float32 CUDA tensor of one value outside the tensors that are
+    written, is taken for the global norm instead of the tensors' own, and
+    returned.  A norm that is not finite gives
     what the formula gives: infinity scales by 0 (NaN where an element is
     infinite), NaN makes everything NaN; `status` receives
     FWB_STATUS_NONFINITE when the norm is computed here."""

@@ -639,7 +639,7 @@ FWB_API int fw_lm_head_log_probs_grad(int dtype, const void* weight, int64_t ldw
  * the one the call runs on) holds partial sums.
  * fw_grad_clip takes the norm from norm_in, one value on the device, if that
  * is given (norm, status and the workspace are not used then), else computes
- * it and writes it to norm.
+ * it and writes it to norm.  norm_in must not lie in a tensor that is written.
  */
 FWB_API int64_t fw_grad_norm_workspace(int64_t n);
 FWB_API int fw_grad_norm(int64_t n, const void* const* grads, const int64_t* numel, const int32_t* dtypes,

@@ -73,3 +73,21 @@ def test_many_interleaved_results():
     g = ones(100, 512)
     fw.clip_grad_norm_([g[:, i] for i in range(512)], 51200 ** 0.5 / 2)
     R.within(g, torch.full_like(g, 0.5).double(), 20 * R.E32)
+
+
+def test_a_norm_in_what_is_written_is_refused():
+    x, m = ones(5000), ones(100, 100)
+    calls = [lambda: fw.clip_grad_norm_([x], 0.5, norm=x[:1]), lambda: fw.clip_grad_norm_([ones(7), x], 0.5, norm=x[4999]),
+             lambda: fw.clip_grad_norm_([ones(5000)], 0.5, out=[x], norm=x[77:78]),
+             lambda: fw.clip_grad_norm_([m[:, ::2]], 0.5, norm=m[3, 4]),
+             lambda: fw.clip_grad_norm_([ones(100, 50, dtype=torch.float16)], 0.5, out=[m.t()[::2].t()], norm=m[99, 98]),
+             lambda: fw.clip_grad_norm_([m.view(torch.bfloat16)[:, 1::2]], 0.5, norm=m[0, 0])]
+    for call in calls:
+        with pytest.raises(ValueError, match="norm must not lie"):
+            call()
+    assert (x == 1).all() and (m == 1).all()
+    # beside what is written, or in what is only read
+    assert float(fw.clip_grad_norm_([m[:, ::2]], 0.5, norm=m[3, 5])) == 1.0 and (m[:, ::2] == 0.5).all() and (m[:, 1::2] == 1).all()
+    out = torch.empty_like(x)
+    assert float(fw.clip_grad_norm_([x], 0.25, out=[out], norm=x[:1])) == 1.0 and (out == 0.25).all()
+    assert float(fw.clip_grad_norm_([x[1:]], 0.5, norm=x[0])) == 1.0 and (x[1:] == 0.5).all() and float(x[0]) == 1.0
