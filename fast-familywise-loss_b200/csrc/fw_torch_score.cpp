@@ -381,6 +381,8 @@ Tensor clip_grad_norm_(const std::vector<Tensor>& grads, double max_norm, const 
     const auto& t = dest[i];
     value_check(!t.requires_grad(), "clip_grad_norm_: written tensors must not require grad (pass p.grad, not p)");
     if (!out.has_value()) continue;
+    value_check(!(at::GradMode::is_enabled() && grads[i].requires_grad()),
+                "clip_grad_norm_: not differentiable; pass gradients (p.grad), or detach");
     type_check(t.is_cuda() && t.layout() == torch::kStrided && is_float(t),
                "clip_grad_norm_: out must hold dense float32, bfloat16 or float16 CUDA tensors");
     value_check(t.device() == grads[0].device() && t.sizes() == grads[i].sizes(),

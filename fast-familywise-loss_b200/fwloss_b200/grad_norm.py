@@ -46,7 +46,8 @@ def clip_grad_norm_(grads, max_norm, out=None, norm=None, status=None):
     grads as for grad_norm; they are changed in place, or left as they are
     where `out` has a tensor for each of them (same shapes, any of the three
     types), which then holds the products, rounded once.  Tensors that are
-    written must not overlap others, nor require grad: pass p.grad, not p.
+    written must not overlap others, nor require grad (with `out`, gradients that
+    do are refused in grad mode): pass p.grad, not p.
     `norm`, a float32 CUDA tensor of one value outside the tensors that are
     written, is taken for the global norm instead of the tensors' own, and
     returned.  A norm that is not finite gives

@@ -91,3 +91,19 @@ def test_a_norm_in_what_is_written_is_refused():
     out = torch.empty_like(x)
     assert float(fw.clip_grad_norm_([x], 0.25, out=[out], norm=x[:1])) == 1.0 and (out == 0.25).all()
     assert float(fw.clip_grad_norm_([x[1:]], 0.5, norm=x[0])) == 1.0 and (x[1:] == 0.5).all() and float(x[0]) == 1.0
+
+
+def test_gradients_of_a_graph_are_refused():
+    """Their graph would be dropped without a word, as grad_norm says."""
+    p, out = ones(8).requires_grad_(True), ones(8)
+    for g in (p, p * 2.0):
+        with pytest.raises(ValueError, match="not differentiable"):
+            fw.clip_grad_norm_([ones(8), g], 1.0, out=[ones(8), out])
+        with pytest.raises(ValueError, match="not differentiable"):
+            fw.grad_norm([ones(8), g])
+    assert (out == 1).all() and (p == 1).all()
+    with torch.no_grad():
+        fw.clip_grad_norm_([p], 2.0 ** 0.5, out=[out])
+    R.within(out, torch.full_like(out, 0.5).double(), 20 * R.E32)
+    fw.clip_grad_norm_([p.detach()], 8.0 ** 0.5 / 4, out=[out])
+    R.within(out, torch.full_like(out, 0.25).double(), 20 * R.E32)
