@@ -52,7 +52,11 @@ def lm_head_log_probs(hidden, weight, tokens, temperature=1.0, ignore_index=-100
 
     Differentiable in hidden and weight through both results.  The backward pass
     forms the logit gradient in pieces of the vocabulary (a bounded workspace)
-    and rounds it to the operands' type, each row without its upstream factor's
-    magnitude; an upstream gradient that is not finite makes its row of hidden's
-    gradient, and all of weight's, NaN."""
+    and rounds it, upstream factors included, to the operands' type; what that
+    takes from the entry of a row's token is added to both gradients.  float16
+    holds the entries relative to the largest factor m of the call: each is off
+    by up to 2^-37 m / temperature, so that in a row whose own factor is 2^-20 m,
+    probabilities under 2^-17 may be lost (its token's entry is not).  bfloat16
+    has the range of float32.  An upstream gradient that is not finite makes its
+    row of hidden's gradient, and all of weight's, NaN."""
     return ext().lm_head_log_probs(hidden, weight, tokens, temperature, ignore_index, status)

@@ -609,7 +609,9 @@ FWB_API int fw_token_log_probs_grad(int dtype, const void* logits, int64_t ld, i
  * fw_lm_head_log_probs_grad writes dhidden [B, D] and dweight [V, D]
  * (contiguous, either may be NULL) for the upstream gradients dlogp and
  * dentropy (fp32 [B]; NULL: none); a factor that is not finite makes its row of
- * dhidden and all of dweight NaN.
+ * dhidden and all of dweight NaN.  float16 operands: entries of the logit
+ * gradient other than the token's are off by up to 2^-37 inv_t of the largest
+ * factor in the call, besides their rounding.
  */
 FWB_API int64_t fw_lm_head_log_probs_state(int64_t B, int64_t D, int64_t V, const void* weight, int64_t ldw);
 FWB_API int64_t fw_lm_head_log_probs_workspace(int64_t B, int64_t D, int64_t V, int backward);
