@@ -50,10 +50,15 @@ def clip_grad_norm_(grads, max_norm, out=None, norm=None, status=None):
     do are refused in grad mode): pass p.grad, not p.
     `norm`, a float32 CUDA tensor of one value outside the tensors that are
     written, is taken for the global norm instead of the tensors' own, and
-    returned.  A norm that is not finite gives
-    what the formula gives: infinity scales by 0 (NaN where an element is
-    infinite), NaN makes everything NaN; `status` receives
-    FWB_STATUS_NONFINITE when the norm is computed here."""
+    returned.  A norm that is not finite gives what the formula gives: infinity
+    scales by 0 (NaN where an element is infinite; under a max_norm of infinity
+    nothing is scaled), NaN makes everything NaN; `status` receives
+    FWB_STATUS_NONFINITE when the norm is computed here.
+
+    Unlike torch.nn.utils.clip_grad_norm_ it takes gradients, not parameters,
+    adds nothing to the norm in the divisor (there 1e-6), and raises ValueError
+    where no gradient is given (there a norm of 0): there is no device to put
+    the norm on, so a step without gradients of its own has to skip the call."""
     grads = _tensors(grads)
     if out is not None:
         out = _tensors(out)
