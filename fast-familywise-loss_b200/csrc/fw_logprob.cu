@@ -12,7 +12,7 @@
 // writes theirs.  4096 x 32000: forward float32 77 us (6.8 TB/s), bfloat16 48
 // (5.5: the exponentials beside it), with 5 alternatives 88 and 60, gradient 167
 // and 86 (6.1 to 6.3 TB/s).  Few rows are bound by latency: 48 x 128256 bfloat16
-// 6.3 us, with 20 alternatives 10.7.
+// 6.3 to 6.8 us (8 CTAs a row), with 20 alternatives 10.7 to 11.3 (4 CTAs a row).
 //
 // The k likeliest columns come without a second pass over the row.  Every
 // thread also knows its largest element; the k-th largest of these (taken over
@@ -41,8 +41,9 @@ constexpr float kFloor = -200.0f;  // 2^kFloor is 0 in fp32; keeps 0 * t finite
 // Slots in flight per thread, and CTAs of 256 threads per SM.  4096 x 32000
 // without and with 5 alternatives, float32: 4 slots and 4 CTAs 82 and 97 us, 4
 // and 5 80 and 93, 8 and 4 77 and 88; bfloat16: 52 and 66, 48 and 60, 48 and 68.
-// Rows split over CTAs, 48 x 128256 bfloat16 without and with 20 alternatives: 4
-// and 4 7.7 and 14.7, 8 and 4 7.8 and 14.7, 8 and 3 7.2 and 13.4.
+// Rows split over CTAs, 48 x 128256 bfloat16 without (8 CTAs a row) and with 20
+// alternatives (4): 4 and 4 7.4 and 11.8, 8 and 4 7.5 and 11.4, 8 and 3 6.7 and
+// 11.2.
 template <class T, int CL>
 constexpr int kBatch = sizeof(T) == 4 || CL > 1 ? 8 : 4;
 constexpr int kSplitCtas = 3;

@@ -46,11 +46,17 @@
 // where a and b differ, and a row of H is then rounded no further.  What the
 // rounding takes from the label's entry, which would show in a whole row of dH
 // and in the largest terms of dW, is kept in fp32 and added to both: that much
-// of the label's row of W, and of the row of H.  Their error is 1.0 to 1.1 times
-// that of a form in 32 bits rounded at the end.
+// of the label's row of W, and of the row of H.  In flat rows their error is that
+// of a form in 32 bits rounded at the end.  It grows where another column than
+// the label's holds much of the probability, whose entry is as large and rounded
+// with nothing kept (512 x 256 into 4000, labels drawn from the rows; mean
+// entropies of 8, 5.5, 4, 3, 1.8, 0.7 and 0.4 nats: 1.00, 1.01, 1.04, 1.06, 1.1,
+// 1.16 and 1.2 times, with factors of the entropies as large as those of the log
+// probabilities 1.00, 1.07, 1.13, 1.13, 1.15, 1.16 and 1.2).
 // |p (l + h)| is at most (log V) / 4 + 0.3, under 5.2, hence 2^13 in the place
-// of 2^15 for float16.  bfloat16, 4014 live rows, 128256 x 4096: 13.4 to 14.0 ms;
-// float16, 1609 live rows, 32000 x 2048: 0.86 to 0.87 ms.
+// of 2^15 for float16.  bfloat16, 4014 live rows, 128256 x 4096: 13.4 to 14.1 ms;
+// float16, 1609 live rows, 32000 x 2048: 0.86 to 0.87 ms; at T < 0.5 (see
+// GradBothTile) 14.4 and 0.90.
 #include <cmath>
 
 #include "fw_reduce.cuh"
