@@ -741,13 +741,13 @@ struct GradTile {
 // A sum over all of K in the accumulator (KC 0) shrinks a logit more than the
 // forward's does (kLseStages), by up to D / 8 ulps of its terms, which T
 // divides too: of a winning logit of 50, D = 2048, a probability of 1 came out
-// 2e-4 too small at T = 1, 2 % at T = 0.01.  Down to kLowT that is a fifth or less
-// of the rounding of G to bfloat16 (2^-9), and once or twice that to float16.  At
-// lower temperatures z is made as in the forward: the same bits, of which the
-// maximum is one, and the probabilities add up to 1 within fp32's rounding
-// whatever T is.  Parts are short, and the epilogue of a tile's last one is then
-// waited for: 1609 live rows, 32000 x 2048 float16 172 and 217 us, 4014 rows,
-// 128256 x 4096 bfloat16 3.32 and 3.96 ms.
+// 2e-4 too small at T = 1, 2 % at T = 0.01.  Down to kLowT that is under
+// the rounding of G (2^-8 of an entry in bfloat16, 2^-11 in float16).  At lower
+// temperatures z is made as in the forward: the same bits, of which the maximum
+// is one, and the probabilities add up to 1 within fp32's rounding whatever T is.
+// Parts are short, and the epilogue of a tile's last one is then waited for: 1609
+// live rows, 32000 x 2048 float16 172 and 217 us, 4014 rows, 128256 x 4096
+// bfloat16 3.32 and 3.96 ms.
 // Nothing in `begin` waits: a row's factors, which are behind row_of, are asked
 // for after the first part, and worked out after the last (with parts: 226 us
 // where the labels' entries are looked at one by one, 217 all at once).
