@@ -117,3 +117,36 @@ def test_waits_that_gave_up_leave_nan(temperature):
     assert not got[0][y == -100].any()
     for x, ref in zip(torch.autograd.grad(out, (h, w), up), want):
         assert torch.equal(x, ref)
+
+
+def test_graphs_of_both_forms():
+    """Steps on either side of T = 0.5 captured one after the other and replayed on new rows."""
+    g = R.gen(60)
+    h = R.normal((300, 600), torch.bfloat16, g).requires_grad_(True)
+    w = R.normal((1000, 600), torch.bfloat16, g, 0.1).requires_grad_(True)
+    y = tokens_for(300, 1000, g, 0.1)
+    a, b = torch.randn(300, generator=g, device="cuda"), torch.randn(300, generator=g, device="cuda")
+
+    def step(temperature):
+        out = fw.lm_head_log_probs(h, w, y, temperature=temperature)
+        return [*(t.detach() for t in out), *torch.autograd.grad(out, (h, w), (a, b))]
+
+    temperatures = (0.5, 0.2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(1.0)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, held = [torch.cuda.CUDAGraph() for _ in temperatures], []
+    for graph, t in zip(graphs, temperatures):
+        with torch.cuda.graph(graph):
+            held.append(step(t))
+    for seed in (1, 2):
+        with torch.no_grad():
+            h.copy_(R.normal((300, 600), torch.bfloat16, R.gen(seed)))
+        y.copy_(tokens_for(300, 1000, R.gen(seed + 9), 0.3))
+        for graph in graphs:
+            graph.replay()
+        for t, captured in zip(temperatures, held):
+            for p, q in zip(captured, step(t)):
+                assert torch.equal(p, q)
